@@ -89,6 +89,13 @@ SIGNATURES = {
     "aw_ops_matmul_add_residual": (_c_int, [_vp, _vp, _vp, _vp, _u32, _u32, _u32, ctypes.c_float, _vp]),
     "aw_ops_matmul_silu_gate": (_c_int, [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _vp]),
     "aw_ops_matmul_qkv": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _vp]),
+    "aw_rotary_frequencies": (_c_int, [_vp, _vp]),
+    "aw_ops_rotary": (_c_int, [_vp, _vp, _vp]),
+    "aw_ops_qk_norm_rotary": (_c_int, [_vp, _vp, _vp]),
+    "aw_ops_append_paged": (_c_int, [_vp, _vp, _vp]),
+    "aw_ops_check_rotary": (_c_int, [_vp, _c_int, ctypes.c_char_p, _sz]),
+    "aw_ops_check_append": (_c_int, [_vp, ctypes.c_char_p, _sz]),
+    "aw_abi_ops_desc_sizes": (None, [ctypes.POINTER(_sz)]),
 }
 
 _cache: dict[str, ctypes.CDLL] = {}

@@ -10,8 +10,10 @@
 namespace aw_engine_internal {
 
 // Bits of the engine's device error word (aw_engine_check_device_errors):
-// 1 hot block ref, 2 cold block ref, 4 atom index (weaver_kernels.hpp), 8 token id.
+// 1 hot block ref, 2 cold block ref, 4 atom index (weaver_kernels.hpp), 8 token id,
+// 16 token counts of a sequence.
 constexpr uint32_t kErrTokenBit = 8u;
+constexpr uint32_t kErrSeqBit = 16u;
 
 int device(const aw_engine* e);        // HIP device ordinal
 uint32_t compute_units(const aw_engine* e);

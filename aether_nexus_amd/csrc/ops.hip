@@ -8,13 +8,17 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
+#include <cstdarg>
 #include <cstdint>
+#include <cstdio>
 #include <tuple>
 
 #include "../../include/aether_ops.h"
 #include "engine_internal.hpp"
 #include "gemm_kernels.hpp"
 #include "ops_kernels.hpp"
+#include "rotary_kernels.hpp"
 
 namespace {
 
@@ -209,6 +213,131 @@ int launch_products(aw_engine* e, const char* what, const uint16_t* a, const Pro
     else
         AW_SKINNY(4, 8);
 #undef AW_SKINNY
+    OPS_HIP(e, hipGetLastError());
+    return AW_OK;
+}
+
+// Whether rows [tokens][heads * hd] at `p` share an element with those at `o`, other
+// than by being the same rows.
+bool rows_clash(const uint16_t* p, uint64_t stride, const uint16_t* o, uint64_t o_stride, uint64_t tokens, uint64_t row) {
+    if (tokens == 0 || (p == o && (stride == o_stride || tokens == 1))) return false;
+    return p < o + (tokens - 1) * o_stride + row && o < p + (tokens - 1) * stride + row;
+}
+
+int refuse(char* msg, size_t len, int code, const char* fmt, ...) __attribute__((format(printf, 4, 5)));
+int refuse(char* msg, size_t len, int code, const char* fmt, ...) {
+    if (msg && len) {
+        va_list ap;
+        va_start(ap, fmt);
+        vsnprintf(msg, len, fmt, ap);
+        va_end(ap);
+    }
+    return code;
+}
+
+constexpr uint64_t kMostStride = 1ull << 30; // elements: tokens * stride * 2 bytes stays below 2^63
+
+// The checks that the three rotary calls share, and their kernel arguments.
+int rotary_args(const char* what, const aw_rotary_desc* d, bool append, awo::RotaryArgs* out, char* msg, size_t len) {
+    auto bad = [&](const char* why) { return refuse(msg, len, AW_E_INVALID_ARG, "%s: %s", what, why); };
+    if (d->reserved) return bad("reserved must be 0");
+    if (d->head_dim == 0) return bad("head_dim is 0");
+    if (d->head_dim > awo::kRotaryMaxDim)
+        return refuse(msg, len, AW_E_UNSUPPORTED, "%s: head_dim %u exceeds %u", what, d->head_dim, awo::kRotaryMaxDim);
+    if (d->rotary_dim % 2 || d->rotary_dim > d->head_dim)
+        return refuse(msg, len, AW_E_INVALID_ARG, "%s: rotary_dim %u must be even and at most head_dim %u", what,
+                      d->rotary_dim, d->head_dim);
+    if (d->layout != AW_ROTARY_HALF && d->layout != AW_ROTARY_INTERLEAVED)
+        return refuse(msg, len, AW_E_INVALID_ARG, "%s: layout %u", what, d->layout);
+    if (d->rotary_dim && !d->inv_freq) return bad("inv_freq is required");
+    if (d->rotary_dim && !std::isfinite(d->magnitude)) return bad("magnitude must be finite");
+    if ((d->q_norm || d->k_norm) && !(d->eps >= 0.0f && std::isfinite(d->eps))) return bad("eps must be finite and not negative");
+    if ((d->q_heads && (!d->q || !d->q_out)) || (d->kv_heads && (!d->k || (!append && !d->k_out)))) return bad("null pointer");
+    if (d->num_tokens > 0x7FFFFFFFu || d->q_heads > 0xFFFFu || d->kv_heads > 0xFFFFu)
+        return refuse(msg, len, AW_E_UNSUPPORTED, "%s: too many tokens or heads", what);
+    awo::RotaryArgs& a = *out;
+    a = awo::RotaryArgs{};
+    const uint64_t q_row = (uint64_t)d->q_heads * d->head_dim, k_row = (uint64_t)d->kv_heads * d->head_dim;
+    a.q_stride = d->q_stride ? d->q_stride : q_row;
+    a.q_out_stride = d->q_out_stride ? d->q_out_stride : q_row;
+    a.k_stride = d->k_stride ? d->k_stride : k_row;
+    a.k_out_stride = d->k_out_stride ? d->k_out_stride : k_row;
+    if (a.q_stride < q_row || a.q_out_stride < q_row || a.k_stride < k_row || a.k_out_stride < k_row)
+        return bad("a stride is shorter than a token's heads");
+    if (std::max(std::max(a.q_stride, a.q_out_stride), std::max(a.k_stride, a.k_out_stride)) > kMostStride)
+        return refuse(msg, len, AW_E_UNSUPPORTED, "%s: a stride exceeds 2^30 elements", what);
+    if ((d->q_heads && rows_clash(d->q, a.q_stride, d->q_out, a.q_out_stride, d->num_tokens, q_row)) ||
+        (d->kv_heads && !append && rows_clash(d->k, a.k_stride, d->k_out, a.k_out_stride, d->num_tokens, k_row)))
+        return bad("the output overlaps its input, and is not the input itself");
+    a.q = d->q;
+    a.k = d->k;
+    a.q_out = d->q_out;
+    a.k_out = d->k_out;
+    a.q_norm = d->q_norm;
+    a.k_norm = d->k_norm;
+    a.positions = d->positions;
+    a.inv_freq = d->inv_freq;
+    a.tokens = d->num_tokens;
+    a.q_heads = d->q_heads;
+    a.kv_heads = d->kv_heads;
+    a.hd = d->head_dim;
+    a.rotary_dim = d->rotary_dim;
+    a.interleaved = d->layout == AW_ROTARY_INTERLEAVED ? 1u : 0u;
+    a.start = d->start_position;
+    a.magnitude = d->magnitude;
+    a.eps = d->eps;
+    return AW_OK;
+}
+
+// aw_ops_rotary (norms false) and aw_ops_qk_norm_rotary.
+int rows_args(const aw_rotary_desc* d, bool norms, awo::RotaryArgs* a, char* msg, size_t len) {
+    const char* what = norms ? "qk_norm_rotary" : "rotary";
+    if (!d) return refuse(msg, len, AW_E_INVALID_ARG, "%s: null descriptor", what);
+    if (!norms && (d->q_norm || d->k_norm))
+        return refuse(msg, len, AW_E_INVALID_ARG, "rotary: norm weights given (qk_norm_rotary takes them)");
+    if (!norms && d->rotary_dim == 0) return refuse(msg, len, AW_E_INVALID_ARG, "rotary: rotary_dim is 0");
+    if (norms && ((d->q_heads && !d->q_norm) || (d->kv_heads && !d->k_norm)))
+        return refuse(msg, len, AW_E_INVALID_ARG, "qk_norm_rotary: norm weights are required");
+    return rotary_args(what, d, false, a, msg, len);
+}
+
+int append_args(const aw_append_desc* d, awo::RotaryArgs* a, char* msg, size_t len) {
+    auto bad = [&](const char* why) { return refuse(msg, len, AW_E_INVALID_ARG, "append_paged: %s", why); };
+    if (!d) return bad("null descriptor");
+    if (int rc = rotary_args("append_paged", &d->rows, true, a, msg, len)) return rc;
+    if (d->reserved) return bad("reserved must be 0");
+    if (d->rows.kv_heads == 0) return bad("kv_heads is 0");
+    if (d->rows.k_out) return bad("k_out must be NULL (k goes to hot_k)");
+    if (d->v && !d->hot_v) return bad("v given without hot_v");
+    if (!d->hot_k || !d->refs || !d->seq_hot || (d->hot_v && !d->v)) return bad("null pointer");
+    if (d->hot_blocks == 0 || d->hot_count == 0) return bad("hot_blocks and hot_count must be >= 1");
+    if (d->hot_blocks > 1ull << 31) return bad("hot_blocks exceeds 2^31, the refs' range");
+    if (d->refs_stride < d->hot_count)
+        return refuse(msg, len, AW_E_INVALID_ARG, "append_paged: refs_stride %u < hot_count %u", d->refs_stride, d->hot_count);
+    if (!d->token_offsets && d->batch && d->rows.num_tokens % d->batch)
+        return refuse(msg, len, AW_E_INVALID_ARG, "append_paged: %u tokens over %u sequences need token_offsets",
+                      d->rows.num_tokens, d->batch);
+    const uint64_t row = (uint64_t)d->rows.kv_heads * d->rows.head_dim;
+    a->v_stride = d->v_stride ? d->v_stride : row;
+    if (a->v_stride < row) return bad("a stride is shorter than a token's heads");
+    if (a->v_stride > kMostStride) return refuse(msg, len, AW_E_UNSUPPORTED, "append_paged: a stride exceeds 2^30 elements");
+    a->v = d->v;
+    a->k_out = d->hot_k;
+    a->v_out = d->hot_v;
+    a->batch = d->batch;
+    a->hot_count = d->hot_count;
+    a->refs_stride = d->refs_stride;
+    a->hot_blocks = d->hot_blocks;
+    a->refs = d->refs;
+    a->seq_hot = d->seq_hot;
+    a->token_offsets = d->token_offsets;
+    return AW_OK;
+}
+
+template <bool APPEND>
+int launch_rotary(aw_engine* e, awo::RotaryArgs& a, hipStream_t st) {
+    a.err = ei::error_word(e);
+    hipLaunchKernelGGL(awo::rotary_kernel<APPEND>, dim3(a.tokens), dim3(256), 0, st, a);
     OPS_HIP(e, hipGetLastError());
     return AW_OK;
 }
@@ -408,6 +537,72 @@ int aw_ops_causal_attention(aw_engine* e, const uint16_t* q, const uint16_t* k, 
                             uint32_t kv_len, uint32_t head_dim, uint64_t cache_tokens, void* stream) {
     if (!e) return AW_E_INVALID_ARG;
     return aw_multihead_attention_device(e, q, k, v, output, kv_len, head_dim, 1, 1, 1, cache_tokens, stream);
+}
+
+int aw_rotary_frequencies(const aw_rotary_scaling* s, double* inv_freq) {
+    if (!s || !inv_freq || s->rotary_dim == 0 || s->rotary_dim % 2) return AW_E_INVALID_ARG;
+    if (!(s->theta > 0.0 && std::isfinite(s->theta)) || s->kind > AW_ROTARY_SCALE_PARTS) return AW_E_INVALID_ARG;
+    if (s->kind != AW_ROTARY_SCALE_NONE && !(s->factor > 0.0 && std::isfinite(s->factor))) return AW_E_INVALID_ARG;
+    if (s->kind == AW_ROTARY_SCALE_NTK && s->rotary_dim == 2) return AW_E_INVALID_ARG;
+    if (s->kind == AW_ROTARY_SCALE_PARTS && !(s->original_length > 0.0 && std::isfinite(s->original_length) &&
+                                              s->low >= 0.0 && s->high > s->low && std::isfinite(s->high)))
+        return AW_E_INVALID_ARG;
+    const double n = (double)s->rotary_dim;
+    const double theta = s->kind == AW_ROTARY_SCALE_NTK ? s->theta * std::pow(s->factor, n / (n - 2.0)) : s->theta;
+    for (uint32_t p = 0; p < s->rotary_dim / 2; ++p) {
+        double f = std::pow(theta, -2.0 * (double)p / n);
+        if (s->kind == AW_ROTARY_SCALE_LINEAR) f /= s->factor;
+        if (s->kind == AW_ROTARY_SCALE_PARTS) {
+            const double turns = s->original_length * f / (2.0 * 3.14159265358979323846);
+            const double keep = std::min(1.0, std::max(0.0, (turns - s->low) / (s->high - s->low)));
+            f = (1.0 - keep) * f / s->factor + keep * f;
+        }
+        inv_freq[p] = f;
+    }
+    return AW_OK;
+}
+
+int aw_ops_check_rotary(const aw_rotary_desc* d, int norms, char* msg, size_t msg_len) {
+    awo::RotaryArgs a;
+    return rows_args(d, norms != 0, &a, msg, msg_len);
+}
+
+int aw_ops_check_append(const aw_append_desc* d, char* msg, size_t msg_len) {
+    awo::RotaryArgs a;
+    return append_args(d, &a, msg, msg_len);
+}
+
+int aw_ops_rotary(aw_engine* e, const aw_rotary_desc* d, void* stream) {
+    int rc = enter(e);
+    if (rc) return rc;
+    awo::RotaryArgs a;
+    char msg[256] = {0};
+    if ((rc = rows_args(d, false, &a, msg, sizeof msg))) return ei::fail(e, rc, "%s", msg);
+    return d->num_tokens && d->q_heads + d->kv_heads ? launch_rotary<false>(e, a, (hipStream_t)stream) : AW_OK;
+}
+
+int aw_ops_qk_norm_rotary(aw_engine* e, const aw_rotary_desc* d, void* stream) {
+    int rc = enter(e);
+    if (rc) return rc;
+    awo::RotaryArgs a;
+    char msg[256] = {0};
+    if ((rc = rows_args(d, true, &a, msg, sizeof msg))) return ei::fail(e, rc, "%s", msg);
+    return d->num_tokens && d->q_heads + d->kv_heads ? launch_rotary<false>(e, a, (hipStream_t)stream) : AW_OK;
+}
+
+int aw_ops_append_paged(aw_engine* e, const aw_append_desc* d, void* stream) {
+    int rc = enter(e);
+    if (rc) return rc;
+    awo::RotaryArgs a;
+    char msg[256] = {0};
+    if ((rc = append_args(d, &a, msg, sizeof msg))) return ei::fail(e, rc, "%s", msg);
+    return d->rows.num_tokens && d->batch ? launch_rotary<true>(e, a, (hipStream_t)stream) : AW_OK;
+}
+
+void aw_abi_ops_desc_sizes(size_t sizes[3]) {
+    sizes[0] = sizeof(aw_rotary_scaling);
+    sizes[1] = sizeof(aw_rotary_desc);
+    sizes[2] = sizeof(aw_append_desc);
 }
 
 int aw_debug_product_tile(uint32_t compute_units, uint32_t m, const uint32_t* n, uint32_t products, uint32_t k,

@@ -1435,10 +1435,11 @@ int aw_engine_check_device_errors(aw_engine* e, void* stream) {
     if (!word) return AW_OK;
     AW_HIP(e, hipMemsetAsync(e->err, 0, 4, st));
     AW_HIP(e, hipStreamSynchronize(st));
-    return fail(e, AW_E_OOB, "device saw out-of-range input:%s%s%s%s (the affected tokens or terms were skipped)",
+    return fail(e, AW_E_OOB, "device saw out-of-range input:%s%s%s%s%s (the affected tokens or terms were skipped)",
                 (word & aw::kErrHotRef) ? " hot block ref" : "", (word & aw::kErrColdRef) ? " cold block ref" : "",
                 (word & aw::kErrAtom) ? " atom index" : "",
-                (word & aw_engine_internal::kErrTokenBit) ? " token id" : "");
+                (word & aw_engine_internal::kErrTokenBit) ? " token id" : "",
+                (word & aw_engine_internal::kErrSeqBit) ? " sequence length" : "");
 }
 
 

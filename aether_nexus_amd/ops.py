@@ -11,8 +11,13 @@ anything is enqueued (the C ABI takes raw pointers).
 """
 from __future__ import annotations
 
+import ctypes
 from typing import Optional
 
+import numpy as np
+
+from . import _lib
+from .types import BLOCK_SIZE, ROTARY_SCALINGS, AppendDesc, RotaryDesc, RotaryScaling
 from .weaver import WeaverEngine, WeaverError, _ptr, _stream
 
 AW_E_INVALID_ARG = -1
@@ -56,6 +61,160 @@ def _checker(*names):
 _f16 = _checker("float16", "int16")  # f16 values or their bit patterns
 _f32 = _checker("float32")
 _u32 = _checker("int32")
+_f64 = _checker("float64")
+
+
+def _token_rows(t, tokens: int, heads: int, head_dim: int, what: str) -> int:
+    """Token stride (elements) of rows [tokens][heads][head_dim]: a contiguous tensor, a
+    raw pointer to one, or a view with contiguous heads whose rows lie further apart
+    (the q, k or v part of a fused product's output)."""
+    row = heads * head_dim
+    if t is None or isinstance(t, int) or not hasattr(t, "is_contiguous") or t.is_contiguous():
+        _f16(t, tokens * row, what)
+        return row
+    inner = ((heads, head_dim), (head_dim, 1)) if t.dim() == 3 else ((row,), (1,))
+    if t.dim() not in (2, 3) or tuple(t.shape[1:]) != inner[0] or t.shape[0] < tokens or \
+            any(n > 1 and s != w for n, s, w in zip(inner[0], t.stride()[1:], inner[1])) or t.stride(0) < row:
+        raise WeaverError(f"{what}: a view must be [tokens][{heads}][{head_dim}] (or flat rows) with contiguous heads "
+                          f"and rows apart, got shape {tuple(t.shape)}, strides {tuple(t.stride())}", AW_E_INVALID_ARG)
+    _f16(t[:0].contiguous(), 0, what)  # dtype and device
+    return t.stride(0)
+
+
+def _one_device(desc, tensors) -> None:
+    """Records the tensors' GPU in the descriptor (raw pointers have none); the call compares it with the engine's."""
+    where = {t.device.index for t in tensors if hasattr(t, "device")}
+    if len(where) > 1:
+        raise WeaverError(f"tensors on several GPUs: {sorted(where)}", AW_E_INVALID_ARG)
+    desc._device = where.pop() if where else None
+    desc._keep = tensors
+
+
+def rotary_frequencies(rotary_dim: int, theta: float, scaling: str = "none", factor: float = 1.0,
+                       original_length: float = 0.0, low: float = 1.0, high: float = 32.0, lib_path=None) -> np.ndarray:
+    """The rotary_dim / 2 frequencies (radians per position, float64) of aw_rotary_frequencies:
+    theta^(-2p / rotary_dim), scaled for contexts longer than a model was trained on.
+    ``scaling``: "none"; "linear" (divided by ``factor``); "ntk" (theta raised by
+    factor^(d / (d - 2))); "parts" (pairs that turn more than ``high`` times over
+    ``original_length`` kept, fewer than ``low`` times divided, a ramp between).  No GPU needed."""
+    if scaling not in ROTARY_SCALINGS:
+        raise WeaverError(f"rotary scaling {scaling!r} (one of {', '.join(ROTARY_SCALINGS)})", AW_E_INVALID_ARG)
+    if rotary_dim < 2 or rotary_dim % 2 or rotary_dim >= 2 ** 32:
+        raise WeaverError(f"rotary_dim {rotary_dim} must be even and at least 2", AW_E_INVALID_ARG)
+    out = np.empty(rotary_dim // 2, dtype=np.float64)
+    s = RotaryScaling(rotary_dim, ROTARY_SCALINGS[scaling], theta, factor, original_length, low, high)
+    if _lib.load(lib_path).aw_rotary_frequencies(ctypes.byref(s), out.ctypes.data):
+        raise WeaverError("rotary_frequencies: theta and factor must be positive, rotary_dim > 2 for ntk, and for parts "
+                          "original_length > 0 and 0 <= low < high", AW_E_INVALID_ARG)
+    return out
+
+
+class Rotary:
+    """A rotation: which dims turn, in which pairs, and the frequencies on the device.
+
+    ``rotary_dim`` dims of each head turn (the others pass), in pairs (p, p +
+    rotary_dim / 2) or, ``interleaved``, (2p, 2p + 1).  Frequencies are those of
+    ``rotary_frequencies``, or ``inv_freq`` (rotary_dim / 2 values in radians per
+    position) as given.  ``magnitude`` multiplies cosines and sines (some long-context
+    scalings sharpen the scores so)."""
+
+    def __init__(self, rotary_dim: int, theta: float = 10000.0, *, interleaved: bool = False, scaling: str = "none",
+                 factor: float = 1.0, original_length: float = 0.0, low: float = 1.0, high: float = 32.0,
+                 magnitude: float = 1.0, inv_freq=None, device="cuda:0"):
+        import torch
+        if inv_freq is None:
+            inv_freq = rotary_frequencies(rotary_dim, theta, scaling, factor, original_length, low, high)
+        self.inv_freq = torch.as_tensor(inv_freq, dtype=torch.float64).to(device).contiguous()
+        if rotary_dim < 2 or rotary_dim % 2 or self.inv_freq.numel() != rotary_dim // 2:
+            raise WeaverError(f"rotary_dim {rotary_dim} must be even, with half as many frequencies "
+                              f"({self.inv_freq.numel()})", AW_E_INVALID_ARG)
+        self.rotary_dim, self.interleaved, self.magnitude = rotary_dim, interleaved, magnitude
+
+
+def _rotary_rows(r: RotaryDesc, *, num_tokens, q_heads, kv_heads, head_dim, rotary, q, k, q_out, k_out, positions,
+                 start_position, q_norm, k_norm, eps) -> list:
+    """Fills the descriptor of the rows; returns the tensors behind it."""
+    r.num_tokens, r.q_heads, r.kv_heads, r.head_dim = num_tokens, q_heads, kv_heads, head_dim
+    r.start_position, r.eps, r.magnitude = start_position, eps, 1.0
+    for t, heads, name in ((q, q_heads, "q"), (k, kv_heads, "k"), (q_out, q_heads, "q_out"), (k_out, kv_heads, "k_out")):
+        setattr(r, name, _ptr(t))
+        setattr(r, name + "_stride", _token_rows(t, num_tokens, heads, head_dim, name))
+    for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+        _f16(t, head_dim, name)
+        setattr(r, name, _ptr(t))
+    _u32(positions, num_tokens, "positions")
+    r.positions = _ptr(positions)
+    if rotary is not None:
+        _f64(rotary.inv_freq, rotary.rotary_dim // 2, "inv_freq")
+        r.rotary_dim, r.layout, r.magnitude = rotary.rotary_dim, int(rotary.interleaved), rotary.magnitude
+        r.inv_freq = _ptr(rotary.inv_freq)
+    return [q, k, q_out, k_out, q_norm, k_norm, positions] + ([rotary.inv_freq] if rotary is not None else [])
+
+
+def make_rotary_desc(*, num_tokens: int, q_heads: int, kv_heads: int, head_dim: int, rotary: Optional[Rotary], q, k,
+                     q_out=None, k_out=None, positions=None, start_position: int = 0, q_norm=None, k_norm=None,
+                     eps: float = 1e-5) -> RotaryDesc:
+    """An ``aw_rotary_desc`` from device tensors (or raw device pointers to contiguous
+    rows), for ``rotary`` and ``qk_norm_rotary``.  q_out and k_out default to q and k
+    (in place); ``positions`` is an int32 tensor of one (unsigned) position per token."""
+    d = RotaryDesc()
+    keep = _rotary_rows(d, num_tokens=num_tokens, q_heads=q_heads, kv_heads=kv_heads, head_dim=head_dim, rotary=rotary,
+                        q=q, k=k, q_out=q if q_out is None else q_out, k_out=k if k_out is None else k_out,
+                        positions=positions, start_position=start_position, q_norm=q_norm, k_norm=k_norm, eps=eps)
+    _one_device(d, keep)
+    return d
+
+
+def _table(refs, batch: int, count: int, stride: Optional[int], what: str) -> int:
+    """Row stride of a block table [batch][>= count]."""
+    if hasattr(refs, "dim") and refs.dim() == 2:
+        if refs.shape[0] < batch or refs.shape[1] < count or (refs.shape[1] > 1 and refs.stride(1) != 1) or \
+                (batch > 1 and refs.stride(0) < count):
+            raise WeaverError(f"{what}: a table of [{batch}][{count}] entries is read, got shape {tuple(refs.shape)}, "
+                              f"strides {tuple(refs.stride())}", AW_E_INVALID_ARG)
+        _u32(refs[:0].contiguous(), 0, what)
+        return refs.stride(0) if batch > 1 else max(refs.stride(0), count)
+    stride = count if stride is None else stride
+    _u32(refs, (batch - 1) * stride + count if batch else 0, what)
+    return stride
+
+
+def make_append_desc(*, batch: int, num_tokens: int, q_heads: int, kv_heads: int, head_dim: int, k, v, hot_k, hot_v,
+                     refs, seq_hot, hot_count: Optional[int] = None, hot_blocks: Optional[int] = None,
+                     refs_stride: Optional[int] = None, token_offsets=None, rotary: Optional[Rotary] = None, q=None,
+                     q_out=None, positions=None, start_position: int = 0, q_norm=None, k_norm=None,
+                     eps: float = 1e-5) -> AppendDesc:
+    """An ``aw_append_desc`` from device tensors (or raw device pointers), for ``append_paged``.
+    ``refs`` [batch][refs_stride] and ``seq_hot`` [batch] (tokens AFTER the append) are the block
+    table and counts of the decode that follows; ``hot_count`` (pages of a sequence) defaults to a
+    2-D table's columns and ``hot_blocks`` to the pool tensor's pages.  Without ``rotary`` k and q
+    keep their positions' angles as they are; without ``q`` (q_heads 0) only k and v move."""
+    d = AppendDesc()
+    if q is None and q_heads:
+        raise WeaverError("append_paged: q_heads without q", AW_E_INVALID_ARG)
+    keep = _rotary_rows(d.rows, num_tokens=num_tokens, q_heads=q_heads, kv_heads=kv_heads, head_dim=head_dim,
+                        rotary=rotary, q=q, k=k, q_out=q if q_out is None else q_out, k_out=None, positions=positions,
+                        start_position=start_position, q_norm=q_norm, k_norm=k_norm, eps=eps)
+    page = BLOCK_SIZE * kv_heads * head_dim
+    if hot_count is None:
+        if not hasattr(refs, "dim") or refs.dim() != 2:
+            raise WeaverError("append_paged: hot_count is required without a 2-D table", AW_E_INVALID_ARG)
+        hot_count = refs.shape[1]
+    if hot_blocks is None:
+        if not hasattr(hot_k, "numel"):
+            raise WeaverError("append_paged: hot_blocks is required for a raw pool pointer", AW_E_INVALID_ARG)
+        hot_blocks = hot_k.numel() // max(page, 1)
+    for t, name in ((hot_k, "hot_k"), (hot_v, "hot_v")):
+        _f16(t, hot_blocks * page, name)
+        setattr(d, name, _ptr(t))
+    d.v_stride = _token_rows(v, num_tokens, kv_heads, head_dim, "v")
+    d.batch, d.hot_count, d.hot_blocks, d.v = batch, hot_count, hot_blocks, _ptr(v)
+    d.refs_stride = _table(refs, batch, hot_count, refs_stride, "refs")
+    _u32(seq_hot, batch, "seq_hot")
+    _u32(token_offsets, batch + 1, "token_offsets")
+    d.refs, d.seq_hot, d.token_offsets = _ptr(refs), _ptr(seq_hot), _ptr(token_offsets)
+    _one_device(d, keep + [v, hot_k, hot_v, refs, seq_hot, token_offsets])
+    return d
 
 
 class OpsEngine:
@@ -223,6 +382,26 @@ class OpsEngine:
             _f16(t, m * n, f"matmul_qkv {w}")
         self._call("aw_ops_matmul_qkv", _ptr(a), _ptr(b_q), _ptr(b_k), _ptr(b_v), _ptr(q), _ptr(k_out), _ptr(v_out),
                    m, n_q, n_kv, k, _stream(stream))
+
+    # -- rotary positions, head norms, paged appends (no reference counterpart): a call's descriptor
+    # holds its tensors and may be used again for as long as they are the call's
+    def _request(self, name: str, desc, stream: Optional[int]) -> None:
+        if desc._device is not None and desc._device != self.engine.device:
+            raise WeaverError(f"{name}: tensors on GPU {desc._device}, the engine on {self.engine.device}", AW_E_INVALID_ARG)
+        self._call(name, ctypes.byref(desc), _stream(stream))
+
+    def rotary(self, desc: RotaryDesc, stream: Optional[int] = None) -> None:
+        """q and k heads turned by their positions (``make_rotary_desc``)."""
+        self._request("aw_ops_rotary", desc, stream)
+
+    def qk_norm_rotary(self, desc: RotaryDesc, stream: Optional[int] = None) -> None:
+        """q and k heads RMS-normed with weights of their own, then turned (``make_rotary_desc``)."""
+        self._request("aw_ops_qk_norm_rotary", desc, stream)
+
+    def append_paged(self, desc: AppendDesc, stream: Optional[int] = None) -> None:
+        """A batch's new k and v rows into their sequences' pages, k and q normed and turned
+        on the way (``make_append_desc``)."""
+        self._request("aw_ops_append_paged", desc, stream)
 
     def multihead_attention(self, q, k_cache, v_cache, output, kv_len: int, head_dim: int, q_heads: int,
                             kv_heads: int, num_queries: int, cache_tokens: Optional[int] = None,

@@ -229,6 +229,52 @@ class EncodeDesc(ctypes.Structure):
     ]
 
 
+class RotaryScaling(ctypes.Structure):
+    """``aw_rotary_scaling`` (include/aether_ops.h)."""
+
+    _fields_ = [
+        ("rotary_dim", ctypes.c_uint32), ("kind", ctypes.c_uint32), ("theta", ctypes.c_double),
+        ("factor", ctypes.c_double), ("original_length", ctypes.c_double), ("low", ctypes.c_double),
+        ("high", ctypes.c_double),
+    ]
+
+
+#: AW_ROTARY_SCALE_* by name.
+ROTARY_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "parts": 3}
+
+
+class RotaryDesc(ctypes.Structure):
+    """``aw_rotary_desc`` (include/aether_ops.h): rows of q and k to norm and turn."""
+
+    _device = None  # the GPU of the tensors behind it, where it was made from tensors
+
+    _fields_ = [
+        ("num_tokens", ctypes.c_uint32), ("q_heads", ctypes.c_uint32), ("kv_heads", ctypes.c_uint32),
+        ("head_dim", ctypes.c_uint32), ("rotary_dim", ctypes.c_uint32), ("layout", ctypes.c_uint32),
+        ("start_position", ctypes.c_uint32), ("magnitude", ctypes.c_float), ("eps", ctypes.c_float),
+        ("reserved", ctypes.c_uint32),
+        ("q_stride", ctypes.c_uint64), ("k_stride", ctypes.c_uint64),
+        ("q_out_stride", ctypes.c_uint64), ("k_out_stride", ctypes.c_uint64),
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("q_out", ctypes.c_void_p), ("k_out", ctypes.c_void_p),
+        ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p), ("inv_freq", ctypes.c_void_p),
+    ]
+
+
+class AppendDesc(ctypes.Structure):
+    """``aw_append_desc`` (include/aether_ops.h): new tokens of a batch into their pages."""
+
+    _device = None  # the GPU of the tensors behind it, where it was made from tensors
+
+    _fields_ = [
+        ("rows", RotaryDesc),
+        ("batch", ctypes.c_uint32), ("hot_count", ctypes.c_uint32), ("refs_stride", ctypes.c_uint32),
+        ("reserved", ctypes.c_uint32), ("v_stride", ctypes.c_uint64), ("hot_blocks", ctypes.c_uint64),
+        ("v", ctypes.c_void_p), ("hot_k", ctypes.c_void_p), ("hot_v", ctypes.c_void_p),
+        ("refs", ctypes.c_void_p), ("seq_hot", ctypes.c_void_p), ("token_offsets", ctypes.c_void_p),
+    ]
+
+
 class PlanInfo(ctypes.Structure):
     """``aw_decode_plan_info``."""
 

@@ -130,6 +130,105 @@ int aw_ops_matmul_qkv(aw_engine* engine, const uint16_t* a, const uint16_t* b_q,
                       const uint16_t* b_v, uint16_t* q, uint16_t* k_out, uint16_t* v_out, uint32_t m, uint32_t n_q,
                       uint32_t n_kv, uint32_t k, void* hip_stream);
 
+/* ---- rotary positions, head norms, paged appends (no reference counterpart) ---
+ * What a batch over pages needs around aw_decode_device that aw_ops_rope and
+ * aw_ops_copy_buffer do not give: a position for each token, either order of
+ * pairs, part of a head, frequencies scaled for long contexts, rows that are
+ * views of a fused q/k/v product, each head normed first, and the rows written
+ * through the block table. */
+
+#define AW_ROTARY_HALF        0u /* pair p is dims (p, p + rotary_dim / 2), as aw_ops_rope's */
+#define AW_ROTARY_INTERLEAVED 1u /* pair p is dims (2 p, 2 p + 1) */
+
+#define AW_ROTARY_SCALE_NONE   0u /* f_p = theta^(-2 p / rotary_dim) */
+#define AW_ROTARY_SCALE_LINEAR 1u /* f_p / factor (position interpolation) */
+#define AW_ROTARY_SCALE_NTK    2u /* theta * factor^(rotary_dim / (rotary_dim - 2)) for theta; rotary_dim > 2 */
+#define AW_ROTARY_SCALE_PARTS  3u /* (1 - g) f_p / factor + g f_p with g = clamp((r_p - low) / (high - low), 0, 1),
+                                     r_p = original_length * f_p / (2 pi) the pair's turns over that length: pairs
+                                     that turn often are kept, those that turn less than `low` times interpolated */
+
+typedef struct aw_rotary_scaling {
+    uint32_t rotary_dim, kind;            /* AW_ROTARY_SCALE_* */
+    double theta, factor;                 /* factor: unused by NONE */
+    double original_length, low, high;    /* PARTS; 0 <= low < high */
+} aw_rotary_scaling;
+
+/* Host only: the rotary_dim / 2 frequencies, in radians per position, into
+ * `inv_freq` (host memory). */
+int aw_rotary_frequencies(const aw_rotary_scaling* scaling, double* inv_freq);
+
+/* One call's rows.  Strides are in f16 elements from token to token, 0 for heads *
+ * head_dim; the heads of a token are contiguous.  Rows of any alignment are taken.
+ * Rows, frequencies, positions and weights are device memory. */
+typedef struct aw_rotary_desc {
+    uint32_t num_tokens, q_heads, kv_heads, head_dim; /* head_dim <= 1024; either head count may be 0 */
+    uint32_t rotary_dim;            /* even, <= head_dim: dims [0, rotary_dim) turn, the others pass */
+    uint32_t layout;                /* AW_ROTARY_HALF or AW_ROTARY_INTERLEAVED */
+    uint32_t start_position;        /* of token 0, where positions is NULL */
+    float    magnitude;             /* cosines and sines are multiplied by it (1: a plain rotation) */
+    float    eps;                   /* aw_ops_qk_norm_rotary and appends with norms */
+    uint32_t reserved;              /* 0 */
+    uint64_t q_stride, k_stride, q_out_stride, k_out_stride;
+    const uint16_t* q;              /* [num_tokens][q_heads][head_dim] */
+    const uint16_t* k;              /* [num_tokens][kv_heads][head_dim] */
+    uint16_t*       q_out;          /* may be q (same stride: in place); no other overlap with an input */
+    uint16_t*       k_out;          /* likewise k; NULL in an append */
+    const uint16_t* q_norm;         /* [head_dim] weights */
+    const uint16_t* k_norm;
+    const uint32_t* positions;      /* [num_tokens], or NULL: start_position + token */
+    const double*   inv_freq;       /* [rotary_dim / 2] */
+} aw_rotary_desc;
+
+/* Pair (x0, x1) of every head of token t becomes magnitude * (x0 cos a - x1 sin a,
+ * x0 sin a + x1 cos a), a = position * inv_freq[p] taken in 64 bits (aw_ops_rope: in
+ * 32); cos, sin and the products in fp32, one rounding at the store.  Dims past
+ * rotary_dim are copied.  q_norm and k_norm must be NULL. */
+int aw_ops_rotary(aw_engine* engine, const aw_rotary_desc* desc, void* hip_stream);
+
+/* x * (1 / sqrt(mean(x^2) + eps)) * weight over each head's head_dim (fp32, as
+ * aw_ops_rms_norm), then aw_ops_rotary of it without rounding in between.  Needs the
+ * weights of every kind of head it is given; rotary_dim may be 0 (norms alone). */
+int aw_ops_qk_norm_rotary(aw_engine* engine, const aw_rotary_desc* desc, void* hip_stream);
+
+/* New tokens of `batch` sequences into their pages: k (normed where k_norm is given,
+ * turned where rotary_dim > 0) and v into the rows that the block table names, q
+ * (likewise) into q_out.  The table and the counts are those of the
+ * aw_decode_device call that follows (AW_F_SEQ_HOT_TOKENS): refs [batch][refs_stride],
+ * of which a sequence's first hot_count entries are its hot pages, and seq_hot
+ * [batch], the tokens of each sequence AFTER the append.  Sequence b's new tokens are
+ * rows token_offsets[b] .. token_offsets[b + 1] - 1 (token_offsets [batch + 1],
+ * ascending, from 0; NULL: num_tokens / batch rows each); the last of them is token
+ * seq_hot[b] - 1.  Their rotary position is start_position + that place, or
+ * rows.positions.  Rows behind the last sequence (a padded batch) are not read, and
+ * nothing is written for them.  A page index past hot_count or a ref past hot_blocks
+ * sets the device error "hot block ref": that token's k and v are not written.  A
+ * sequence with more new tokens than seq_hot, or offsets that descend, set "sequence
+ * length": nothing of those tokens is written (aw_engine_check_device_errors).  Two
+ * tokens must not share a row of the pools: which is kept is then undefined. */
+typedef struct aw_append_desc {
+    aw_rotary_desc rows;            /* k_out NULL; q may be absent (q_heads 0) */
+    uint32_t batch, hot_count, refs_stride, reserved;
+    uint64_t v_stride, hot_blocks;
+    const uint16_t* v;              /* [num_tokens][kv_heads][head_dim], NULL with hot_v */
+    uint16_t* hot_k;                /* [hot_blocks][16][kv_heads][head_dim] */
+    uint16_t* hot_v;                /* likewise, or NULL: the K row is the value (aw_decode_desc) */
+    const uint32_t* refs;
+    const uint32_t* seq_hot;
+    const uint32_t* token_offsets;
+} aw_append_desc;
+
+int aw_ops_append_paged(aw_engine* engine, const aw_append_desc* desc, void* hip_stream);
+
+/* The host checks of the calls above (aw_ops_qk_norm_rotary's where `norms` is not 0),
+ * without an engine or a GPU: AW_OK or the code that the call returns, and its text in
+ * `msg` (may be NULL).  What the tables and counts in device memory hold is checked by
+ * the kernel alone. */
+int aw_ops_check_rotary(const aw_rotary_desc* desc, int norms, char* msg, size_t msg_len);
+int aw_ops_check_append(const aw_append_desc* desc, char* msg, size_t msg_len);
+
+/* sizeof(aw_rotary_scaling), sizeof(aw_rotary_desc), sizeof(aw_append_desc), for bindings. */
+void aw_abi_ops_desc_sizes(size_t sizes[3]);
+
 /* The tile that a call's product (matmul_qkv: 3, of n[0 .. products) weight rows)
  * of m > 64 rows with 16-byte aligned rows takes on a GPU of `compute_units`, for
  * testing: {activation rows, weight rows, LDS buffers of 64 k}.  Host only.
