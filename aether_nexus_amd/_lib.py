@@ -41,6 +41,9 @@ SIGNATURES = {
     "aw_debug_read_pools": (_c_int, [_vp, _vp, _vp, _vp]),
     "aw_debug_project": (_c_int, [_vp, _vp, _vp, _vp]),
     "aw_multihead_attention_device": (_c_int, [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u64, _vp]),
+    "aw_shared_prefix_plan": (_c_int, [_vp, _u32, _vp, ctypes.c_char_p, _sz]),
+    "aw_shared_prefix_attention_device": (_c_int, [_vp, _vp, _vp]),
+    "aw_abi_prefix_sizes": (None, [ctypes.POINTER(_sz)]),
     "aw_engine_check_device_errors": (_c_int, [_vp, _vp]),
     "aw_debug_product_tile": (_c_int, [_u32, _u32, _vp, _u32, _u32, _vp]),
     "aw_debug_gather_codes": (_c_int, [_vp, _vp, _sz, _vp, _u32, _u32, _vp, _vp, _vp, _vp]),

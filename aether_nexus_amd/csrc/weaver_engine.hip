@@ -18,6 +18,7 @@
 #include "../../include/aether_fabric.h"
 #include "engine_internal.hpp"
 #include "prefill_kernels.hpp"
+#include "prefix_kernels.hpp"
 #include "weaver_kernels.hpp"
 
 static_assert(sizeof(aw_sparse_code) == 16, "SparseCode is 16 bytes (types.rs:227)");
@@ -1007,6 +1008,104 @@ int launch_prefill(aw_engine* e, const aw_decode_desc* d, uint32_t n, uint32_t k
     return enqueue_merge<HD>(e, m, st);
 }
 
+// ---- a batch that shares a prefix ------------------------------------------------
+
+// Parts of `tokens` tokens so that `items` work items of one part each become about
+// `want`: at most `most` parts of at least `least` tokens, a multiple of 32.
+void prefix_parts(uint64_t items, uint64_t want, uint32_t tokens, uint32_t least, uint32_t most, uint32_t* parts, uint32_t* span) {
+    *parts = *span = 0;
+    if (tokens == 0) return;
+    const uint64_t n = std::max<uint64_t>(1, std::min<uint64_t>({want / std::max<uint64_t>(items, 1), most, cdiv(tokens, least)}));
+    *span = (uint32_t)align_up(cdiv(tokens, n), 32);
+    *parts = cdiv(tokens, *span);
+}
+
+// Checks a request and fills its kernel arguments but for addresses of scratch.
+int prefix_plan(const aw_prefix_desc* d, uint32_t n_cu, aw::PrefixArgs* out, aw_prefix_plan_info* info, char* msg, size_t len) {
+    auto refuse = [&](int code, const char* why) {
+        put_msg(msg, len, "shared_prefix_attention: %s", why);
+        return code;
+    };
+    if (!d) return refuse(AW_E_INVALID_ARG, "null descriptor");
+    if (d->batch == 0 || d->queries == 0) return refuse(AW_E_INVALID_ARG, "batch and queries must be >= 1");
+    if (d->kv_heads == 0 || d->q_heads == 0 || d->q_heads % d->kv_heads)
+        return refuse(AW_E_INVALID_ARG, "q_heads must be a positive multiple of kv_heads");
+    if (!supported_head_dim(d->head_dim)) return refuse(AW_E_UNSUPPORTED, "head_dim must be 64 or 128");
+    if (d->flags & ~AW_F_CAUSAL) return refuse(AW_E_INVALID_ARG, "unknown flags");
+    if (!std::isfinite(d->scale)) return refuse(AW_E_INVALID_ARG, "scale must be finite");
+    if (d->refs_stride < d->own_count) return refuse(AW_E_INVALID_ARG, "refs_stride is less than own_count");
+    const uint64_t gqa = d->q_heads / d->kv_heads, rows = (uint64_t)d->batch * d->queries * gqa;
+    if (d->prefix_tokens > 1u << 26 || d->own_count > 1u << 18) return refuse(AW_E_UNSUPPORTED, "too many tokens");
+    if (rows > 1u << 26 || (uint64_t)d->batch * d->queries > 1u << 26 || gqa > 1u << 16 || rows * d->kv_heads > 1u << 28)
+        return refuse(AW_E_UNSUPPORTED, "too many query rows");
+    if ((uint64_t)d->kv_heads * d->head_dim > 1u << 16) return refuse(AW_E_UNSUPPORTED, "too many kv heads");
+    if (!d->q || !d->out) return refuse(AW_E_INVALID_ARG, "q and out are required");
+    if (d->prefix_tokens && !d->prefix_refs) return refuse(AW_E_INVALID_ARG, "prefix_refs is required");
+    if (d->own_count && !d->refs) return refuse(AW_E_INVALID_ARG, "refs is required");
+    if ((d->prefix_tokens || d->own_count) && (!d->hot_k || d->hot_blocks == 0))
+        return refuse(AW_E_INVALID_ARG, "hot_k and hot_blocks are required");
+    if (d->hot_blocks > 1ull << 31) return refuse(AW_E_INVALID_ARG, "hot_blocks exceeds 2^31, the refs' range");
+    if (((uintptr_t)d->q | (uintptr_t)d->hot_k | (uintptr_t)d->hot_v) & 15u)
+        return refuse(AW_E_ALIGN, "q, hot_k and hot_v must be 16-byte aligned");
+    if ((uintptr_t)d->out & 7u) return refuse(AW_E_ALIGN, "out must be 8-byte aligned");
+    aw::PrefixArgs& a = *out;
+    a = aw::PrefixArgs{};
+    a.q = d->q;
+    a.k = d->hot_k;
+    a.v = d->hot_v ? d->hot_v : d->hot_k;
+    a.prefix_refs = d->prefix_refs;
+    a.refs = d->refs;
+    a.seq_own = d->seq_own;
+    a.out = d->out;
+    a.batch = d->batch;
+    a.queries = d->queries;
+    a.q_heads = d->q_heads;
+    a.kv_heads = d->kv_heads;
+    a.gqa = (uint32_t)gqa;
+    a.causal = d->flags & AW_F_CAUSAL;
+    a.rows = (uint32_t)rows;
+    a.own_rows = (uint32_t)(d->queries * gqa);
+    a.prefix_tokens = d->prefix_tokens;
+    a.own_max = d->own_count * kBlock;
+    a.refs_stride = d->refs_stride;
+    a.blocks = d->hot_blocks;
+    a.scale_log2 = d->scale * aw::kLog2e;
+    a.prefix_tiles = cdiv(rows, 16);
+    a.own_tiles = cdiv(a.own_rows, 16);
+    const uint64_t own_items = (uint64_t)d->batch * d->kv_heads * a.own_tiles;
+    prefix_parts((uint64_t)a.prefix_tiles * d->kv_heads, 8ull * n_cu, a.prefix_tokens, 128, 48, &a.prefix_splits, &a.prefix_span);
+    prefix_parts(own_items, 8ull * n_cu, a.own_max, 128, 16, &a.own_splits, &a.own_span);
+    a.splits = a.prefix_splits + a.own_splits;
+    const uint64_t prefix_items = (uint64_t)a.prefix_tiles * d->kv_heads * a.prefix_splits;
+    if (prefix_items + own_items * a.own_splits > 0x7FFFFFFFull) return refuse(AW_E_UNSUPPORTED, "grid too large");
+    a.prefix_items = (uint32_t)prefix_items;
+    if (info) {
+        *info = aw_prefix_plan_info{};
+        info->prefix_splits = a.prefix_splits;
+        info->prefix_tokens_per_split = a.prefix_span;
+        info->own_splits = a.own_splits;
+        info->own_tokens_per_split = a.own_span;
+        info->row_tile = 16;
+        const uint64_t parts = (uint64_t)d->kv_heads * a.splits * a.rows;
+        info->workspace_bytes = 2 * align_up(parts * 4, kAlign) + parts * d->head_dim * 4;
+    }
+    return AW_OK;
+}
+
+template <int HD>
+int launch_prefix(aw_engine* e, aw::PrefixArgs& a, hipStream_t st) {
+    const uint64_t own = (uint64_t)a.batch * a.kv_heads * a.own_tiles * a.own_splits;
+    {
+        StageTimer t(e, AW_STAGE_HOT, st);
+        if (a.splits) hipLaunchKernelGGL(aw::prefix_kernel<HD>, dim3((uint32_t)(a.prefix_items + own)), dim3(64), 0, st, a);
+        AW_HIP(e, hipGetLastError());
+    }
+    StageTimer t(e, AW_STAGE_MERGE, st);
+    hipLaunchKernelGGL(aw::prefix_merge_kernel<HD>, dim3(cdiv((uint64_t)a.kv_heads * a.rows, 4)), dim3(256), 0, st, a);
+    AW_HIP(e, hipGetLastError());
+    return AW_OK;
+}
+
 template <typename F>
 int check_kernel(aw_engine* e, F* fn, const char* name) {
     hipFuncAttributes attr;
@@ -1423,6 +1522,35 @@ int aw_multihead_attention_device(aw_engine* e, const uint16_t* q, const uint16_
         if (rc) return rc;
     }
     return AW_OK;
+}
+
+int aw_shared_prefix_plan(const aw_prefix_desc* d, uint32_t compute_units, aw_prefix_plan_info* info, char* msg, size_t mlen) {
+    aw::PrefixArgs a;
+    return prefix_plan(d, compute_units ? compute_units : 256, &a, info, msg, mlen);
+}
+
+int aw_shared_prefix_attention_device(aw_engine* e, const aw_prefix_desc* d, void* stream) {
+    if (!e) return AW_E_INVALID_ARG;
+    aw::PrefixArgs a;
+    aw_prefix_plan_info info;
+    char msg[256] = {0};
+    int rc = prefix_plan(d, e->n_cu, &a, &info, msg, sizeof msg);
+    if (rc) return fail(e, rc, "%s", msg);
+    AW_HIP(e, hipSetDevice(e->device));
+    hipStream_t st = (hipStream_t)stream; // NULL is HIP's null stream
+    if ((rc = ensure_keep(e->ws, info.workspace_bytes, e->retired_ws, e->last_error, st))) return rc;
+    char* ws = (char*)e->ws.ptr;
+    const size_t stat = align_up((uint64_t)a.kv_heads * a.splits * a.rows * 4, kAlign);
+    a.part_m = (float*)ws;
+    a.part_l = (float*)(ws + stat);
+    a.part_o = (float*)(ws + 2 * stat);
+    a.err = e->err;
+    return d->head_dim == 64 ? launch_prefix<64>(e, a, st) : launch_prefix<128>(e, a, st);
+}
+
+void aw_abi_prefix_sizes(size_t sizes[2]) {
+    sizes[0] = sizeof(aw_prefix_desc);
+    sizes[1] = sizeof(aw_prefix_plan_info);
 }
 
 int aw_engine_check_device_errors(aw_engine* e, void* stream) {

@@ -17,7 +17,8 @@ from typing import Optional
 import numpy as np
 
 from . import _lib
-from .types import BLOCK_SIZE, ROTARY_SCALINGS, AppendDesc, RotaryDesc, RotaryScaling
+from .types import (AW_F_CAUSAL, BLOCK_SIZE, ROTARY_SCALINGS, AppendDesc, PrefixDesc, PrefixPlanInfo, RotaryDesc,
+                    RotaryScaling)
 from .weaver import WeaverEngine, WeaverError, _ptr, _stream
 
 AW_E_INVALID_ARG = -1
@@ -217,6 +218,46 @@ def make_append_desc(*, batch: int, num_tokens: int, q_heads: int, kv_heads: int
     return d
 
 
+def make_prefix_desc(*, batch: int, queries: int, q_heads: int, kv_heads: int, head_dim: int, prefix_tokens: int, q, out,
+                     hot_k, hot_v=None, prefix_refs=None, own_count: int = 0, refs=None, refs_stride: Optional[int] = None,
+                     seq_own=None, hot_blocks: Optional[int] = None, scale: Optional[float] = None,
+                     causal: bool = True) -> PrefixDesc:
+    """An ``aw_prefix_desc`` from device tensors (or raw device pointers), for
+    ``shared_prefix_attention``: q and out [batch][queries][q_heads][head_dim], the prefix'
+    pages in ``prefix_refs``, each sequence's own in its row of ``refs`` and their number of
+    tokens in ``seq_own``.  ``scale`` defaults to 1 / sqrt(head_dim), ``hot_blocks`` to the
+    pool tensor's pages."""
+    d = PrefixDesc()
+    d.batch, d.queries, d.q_heads, d.kv_heads, d.head_dim = batch, queries, q_heads, kv_heads, head_dim
+    d.prefix_tokens, d.own_count, d.flags = prefix_tokens, own_count, AW_F_CAUSAL if causal else 0
+    d.scale = head_dim ** -0.5 if scale is None else scale
+    page = BLOCK_SIZE * kv_heads * head_dim
+    if hot_blocks is None:
+        if not hasattr(hot_k, "numel"):
+            raise WeaverError("shared_prefix_attention: hot_blocks is required for a raw pool pointer", AW_E_INVALID_ARG)
+        hot_blocks = hot_k.numel() // max(page, 1)
+    d.hot_blocks = hot_blocks
+    for t, need, name in ((q, batch * queries * q_heads * head_dim, "q"), (out, batch * queries * q_heads * head_dim, "out"),
+                          (hot_k, hot_blocks * page, "hot_k"), (hot_v, hot_blocks * page, "hot_v")):
+        _f16(t, need, name)
+        setattr(d, name, _ptr(t))
+    _u32(prefix_refs, -(-prefix_tokens // BLOCK_SIZE), "prefix_refs")
+    _u32(seq_own, batch, "seq_own")
+    d.refs_stride = _table(refs, batch, own_count, refs_stride, "refs") if refs is not None else own_count
+    d.prefix_refs, d.refs, d.seq_own = _ptr(prefix_refs), _ptr(refs), _ptr(seq_own)
+    _one_device(d, [q, out, hot_k, hot_v, prefix_refs, refs, seq_own])
+    return d
+
+
+def prefix_plan(desc: PrefixDesc, compute_units: int = 0, lib_path=None) -> PrefixPlanInfo:
+    """Validate a ``shared_prefix_attention`` request and return how it is split (no GPU needed)."""
+    info, msg = PrefixPlanInfo(), ctypes.create_string_buffer(256)
+    rc = _lib.load(lib_path).aw_shared_prefix_plan(ctypes.byref(desc), compute_units, ctypes.byref(info), msg, 256)
+    if rc:
+        raise WeaverError(msg.value.decode(), rc)
+    return info
+
+
 class OpsEngine:
     """``Ops`` (ops.rs:21-462) on MI355X.  Shares a ``WeaverEngine`` (device,
     device error word, last-error text) or creates its own."""
@@ -402,6 +443,11 @@ class OpsEngine:
         """A batch's new k and v rows into their sequences' pages, k and q normed and turned
         on the way (``make_append_desc``)."""
         self._request("aw_ops_append_paged", desc, stream)
+
+    def shared_prefix_attention(self, desc: PrefixDesc, stream: Optional[int] = None) -> None:
+        """Attention over pages of a batch whose sequences share a prefix, read once for all
+        (aw_shared_prefix_attention_device; ``make_prefix_desc``)."""
+        self._request("aw_shared_prefix_attention_device", desc, stream)
 
     def multihead_attention(self, q, k_cache, v_cache, output, kv_len: int, head_dim: int, q_heads: int,
                             kv_heads: int, num_queries: int, cache_tokens: Optional[int] = None,

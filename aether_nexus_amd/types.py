@@ -275,6 +275,32 @@ class AppendDesc(ctypes.Structure):
     ]
 
 
+class PrefixDesc(ctypes.Structure):
+    """``aw_prefix_desc`` (include/aether_weaver.h): attention of a batch that shares a prefix."""
+
+    _device = None  # the GPU of the tensors behind it, where it was made from tensors
+
+    _fields_ = [
+        ("batch", ctypes.c_uint32), ("queries", ctypes.c_uint32), ("q_heads", ctypes.c_uint32),
+        ("kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32), ("prefix_tokens", ctypes.c_uint32),
+        ("own_count", ctypes.c_uint32), ("refs_stride", ctypes.c_uint32), ("flags", ctypes.c_uint32),
+        ("scale", ctypes.c_float), ("hot_blocks", ctypes.c_uint64),
+        ("q", ctypes.c_void_p), ("hot_k", ctypes.c_void_p), ("hot_v", ctypes.c_void_p),
+        ("prefix_refs", ctypes.c_void_p), ("refs", ctypes.c_void_p), ("seq_own", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+    ]
+
+
+class PrefixPlanInfo(ctypes.Structure):
+    """``aw_prefix_plan_info``."""
+
+    _fields_ = [
+        ("prefix_splits", ctypes.c_uint32), ("prefix_tokens_per_split", ctypes.c_uint32),
+        ("own_splits", ctypes.c_uint32), ("own_tokens_per_split", ctypes.c_uint32),
+        ("row_tile", ctypes.c_uint32), ("reserved", ctypes.c_uint32), ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
 class PlanInfo(ctypes.Structure):
     """``aw_decode_plan_info``."""
 

@@ -310,6 +310,63 @@ int aw_multihead_attention_device(aw_engine* engine, const uint16_t* q, const ui
                                   uint32_t head_dim, uint32_t q_heads, uint32_t kv_heads,
                                   uint32_t num_queries, uint64_t cache_tokens, void* hip_stream);
 
+/* ---- a batch that shares a prefix (no reference counterpart) ------------------
+ * Attention of the newest `queries` tokens of each of `batch` sequences that all
+ * begin with the same prefix_tokens tokens (an instruction, a document), over
+ * pages of one pool: the prefix' keys and values are read once for the whole
+ * batch instead of once for each sequence (aw_decode_device with the prefix'
+ * refs in every row of its table), each sequence's own pages beside them, and
+ * the parts are joined by their log-sum-exp.  Device pointers, f16:
+ *   q, out       [batch][queries][q_heads][head_dim]; q 16-byte, out 8-byte aligned
+ *   hot_k, hot_v [hot_blocks][16][kv_heads][head_dim], 16-byte aligned; hot_v NULL: V is the K row
+ *   prefix_refs  [ceil(prefix_tokens / 16)]: the prefix may end inside its last page, whose other rows are not used
+ *   refs         [batch][refs_stride]: the pages of a sequence's tokens behind the prefix, which begin a page of their own
+ *   seq_own      [batch] own tokens, the new ones among them; NULL: own_count * 16 each
+ * Query i of Q sees every prefix token and, with AW_F_CAUSAL, own tokens p <
+ * seq_own - Q + 1 + i (else all of them); a row that sees no token is zeros.  Bit
+ * 31 of a ref is masked.  A ref >= hot_blocks hides its tokens and sets the
+ * device error "hot block ref", a seq_own over own_count * 16 is taken as that and
+ * sets "sequence length" (aw_engine_check_device_errors).  Values of tokens that a
+ * row does not see never reach it, infinities and NaNs neither.
+ * Any number of queries; head_dim 64 or 128; up to 2^26 prefix and 2^22 own tokens.
+ * Scratch is the engine's workspace, as in aw_decode_device, also under capture. */
+typedef struct aw_prefix_desc {
+    uint32_t batch, queries;
+    uint32_t q_heads, kv_heads, head_dim;
+    uint32_t prefix_tokens;          /* 0: no shared tokens */
+    uint32_t own_count;              /* table entries of a sequence (0: no own tokens, refs NULL) */
+    uint32_t refs_stride;            /* >= own_count */
+    uint32_t flags;                  /* 0 or AW_F_CAUSAL */
+    float    scale;
+    uint64_t hot_blocks;
+    const uint16_t* q;
+    const uint16_t* hot_k;
+    const uint16_t* hot_v;
+    const uint32_t* prefix_refs;
+    const uint32_t* refs;
+    const uint32_t* seq_own;
+    uint16_t*       out;
+} aw_prefix_desc;
+
+/* How a request is split; filled by aw_shared_prefix_plan. */
+typedef struct aw_prefix_plan_info {
+    uint32_t prefix_splits, prefix_tokens_per_split; /* parts of the prefix (0: none) */
+    uint32_t own_splits, own_tokens_per_split;       /* parts of each sequence's own tokens (0: none) */
+    uint32_t row_tile;                               /* query rows of a kv head that read the prefix together */
+    uint32_t reserved;
+    uint64_t workspace_bytes;
+} aw_prefix_plan_info;
+
+/* The host checks of the call below and its plan on a GPU of `compute_units` (0: 256),
+ * without an engine or a GPU; info and msg may be NULL. */
+int aw_shared_prefix_plan(const aw_prefix_desc* desc, uint32_t compute_units, aw_prefix_plan_info* info, char* msg,
+                          size_t msg_len);
+
+int aw_shared_prefix_attention_device(aw_engine* engine, const aw_prefix_desc* desc, void* hip_stream);
+
+/* sizeof(aw_prefix_desc) and sizeof(aw_prefix_plan_info), for bindings. */
+void aw_abi_prefix_sizes(size_t sizes[2]);
+
 /* Wait for `hip_stream` and report AW_E_OOB if any kernel since the last check
  * met an out-of-range block ref or atom index (then clears the record). */
 int aw_engine_check_device_errors(aw_engine* engine, void* hip_stream);

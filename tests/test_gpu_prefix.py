@@ -1,0 +1,369 @@
+"""Shared-prefix attention on cuda:0 through the C ABI against the float64 oracle
+(oracle/paged_oracle.py).
+
+Tolerance of an output o = sum p v / sum p over n tokens, with A = sum p |v| / sum p:
+half a step of the f16 store, 2^-11 |o|; the weights as f16 operands, each off by half a
+step, together 2^-11 A at most, or 2^-25 (of the largest weight, 1) among the subnormals,
+together n 2^-25 max |v|; the scores' fp32 sums of head_dim products, off by at most
+head_dim 2^-24 scale sum |q k| <= 128 2^-24 12 = 0.2 2^-11 for the values drawn here, in
+the weights and in their sum: 0.4 2^-11 A; exp2, rescaling and joining a few 2^-24 A.
+Together 2^-11 |o| + 1.5 2^-11 A + n 2^-25 max |v| + 2^-25."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from oracle import paged_oracle as P
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops(engine):
+    from aether_nexus_amd.ops import OpsEngine
+    return OpsEngine(engine)
+
+
+def dev(a):
+    import torch
+    a = np.ascontiguousarray(a)
+    if a.dtype == np.float16:
+        return torch.from_numpy(a.view(np.int16).copy()).cuda().view(torch.float16)
+    return torch.from_numpy(a.astype(np.uint32).view(np.int32).copy()).cuda()
+
+
+def host(t):
+    import torch
+    torch.cuda.synchronize()
+    return t.contiguous().cpu().view(torch.int16).numpy().view(np.float16)
+
+
+class Case:
+    """Inputs of one request: pages in a mixed order, stale rows (NaN, inf) wherever no token is."""
+
+    def __init__(self, seed, batch, queries, hq, hk, hd, prefix, own, *, causal=True, stale=True, qscale=1.5, spare=0):
+        rng = self.rng = np.random.default_rng(seed)
+        self.shape = (batch, queries, hq, hk, hd)
+        self.prefix, self.own, self.causal = prefix, np.asarray(own), causal
+        pages = [-(-int(n) // 16) for n in own]
+        np_ = -(-prefix // 16)
+        self.blocks = np_ + sum(pages) + 2
+        order = rng.permutation(self.blocks).astype(np.int64)
+        self.count = max(pages + [0]) + spare
+        self.prefix_refs = order[:np_]
+        self.refs = np.full((batch, max(self.count, 1)), 0x7FFFFFFF, dtype=np.int64)
+        at = np_
+        for b, n in enumerate(pages):
+            self.refs[b, :n] = order[at:at + n]
+            at += n
+        self.q = (rng.standard_normal((batch, queries, hq, hd)) * qscale).astype(np.float16)
+        bad = np.array([np.nan, np.inf, -np.inf, 65504.0], dtype=np.float16)
+        self.k, self.v = (rng.standard_normal((self.blocks, 16, hk, hd)).astype(np.float16) for _ in range(2))
+        if stale:
+            live = np.zeros((self.blocks, 16), dtype=bool)
+            for table, n in [(self.prefix_refs, prefix)] + [(self.refs[b], int(n)) for b, n in enumerate(own)]:
+                t = np.arange(n)
+                live[table[t // 16], t % 16] = True
+            for p in (self.k, self.v):
+                p[~live] = bad[rng.integers(0, 4, p[~live].shape)]
+        self.prefix_refs[::2] |= 1 << 31  # masked
+        self.dq, self.dk, self.dv = dev(self.q), dev(self.k), dev(self.v)
+        self.drefs, self.dprefix, self.down = dev(self.refs), dev(self.prefix_refs), dev(self.own)
+
+    def desc(self, **kw):
+        import torch
+        from aether_nexus_amd import ops as O
+        batch, queries, hq, hk, hd = self.shape
+        self.out = torch.full((batch, queries, hq, hd), float("nan"), dtype=torch.float16, device="cuda:0")
+        base = dict(batch=batch, queries=queries, q_heads=hq, kv_heads=hk, head_dim=hd, prefix_tokens=self.prefix, q=self.dq,
+                    out=self.out, hot_k=self.dk, hot_v=self.dv, prefix_refs=self.dprefix if self.prefix else None,
+                    own_count=self.count, refs=self.drefs if self.count else None, seq_own=self.down, causal=self.causal)
+        return O.make_prefix_desc(**{**base, **kw})
+
+    def want(self, own=None, scale=None, values=None, refs=None, prefix_refs=None):
+        scale = self.shape[4] ** -0.5 if scale is None else scale
+        a = (self.prefix_refs if prefix_refs is None else prefix_refs, self.prefix, self.refs if refs is None else refs,
+             self.own if own is None else own, scale, self.causal)
+        v = self.v if values is None else values
+        with np.errstate(all="ignore"):
+            return (P.shared_prefix_attention(self.q, self.k, v, *a), P.shared_prefix_attention(self.q, self.k, np.abs(v), *a))
+
+    def check(self, what, **kw):
+        want, absolute = self.want(**kw)
+        got = host(self.out).astype(np.float64)
+        n = self.prefix + int(self.own.max(initial=0))
+        tol = 2.0 ** -11 * np.abs(want) + 1.5 * 2.0 ** -11 * absolute + (n * 6.0 + 1) * 2.0 ** -25
+        d = np.abs(got - want)
+        print(f"{what}: worst error over tolerance {float((d / tol).max()):.3f}, rel {np.linalg.norm(d) / max(np.linalg.norm(want), 1e-30):.2e}",
+              flush=True)
+        assert np.isfinite(got).all() and np.all(d <= tol), what
+
+
+# batch, queries, q heads, kv heads, head_dim, prefix, own tokens of each sequence
+CASES = [
+    (1, 1, 1, 1, 64, 1, [1]), (1, 1, 4, 1, 128, 0, [1]), (2, 1, 14, 2, 64, 117, [9, 1]), (3, 1, 32, 8, 128, 16, [16, 17, 15]),
+    (4, 1, 32, 8, 128, 1000, [1, 33, 64, 200]), (2, 2, 8, 2, 64, 33, [2, 40]), (3, 8, 32, 8, 64, 515, [8, 100, 47]),
+    (2, 5, 12, 2, 128, 64, [300, 5]), (5, 1, 8, 8, 128, 257, [0, 1, 0, 31, 32]), (1, 40, 14, 2, 64, 77, [53]),
+    (2, 70, 4, 2, 128, 130, [70, 150]), (33, 1, 32, 8, 128, 300, list(range(33))), (1, 1, 32, 8, 128, 5000, [1]),
+    (130, 1, 12, 2, 128, 95, [7] * 130), (1, 3, 70, 1, 64, 31, [4]), (2, 1, 4, 2, 128, 48, [1000, 2]), (7, 1, 2, 1, 64, 0, [0, 5, 0, 16, 3, 0, 1]),
+    (3, 2, 6, 3, 128, 63, [0, 1, 2]), (16, 8, 32, 8, 64, 640, [8 + i for i in range(16)]), (1, 1, 2, 2, 64, 20000, [0]),
+]
+
+
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "full"])
+@pytest.mark.parametrize("case", CASES, ids=["-".join(map(str, c[:6])) for c in CASES])
+def test_against_float64(ops, engine, case, causal):
+    c = Case(sum(case[:6]), *case, causal=causal)
+    ops.shared_prefix_attention(c.desc())
+    engine.check_device_errors()
+    c.check(f"{case[:6]}")
+
+
+def test_own_pages_only_and_prefix_only(ops, engine):
+    c = Case(1, 3, 2, 8, 2, 128, 0, [5, 40, 17])
+    ops.shared_prefix_attention(c.desc(prefix_refs=None))
+    c.check("own pages only")
+    c = Case(2, 3, 2, 8, 2, 128, 70, [0, 0, 0])
+    ops.shared_prefix_attention(c.desc(own_count=0, refs=None, seq_own=None))
+    c.check("prefix only")
+    c = Case(3, 2, 1, 8, 2, 64, 10, [32, 32])  # every own row is taken without counts
+    ops.shared_prefix_attention(c.desc(seq_own=None))
+    c.check("without counts")
+    c = Case(4, 3, 2, 8, 2, 128, 0, [0, 0, 0])
+    ops.shared_prefix_attention(c.desc(own_count=0, refs=None))
+    assert not host(c.out).any()  # nothing to see
+    engine.check_device_errors()
+
+
+def test_keys_that_are_the_values(ops):
+    c = Case(5, 3, 1, 8, 2, 128, 100, [5, 40, 17])
+    ops.shared_prefix_attention(c.desc(hot_v=None))
+    c.check("K rows as values", values=c.k)
+
+
+def test_peaked_and_flat_scores(ops):
+    """Scores so far apart that one token takes all of the weight, the largest in the last part; equal scores."""
+    c = Case(6, 2, 1, 8, 2, 128, 900, [40, 8], qscale=40.0)
+    ops.shared_prefix_attention(c.desc(scale=0.25))
+    want, _ = c.want(scale=0.25)
+    got = host(c.out).astype(np.float64)
+    # scores are off by at most 128 2^-24 scale sum |q k| < 128 2^-24 0.25 128 40 6.25 = 0.061 where they are largest; but sums
+    # of random signs are far from that bound, and rows whose two best scores are closer than 0.1 are left out
+    k = np.concatenate([c.k[c.prefix_refs & P.REF_MASK].reshape(-1, 2, 128)[:900], c.k[c.refs[0, :3]].reshape(-1, 2, 128)[:40]])
+    s = np.einsum("hd,nhd->hn", c.q[0, 0].astype(np.float64), np.repeat(k, 4, axis=1).astype(np.float64)) * 0.25
+    top = np.sort(s, axis=1)
+    rows = top[:, -1] - top[:, -2] > 12.0  # the next weights are below e^-12: 900 of them under 2^-7... of the largest
+    assert rows.sum() >= 4
+    v = np.concatenate([c.v[c.prefix_refs & P.REF_MASK].reshape(-1, 2, 128)[:900], c.v[c.refs[0, :3]].reshape(-1, 2, 128)[:40]])
+    best = np.take_along_axis(np.repeat(v, 4, axis=1).astype(np.float64), s.argmax(1)[None, :, None], 0)[0]
+    assert np.all(np.abs(got[0, 0][rows] - best[rows]) <= 900 * np.exp(-11.9) * 12 + 2.0 ** -11 * np.abs(best[rows]))
+    assert np.isfinite(got).all()
+    c = Case(7, 2, 1, 8, 2, 128, 900, [40, 8], qscale=0.0)
+    ops.shared_prefix_attention(c.desc())
+    c.check("equal scores")
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_infinities_reach_only_the_rows_that_see_them(ops, hd):
+    """Draft tokens whose values hold infinities and NaNs are hidden from earlier drafts; those that see them get
+    them in those dims alone.  The same in the prefix, which every row sees."""
+    for queries, prefix in ((4, 50), (9, 0), (1, 200)):
+        c = Case(8 + queries, 2, queries, 8, 2, hd, prefix, [queries + 10, queries])
+        values = c.v.copy()
+
+        def put(b, token, g, dim, x):
+            values[c.refs[b, token // 16], token % 16, g, dim] = x
+        put(0, queries + 9, 0, 3, np.inf)            # the last draft: only the last row sees it
+        put(1, queries - 1, 1, hd - 1, np.nan)
+        if queries > 2:
+            put(0, queries + 7, 1, 17, -np.inf)      # the third last
+        if prefix:
+            at = c.prefix_refs[2] & P.REF_MASK
+            values[at, 5, 0, 9] = np.inf             # every row of head 0
+        c.v, c.dv = values, dev(values)
+        ops.shared_prefix_attention(c.desc())
+        got = host(c.out).astype(np.float64)
+        finite = np.where(np.isfinite(values), values, 0).astype(np.float16)
+        want, absolute = c.want(values=finite)
+        bad = np.zeros(got.shape, dtype=bool)
+        bad[0, queries - 1, :4, 3] = bad[1, queries - 1, 4:, hd - 1] = True
+        if queries > 2:
+            bad[0, queries - 3:, 4:, 17] = True
+        if prefix:
+            bad[:, :, :4, 9] = True
+        assert np.array_equal(~np.isfinite(got), bad), (queries, prefix)
+        assert np.all(np.isposinf(got[0, queries - 1, :4, 3])) and np.all(np.isnan(got[1, queries - 1, 4:, hd - 1]))
+        tol = 2.0 ** -11 * np.abs(want) + 1.5 * 2.0 ** -11 * absolute + 1500 * 2.0 ** -25
+        assert np.all((np.abs(got - want) <= tol)[~bad])
+
+
+def test_nan_keys_make_nan_rows(ops):
+    """A NaN in a key that a row sees makes the row NaN, whichever part it lies in; other rows and heads stay."""
+    for where in ("prefix", "own"):
+        c = Case(20, 2, 1, 8, 2, 128, 1500, [40, 17])
+        k = c.k.copy()
+        at = (c.prefix_refs[70] & P.REF_MASK) if where == "prefix" else c.refs[0, 1]
+        k[at, 3, 1, 5] = np.nan
+        c.dk = dev(k)
+        ops.shared_prefix_attention(c.desc())
+        got = host(c.out)
+        nan = np.zeros(got.shape, dtype=bool)
+        nan[(slice(None) if where == "prefix" else 0), :, 4:] = True
+        assert np.array_equal(np.isnan(got), nan), where
+
+
+def test_bad_refs_and_counts(ops, engine):
+    from aether_nexus_amd.types import AW_E_OOB
+    from aether_nexus_amd.weaver import WeaverError
+
+    def error(word):
+        with pytest.raises(WeaverError) as e:
+            engine.check_device_errors()
+        assert e.value.status == AW_E_OOB and word in str(e.value)
+        engine.check_device_errors()
+
+    c = Case(30, 3, 2, 8, 2, 128, 150, [20, 40, 3])
+    c.prefix_refs[4] = c.blocks
+    c.dprefix = dev(c.prefix_refs)
+    ops.shared_prefix_attention(c.desc())
+    error("hot block ref")
+    c.check("bad prefix page")
+    c = Case(31, 3, 2, 8, 2, 64, 150, [20, 40, 3])
+    c.refs[1, 0] = 0x7FFFFFFE
+    c.drefs = dev(c.refs)
+    ops.shared_prefix_attention(c.desc())
+    error("hot block ref")
+    c.check("bad own page")
+    c = Case(32, 2, 1, 8, 2, 64, 15, [32, 32])  # two pages each, all rows live
+    ops.shared_prefix_attention(c.desc(seq_own=dev(np.array([33, 32]))))
+    error("sequence length")
+    c.check("count past the table")
+
+
+def test_results_do_not_depend_on_the_batch_order_or_run(ops):
+    c = Case(40, 6, 2, 8, 2, 128, 700, [2, 30, 17, 90, 2, 5])
+    ops.shared_prefix_attention(c.desc())
+    first = host(c.out).copy()
+    for _ in range(3):
+        ops.shared_prefix_attention(c.desc())
+        assert np.array_equal(host(c.out).view(np.int16), first.view(np.int16))
+
+
+def test_another_stream_and_graph_replays(ops, engine):
+    """Captured once, replayed while counts grow in device memory, with eager calls of another shape between:
+    every replay gives the eager call's bits."""
+    import torch
+    c, other = Case(41, 3, 1, 8, 2, 128, 700, [20, 40, 3], spare=1), Case(42, 2, 3, 8, 2, 128, 300, [9, 3])
+    down = c.down.clone()
+    d, d2 = c.desc(seq_own=down), other.desc()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        ops.shared_prefix_attention(d)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            ops.shared_prefix_attention(d, stream=torch.cuda.current_stream().cuda_stream)
+        for step, own in enumerate(([20, 40, 3], [19, 39, 2], [1, 1, 1], [20, 40, 3])):
+            down.copy_(torch.tensor(own, dtype=torch.int32))
+            ops.shared_prefix_attention(d)
+            eager = c.out.clone()
+            c.out.fill_(float("nan"))
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(c.out.view(torch.int16), eager.view(torch.int16)), step
+            c.own = np.array(own)
+            c.check(f"replay {step}")
+            ops.shared_prefix_attention(d2)
+            _ = (other.out.float() * 2).sum()
+            torch.cuda.synchronize()
+    other.check("the other shape")
+    engine.check_device_errors(s.cuda_stream)
+    del g
+
+
+def test_capture_refuses_workspace_growth():
+    import torch
+    from aether_nexus_amd.ops import OpsEngine
+    from aether_nexus_amd.types import AW_E_UNSUPPORTED
+    from aether_nexus_amd.weaver import WeaverError
+    fresh = OpsEngine()
+    try:
+        c = Case(43, 2, 1, 8, 2, 64, 100, [20, 3])
+        d = c.desc()
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            g = torch.cuda.CUDAGraph()
+            with pytest.raises(WeaverError) as e:
+                with torch.cuda.graph(g, stream=s):
+                    fresh.shared_prefix_attention(d, stream=torch.cuda.current_stream().cuda_stream)
+            assert e.value.status == AW_E_UNSUPPORTED and "eager" in str(e.value)
+            del g
+            torch.cuda.synchronize()
+            assert np.isnan(host(c.out)).all()
+            fresh.shared_prefix_attention(d)
+        c.check("after the refusal")
+    finally:
+        torch.cuda.synchronize()
+        fresh.close()
+
+
+def test_a_decode_loop_of_all_of_them(ops, engine):
+    """Three steps of four conversations behind one instruction: head norms and rotation on the way into the pages
+    (the prefix first, then each conversation's tokens), then attention; against float64 over the tokens end to end."""
+    import torch
+    from aether_nexus_amd import ops as O
+    rng = np.random.default_rng(44)
+    batch, hq, hk, hd, prefix, count = 4, 8, 2, 128, 43, 4
+    rotary = O.Rotary(hd, 10000.0, scaling="parts", factor=4.0, original_length=2048.0)
+    f = rotary.inv_freq.cpu().numpy()
+    wq, wk = ((1 + 0.1 * rng.standard_normal(hd)).astype(np.float16) for _ in range(2))
+    blocks = 3 + batch * count
+    pool_k, pool_v = (torch.full((blocks, 16, hk, hd), float("nan"), dtype=torch.float16, device="cuda:0") for _ in range(2))
+    order = rng.permutation(blocks)
+    prefix_refs, refs = dev(order[:3]), dev(order[3:].reshape(batch, count))
+    keys, values = [[] for _ in range(batch + 1)], [[] for _ in range(batch + 1)]
+
+    def feed(new, held, table, seqs, start):
+        """New rows of the sequences through append_paged; returns their turned q."""
+        x = (rng.standard_normal((sum(new), hq + 2 * hk, hd)) * 1.5).astype(np.float16)
+        d = dev(x)
+        q_out = torch.empty(sum(new), hq, hd, dtype=torch.float16, device="cuda:0")
+        ops.append_paged(O.make_append_desc(
+            batch=len(new), num_tokens=sum(new), q_heads=hq, kv_heads=hk, head_dim=hd, q=d[:, :hq], q_out=q_out, k=d[:, hq:hq + hk],
+            v=d[:, hq + hk:], hot_k=pool_k, hot_v=pool_v, refs=table, seq_hot=dev(np.array(held) + np.array(new)),
+            token_offsets=dev(np.concatenate([[0], np.cumsum(new)])), rotary=rotary, q_norm=dev(wq), k_norm=dev(wk),
+            start_position=start))
+        at = 0
+        for i, n, h in zip(seqs, new, held):
+            pos = start + h + np.arange(n)
+            k = P.rotary(P.head_norm(x[at:at + n, hq:hq + hk], wk, 1e-5), pos, f)
+            keys[i].append(k.astype(np.float16).astype(np.float64))
+            values[i].append(x[at:at + n, hq + hk:].astype(np.float64))
+            at += n
+        return q_out
+    feed([prefix], [0], prefix_refs.view(1, 3), [batch], 0)
+    held = [0] * batch
+    for queries in (20, 1, 3):
+        q = feed([queries] * batch, held, refs, range(batch), prefix)
+        held = [h + queries for h in held]
+        out = torch.empty(batch, queries, hq, hd, dtype=torch.float16, device="cuda:0")
+        ops.shared_prefix_attention(O.make_prefix_desc(
+            batch=batch, queries=queries, q_heads=hq, kv_heads=hk, head_dim=hd, prefix_tokens=prefix, q=q.view_as(out), out=out,
+            hot_k=pool_k, hot_v=pool_v, prefix_refs=prefix_refs, own_count=count, refs=refs, seq_own=dev(np.array(held))))
+        engine.check_device_errors()
+        got, qs = host(out).astype(np.float64), host(q).astype(np.float64).reshape(batch, queries, hq, hd)
+        for b in range(batch):
+            k, v = (np.concatenate(x[batch] + x[b]) for x in (keys, values))
+            for i in range(queries):
+                n = prefix + held[b] - queries + 1 + i
+                for h in range(hq):
+                    s = k[:n, h // 4] @ qs[b, i, h] * hd ** -0.5
+                    w = np.exp(s - s.max())
+                    w /= w.sum()
+                    want, a = w @ v[:n, h // 4], w @ np.abs(v[:n, h // 4])
+                    # besides the kernel's own errors, the oracle's keys are rounded to f16 from 64 bits and may differ by a
+                    # step from the kernel's: 2^-10 of each product, in weights and sum
+                    grow = 2 * 2.0 ** -10 * np.abs(k[:n, h // 4] * qs[b, i, h]).sum(1).max() * hd ** -0.5
+                    assert np.all(np.abs(got[b, i, h] - want) <= 2.0 ** -11 * np.abs(want) + (1.5 * 2.0 ** -11 + grow) * a + 2.0 ** -20)
