@@ -235,6 +235,7 @@ int refuse(char* msg, size_t len, int code, const char* fmt, ...) {
     return code;
 }
 
+constexpr uint64_t kRotaryWaves = 8; // waves per CU that a token's heads are cut for
 constexpr uint64_t kMostStride = 1ull << 30; // elements: tokens * stride * 2 bytes stays below 2^63
 
 // The checks that the three rotary calls share, and their kernel arguments.
@@ -337,7 +338,25 @@ int append_args(const aw_append_desc* d, awo::RotaryArgs* a, char* msg, size_t l
 template <bool APPEND>
 int launch_rotary(aw_engine* e, awo::RotaryArgs& a, hipStream_t st) {
     a.err = ei::error_word(e);
-    hipLaunchKernelGGL(awo::rotary_kernel<APPEND>, dim3(a.tokens), dim3(256), 0, st, a);
+    if (!awo::rotary_rows_take(a.hd, a.rotary_dim)) {
+        hipLaunchKernelGGL(awo::rotary_kernel<APPEND>, dim3(a.tokens), dim3(256), 0, st, a);
+        OPS_HIP(e, hipGetLastError());
+        return AW_OK;
+    }
+    const uint32_t lanes = awo::rotary_turn_lanes(a.rotary_dim) + awo::rotary_pass_lanes(a.hd, a.rotary_dim);
+    while ((1u << a.lanes_log) < lanes) ++a.lanes_log;
+    const uint32_t heads = a.q_heads + a.kv_heads + (APPEND && a.v_out ? a.kv_heads : 0u);
+    const uint64_t steps = cdiv64(heads, 64u >> a.lanes_log);
+    // Few tokens: a token's heads over several waves.
+    a.slices = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(steps, cdiv64(kRotaryWaves * (uint64_t)ei::compute_units(e), a.tokens)));
+    const uint64_t groups = cdiv64((uint64_t)a.tokens * a.slices, 4);
+    if (groups > 0x20000000ull) return ei::fail(e, AW_E_UNSUPPORTED, "rotary: grid too large");
+    const dim3 grid((uint32_t)groups), block(256);
+    const bool norm = a.q_norm || a.k_norm;
+    if (norm && a.interleaved) hipLaunchKernelGGL((awo::rotary_rows_kernel<APPEND, true, true>), grid, block, 0, st, a);
+    else if (norm) hipLaunchKernelGGL((awo::rotary_rows_kernel<APPEND, true, false>), grid, block, 0, st, a);
+    else if (a.interleaved) hipLaunchKernelGGL((awo::rotary_rows_kernel<APPEND, false, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((awo::rotary_rows_kernel<APPEND, false, false>), grid, block, 0, st, a);
     OPS_HIP(e, hipGetLastError());
     return AW_OK;
 }

@@ -32,6 +32,9 @@ struct RotaryArgs {
     uint64_t hot_blocks;
     const uint32_t *refs, *seq_hot, *token_offsets; // token_offsets null: tokens / batch each
     uint32_t* err;
+    // rotary_rows_kernel
+    uint32_t slices;    // waves of a token
+    uint32_t lanes_log; // log2 of the lanes of a head
 };
 
 // Where a token of an append goes.
@@ -85,8 +88,199 @@ __device__ inline float2 turn_of(const RotaryArgs& a, uint32_t p, uint32_t posit
     return make_float2(c * a.magnitude, s * a.magnitude);
 }
 
-// Any head_dim, rotary_dim, stride and alignment: work-group = one token, a wave per
-// head in turn, lanes over the pairs and then over the dims that pass.
+// 16 bytes at an element's alignment: one access on gfx950.
+typedef uint32_t uint4_el_t __attribute__((ext_vector_type(4), aligned(2)));
+
+// Sum over the 2^log lanes of a head, in each of them: quad permutes and row mirrors up
+// to 16 lanes (a mirror meets a lane of the other half, whose lanes hold equal sums).
+__device__ inline float lanes_sum(float x, uint32_t log) {
+#define AWO_DPP_ADD(n, ctrl) \
+    if (log > n) x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), ctrl, 0xF, 0xF, false))
+    AWO_DPP_ADD(0, 0xB1);  // quad_perm [1,0,3,2]
+    AWO_DPP_ADD(1, 0x4E);  // quad_perm [2,3,0,1]
+    AWO_DPP_ADD(2, 0x141); // row_half_mirror
+    AWO_DPP_ADD(3, 0x140); // row_mirror
+#undef AWO_DPP_ADD
+    if (log > 4) x += __shfl_xor(x, 16);
+    if (log > 5) x += __shfl_xor(x, 32);
+    return x;
+}
+
+// Heads whose turned dims are none or at least 16 and whose passing dims are none or at
+// least 8 (rotary_rows_take): 16 dims of a head in a lane, as two 16-byte pieces, the
+// heads of a wave's step side by side.  A turned lane holds 8 pairs from p0 on: dims p0
+// .. and rotary_dim / 2 + p0 .. (half), or 2 p0 .. 2 p0 + 15 (interleaved), so the same 8
+// cosines and sines serve every head of its token; a passing lane holds dims as they
+// lie.  Where the dims do not divide, the last lane starts earlier and makes some values
+// twice, the same bits (`skip` keeps them out of the norm's sum).  Work-group = 4
+// waves, each a token or a slice of its heads, none waiting for another: a wave works its
+// token's cosines and sines out once, a pair a lane, into LDS of its own, while its
+// first kStep steps of rows are on the way.
+constexpr int kRotaryStep = 4;
+
+__host__ __device__ inline bool rotary_rows_take(uint32_t hd, uint32_t n) {
+    return (n == 0 || n >= 16) && (hd == n || hd - n >= 8);
+}
+// Lanes of turned and of passing dims of a head.
+__host__ __device__ inline uint32_t rotary_turn_lanes(uint32_t n) { return (n + 15u) / 16u; }
+__host__ __device__ inline uint32_t rotary_pass_lanes(uint32_t hd, uint32_t n) { return (hd - n + 15u) / 16u; }
+
+template <bool APPEND, bool NORM, bool INTER>
+__global__ __launch_bounds__(256) void rotary_rows_kernel(RotaryArgs a) {
+    __shared__ float2 s_turns[4][kRotaryMaxDim / 2];
+    const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const uint32_t id = blockIdx.x * 4u + wave; // below 2^31 + 4
+    const uint32_t t = (uint32_t)__builtin_amdgcn_readfirstlane((int)(id / a.slices)), slice = id - t * a.slices;
+    if (t >= a.tokens) return; // no barrier follows
+    const uint32_t n = a.rotary_dim, half = n / 2, hd = a.hd;
+    const uint32_t u = lane & ((1u << a.lanes_log) - 1u), slot = lane >> a.lanes_log, per = 64u >> a.lanes_log;
+    const uint32_t turn_lanes = rotary_turn_lanes(n), unit = u - turn_lanes;
+    const bool turning = u < turn_lanes, used = u < turn_lanes + rotary_pass_lanes(hd, n);
+    uint32_t at0, at1, p0 = 0, skip0, skip1; // dims of the pieces, leading values that another lane holds too
+    if (turning) {
+        p0 = min(8u * u, half - 8u);
+        at0 = INTER ? 2u * p0 : p0;
+        at1 = INTER ? 2u * p0 + 8u : half + p0;
+        const uint32_t twice = 8u * u - p0; // pairs
+        skip0 = INTER ? min(2u * twice, 8u) : twice;
+        skip1 = INTER ? 2u * twice - skip0 : twice;
+    } else {
+        const uint32_t d = n + 16u * unit;
+        at0 = min(d, hd - 8u);
+        at1 = min(d + 8u, hd - 8u);
+        skip0 = d - at0;
+        skip1 = d + 8u - at1;
+    }
+    const uint32_t heads = a.q_heads + a.kv_heads + (APPEND && a.v_out ? a.kv_heads : 0u);
+    const uint32_t steps = (heads + per - 1u) / per;
+    const uint32_t s1 = (uint32_t)((uint64_t)steps * (slice + 1u) / a.slices);
+    uint32_t s = (uint32_t)((uint64_t)steps * slice / a.slices);
+    uint4_el_t x0[kRotaryStep], x1[kRotaryStep];
+    auto load = [&] {
+#pragma unroll
+        for (int j = 0; j < kRotaryStep; ++j) {
+            const uint32_t h = (s + (uint32_t)j) * per + slot;
+            if (s + (uint32_t)j >= s1 || h >= heads || !used) continue;
+            const bool is_q = h < a.q_heads, is_v = APPEND && h >= a.q_heads + a.kv_heads;
+            const uint16_t* p = is_q ? a.q + t * a.q_stride + (uint64_t)h * hd
+                                     : (is_v ? a.v + t * a.v_stride + (uint64_t)(h - a.q_heads - a.kv_heads) * hd
+                                             : a.k + t * a.k_stride + (uint64_t)(h - a.q_heads) * hd);
+            x0[j] = *(const uint4_el_t*)(p + at0);
+            x1[j] = *(const uint4_el_t*)(p + at1);
+        }
+    };
+    load();
+    uint4_el_t w0[2] = {}, w1[2] = {}; // weights of q, of k
+    if constexpr (NORM) {
+        if (used && a.q_norm) {
+            w0[0] = *(const uint4_el_t*)(a.q_norm + at0);
+            w1[0] = *(const uint4_el_t*)(a.q_norm + at1);
+        }
+        if (used && a.k_norm) {
+            w0[1] = *(const uint4_el_t*)(a.k_norm + at0);
+            w1[1] = *(const uint4_el_t*)(a.k_norm + at1);
+        }
+    }
+    Place place{true, true, t, 0};
+    if constexpr (APPEND) place = find_place(a, t, lane, slice == 0);
+    if (!place.rows) return;
+    float c[8], sn[8];
+    if (n) {
+        const uint32_t position = a.positions ? a.positions[t] : a.start + place.at;
+        for (uint32_t p = lane; p < half; p += 64u) s_turns[wave][p] = turn_of(a, p, position);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float2 cs = s_turns[wave][p0 + (uint32_t)e]; // p0 = 0 in passing lanes
+            c[e] = cs.x;
+            sn[e] = cs.y;
+        }
+    }
+    auto half_of = [](const uint4_el_t& v, int e) { return (uint16_t)(v[e / 2] >> (16 * (e % 2))); };
+    for (;;) {
+#pragma unroll
+        for (int j = 0; j < kRotaryStep; ++j) {
+            if (s + (uint32_t)j >= s1) break; // wave-uniform
+            const uint32_t h = (s + (uint32_t)j) * per + slot;
+            const bool is_q = h < a.q_heads, is_v = APPEND && h >= a.q_heads + a.kv_heads;
+            float f0[8], f1[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                f0[e] = h2f(half_of(x0[j], e));
+                f1[e] = h2f(half_of(x1[j], e));
+            }
+            if constexpr (NORM) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    sum += used && (uint32_t)e >= skip0 ? f0[e] * f0[e] : 0.0f;
+                    sum += used && (uint32_t)e >= skip1 ? f1[e] * f1[e] : 0.0f;
+                }
+                sum = lanes_sum(sum, a.lanes_log);
+                if (is_q ? a.q_norm != nullptr : a.k_norm != nullptr) {
+                    const float inv = 1.0f / sqrtf(sum / (float)hd + a.eps);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        f0[e] = f0[e] * inv * h2f(half_of(is_q ? w0[0] : w0[1], e));
+                        f1[e] = f1[e] * inv * h2f(half_of(is_q ? w1[0] : w1[1], e));
+                    }
+                }
+            }
+            if (h >= heads || !used) continue;
+            uint16_t* y;
+            if (is_q) {
+                y = a.q_out + t * a.q_out_stride + (uint64_t)h * hd;
+            } else if constexpr (APPEND) {
+                if (!place.page) continue;
+                y = is_v ? a.v_out + (place.row * a.kv_heads + (h - a.q_heads - a.kv_heads)) * hd
+                         : a.k_out + (place.row * a.kv_heads + (h - a.q_heads)) * hd;
+            } else {
+                y = a.k_out + t * a.k_out_stride + (uint64_t)(h - a.q_heads) * hd;
+            }
+            uint4_el_t r0 = x0[j], r1 = x1[j];
+            const bool turn = turning && !is_v;
+            if (turn) {
+                float g0[8], g1[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if constexpr (INTER) { // pairs of neighbours: e and e + 1 of one piece
+                        float(&f)[8] = e < 4 ? f0 : f1;
+                        float(&g)[8] = e < 4 ? g0 : g1;
+                        const int i = 2 * (e % 4);
+                        g[i] = f[i] * c[e] - f[i + 1] * sn[e];
+                        g[i + 1] = f[i] * sn[e] + f[i + 1] * c[e];
+                    } else {
+                        g0[e] = f0[e] * c[e] - f1[e] * sn[e];
+                        g1[e] = f0[e] * sn[e] + f1[e] * c[e];
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    f0[e] = g0[e];
+                    f1[e] = g1[e];
+                }
+            }
+            if (turn || (NORM && !is_v && (is_q ? a.q_norm != nullptr : a.k_norm != nullptr))) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    r0[i] = (uint32_t)f2h(f0[2 * i]) | ((uint32_t)f2h(f0[2 * i + 1]) << 16);
+                    r1[i] = (uint32_t)f2h(f1[2 * i]) | ((uint32_t)f2h(f1[2 * i + 1]) << 16);
+                }
+            }
+            *(uint4_el_t*)(y + at0) = r0;
+            *(uint4_el_t*)(y + at1) = r1;
+        }
+        s += (uint32_t)kRotaryStep;
+        if (s >= s1) return;
+        load();
+    }
+}
+
+// The other heads (fewer than 16 turned dims, fewer than 8 passing ones): work-group =
+// one token, a wave per head in turn, lanes over the pairs and then over the dims that
+// pass.
 template <bool APPEND>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
     __shared__ float2 s_turn[kRotaryMaxDim / 2];

@@ -199,8 +199,8 @@ int aw_ops_qk_norm_rotary(aw_engine* engine, const aw_rotary_desc* desc, void* h
  * rows token_offsets[b] .. token_offsets[b + 1] - 1 (token_offsets [batch + 1],
  * ascending, from 0; NULL: num_tokens / batch rows each); the last of them is token
  * seq_hot[b] - 1.  Their rotary position is start_position + that place, or
- * rows.positions.  Rows behind the last sequence (a padded batch) are not read, and
- * nothing is written for them.  A page index past hot_count or a ref past hot_blocks
+ * rows.positions.  For rows behind the last sequence (a padded batch)
+ * nothing is written.  A page index past hot_count or a ref past hot_blocks
  * sets the device error "hot block ref": that token's k and v are not written.  A
  * sequence with more new tokens than seq_hot, or offsets that descend, set "sequence
  * length": nothing of those tokens is written (aw_engine_check_device_errors).  Two
