@@ -116,7 +116,7 @@ __device__ inline float lanes_sum(float x, uint32_t log) {
 // waves, each a token or a slice of its heads, none waiting for another: a wave works its
 // token's cosines and sines out once, a pair a lane, into LDS of its own, while its
 // first kStep steps of rows are on the way.
-constexpr int kRotaryStep = 4;
+constexpr int kRotaryStep = 2;
 
 __host__ __device__ inline bool rotary_rows_take(uint32_t hd, uint32_t n) {
     return (n == 0 || n >= 16) && (hd == n || hd - n >= 8);
