@@ -28,17 +28,32 @@ struct PrefixArgs {
     uint32_t prefix_tokens, own_max, refs_stride;
     uint32_t prefix_splits, own_splits, splits; // splits = prefix_splits + own_splits
     uint32_t prefix_span, own_span;             // tokens of a split, a multiple of 32
-    uint32_t prefix_items, prefix_tiles, own_tiles;
+    uint32_t prefix_wgs;                        // work-groups of PrefixTile parts
+    uint32_t prefix_items, own_items;           // one-wave parts
+    uint32_t prefix_tiles, own_tiles;
     uint64_t blocks;
-    float scale_log2;
+    float scale_log2;           // > 0
+    uint32_t q_and, q_xor;      // of two halves of q: the sign of the scale, or all zero for a scale of 0
 };
 
-// 16 query rows of one kv head x the tokens [t0, t1) of one table, one wave, as in the
-// decode over hot blocks: S^T = K Q^T and O^T += V^T P^T on 16 x 16 x 32 MFMAs, 32
-// tokens a step, V read back from LDS transposed.  A row's softmax keeps its running
-// maximum and sum in fp32; weights are f16 operands of the second product (each off by
-// 2^-12 of itself, independently: less than the f16 store of the output).
-// Tokens past `end` and tokens of a bad ref load as zeros and score -inf.
+// 8 halves of a query row.
+__device__ __forceinline__ half8_t prefix_query(const PrefixArgs& a, const uint16_t* p) {
+    uint4_t w = *(const uint4_t*)p;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = (w[e] & a.q_and) ^ a.q_xor;
+    return as_h8(w);
+}
+
+// Few rows to a table (a sequence's own pages; a prefix that at most kPrefixFewRows rows
+// see): 16 query rows of one kv head x the tokens [t0, t1), one wave, as in the decode
+// over hot blocks: S^T = K Q^T and O^T += V^T P^T on 16 x 16 x 32 MFMAs, 32 tokens a
+// step, the next step's rows loading while this one is multiplied, V read back from LDS
+// transposed.  A row's softmax keeps its running maximum and sum in fp32; weights are f16
+// operands of the second product (each off by 2^-12 of itself, independently: less than
+// the f16 store of the output).  Bound: HBM, the pages' bytes.
+// Tokens past `end` and tokens of a bad ref count as zeros that score -inf.
+constexpr uint32_t kPrefixFewRows = 32;
+
 template <int HD>
 struct PrefixWave {
     static constexpr int KS = HD / 32, NB = HD / 16, P = HD + 16;
@@ -57,30 +72,40 @@ struct PrefixWave {
         l_run = 0.0f;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) oacc[nb] = (float4_t)0.0f;
-        uint32_t held = ~0u, refv = 0;
-        for (uint32_t c0 = t0; c0 < t1; c0 += 32u) {
-            uint4_t kr[2][KS], vr[2][KS];
-            bool ok[2];
+        if (t0 >= t1) return;
+        // Refs of 64 blocks, one in each lane, and of the next 64.
+        const uint32_t last = (end - 1u) / kBlockTokens, first = t0 / kBlockTokens;
+        uint32_t held = 0;
+        uint32_t refv = table[min(first + (uint32_t)lane, last)] & kRefMask;
+        uint32_t refn = table[min(first + 64u + (uint32_t)lane, last)] & kRefMask;
+        // The 32 tokens from c0 on: this lane's pieces of K and V (loads that nothing masks:
+        // a bad ref reads block 0), and whether each block counts.
+        auto load = [&](uint32_t c0, uint4_t (&kr)[2][KS], uint4_t (&vr)[2][KS], bool (&ok)[2]) {
+            const uint32_t b0 = c0 / kBlockTokens - first;
+            if (b0 / 64u != held) { // a step's two blocks lie in one run of 64
+                held = b0 / 64u;
+                refv = refn;
+                refn = table[min(first + (held + 1u) * 64u + (uint32_t)lane, last)] & kRefMask;
+            }
 #pragma unroll
             for (int tb = 0; tb < 2; ++tb) {
-                const uint32_t tok = c0 + 16u * tb, blk = tok / kBlockTokens;
-                const bool in = tok < end; // wave-uniform
-                if (in && blk / 64u != held) { // the refs of 64 blocks, one in each lane
-                    held = blk / 64u;
-                    const uint32_t i = min(held * 64u + (uint32_t)lane, (end - 1u) / kBlockTokens);
-                    refv = table[i] & kRefMask;
-                }
-                const uint32_t ref = (uint32_t)__builtin_amdgcn_readlane((int)refv, (int)(blk & 63u));
+                const uint32_t ref = (uint32_t)__builtin_amdgcn_readlane((int)refv, (int)((b0 + (uint32_t)tb) & 63u));
+                const bool in = c0 + 16u * tb < end;
                 ok[tb] = in && ref < a.blocks;
                 bad |= in && !ok[tb];
                 const uint64_t at = (((uint64_t)(ok[tb] ? ref : 0u) * kBlockTokens + li) * a.kv_heads + g) * HD + 8 * lg;
-                const bool row = ok[tb] && tok + (uint32_t)li < end;
 #pragma unroll
-                for (int j = 0; j < KS; ++j) {
-                    kr[tb][j] = row ? *(const uint4_t*)(a.k + at + 32 * j) : (uint4_t)0u;
-                    vr[tb][j] = row ? *(const uint4_t*)(a.v + at + 32 * j) : (uint4_t)0u;
-                }
+                for (int j = 0; j < KS; ++j) kr[tb][j] = *(const uint4_t*)(a.k + at + 32 * j);
+#pragma unroll
+                for (int j = 0; j < KS; ++j) vr[tb][j] = *(const uint4_t*)(a.v + at + 32 * j);
             }
+        };
+        auto process = [&](uint32_t c0, uint4_t (&kr)[2][KS], uint4_t (&vr)[2][KS], const bool (&ok)[2]) {
+#pragma unroll
+            for (int tb = 0; tb < 2; ++tb)
+                if (!ok[tb] || c0 + 16u * tb + (uint32_t)li >= end)
+#pragma unroll
+                    for (int j = 0; j < KS; ++j) kr[tb][j] = vr[tb][j] = (uint4_t)0u;
             float4_t sacc[2];
 #pragma unroll
             for (int tb = 0; tb < 2; ++tb) {
@@ -88,12 +113,12 @@ struct PrefixWave {
 #pragma unroll
                 for (int j = 0; j < KS; ++j) sacc[tb] = mfma16x16x32(as_h8(kr[tb][j]), qop[j], sacc[tb]);
             }
-            __syncthreads(); // one wave
+            wave_lds_order(); // the reads of the last step
 #pragma unroll
             for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
                 for (int j = 0; j < KS; ++j) *(uint4_t*)(lds + (16 * tb + li) * P + 32 * j + 8 * lg) = vr[tb][j];
-            __syncthreads(); // one wave
+            wave_lds_order();
             float pf[8], mx = -INFINITY;
 #pragma unroll
             for (int tb = 0; tb < 2; ++tb)
@@ -161,9 +186,28 @@ struct PrefixWave {
                     }
                 }
             }
+        };
+        // Two sets of registers in turn.
+        uint4_t k0[2][KS], v0[2][KS], k1[2][KS], v1[2][KS];
+        bool ok0[2], ok1[2];
+        load(t0, k0, v0, ok0);
+        for (uint32_t c0 = t0; c0 < t1; c0 += 64u) {
+            const bool more = c0 + 32u < t1;
+            if (more) load(c0 + 32u, k1, v1, ok1);
+            process(c0, k0, v0, ok0);
+            if (!more) break;
+            if (c0 + 64u < t1) load(c0 + 64u, k0, v0, ok0);
+            process(c0 + 32u, k1, v1, ok1);
         }
         l_run += __shfl_xor(l_run, 16);
         l_run += __shfl_xor(l_run, 32);
+    }
+
+    // LDS that one wave alone uses is written and read in order by the hardware; this keeps the compiler to it.
+    static __device__ __forceinline__ void wave_lds_order() {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
 
     __device__ __forceinline__ void run(const PrefixArgs& a, const uint32_t* table, uint32_t g, uint32_t row, bool valid,
@@ -173,7 +217,7 @@ struct PrefixWave {
         const uint32_t head = g * a.gqa + row % a.gqa;
         const uint16_t* p = a.q + ((uint64_t)(row / a.gqa) * a.q_heads + head) * HD;
 #pragma unroll
-        for (int j = 0; j < KS; ++j) qop[j] = as_h8(*(const uint4_t*)(p + 32 * j + 8 * lg));
+        for (int j = 0; j < KS; ++j) qop[j] = prefix_query(a, p + 32 * j + 8 * lg);
         bad = false;
         pass<false>(a, table, g, t0, t1, end, lim, lds, lane);
         // An inf or NaN among the sums under finite weights comes from the values, and may
@@ -198,22 +242,334 @@ struct PrefixWave {
     }
 };
 
+// Many rows to the prefix: a work-group takes kPrefixRows rows of one kv head, of
+// whatever sequences (row r: sequence and query r / G, head r % G), x one part of the
+// prefix, so that its pages are read once for all of them; 4 waves of 32 rows, TOK
+// tokens a step.  K and V of a step go from memory straight into LDS, TOK / 16 pages of
+// any place in the pool, each through a buffer resource of its own whose range ends with
+// the page's last token: rows past the prefix, and pages of a bad ref, load as zeros.
+//   S^T = K Q^T on v_mfma_f32_32x32x16_f16 (lane l: row l % 32, hf = l / 32):
+//     A = K (token l % 32, dims 16 j + 8 hf ..), B = Q^T from registers; a lane ends
+//     with 16 of 32 tokens, 8 (i / 4) + 4 hf + i % 4, of its row: the softmax is per
+//     lane but for one exchange with lane l ^ 32, and
+//   O^T += V^T P^T takes P from the same registers: k-index 8 hf + j is token 4 hf + j
+//     (j < 4) or 8 + 4 hf + j - 4; A = V^T by transposing LDS reads.
+// Staged rows are HD / 8 16-byte chunks, chunk c of K row r at c ^ (r % chunks), of V
+// row r at c ^ 4 (r % 4) ^ (r / 4) % 4 (128 dims): no bank conflict at 128 dims.
+constexpr uint32_t kPrefixRows = 128;
+constexpr int kPrefixThreads = 256;
+constexpr int kPrefixTok = 64, kPrefixBufs = 2;
+constexpr size_t prefix_lds_bytes(int HD) { return (size_t)kPrefixBufs * 2 * kPrefixTok * HD * 2; }
+
 template <int HD>
-__global__ __launch_bounds__(64) void prefix_kernel(PrefixArgs a) {
-    __shared__ __attribute__((aligned(16))) _Float16 lds[32 * (HD + 16)];
-    const int lane = threadIdx.x;
+struct PrefixTile {
+    static constexpr int TOK = kPrefixTok, BUFS = kPrefixBufs, PAGES = TOK / 16, TB = TOK / 32;
+    static constexpr int CH = HD / 8, KS = HD / 16, NB = HD / 32;
+    static constexpr int LPT = TOK * CH / kPrefixThreads; // loads per thread, operand and step
+    static constexpr uint32_t OP = TOK * HD;              // halves per staged operand
+    static_assert(prefix_lds_bytes(HD) >= (size_t)4 * 32 * (HD + 16) * 2, "the one-wave parts' LDS");
+
+    static __device__ __forceinline__ uint32_t ksw(uint32_t row) { return row & (uint32_t)(CH - 1); }
+    static __device__ __forceinline__ uint32_t vsw(uint32_t row) {
+        return CH == 16 ? ((row & 3u) << 2) | ((row >> 2) & 3u) : ((row >> 1) & 1u) << 2;
+    }
+    static __device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
+    static __device__ __forceinline__ void barrier() {
+        __asm__ volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        __asm__ volatile("" ::: "memory");
+    }
+
+    static __device__ __forceinline__ void run(const PrefixArgs& a, uint32_t g, uint32_t tile, uint32_t s, _Float16* lds) {
+        const int tid = threadIdx.x, lane = tid & 63, li = lane & 31, hf = lane >> 5;
+        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        const uint32_t t0 = s * a.prefix_span, t1 = min(t0 + a.prefix_span, a.prefix_tokens); // t0 < t1
+        const uint32_t row = tile * kPrefixRows + 32u * (uint32_t)wave + (uint32_t)li;
+        const bool wave_rows = tile * kPrefixRows + 32u * (uint32_t)wave < a.rows;
+
+        half8_t qop[KS];
+        {
+            const uint32_t r = min(row, a.rows - 1u);
+            const uint16_t* p = a.q + ((uint64_t)(r / a.gqa) * a.q_heads + g * a.gqa + r % a.gqa) * HD;
+#pragma unroll
+            for (int j = 0; j < KS; ++j) qop[j] = prefix_query(a, p + 16 * j + 8 * hf);
+        }
+
+        // Staging: load j fills slots tid + 256 j of the operand (slot -> row, chunk); a
+        // wave's slots of one load lie in one page.
+        const uint32_t rstride = a.kv_heads * (uint32_t)HD; // halves
+        uint32_t koff[LPT], voff[LPT];
+#pragma unroll
+        for (int j = 0; j < LPT; ++j) {
+            const uint32_t q = (uint32_t)tid + (uint32_t)(kPrefixThreads * j), r = q / CH, c = q % CH;
+            koff[j] = ((r & 15u) * rstride + 8u * (c ^ ksw(r))) * 2u;
+            voff[j] = ((r & 15u) * rstride + 8u * (c ^ vsw(r))) * 2u;
+        }
+        // Refs of 64 pages from the part's first on, one in each lane, and of the next 64.
+        const uint32_t last = (a.prefix_tokens - 1u) / kBlockTokens, first = t0 / kBlockTokens;
+        const uint64_t page_halves = (uint64_t)kBlockTokens * rstride;
+        uint32_t held, refv, refn;
+        bool bad = false;
+        auto refs_from = [&](uint32_t run) {
+            return a.prefix_refs[min(first + 64u * run + (uint32_t)lane, last)] & kRefMask;
+        };
+        // Loads the step of tokens c0 .. into buffer `buf`; returns a bit for each page that counts.
+        auto issue = [&](uint32_t c0, uint32_t buf) -> uint32_t {
+            const uint32_t b0 = (c0 - t0) / kBlockTokens;
+            if (b0 / 64u != held) { // a step's pages lie in one run of 64
+                held = b0 / 64u;
+                refv = refn;
+                refn = refs_from(held + 1u);
+            }
+            uint32_t oks = 0;
+            __amdgpu_buffer_rsrc_t rk[PAGES], rv[PAGES];
+#pragma unroll
+            for (int p = 0; p < PAGES; ++p) {
+                const uint32_t ref = (uint32_t)__builtin_amdgcn_readlane((int)refv, (int)((b0 + (uint32_t)p) & 63u));
+                const uint32_t at = c0 + 16u * p;
+                const bool in = at < t1, ok = in && ref < a.blocks;
+                bad |= in && !ok;
+                oks |= ok ? 1u << p : 0u;
+                const uint64_t base = (ok ? ref : 0u) * page_halves + (uint64_t)g * HD;
+                const uint32_t rows = ok ? min(16u, t1 - at) : 0u;
+                const int bytes = ok ? (int)(((rows - 1u) * rstride + (uint32_t)HD) * 2u) : 0;
+                rk[p] = __builtin_amdgcn_make_buffer_rsrc((void*)(a.k + base), (short)0, bytes, (int)kBufferWord3);
+                rv[p] = __builtin_amdgcn_make_buffer_rsrc((void*)(a.v + base), (short)0, bytes, (int)kBufferWord3);
+            }
+            _Float16* dst = lds + buf * 2u * OP;
+#pragma unroll
+            for (int o = 0; o < 2; ++o)
+#pragma unroll
+                for (int j = 0; j < LPT; ++j) {
+                    _Float16* d = dst + (uint32_t)o * OP + ((uint32_t)wave * 64u + (uint32_t)(kPrefixThreads * j)) * 8u; // wave-uniform
+                    const int off = (int)(o ? voff[j] : koff[j]);
+                    auto go = [&](__amdgpu_buffer_rsrc_t r) {
+                        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)d, 16, off, 0, 0, 0);
+                    };
+                    if constexpr (CH == 16) go(o ? rv[j] : rk[j]); // 16 rows a load
+                    else if (wave < 2) go(o ? rv[2 * j] : rk[2 * j]); // 32 rows a load, two pages
+                    else go(o ? rv[2 * j + 1] : rk[2 * j + 1]);
+                }
+            return oks;
+        };
+
+        // LDS offsets (halves) of this lane's operands in a staged step.
+        uint32_t kat[KS], va[NB], vb[NB];
+#pragma unroll
+        for (int j = 0; j < KS; ++j) kat[j] = (uint32_t)li * HD + 8u * (((uint32_t)(2 * j + hf)) ^ ksw((uint32_t)li));
+        {
+            const uint32_t i16 = (uint32_t)lane & 15u, ra = 4u * (uint32_t)hf + (i16 >> 2), rb = ra + 8u;
+            const uint32_t c = (((uint32_t)lane >> 4) & 1u) * 2u + ((i16 & 3u) >> 1), lo = 4u * (i16 & 1u);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                va[nb] = OP + ra * HD + 8u * ((4u * nb + c) ^ vsw(ra)) + lo;
+                vb[nb] = OP + rb * HD + 8u * ((4u * nb + c) ^ vsw(rb)) + lo;
+            }
+        }
+
+        float m_run, l_run;
+        float16_t oacc[NB];
+        // SPLIT: as in PrefixWave.
+        auto process = [&](auto split, uint32_t c0, uint32_t buf, uint32_t oks) {
+            constexpr bool SPLIT = decltype(split)::value;
+            const _Float16* sb = lds + buf * 2u * OP;
+            float16_t sacc[TB];
+#pragma unroll
+            for (int tb = 0; tb < TB; ++tb) {
+                sacc[tb] = (float16_t)0.0f;
+#pragma unroll
+                for (int j = 0; j < KS; ++j)
+                    sacc[tb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8_t*)(sb + kat[j] + tb * 32 * HD), qop[j],
+                                                                      sacc[tb], 0, 0, 0);
+            }
+            if (c0 + (uint32_t)TOK > t1 || oks != (1u << PAGES) - 1u) { // wave-uniform
+                int see = (int)(t1 - c0) - 4 * hf;
+                __asm__ volatile("" : "+v"(see)); // compared with constants here, not as 32 values kept over the loop
+#pragma unroll
+                for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (32 * tb + 8 * (i / 4) + i % 4 >= see || !((oks >> (2 * tb + i / 8)) & 1u)) sacc[tb][i] = -INFINITY;
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sacc[tb][i]);
+            const auto sw = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, mx), __builtin_bit_cast(uint32_t, mx), false, false);
+            const uint32_t sw0 = sw[0], sw1 = sw[1]; // the row's two halves
+            mx = fmaxf(__builtin_bit_cast(float, sw0), __builtin_bit_cast(float, sw1)) * a.scale_log2;
+            if (__any(mx > m_run)) {
+                const float mnew = fmaxf(m_run, mx);
+                const float alpha = mnew == -INFINITY ? 1.0f : fast_exp2(m_run - mnew);
+                m_run = mnew;
+                l_run *= alpha;
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) oacc[nb] *= alpha;
+            }
+            const float mref = m_run == -INFINITY ? 0.0f : m_run;
+            half8_t pop[TB][2];
+            float ps0 = 0.0f, ps1 = 0.0f;
+#pragma unroll
+            for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const float p0 = fast_exp2(fmaf(sacc[tb][i], a.scale_log2, -mref));
+                    const float p1 = fast_exp2(fmaf(sacc[tb][i + 1], a.scale_log2, -mref));
+                    ps0 += p0;
+                    ps1 += p1;
+                    pop[tb][i / 8][i % 8] = (_Float16)p0;
+                    pop[tb][i / 8][i % 8 + 1] = (_Float16)p1;
+                }
+            l_run += ps0 + ps1;
+#pragma unroll
+            for (int x = 0; x < 2 * TB * NB; ++x) {
+                const int tb = x / (2 * NB), kk = (x / NB) % 2, nb = x % NB, ro = (32 * tb + 16 * kk) * HD;
+                half8_t v = __builtin_bit_cast(half8_t, __builtin_shufflevector(lds_read_tr16(sb + va[nb] + ro),
+                                                                                lds_read_tr16(sb + vb[nb] + ro), 0, 1, 2, 3, 4, 5, 6, 7));
+                if constexpr (SPLIT) v = finite_part(v);
+                oacc[nb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pop[tb][kk], oacc[nb], 0, 0, 0);
+                if constexpr (SPLIT) __builtin_amdgcn_sched_barrier(0); // fewer fragments at once: no spills
+            }
+            if constexpr (SPLIT) {
+                auto nonfinite = [&](uint32_t r, uint32_t c) -> bool { // slot c of V row r
+                    const uint4_t w = *(const uint4_t*)(sb + OP + r * HD + 8u * c);
+                    bool any = false;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t v = w[e];
+                        any |= (v & 0x7C00u) == 0x7C00u || (v & 0x7C000000u) == 0x7C000000u;
+                    }
+                    return any;
+                };
+                bool any = false; // row `lane`, from another slot on in each lane (banks)
+#pragma unroll 4
+                for (uint32_t c = 0; c < (uint32_t)CH; ++c)
+                    any |= lane < TOK && nonfinite((uint32_t)lane % (uint32_t)TOK, (c + (uint32_t)lane) % (uint32_t)CH);
+#pragma unroll 1
+                for (uint64_t todo = __ballot(any); todo; todo &= todo - 1u) {
+                    const uint32_t at = (uint32_t)__builtin_ctzll(todo);
+                    const uint32_t slots = (uint32_t)__ballot(lane < CH && nonfinite(at, (uint32_t)lane % (uint32_t)CH));
+                    float x = 0.0f; // the score again
+#pragma unroll
+                    for (int j = 0; j < KS; ++j) {
+                        const half8_t kv = *(const half8_t*)(sb + at * HD + 8u * (((uint32_t)(2 * j + hf)) ^ ksw(at)));
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x = fmaf((float)qop[j][e], (float)kv[e], x);
+                    }
+                    x += __shfl_xor(x, 32);
+                    const float p = fast_exp2(fmaf(x, a.scale_log2, -mref));
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4) {
+                            const uint32_t slot = (uint32_t)(4 * nb + i / 4) ^ vsw(at);
+                            if (!((slots >> slot) & 1u)) continue; // uniform
+                            const half4_t v = *(const half4_t*)(sb + OP + at * HD + 8u * slot + 4 * hf);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float f = (float)v[e];
+                                if (!(fabsf(f) < INFINITY)) oacc[nb][i + e] = fmaf(p, f, oacc[nb][i + e]);
+                            }
+                        }
+                }
+            }
+        };
+
+        constexpr short kWaitAll = (short)0x0070; // vmcnt(0), lgkmcnt(0): this wave's loads are in LDS, its LDS reads done
+        auto pass = [&](auto split) {
+            m_run = -INFINITY;
+            l_run = 0.0f;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) oacc[nb] = (float16_t)0.0f;
+            held = 0;
+            refv = refs_from(0);
+            refn = refs_from(1);
+            uint32_t buf = 0, oks = issue(t0, 0);
+            __builtin_amdgcn_s_waitcnt(kWaitAll);
+            barrier();
+            for (uint32_t c0 = t0; c0 < t1; c0 += (uint32_t)TOK) {
+                uint32_t next = 0;
+                if (c0 + (uint32_t)TOK < t1) next = issue(c0 + (uint32_t)TOK, buf ^ 1u); // its readers passed the last barrier
+                if (wave_rows) process(split, c0, buf, oks);
+                __builtin_amdgcn_s_waitcnt(kWaitAll);
+                barrier();
+                buf ^= 1u;
+                oks = next;
+            }
+        };
+        pass(std::false_type{});
+        // An inf or NaN among the sums under finite weights: it comes from the values, and a
+        // weight that f16 rounds to 0 makes it NaN.  The work-group then takes its part again.
+        float l = l_run + __shfl_xor(l_run, 32), chk = 0.0f;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) chk = fmaf(oacc[nb][i], 0.0f, chk);
+        uint32_t* flags = (uint32_t*)lds; // every step has been read
+        const bool redo = __any(wave_rows && row < a.rows && chk != 0.0f && l * 0.0f == 0.0f);
+        if (lane == 0) flags[wave] = redo ? 1u : 0u;
+        __syncthreads();
+        const uint32_t again = flags[0] | flags[1] | flags[2] | flags[3];
+        __syncthreads();
+        if (again) { // the same in every wave
+            pass(std::true_type{});
+            l = l_run + __shfl_xor(l_run, 32);
+        }
+        if (bad && lane == 0 && wave == 0) flag_error(a.err, kErrHotRef);
+        uint32_t ro = row;
+        __asm__ volatile("" : "+v"(ro)); // its addresses are made here, not kept over the loops
+        if (ro >= a.rows) return;
+        const uint64_t at = ((uint64_t)g * a.splits + s) * a.rows + ro;
+        if (hf == 0) {
+            a.part_m[at] = m_run;
+            a.part_l[at] = l;
+        }
+        if (l == 0.0f) return;
+        float* po = a.part_o + at * HD;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *(float4_t*)(po + 32 * nb + 2 * i + 4 * hf) =
+                    (float4_t){oacc[nb][i], oacc[nb][i + 1], oacc[nb][i + 2], oacc[nb][i + 3]};
+    }
+};
+
+// Work-groups 0 .. prefix_wgs - 1 take the prefix, the others four one-wave parts each.
+// TILES: the prefix in PrefixTile's parts; else in one-wave parts too.
+// Work-group b runs on XCD b % 8: the row tiles of one part of the prefix follow one
+// another on one XCD, so its pages come from memory once.
+template <int HD, bool TILES>
+__global__ __launch_bounds__(kPrefixThreads) __attribute__((amdgpu_waves_per_eu(2))) void prefix_kernel(PrefixArgs a) {
+    extern __shared__ __attribute__((aligned(16))) _Float16 prefix_lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    if constexpr (TILES) {
+        if (blockIdx.x < a.prefix_wgs) {
+            auto uniform = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }; // divisions run on the vector ALUs
+            const uint32_t j = blockIdx.x >> 3, part = uniform(j / a.prefix_tiles) * 8u + (blockIdx.x & 7u);
+            if (part >= a.kv_heads * a.prefix_splits) return;
+            const uint32_t tile = j % a.prefix_tiles, s = uniform(part / a.kv_heads);
+            PrefixTile<HD>::run(a, part - s * a.kv_heads, uniform(tile), s, prefix_lds);
+            return;
+        }
+    }
+    _Float16* lds = prefix_lds + wave * 32 * (HD + 16);
     const uint32_t li = (uint32_t)lane & 15u;
     PrefixWave<HD> w;
-    uint32_t t = blockIdx.x;
-    if (t < a.prefix_items) {
-        const uint32_t s = t % a.prefix_splits;
-        t /= a.prefix_splits;
-        const uint32_t tile = t % a.prefix_tiles, g = t / a.prefix_tiles, r = tile * 16u + li;
-        const uint32_t t0 = s * a.prefix_span, t1 = min(t0 + a.prefix_span, a.prefix_tokens);
-        w.run(a, a.prefix_refs, g, min(r, a.rows - 1u), r < a.rows, t0, t1, a.prefix_tokens, a.prefix_tokens, s, lds, lane);
-        return;
+    uint32_t t = (blockIdx.x - (TILES ? a.prefix_wgs : 0u)) * 4u + (uint32_t)wave;
+    if constexpr (!TILES) {
+        if (t < a.prefix_items) {
+            const uint32_t s = t % a.prefix_splits;
+            t /= a.prefix_splits;
+            const uint32_t tile = t % a.prefix_tiles, g = t / a.prefix_tiles, r = tile * 16u + li;
+            const uint32_t t0 = s * a.prefix_span, t1 = min(t0 + a.prefix_span, a.prefix_tokens);
+            w.run(a, a.prefix_refs, g, min(r, a.rows - 1u), r < a.rows, t0, t1, a.prefix_tokens, a.prefix_tokens, s, lds, lane);
+            return;
+        }
+        t -= a.prefix_items;
     }
-    t -= a.prefix_items;
+    if (t >= a.own_items) return;
     const uint32_t s = t % a.own_splits;
     t /= a.own_splits;
     const uint32_t g = t % a.kv_heads;

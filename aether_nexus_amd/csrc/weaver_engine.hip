@@ -1069,23 +1069,30 @@ int prefix_plan(const aw_prefix_desc* d, uint32_t n_cu, aw::PrefixArgs* out, aw_
     a.own_max = d->own_count * kBlock;
     a.refs_stride = d->refs_stride;
     a.blocks = d->hot_blocks;
-    a.scale_log2 = d->scale * aw::kLog2e;
-    a.prefix_tiles = cdiv(rows, 16);
+    a.q_and = d->scale == 0.0f ? 0u : ~0u;
+    a.q_xor = d->scale < 0.0f ? 0x80008000u : 0u;
+    a.scale_log2 = d->scale == 0.0f ? 1.0f : std::fabs(d->scale) * aw::kLog2e;
+    const bool tiles = rows > aw::kPrefixFewRows;
+    a.prefix_tiles = cdiv(rows, tiles ? aw::kPrefixRows : 16);
     a.own_tiles = cdiv(a.own_rows, 16);
-    const uint64_t own_items = (uint64_t)d->batch * d->kv_heads * a.own_tiles;
-    prefix_parts((uint64_t)a.prefix_tiles * d->kv_heads, 8ull * n_cu, a.prefix_tokens, 128, 48, &a.prefix_splits, &a.prefix_span);
-    prefix_parts(own_items, 8ull * n_cu, a.own_max, 128, 16, &a.own_splits, &a.own_span);
+    const uint64_t own_parts = (uint64_t)d->batch * d->kv_heads * a.own_tiles, prefix_parts_n = (uint64_t)a.prefix_tiles * d->kv_heads;
+    if (tiles) prefix_parts(prefix_parts_n, n_cu, a.prefix_tokens, 128, 48, &a.prefix_splits, &a.prefix_span);
+    else prefix_parts(prefix_parts_n, 8ull * n_cu, a.prefix_tokens, 128, 48, &a.prefix_splits, &a.prefix_span);
+    prefix_parts(own_parts, 8ull * n_cu, a.own_max, 128, 16, &a.own_splits, &a.own_span);
     a.splits = a.prefix_splits + a.own_splits;
-    const uint64_t prefix_items = (uint64_t)a.prefix_tiles * d->kv_heads * a.prefix_splits;
-    if (prefix_items + own_items * a.own_splits > 0x7FFFFFFFull) return refuse(AW_E_UNSUPPORTED, "grid too large");
-    a.prefix_items = (uint32_t)prefix_items;
+    const uint64_t items = prefix_parts_n * a.prefix_splits, own_items = own_parts * a.own_splits;
+    const uint64_t wgs = tiles ? (uint64_t)cdiv((uint64_t)d->kv_heads * a.prefix_splits, 8) * 8 * a.prefix_tiles : 0;
+    if (items + own_items > 0x7FFFFFFFull || wgs + own_items > 0x7FFFFFFFull) return refuse(AW_E_UNSUPPORTED, "grid too large");
+    a.prefix_wgs = (uint32_t)wgs;
+    a.prefix_items = tiles ? 0u : (uint32_t)items;
+    a.own_items = (uint32_t)own_items;
     if (info) {
         *info = aw_prefix_plan_info{};
         info->prefix_splits = a.prefix_splits;
         info->prefix_tokens_per_split = a.prefix_span;
         info->own_splits = a.own_splits;
         info->own_tokens_per_split = a.own_span;
-        info->row_tile = 16;
+        info->row_tile = tiles ? aw::kPrefixRows : 16;
         const uint64_t parts = (uint64_t)d->kv_heads * a.splits * a.rows;
         info->workspace_bytes = 2 * align_up(parts * 4, kAlign) + parts * d->head_dim * 4;
     }
@@ -1094,10 +1101,13 @@ int prefix_plan(const aw_prefix_desc* d, uint32_t n_cu, aw::PrefixArgs* out, aw_
 
 template <int HD>
 int launch_prefix(aw_engine* e, aw::PrefixArgs& a, hipStream_t st) {
-    const uint64_t own = (uint64_t)a.batch * a.kv_heads * a.own_tiles * a.own_splits;
-    {
+    const dim3 grid(a.prefix_wgs + cdiv((uint64_t)a.prefix_items + a.own_items, 4)), block(aw::kPrefixThreads);
+    if (a.splits) {
         StageTimer t(e, AW_STAGE_HOT, st);
-        if (a.splits) hipLaunchKernelGGL(aw::prefix_kernel<HD>, dim3((uint32_t)(a.prefix_items + own)), dim3(64), 0, st, a);
+        if (a.prefix_wgs)
+            hipLaunchKernelGGL((aw::prefix_kernel<HD, true>), grid, block, aw::prefix_lds_bytes(HD), st, a);
+        else
+            hipLaunchKernelGGL((aw::prefix_kernel<HD, false>), grid, block, (size_t)4 * 32 * (HD + 16) * 2, st, a);
         AW_HIP(e, hipGetLastError());
     }
     StageTimer t(e, AW_STAGE_MERGE, st);

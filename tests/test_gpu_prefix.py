@@ -141,6 +141,15 @@ def test_keys_that_are_the_values(ops):
     c.check("K rows as values", values=c.k)
 
 
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 2.0 ** -30])
+def test_scales(ops, scale):
+    """A negative scale turns the order of the scores round; a scale of 0 weighs every token that is seen alike."""
+    for batch in (2, 20):
+        c = Case(50, batch, 2, 8, 2, 128, 100, [5, 40] + [3] * (batch - 2))
+        ops.shared_prefix_attention(c.desc(scale=scale))
+        c.check(f"scale {scale}", scale=scale)
+
+
 def test_peaked_and_flat_scores(ops):
     """Scores so far apart that one token takes all of the weight, the largest in the last part; equal scores."""
     c = Case(6, 2, 1, 8, 2, 128, 900, [40, 8], qscale=40.0)
