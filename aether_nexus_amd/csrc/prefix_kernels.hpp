@@ -28,8 +28,8 @@ struct PrefixArgs {
     uint32_t prefix_tokens, own_max, refs_stride;
     uint32_t prefix_splits, own_splits, splits; // splits = prefix_splits + own_splits
     uint32_t prefix_span, own_span;             // tokens of a split, a multiple of 32
-    uint32_t prefix_wgs;                        // work-groups of PrefixTile parts
-    uint32_t prefix_items, own_items;           // one-wave parts
+    uint32_t prefix_wgs, work_groups;           // work-groups of PrefixTile parts, all
+    uint32_t prefix_units, own_units;           // one-wave parts, kv_heads each
     uint32_t prefix_tiles, own_tiles;
     uint64_t blocks;
     float scale_log2;           // > 0
@@ -257,8 +257,9 @@ struct PrefixWave {
 // Staged rows are HD / 8 16-byte chunks, chunk c of K row r at c ^ (r % chunks), of V
 // row r at c ^ 4 (r % 4) ^ (r / 4) % 4 (128 dims): no bank conflict at 128 dims.
 constexpr uint32_t kPrefixRows = 128;
+constexpr float kPrefixGrow = 8.0f;
 constexpr int kPrefixThreads = 256;
-constexpr int kPrefixTok = 64, kPrefixBufs = 2;
+constexpr int kPrefixTok = 64, kPrefixBufs = 2; // tokens a step, steps of K (and of V) in LDS
 constexpr size_t prefix_lds_bytes(int HD) { return (size_t)kPrefixBufs * 2 * kPrefixTok * HD * 2; }
 
 template <int HD>
@@ -267,23 +268,29 @@ struct PrefixTile {
     static constexpr int CH = HD / 8, KS = HD / 16, NB = HD / 32;
     static constexpr int LPT = TOK * CH / kPrefixThreads; // loads per thread, operand and step
     static constexpr uint32_t OP = TOK * HD;              // halves per staged operand
+    static constexpr int NS = TB * KS, NV = 2 * TB * NB;  // MFMAs of a step's scores, of its output
+    static constexpr int EXP = 16 * TB / NS;              // weights worked out beside one MFMA of the scores
+    static constexpr int AHEAD = 4;                       // fragments read ahead of their MFMAs
     static_assert(prefix_lds_bytes(HD) >= (size_t)4 * 32 * (HD + 16) * 2, "the one-wave parts' LDS");
+    static_assert(EXP % 2 == 0 && 16 * TB % NS == 0 && NS >= AHEAD && NV >= AHEAD, "");
 
     static __device__ __forceinline__ uint32_t ksw(uint32_t row) { return row & (uint32_t)(CH - 1); }
     static __device__ __forceinline__ uint32_t vsw(uint32_t row) {
         return CH == 16 ? ((row & 3u) << 2) | ((row >> 2) & 3u) : ((row >> 1) & 1u) << 2;
     }
-    static __device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
     static __device__ __forceinline__ void barrier() {
+        __builtin_amdgcn_sched_barrier(0);
         __asm__ volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         __asm__ volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
     }
 
     static __device__ __forceinline__ void run(const PrefixArgs& a, uint32_t g, uint32_t tile, uint32_t s, _Float16* lds) {
         const int tid = threadIdx.x, lane = tid & 63, li = lane & 31, hf = lane >> 5;
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         const uint32_t t0 = s * a.prefix_span, t1 = min(t0 + a.prefix_span, a.prefix_tokens); // t0 < t1
+        const int steps = (int)((t1 - t0 + (uint32_t)TOK - 1u) / (uint32_t)TOK);
         const uint32_t row = tile * kPrefixRows + 32u * (uint32_t)wave + (uint32_t)li;
         const bool wave_rows = tile * kPrefixRows + 32u * (uint32_t)wave < a.rows;
 
@@ -295,16 +302,11 @@ struct PrefixTile {
             for (int j = 0; j < KS; ++j) qop[j] = prefix_query(a, p + 16 * j + 8 * hf);
         }
 
-        // Staging: load j fills slots tid + 256 j of the operand (slot -> row, chunk); a
-        // wave's slots of one load lie in one page.
+        // Staging: load j fills slots tid + 256 j of the operand (slot -> row, chunk); a wave's
+        // slots of one load lie in one page, at the same place of it for every j.
         const uint32_t rstride = a.kv_heads * (uint32_t)HD; // halves
-        uint32_t koff[LPT], voff[LPT];
-#pragma unroll
-        for (int j = 0; j < LPT; ++j) {
-            const uint32_t q = (uint32_t)tid + (uint32_t)(kPrefixThreads * j), r = q / CH, c = q % CH;
-            koff[j] = ((r & 15u) * rstride + 8u * (c ^ ksw(r))) * 2u;
-            voff[j] = ((r & 15u) * rstride + 8u * (c ^ vsw(r))) * 2u;
-        }
+        const uint32_t srow = ((uint32_t)tid / CH) & 15u, schunk = (uint32_t)tid % CH;
+        const int koff = (int)((srow * rstride + 8u * (schunk ^ ksw(srow))) * 2u), voff = (int)((srow * rstride + 8u * (schunk ^ vsw(srow))) * 2u);
         // Refs of 64 pages from the part's first on, one in each lane, and of the next 64.
         const uint32_t last = (a.prefix_tokens - 1u) / kBlockTokens, first = t0 / kBlockTokens;
         const uint64_t page_halves = (uint64_t)kBlockTokens * rstride;
@@ -313,45 +315,47 @@ struct PrefixTile {
         auto refs_from = [&](uint32_t run) {
             return a.prefix_refs[min(first + 64u * run + (uint32_t)lane, last)] & kRefMask;
         };
-        // Loads the step of tokens c0 .. into buffer `buf`; returns a bit for each page that counts.
-        auto issue = [&](uint32_t c0, uint32_t buf) -> uint32_t {
-            const uint32_t b0 = (c0 - t0) / kBlockTokens;
+        uint64_t page_at[PAGES]; // of the newest step of K: the step of V that is loaded next
+        int page_bytes[PAGES];
+        uint32_t oks = 0; // PAGES bits for each of 4 steps: the pages that count
+        auto load = [&](const uint16_t* pool, uint32_t buf, int off, _Float16* dst) {
+            dst += buf * OP + (uint32_t)wave * 512u;
+#pragma unroll
+            for (int j = 0; j < LPT; ++j) {
+                auto go = [&](int p) {
+                    const __amdgpu_buffer_rsrc_t r =
+                        __builtin_amdgcn_make_buffer_rsrc((void*)(pool + page_at[p]), (short)0, page_bytes[p], (int)kBufferWord3);
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                        r, (__attribute__((address_space(3))) void*)(dst + kPrefixThreads * 8 * j), 16, off, 0, 0, 0);
+                };
+                if constexpr (CH == 16) go(j);      // 16 rows a load
+                else if (wave < 2) go(2 * j);       // 32 rows a load, two pages
+                else go(2 * j + 1);
+            }
+        };
+        auto load_k = [&](int step, uint32_t buf) {
+            const uint32_t b0 = (uint32_t)step * (uint32_t)PAGES;
             if (b0 / 64u != held) { // a step's pages lie in one run of 64
                 held = b0 / 64u;
                 refv = refn;
                 refn = refs_from(held + 1u);
             }
-            uint32_t oks = 0;
-            __amdgpu_buffer_rsrc_t rk[PAGES], rv[PAGES];
+            uint32_t ok4 = 0;
 #pragma unroll
             for (int p = 0; p < PAGES; ++p) {
                 const uint32_t ref = (uint32_t)__builtin_amdgcn_readlane((int)refv, (int)((b0 + (uint32_t)p) & 63u));
-                const uint32_t at = c0 + 16u * p;
+                const uint32_t at = t0 + 16u * (b0 + (uint32_t)p);
                 const bool in = at < t1, ok = in && ref < a.blocks;
                 bad |= in && !ok;
-                oks |= ok ? 1u << p : 0u;
-                const uint64_t base = (ok ? ref : 0u) * page_halves + (uint64_t)g * HD;
-                const uint32_t rows = ok ? min(16u, t1 - at) : 0u;
-                const int bytes = ok ? (int)(((rows - 1u) * rstride + (uint32_t)HD) * 2u) : 0;
-                rk[p] = __builtin_amdgcn_make_buffer_rsrc((void*)(a.k + base), (short)0, bytes, (int)kBufferWord3);
-                rv[p] = __builtin_amdgcn_make_buffer_rsrc((void*)(a.v + base), (short)0, bytes, (int)kBufferWord3);
+                ok4 |= ok ? 1u << p : 0u;
+                page_at[p] = (ok ? ref : 0u) * page_halves + (uint64_t)g * HD;
+                page_bytes[p] = ok ? (int)(((min(16u, t1 - at) - 1u) * rstride + (uint32_t)HD) * 2u) : 0;
             }
-            _Float16* dst = lds + buf * 2u * OP;
-#pragma unroll
-            for (int o = 0; o < 2; ++o)
-#pragma unroll
-                for (int j = 0; j < LPT; ++j) {
-                    _Float16* d = dst + (uint32_t)o * OP + ((uint32_t)wave * 64u + (uint32_t)(kPrefixThreads * j)) * 8u; // wave-uniform
-                    const int off = (int)(o ? voff[j] : koff[j]);
-                    auto go = [&](__amdgpu_buffer_rsrc_t r) {
-                        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)d, 16, off, 0, 0, 0);
-                    };
-                    if constexpr (CH == 16) go(o ? rv[j] : rk[j]); // 16 rows a load
-                    else if (wave < 2) go(o ? rv[2 * j] : rk[2 * j]); // 32 rows a load, two pages
-                    else go(o ? rv[2 * j + 1] : rk[2 * j + 1]);
-                }
-            return oks;
+            const uint32_t sh = ((uint32_t)step & 3u) * (uint32_t)PAGES;
+            oks = (oks & ~(((1u << PAGES) - 1u) << sh)) | ok4 << sh;
+            load(a.k, buf, koff, lds);
         };
+        auto load_v = [&](uint32_t buf) { load(a.v, buf, voff, lds + BUFS * OP); };
 
         // LDS offsets (halves) of this lane's operands in a staged step.
         uint32_t kat[KS], va[NB], vb[NB];
@@ -362,44 +366,47 @@ struct PrefixTile {
             const uint32_t c = (((uint32_t)lane >> 4) & 1u) * 2u + ((i16 & 3u) >> 1), lo = 4u * (i16 & 1u);
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-                va[nb] = OP + ra * HD + 8u * ((4u * nb + c) ^ vsw(ra)) + lo;
-                vb[nb] = OP + rb * HD + 8u * ((4u * nb + c) ^ vsw(rb)) + lo;
+                va[nb] = ra * HD + 8u * ((4u * nb + c) ^ vsw(ra)) + lo;
+                vb[nb] = rb * HD + 8u * ((4u * nb + c) ^ vsw(rb)) + lo;
             }
         }
+        // MFMA x of the scores: tokens 32 (x % TB) .., k-step x / TB; of the output: tokens
+        // 32 (x / 2 NB) + 16 (x / NB % 2) .., dims 32 (x % NB) ..
+        auto kfrag = [&](const _Float16* sk, int x) { return *(const half8_t*)(sk + kat[x / TB] + (x % TB) * 32 * HD); };
+        auto vfrag = [&](const _Float16* sv, int x) {
+            const int nb = x % NB, ro = (32 * (x / (2 * NB)) + 16 * ((x / NB) % 2)) * HD;
+            return __builtin_bit_cast(half8_t, __builtin_shufflevector(lds_read_tr16(sv + va[nb] + ro), lds_read_tr16(sv + vb[nb] + ro),
+                                                                       0, 1, 2, 3, 4, 5, 6, 7));
+        };
 
         float m_run, l_run;
         float16_t oacc[NB];
-        // SPLIT: as in PrefixWave.
-        auto process = [&](auto split, uint32_t c0, uint32_t buf, uint32_t oks) {
+        // One step: the weights of `sc` (this step's scores), this step's output, and beside
+        // the weights the next step's scores into `sn`.  SPLIT: as in PrefixWave.
+        auto process = [&](auto split, int step, const _Float16* sk, const _Float16* sv, float16_t (&sc)[TB], float16_t (&sn)[TB]) {
             constexpr bool SPLIT = decltype(split)::value;
-            const _Float16* sb = lds + buf * 2u * OP;
-            float16_t sacc[TB];
+            const uint32_t c0 = t0 + (uint32_t)step * (uint32_t)TOK, ok4 = (oks >> (((uint32_t)step & 3u) * (uint32_t)PAGES)) & ((1u << PAGES) - 1u);
+            half8_t kf[AHEAD], vf[AHEAD];
 #pragma unroll
-            for (int tb = 0; tb < TB; ++tb) {
-                sacc[tb] = (float16_t)0.0f;
-#pragma unroll
-                for (int j = 0; j < KS; ++j)
-                    sacc[tb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8_t*)(sb + kat[j] + tb * 32 * HD), qop[j],
-                                                                      sacc[tb], 0, 0, 0);
-            }
-            if (c0 + (uint32_t)TOK > t1 || oks != (1u << PAGES) - 1u) { // wave-uniform
+            for (int x = 0; x < AHEAD; ++x) kf[x] = kfrag(sk, x);
+            if (c0 + (uint32_t)TOK > t1 || ok4 != (1u << PAGES) - 1u) { // wave-uniform
                 int see = (int)(t1 - c0) - 4 * hf;
                 __asm__ volatile("" : "+v"(see)); // compared with constants here, not as 32 values kept over the loop
 #pragma unroll
                 for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
-                        if (32 * tb + 8 * (i / 4) + i % 4 >= see || !((oks >> (2 * tb + i / 8)) & 1u)) sacc[tb][i] = -INFINITY;
+                        if (32 * tb + 8 * (i / 4) + i % 4 >= see || !((ok4 >> (2 * tb + i / 8)) & 1u)) sc[tb][i] = -INFINITY;
             }
             float mx = -INFINITY;
 #pragma unroll
             for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sacc[tb][i]);
+                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[tb][i]);
             const auto sw = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, mx), __builtin_bit_cast(uint32_t, mx), false, false);
             const uint32_t sw0 = sw[0], sw1 = sw[1]; // the row's two halves
             mx = fmaxf(__builtin_bit_cast(float, sw0), __builtin_bit_cast(float, sw1)) * a.scale_log2;
-            if (__any(mx > m_run)) {
+            if (__any(mx > m_run + kPrefixGrow)) {
                 const float mnew = fmaxf(m_run, mx);
                 const float alpha = mnew == -INFINITY ? 1.0f : fast_exp2(m_run - mnew);
                 m_run = mnew;
@@ -409,31 +416,38 @@ struct PrefixTile {
             }
             const float mref = m_run == -INFINITY ? 0.0f : m_run;
             half8_t pop[TB][2];
-            float ps0 = 0.0f, ps1 = 0.0f;
+            float ps[2] = {0.0f, 0.0f};
 #pragma unroll
-            for (int tb = 0; tb < TB; ++tb)
+            for (int tb = 0; tb < TB; ++tb) sn[tb] = (float16_t)0.0f;
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    const float p0 = fast_exp2(fmaf(sacc[tb][i], a.scale_log2, -mref));
-                    const float p1 = fast_exp2(fmaf(sacc[tb][i + 1], a.scale_log2, -mref));
-                    ps0 += p0;
-                    ps1 += p1;
-                    pop[tb][i / 8][i % 8] = (_Float16)p0;
-                    pop[tb][i / 8][i % 8 + 1] = (_Float16)p1;
+            for (int x = 0; x < NS; ++x) {
+                sn[x % TB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[x % AHEAD], qop[x / TB], sn[x % TB], 0, 0, 0);
+                if (x + AHEAD < NS) kf[x % AHEAD] = kfrag(sk, x + AHEAD);
+                else vf[x + AHEAD - NS] = vfrag(sv, x + AHEAD - NS);
+#pragma unroll
+                for (int e = 0; e < EXP; ++e) {
+                    const int at = x * EXP + e, tb = at / 16, i = at % 16;
+                    const float p = fast_exp2(fmaf(sc[tb][i], a.scale_log2, -mref));
+                    ps[e % 2] += p;
+                    pop[tb][i / 8][i % 8] = (_Float16)p;
+                    if constexpr (SPLIT) sc[tb][i] = p;
                 }
-            l_run += ps0 + ps1;
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            l_run += ps[0] + ps[1];
 #pragma unroll
-            for (int x = 0; x < 2 * TB * NB; ++x) {
-                const int tb = x / (2 * NB), kk = (x / NB) % 2, nb = x % NB, ro = (32 * tb + 16 * kk) * HD;
-                half8_t v = __builtin_bit_cast(half8_t, __builtin_shufflevector(lds_read_tr16(sb + va[nb] + ro),
-                                                                                lds_read_tr16(sb + vb[nb] + ro), 0, 1, 2, 3, 4, 5, 6, 7));
+            for (int x = 0; x < NV; ++x) {
+                const int nb = x % NB;
+                half8_t v = vf[x % AHEAD];
                 if constexpr (SPLIT) v = finite_part(v);
-                oacc[nb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pop[tb][kk], oacc[nb], 0, 0, 0);
-                if constexpr (SPLIT) __builtin_amdgcn_sched_barrier(0); // fewer fragments at once: no spills
+                oacc[nb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pop[x / (2 * NB)][(x / NB) % 2], oacc[nb], 0, 0, 0);
+                if (x + AHEAD < NV) vf[x % AHEAD] = vfrag(sv, x + AHEAD);
+                __builtin_amdgcn_sched_barrier(0);
             }
             if constexpr (SPLIT) {
                 auto nonfinite = [&](uint32_t r, uint32_t c) -> bool { // slot c of V row r
-                    const uint4_t w = *(const uint4_t*)(sb + OP + r * HD + 8u * c);
+                    const uint4_t w = *(const uint4_t*)(sv + r * HD + 8u * c);
                     bool any = false;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -443,29 +457,27 @@ struct PrefixTile {
                     return any;
                 };
                 bool any = false; // row `lane`, from another slot on in each lane (banks)
-#pragma unroll 4
+#pragma unroll 1
                 for (uint32_t c = 0; c < (uint32_t)CH; ++c)
                     any |= lane < TOK && nonfinite((uint32_t)lane % (uint32_t)TOK, (c + (uint32_t)lane) % (uint32_t)CH);
 #pragma unroll 1
                 for (uint64_t todo = __ballot(any); todo; todo &= todo - 1u) {
                     const uint32_t at = (uint32_t)__builtin_ctzll(todo);
                     const uint32_t slots = (uint32_t)__ballot(lane < CH && nonfinite(at, (uint32_t)lane % (uint32_t)CH));
-                    float x = 0.0f; // the score again
+                    float p = 0.0f; // token `at`'s weight: register (at / 8 % 4) 4 + at % 4 of the half at / 4 % 2
 #pragma unroll
-                    for (int j = 0; j < KS; ++j) {
-                        const half8_t kv = *(const half8_t*)(sb + at * HD + 8u * (((uint32_t)(2 * j + hf)) ^ ksw(at)));
+                    for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) x = fmaf((float)qop[j][e], (float)kv[e], x);
-                    }
-                    x += __shfl_xor(x, 32);
-                    const float p = fast_exp2(fmaf(x, a.scale_log2, -mref));
+                        for (int i = 0; i < 16; ++i)
+                            if ((at & ~4u) == (uint32_t)(32 * tb + 8 * (i / 4) + i % 4)) p = sc[tb][i];
+                    p = __shfl(p, li + 32 * (int)((at >> 2) & 1u));
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                         for (int i = 0; i < 16; i += 4) {
                             const uint32_t slot = (uint32_t)(4 * nb + i / 4) ^ vsw(at);
                             if (!((slots >> slot) & 1u)) continue; // uniform
-                            const half4_t v = *(const half4_t*)(sb + OP + at * HD + 8u * slot + 4 * hf);
+                            const half4_t v = *(const half4_t*)(sv + at * HD + 8u * slot + 4 * hf);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 const float f = (float)v[e];
@@ -476,8 +488,18 @@ struct PrefixTile {
             }
         };
 
-        constexpr short kWaitAll = (short)0x0070; // vmcnt(0), lgkmcnt(0): this wave's loads are in LDS, its LDS reads done
+        // Waits until at most `pairs` of this wave's newest steps of V and K, and `more` loads besides, are in
+        // flight, and its LDS reads are done.
+        auto wait = [](auto pairs, auto more) {
+            constexpr uint32_t vm = (uint32_t)(decltype(pairs)::value * 2 + decltype(more)::value) * (uint32_t)LPT;
+            __builtin_amdgcn_s_waitcnt((short)((vm & 15u) | ((vm >> 4) << 14) | (7u << 4))); // vmcnt(vm), lgkmcnt(0)
+        };
+        // Step i of K sits in buffer i % BUFS of K, of V likewise.  While step i is worked, V of
+        // i and K of i + 1 are read, and V up to i + BUFS - 1 and K up to i + BUFS are on the
+        // way: loads are issued in pairs (V of i + BUFS - 1, K of i + BUFS) once every wave has
+        // read what was there.
         auto pass = [&](auto split) {
+            using I0 = std::integral_constant<int, 0>;
             m_run = -INFINITY;
             l_run = 0.0f;
 #pragma unroll
@@ -485,18 +507,43 @@ struct PrefixTile {
             held = 0;
             refv = refs_from(0);
             refn = refs_from(1);
-            uint32_t buf = 0, oks = issue(t0, 0);
-            __builtin_amdgcn_s_waitcnt(kWaitAll);
+            float16_t s0[TB], s1[TB];
+            load_k(0, 0);
+#pragma unroll
+            for (int i = 1; i < BUFS; ++i)
+                if (i - 1 < steps) {
+                    load_v((uint32_t)(i - 1));
+                    if (i < steps) load_k(i, (uint32_t)i);
+                }
+            if (steps >= BUFS) wait(std::integral_constant<int, BUFS - 1>{}, I0{});
+            else wait(I0{}, I0{});
             barrier();
-            for (uint32_t c0 = t0; c0 < t1; c0 += (uint32_t)TOK) {
-                uint32_t next = 0;
-                if (c0 + (uint32_t)TOK < t1) next = issue(c0 + (uint32_t)TOK, buf ^ 1u); // its readers passed the last barrier
-                if (wave_rows) process(split, c0, buf, oks);
-                __builtin_amdgcn_s_waitcnt(kWaitAll);
+#pragma unroll
+            for (int tb = 0; tb < TB; ++tb) s0[tb] = (float16_t)0.0f;
+            if (wave_rows)
+#pragma unroll
+                for (int x = 0; x < NS; ++x)
+                    s0[x % TB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kfrag(lds, x), qop[x / TB], s0[x % TB], 0, 0, 0);
+            uint32_t cur = 0, nxt = BUFS > 1 ? 1u : 0u, old = BUFS - 1; // buffers i, i + 1, i - 1 (mod BUFS)
+            auto step = [&](int i, float16_t (&sc)[TB], float16_t (&sn)[TB]) {
+                if (i - 1 + BUFS < steps) wait(std::integral_constant<int, BUFS - 2>{}, I0{}); // every pair so far was a whole one
+                else wait(I0{}, I0{});
                 barrier();
-                buf ^= 1u;
-                oks = next;
+                if (i + BUFS - 1 < steps) {
+                    load_v(old);
+                    if (i + BUFS < steps) load_k(i + BUFS, cur);
+                }
+                if (wave_rows) process(split, i, lds + nxt * OP, lds + (BUFS + cur) * OP, sc, sn);
+                old = cur;
+                cur = nxt;
+                nxt = nxt + 1u == (uint32_t)BUFS ? 0u : nxt + 1u;
+            };
+            for (int i = 0; i < steps; i += 2) {
+                step(i, s0, s1);
+                if (i + 1 < steps) step(i + 1, s1, s0);
             }
+            wait(I0{}, I0{});
+            barrier(); // every step has been read
         };
         pass(std::false_type{});
         // An inf or NaN among the sums under finite weights: it comes from the values, and a
@@ -506,7 +553,7 @@ struct PrefixTile {
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int i = 0; i < 16; ++i) chk = fmaf(oacc[nb][i], 0.0f, chk);
-        uint32_t* flags = (uint32_t*)lds; // every step has been read
+        uint32_t* flags = (uint32_t*)lds;
         const bool redo = __any(wave_rows && row < a.rows && chk != 0.0f && l * 0.0f == 0.0f);
         if (lane == 0) flags[wave] = redo ? 1u : 0u;
         __syncthreads();
@@ -538,43 +585,48 @@ struct PrefixTile {
 
 // Work-groups 0 .. prefix_wgs - 1 take the prefix, the others four one-wave parts each.
 // TILES: the prefix in PrefixTile's parts; else in one-wave parts too.
-// Work-group b runs on XCD b % 8: the row tiles of one part of the prefix follow one
-// another on one XCD, so its pages come from memory once.
+// Work-group b runs on XCD b % 8.  A head's rows lie kv_heads * HD apart, so an XCD that
+// read one head alone would use a few of its L2's channels: each XCD takes all heads of
+// what it reads, the parts of one stretch of tokens after another (tiles: a run of
+// parts, each part's row tiles side by side, so that its pages come from memory once;
+// one-wave parts: the heads of four units, a unit one sequence's part, in turn over the
+// XCDs, since sequences differ in length).
 template <int HD, bool TILES>
 __global__ __launch_bounds__(kPrefixThreads) __attribute__((amdgpu_waves_per_eu(2))) void prefix_kernel(PrefixArgs a) {
     extern __shared__ __attribute__((aligned(16))) _Float16 prefix_lds[];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    auto uniform = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }; // divisions run on the vector ALUs
+    const int lane = threadIdx.x & 63;
+    const uint32_t wave = uniform(threadIdx.x >> 6), xcd = blockIdx.x & 7u;
+    uint32_t j = blockIdx.x >> 3;
     if constexpr (TILES) {
-        if (blockIdx.x < a.prefix_wgs) {
-            auto uniform = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }; // divisions run on the vector ALUs
-            const uint32_t j = blockIdx.x >> 3, part = uniform(j / a.prefix_tiles) * 8u + (blockIdx.x & 7u);
-            if (part >= a.kv_heads * a.prefix_splits) return;
-            const uint32_t tile = j % a.prefix_tiles, s = uniform(part / a.kv_heads);
-            PrefixTile<HD>::run(a, part - s * a.kv_heads, uniform(tile), s, prefix_lds);
+        if (blockIdx.x < a.prefix_wgs) { // a multiple of 8
+            const uint32_t parts = a.kv_heads * a.prefix_splits, each = (parts + 7u) >> 3, i = uniform(j / a.prefix_tiles);
+            const uint32_t part = xcd * each + i;
+            if (part >= parts) return;
+            const uint32_t s = uniform(part / a.kv_heads);
+            PrefixTile<HD>::run(a, part - s * a.kv_heads, j - i * a.prefix_tiles, s, prefix_lds);
             return;
         }
+        j -= a.prefix_wgs >> 3;
     }
+    const uint32_t chunk = uniform(j / a.kv_heads), item = (j - chunk * a.kv_heads) * 4u + wave; // of a chunk's 4 kv_heads items
+    uint32_t unit = (chunk * 8u + xcd) * 4u + uniform(item / a.kv_heads);
+    const uint32_t g = uniform(item % a.kv_heads);
     _Float16* lds = prefix_lds + wave * 32 * (HD + 16);
     const uint32_t li = (uint32_t)lane & 15u;
     PrefixWave<HD> w;
-    uint32_t t = (blockIdx.x - (TILES ? a.prefix_wgs : 0u)) * 4u + (uint32_t)wave;
     if constexpr (!TILES) {
-        if (t < a.prefix_items) {
-            const uint32_t s = t % a.prefix_splits;
-            t /= a.prefix_splits;
-            const uint32_t tile = t % a.prefix_tiles, g = t / a.prefix_tiles, r = tile * 16u + li;
+        if (unit < a.prefix_units) {
+            const uint32_t s = uniform(unit / a.prefix_tiles), r = (unit - s * a.prefix_tiles) * 16u + li;
             const uint32_t t0 = s * a.prefix_span, t1 = min(t0 + a.prefix_span, a.prefix_tokens);
             w.run(a, a.prefix_refs, g, min(r, a.rows - 1u), r < a.rows, t0, t1, a.prefix_tokens, a.prefix_tokens, s, lds, lane);
             return;
         }
-        t -= a.prefix_items;
+        unit -= a.prefix_units;
     }
-    if (t >= a.own_items) return;
-    const uint32_t s = t % a.own_splits;
-    t /= a.own_splits;
-    const uint32_t g = t % a.kv_heads;
-    t /= a.kv_heads;
-    const uint32_t tile = t % a.own_tiles, b = t / a.own_tiles, r = tile * 16u + li, rc = min(r, a.own_rows - 1u);
+    if (unit >= a.own_units) return;
+    const uint32_t s = uniform(unit / (a.batch * a.own_tiles)), bt = unit - s * a.batch * a.own_tiles, b = uniform(bt / a.own_tiles);
+    const uint32_t r = (bt - b * a.own_tiles) * 16u + li, rc = min(r, a.own_rows - 1u);
     uint32_t n = a.seq_own ? a.seq_own[b] : a.own_max;
     if (n > a.own_max) {
         n = a.own_max;
@@ -587,34 +639,71 @@ __global__ __launch_bounds__(kPrefixThreads) __attribute__((amdgpu_waves_per_eu(
           a.prefix_splits + s, lds, lane);
 }
 
-// Joins a row's splits: the largest maximum, each split's sums times 2^(its maximum -
-// that), in the order of the splits; zeros where no split saw a token.  An inf or NaN
-// in a split's sum stays in the result.  Wave per row.
-template <int HD>
+// A batch that sees no token at all: rows of zeros, 4 halves a lane.
+__global__ __launch_bounds__(256) void prefix_zero_kernel(uint16_t* out, uint64_t n4) {
+    for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < n4; i += (uint64_t)gridDim.x * 256u)
+        ((half4_t*)out)[i] = (half4_t)(_Float16)0;
+}
+
+// Joins a row's parts: the largest maximum, each part's sums times 2^(its maximum -
+// that), added in an order of their own; zeros where no part saw a token.  An inf or NaN
+// in a part's sum stays in the result.  W waves a row (4 where rows are few, their sums
+// added in the order of the waves); a row of a part is HD / 4 lanes' float4, U loads in
+// flight before the parts' factors are known.
+template <int HD, int U, int W>
 __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a) {
-    constexpr int V = HD / 64;
-    const uint32_t lane = threadIdx.x & 63u;
-    const uint64_t id = (uint64_t)blockIdx.x * 4u + (threadIdx.x >> 6);
-    if (id >= (uint64_t)a.kv_heads * a.rows) return;
-    const uint32_t g = (uint32_t)(id / a.rows), r = (uint32_t)(id % a.rows);
-    const uint64_t at = (uint64_t)g * a.splits * a.rows + r;
-    const bool in = lane < a.splits;
-    const float l = in ? a.part_l[at + (uint64_t)lane * a.rows] : 0.0f;
-    const float m = l != 0.0f ? a.part_m[at + (uint64_t)lane * a.rows] : -INFINITY;
+    constexpr int LP = HD / 4, PG = 64 / LP; // lanes of a part's row, parts of one load
+    __shared__ float4_t s_sum[W > 1 ? W : 1][LP];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, w = W > 1 ? wave : 0u;
+    const uint64_t id = W > 1 ? (uint64_t)blockIdx.x : (uint64_t)blockIdx.x * 4u + wave;
+    if (id >= (uint64_t)a.kv_heads * a.rows) return; // W > 1: the grid is exact
+    const uint32_t g = (uint32_t)(id / a.rows), r = (uint32_t)(id % a.rows), S = a.splits;
+    const uint64_t at = (uint64_t)g * S * a.rows + r;
+    const uint32_t sub = lane / LP, d = 4u * (lane % LP);
+    const float* po = a.part_o + at * HD + d;
+    auto part = [&](uint32_t p0, int j) { return p0 + (uint32_t)(j * W * PG) + w * PG + sub; };
+    float4_t v[U];
+    auto load = [&](uint32_t p0) {
+#pragma unroll
+        for (int j = 0; j < U; ++j) v[j] = *(const float4_t*)(po + (uint64_t)min(part(p0, j), S - 1u) * a.rows * HD);
+    };
+    const uint64_t mine = at + (uint64_t)min(lane, S - 1u) * a.rows;
+    float l = a.part_l[mine], m = a.part_m[mine];
+    load(0);
+    if (lane >= S) l = 0.0f;
+    if (l == 0.0f) m = -INFINITY;
     const float M = wave_max(m);
     const float f = l != 0.0f ? fast_exp2(m - M) : 0.0f;
     const float L = wave_sum(f * l);
-    float acc[V] = {};
-    for (uint32_t s = 0; s < a.splits; ++s) {
-        const float fs = __shfl(f, (int)s);
-        if (fs == 0.0f) continue; // uniform
-        const float* po = a.part_o + (at + (uint64_t)s * a.rows) * HD + V * lane;
+    float4_t acc = (float4_t)0.0f;
+    for (uint32_t p0 = 0; p0 < S; p0 += (uint32_t)(U * W * PG)) {
+        if (p0) load(p0);
 #pragma unroll
-        for (int e = 0; e < V; ++e) acc[e] = fmaf(fs, po[e], acc[e]);
+        for (int j = 0; j < U; ++j) {
+            const uint32_t p = part(p0, j);
+            const float fp = __shfl(f, (int)min(p, S - 1u));
+            if (p < S && fp != 0.0f) // a part that saw nothing holds no sums
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[e] = fmaf(fp, v[j][e], acc[e]);
+        }
     }
-    uint16_t* out = a.out + ((uint64_t)(r / a.gqa) * a.q_heads + g * a.gqa + r % a.gqa) * HD + V * lane;
 #pragma unroll
-    for (int e = 0; e < V; ++e) out[e] = __builtin_bit_cast(uint16_t, (_Float16)(L == 0.0f ? 0.0f : acc[e] / L));
+    for (int o = LP; o < 64; o *= 2)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], o);
+    if constexpr (W > 1) {
+        if (sub == 0) s_sum[wave][lane] = acc;
+        __syncthreads();
+        if (wave != 0) return;
+        acc = s_sum[0][lane % LP];
+#pragma unroll
+        for (int i = 1; i < W; ++i) acc += s_sum[i][lane % LP];
+    }
+    if (sub != 0) return;
+    half4_t h;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[e] = (_Float16)(L == 0.0f ? 0.0f : acc[e] / L);
+    *(half4_t*)(a.out + ((uint64_t)(r / a.gqa) * a.q_heads + g * a.gqa + r % a.gqa) * HD + d) = h;
 }
 
 } // namespace aw

@@ -1020,6 +1020,8 @@ void prefix_parts(uint64_t items, uint64_t want, uint32_t tokens, uint32_t least
     *parts = cdiv(tokens, *span);
 }
 
+constexpr uint64_t kPrefixTilesPerCu = 1;
+
 // Checks a request and fills its kernel arguments but for addresses of scratch.
 int prefix_plan(const aw_prefix_desc* d, uint32_t n_cu, aw::PrefixArgs* out, aw_prefix_plan_info* info, char* msg, size_t len) {
     auto refuse = [&](int code, const char* why) {
@@ -1076,16 +1078,19 @@ int prefix_plan(const aw_prefix_desc* d, uint32_t n_cu, aw::PrefixArgs* out, aw_
     a.prefix_tiles = cdiv(rows, tiles ? aw::kPrefixRows : 16);
     a.own_tiles = cdiv(a.own_rows, 16);
     const uint64_t own_parts = (uint64_t)d->batch * d->kv_heads * a.own_tiles, prefix_parts_n = (uint64_t)a.prefix_tiles * d->kv_heads;
-    if (tiles) prefix_parts(prefix_parts_n, n_cu, a.prefix_tokens, 128, 48, &a.prefix_splits, &a.prefix_span);
+    if (tiles) prefix_parts(prefix_parts_n, kPrefixTilesPerCu * n_cu, a.prefix_tokens, 128, 48, &a.prefix_splits, &a.prefix_span);
     else prefix_parts(prefix_parts_n, 8ull * n_cu, a.prefix_tokens, 128, 48, &a.prefix_splits, &a.prefix_span);
     prefix_parts(own_parts, 8ull * n_cu, a.own_max, 128, 16, &a.own_splits, &a.own_span);
     a.splits = a.prefix_splits + a.own_splits;
-    const uint64_t items = prefix_parts_n * a.prefix_splits, own_items = own_parts * a.own_splits;
     const uint64_t wgs = tiles ? (uint64_t)cdiv((uint64_t)d->kv_heads * a.prefix_splits, 8) * 8 * a.prefix_tiles : 0;
-    if (items + own_items > 0x7FFFFFFFull || wgs + own_items > 0x7FFFFFFFull) return refuse(AW_E_UNSUPPORTED, "grid too large");
+    const uint64_t prefix_units = tiles ? 0 : (uint64_t)a.prefix_tiles * a.prefix_splits;
+    const uint64_t own_units = (uint64_t)d->batch * a.own_tiles * a.own_splits;
+    const uint64_t wave_wgs = (uint64_t)cdiv(prefix_units + own_units, 32) * 8 * d->kv_heads; // chunks of 4 units, in eights
+    if (wgs + wave_wgs > 0x7FFFFFFFull || prefix_units + own_units > 0x7FFFFFFFull) return refuse(AW_E_UNSUPPORTED, "grid too large");
     a.prefix_wgs = (uint32_t)wgs;
-    a.prefix_items = tiles ? 0u : (uint32_t)items;
-    a.own_items = (uint32_t)own_items;
+    a.prefix_units = (uint32_t)prefix_units;
+    a.own_units = (uint32_t)own_units;
+    a.work_groups = (uint32_t)(wgs + wave_wgs);
     if (info) {
         *info = aw_prefix_plan_info{};
         info->prefix_splits = a.prefix_splits;
@@ -1101,7 +1106,7 @@ int prefix_plan(const aw_prefix_desc* d, uint32_t n_cu, aw::PrefixArgs* out, aw_
 
 template <int HD>
 int launch_prefix(aw_engine* e, aw::PrefixArgs& a, hipStream_t st) {
-    const dim3 grid(a.prefix_wgs + cdiv((uint64_t)a.prefix_items + a.own_items, 4)), block(aw::kPrefixThreads);
+    const dim3 grid(a.work_groups), block(aw::kPrefixThreads);
     if (a.splits) {
         StageTimer t(e, AW_STAGE_HOT, st);
         if (a.prefix_wgs)
@@ -1110,8 +1115,21 @@ int launch_prefix(aw_engine* e, aw::PrefixArgs& a, hipStream_t st) {
             hipLaunchKernelGGL((aw::prefix_kernel<HD, false>), grid, block, (size_t)4 * 32 * (HD + 16) * 2, st, a);
         AW_HIP(e, hipGetLastError());
     }
+    if (!a.splits) { // nothing to see
+        hipLaunchKernelGGL(aw::prefix_zero_kernel, dim3(std::min<uint32_t>(cdiv((uint64_t)a.batch * a.queries * a.q_heads * HD, 1024), 4096)),
+                           dim3(256), 0, st, a.out, (uint64_t)a.batch * a.queries * a.q_heads * HD / 4);
+        AW_HIP(e, hipGetLastError());
+        return AW_OK;
+    }
     StageTimer t(e, AW_STAGE_MERGE, st);
-    hipLaunchKernelGGL(aw::prefix_merge_kernel<HD>, dim3(cdiv((uint64_t)a.kv_heads * a.rows, 4)), dim3(256), 0, st, a);
+    const uint64_t all = (uint64_t)a.kv_heads * a.rows;
+    // Fewer rows than waves that the CUs hold: four waves a row.
+    if (all <= 4ull * e->n_cu && a.splits > 8)
+        hipLaunchKernelGGL((aw::prefix_merge_kernel<HD, 4, 4>), dim3((uint32_t)all), dim3(256), 0, st, a);
+    else if (a.splits > 8)
+        hipLaunchKernelGGL((aw::prefix_merge_kernel<HD, 8, 1>), dim3(cdiv(all, 4)), dim3(256), 0, st, a);
+    else
+        hipLaunchKernelGGL((aw::prefix_merge_kernel<HD, 4, 1>), dim3(cdiv(all, 4)), dim3(256), 0, st, a);
     AW_HIP(e, hipGetLastError());
     return AW_OK;
 }
@@ -1337,6 +1355,8 @@ int aw_engine_create(int device, aw_engine** out) {
         set_lds((const void*)aw::encode_lds_kernel<128>);
         set_lds((const void*)aw::prefill_kernel<64>);
         set_lds((const void*)aw::prefill_kernel<128>);
+        set_lds((const void*)aw::prefix_kernel<64, true>);
+        set_lds((const void*)aw::prefix_kernel<128, true>);
         if (!aw_engine_internal::ops_set_lds_limits(e->max_lds)) attr_ok = false;
     }
     if (!attr_ok) {
