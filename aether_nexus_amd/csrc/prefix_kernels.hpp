@@ -11,6 +11,11 @@
 
 namespace aw {
 
+// lds_read_tr16 of data whose loads into LDS this kernel has waited for itself.  Without
+// the restrict (any alias information does) the compiler puts a wait for every load into
+// LDS before such a read.
+__device__ __forceinline__ short4_t lds_read_tr16_waited(const _Float16* __restrict__ p) { return lds_read_tr16(p); }
+
 struct PrefixArgs {
     const uint16_t* q;          // [batch][queries][q_heads][HD]
     const uint16_t* k;          // pools [blocks][16][kv_heads][HD]
@@ -246,8 +251,7 @@ struct PrefixWave {
 // whatever sequences (row r: sequence and query r / G, head r % G), x one part of the
 // prefix, so that its pages are read once for all of them; 4 waves of 32 rows, TOK
 // tokens a step.  K and V of a step go from memory straight into LDS, TOK / 16 pages of
-// any place in the pool, each through a buffer resource of its own whose range ends with
-// the page's last token: rows past the prefix, and pages of a bad ref, load as zeros.
+// any place in the pool; tokens of a bad ref (page 0 is read) score -inf.
 //   S^T = K Q^T on v_mfma_f32_32x32x16_f16 (lane l: row l % 32, hf = l / 32):
 //     A = K (token l % 32, dims 16 j + 8 hf ..), B = Q^T from registers; a lane ends
 //     with 16 of 32 tokens, 8 (i / 4) + 4 hf + i % 4, of its row: the softmax is per
@@ -272,7 +276,7 @@ struct PrefixTile {
     static constexpr int EXP = 16 * TB / NS;              // weights worked out beside one MFMA of the scores
     static constexpr int AHEAD = 4;                       // fragments read ahead of their MFMAs
     static_assert(prefix_lds_bytes(HD) >= (size_t)4 * 32 * (HD + 16) * 2, "the one-wave parts' LDS");
-    static_assert(EXP % 2 == 0 && 16 * TB % NS == 0 && NS >= AHEAD && NV >= AHEAD, "");
+    static_assert(BUFS >= 2 && EXP % 2 == 0 && 16 * TB % NS == 0 && NS >= 2 * LPT && NS >= AHEAD && NV >= AHEAD, "");
 
     static __device__ __forceinline__ uint32_t ksw(uint32_t row) { return row & (uint32_t)(CH - 1); }
     static __device__ __forceinline__ uint32_t vsw(uint32_t row) {
@@ -304,88 +308,82 @@ struct PrefixTile {
 
         // Staging: load j fills slots tid + 256 j of the operand (slot -> row, chunk); a wave's
         // slots of one load lie in one page, at the same place of it for every j.
-        const uint32_t rstride = a.kv_heads * (uint32_t)HD; // halves
+        const uint32_t rstride = a.kv_heads * (uint32_t)HD, page_halves = kBlockTokens * rstride; // halves
         const uint32_t srow = ((uint32_t)tid / CH) & 15u, schunk = (uint32_t)tid % CH;
-        const int koff = (int)((srow * rstride + 8u * (schunk ^ ksw(srow))) * 2u), voff = (int)((srow * rstride + 8u * (schunk ^ vsw(srow))) * 2u);
-        // Refs of 64 pages from the part's first on, one in each lane, and of the next 64.
-        const uint32_t last = (a.prefix_tokens - 1u) / kBlockTokens, first = t0 / kBlockTokens;
-        const uint64_t page_halves = (uint64_t)kBlockTokens * rstride;
-        uint32_t held, refv, refn;
+        const uint16_t* kfrom = a.k + (uint64_t)g * HD + srow * rstride + 8u * (schunk ^ ksw(srow));
+        const uint16_t* vfrom = a.v + (uint64_t)g * HD + srow * rstride + 8u * (schunk ^ vsw(srow));
+        // Rows past the part's last token load that token's (and count for nothing).
+        const uint32_t first = t0 / kBlockTokens, last = (t1 - 1u) / kBlockTokens - first;
+        const int back = ((int)min(srow, (t1 - 1u) % kBlockTokens) - (int)srow) * (int)rstride;
+        // Refs of 64 pages, one in each lane, and which of them count: the run of the newest K
+        // step, the one before it, and (refs alone) the next.
+        uint32_t held, ref_cur, ref_old, ref_next;
+        uint64_t ok_cur, ok_old;
         bool bad = false;
-        auto refs_from = [&](uint32_t run) {
-            return a.prefix_refs[min(first + 64u * run + (uint32_t)lane, last)] & kRefMask;
+        auto refs_from = [&](uint32_t run) { return a.prefix_refs[first + min(64u * run + (uint32_t)lane, last)] & kRefMask; };
+        auto take = [&](uint32_t run) {
+            held = run;
+            ref_old = ref_cur;
+            ok_old = ok_cur;
+            const bool ok = ref_next < a.blocks;
+            ref_cur = ok ? ref_next : 0u;
+            ok_cur = __ballot(ok);
+            bad |= !ok;
+            ref_next = refs_from(run + 1u);
         };
-        uint64_t page_at[PAGES]; // of the newest step of K: the step of V that is loaded next
-        int page_bytes[PAGES];
-        uint32_t oks = 0; // PAGES bits for each of 4 steps: the pages that count
-        auto load = [&](const uint16_t* pool, uint32_t buf, int off, _Float16* dst) {
-            dst += buf * OP + (uint32_t)wave * 512u;
-#pragma unroll
-            for (int j = 0; j < LPT; ++j) {
-                auto go = [&](int p) {
-                    const __amdgpu_buffer_rsrc_t r =
-                        __builtin_amdgcn_make_buffer_rsrc((void*)(pool + page_at[p]), (short)0, page_bytes[p], (int)kBufferWord3);
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                        r, (__attribute__((address_space(3))) void*)(dst + kPrefixThreads * 8 * j), 16, off, 0, 0, 0);
-                };
-                if constexpr (CH == 16) go(j);      // 16 rows a load
-                else if (wave < 2) go(2 * j);       // 32 rows a load, two pages
-                else go(2 * j + 1);
+        // Load j of a step of K or V; INNER: the step is not the part's last.
+        auto load = [&](auto inner, const uint16_t* from, uint32_t refs, int step, _Float16* dst, int j) {
+            const uint32_t p = (uint32_t)(CH == 16 ? j : 2 * j + (wave >> 1)); // page: 16 rows a load, or 32
+            const uint32_t b = (uint32_t)step * (uint32_t)PAGES + p, at = decltype(inner)::value ? b : min(b, last);
+            const uint32_t ref = (uint32_t)__builtin_amdgcn_readlane((int)refs, (int)(at & 63u));
+            const uint16_t* src = from + (uint64_t)ref * page_halves;
+            if constexpr (!decltype(inner)::value) src += b >= last ? back : 0;
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                             (__attribute__((address_space(3))) void*)(dst + ((uint32_t)wave * 512u + (uint32_t)(kPrefixThreads * 8 * j))), 16, 0, 0);
+        };
+        // The pair (V of step v into its buffer vbuf, K of step v + 1 into kbuf): 2 LPT loads, x < LPT of V.  ready() first.
+        uint32_t vrefs;
+        auto ready = [&](int v) {
+            if (v + 1 < steps && (uint32_t)(v + 1) * (uint32_t)PAGES / 64u != held) take(held + 1u); // a step's pages lie in one run of 64
+            vrefs = (uint32_t)v * (uint32_t)PAGES / 64u == held ? ref_cur : ref_old;
+        };
+        auto load_pair = [&](auto inner, int x, int v, uint32_t vbuf, uint32_t kbuf) {
+            constexpr bool INNER = decltype(inner)::value;
+            if (x < LPT) {
+                if (INNER || (v >= 0 && v < steps)) load(inner, vfrom, vrefs, v, lds + (BUFS + vbuf) * OP, x);
+            } else if (INNER || v + 1 < steps) {
+                load(inner, kfrom, ref_cur, v + 1, lds + kbuf * OP, x - LPT);
             }
         };
-        auto load_k = [&](int step, uint32_t buf) {
-            const uint32_t b0 = (uint32_t)step * (uint32_t)PAGES;
-            if (b0 / 64u != held) { // a step's pages lie in one run of 64
-                held = b0 / 64u;
-                refv = refn;
-                refn = refs_from(held + 1u);
-            }
-            uint32_t ok4 = 0;
-#pragma unroll
-            for (int p = 0; p < PAGES; ++p) {
-                const uint32_t ref = (uint32_t)__builtin_amdgcn_readlane((int)refv, (int)((b0 + (uint32_t)p) & 63u));
-                const uint32_t at = t0 + 16u * (b0 + (uint32_t)p);
-                const bool in = at < t1, ok = in && ref < a.blocks;
-                bad |= in && !ok;
-                ok4 |= ok ? 1u << p : 0u;
-                page_at[p] = (ok ? ref : 0u) * page_halves + (uint64_t)g * HD;
-                page_bytes[p] = ok ? (int)(((min(16u, t1 - at) - 1u) * rstride + (uint32_t)HD) * 2u) : 0;
-            }
-            const uint32_t sh = ((uint32_t)step & 3u) * (uint32_t)PAGES;
-            oks = (oks & ~(((1u << PAGES) - 1u) << sh)) | ok4 << sh;
-            load(a.k, buf, koff, lds);
-        };
-        auto load_v = [&](uint32_t buf) { load(a.v, buf, voff, lds + BUFS * OP); };
 
-        // LDS offsets (halves) of this lane's operands in a staged step.
-        uint32_t kat[KS], va[NB], vb[NB];
-#pragma unroll
-        for (int j = 0; j < KS; ++j) kat[j] = (uint32_t)li * HD + 8u * (((uint32_t)(2 * j + hf)) ^ ksw((uint32_t)li));
+        // LDS offsets (halves) of this lane's operands in a staged step, of the first k-step
+        // and dim block; the others lie at these with a chunk's bits turned over.
+        uint32_t kat, va, vb;
         {
             const uint32_t i16 = (uint32_t)lane & 15u, ra = 4u * (uint32_t)hf + (i16 >> 2), rb = ra + 8u;
             const uint32_t c = (((uint32_t)lane >> 4) & 1u) * 2u + ((i16 & 3u) >> 1), lo = 4u * (i16 & 1u);
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                va[nb] = ra * HD + 8u * ((4u * nb + c) ^ vsw(ra)) + lo;
-                vb[nb] = rb * HD + 8u * ((4u * nb + c) ^ vsw(rb)) + lo;
-            }
+            kat = (uint32_t)li * HD + 8u * ((uint32_t)hf ^ ksw((uint32_t)li));
+            va = ra * HD + 8u * (c ^ vsw(ra)) + lo;
+            vb = rb * HD + 8u * (c ^ vsw(rb)) + lo;
         }
         // MFMA x of the scores: tokens 32 (x % TB) .., k-step x / TB; of the output: tokens
         // 32 (x / 2 NB) + 16 (x / NB % 2) .., dims 32 (x % NB) ..
-        auto kfrag = [&](const _Float16* sk, int x) { return *(const half8_t*)(sk + kat[x / TB] + (x % TB) * 32 * HD); };
+        auto kfrag = [&](const _Float16* sk, int x) { return *(const half8_t*)(sk + (kat ^ (16u * (x / TB))) + (x % TB) * 32 * HD); };
         auto vfrag = [&](const _Float16* sv, int x) {
             const int nb = x % NB, ro = (32 * (x / (2 * NB)) + 16 * ((x / NB) % 2)) * HD;
-            return __builtin_bit_cast(half8_t, __builtin_shufflevector(lds_read_tr16(sv + va[nb] + ro), lds_read_tr16(sv + vb[nb] + ro),
-                                                                       0, 1, 2, 3, 4, 5, 6, 7));
+            return __builtin_bit_cast(half8_t, __builtin_shufflevector(lds_read_tr16_waited(sv + (va ^ (32u * nb)) + ro),
+                                                                       lds_read_tr16_waited(sv + (vb ^ (32u * nb)) + ro), 0, 1, 2, 3, 4, 5, 6, 7));
         };
 
         float m_run, l_run;
         float16_t oacc[NB];
         // One step: the weights of `sc` (this step's scores), this step's output, and beside
         // the weights the next step's scores into `sn`.  SPLIT: as in PrefixWave.
-        auto process = [&](auto split, int step, const _Float16* sk, const _Float16* sv, float16_t (&sc)[TB], float16_t (&sn)[TB]) {
+        auto process = [&](auto split, int step, const _Float16* sk, const _Float16* sv, float16_t (&sc)[TB], float16_t (&sn)[TB], auto load_x) {
             constexpr bool SPLIT = decltype(split)::value;
-            const uint32_t c0 = t0 + (uint32_t)step * (uint32_t)TOK, ok4 = (oks >> (((uint32_t)step & 3u) * (uint32_t)PAGES)) & ((1u << PAGES) - 1u);
+            const uint32_t c0 = t0 + (uint32_t)step * (uint32_t)TOK, b0 = (uint32_t)step * (uint32_t)PAGES;
+            const uint32_t ok4 = (uint32_t)((b0 / 64u == held ? ok_cur : ok_old) >> (b0 & 63u)) & ((1u << PAGES) - 1u);
+            __asm__ volatile("" : "+v"(kat), "+v"(va), "+v"(vb)); // their other forms are made in each step, not kept: no spills
             half8_t kf[AHEAD], vf[AHEAD];
 #pragma unroll
             for (int x = 0; x < AHEAD; ++x) kf[x] = kfrag(sk, x);
@@ -425,6 +423,7 @@ struct PrefixTile {
                 sn[x % TB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[x % AHEAD], qop[x / TB], sn[x % TB], 0, 0, 0);
                 if (x + AHEAD < NS) kf[x % AHEAD] = kfrag(sk, x + AHEAD);
                 else vf[x + AHEAD - NS] = vfrag(sv, x + AHEAD - NS);
+                if (x < 2 * LPT) load_x(x);
 #pragma unroll
                 for (int e = 0; e < EXP; ++e) {
                     const int at = x * EXP + e, tb = at / 16, i = at % 16;
@@ -476,7 +475,7 @@ struct PrefixTile {
 #pragma unroll
                         for (int i = 0; i < 16; i += 4) {
                             const uint32_t slot = (uint32_t)(4 * nb + i / 4) ^ vsw(at);
-                            if (!((slots >> slot) & 1u)) continue; // uniform
+                            if (!((slots >> slot) & 1u) || c0 + at >= t1 || !((ok4 >> (at / 16u)) & 1u)) continue; // uniform
                             const half4_t v = *(const half4_t*)(sv + at * HD + 8u * slot + 4 * hf);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
@@ -488,35 +487,33 @@ struct PrefixTile {
             }
         };
 
-        // Waits until at most `pairs` of this wave's newest steps of V and K, and `more` loads besides, are in
-        // flight, and its LDS reads are done.
-        auto wait = [](auto pairs, auto more) {
-            constexpr uint32_t vm = (uint32_t)(decltype(pairs)::value * 2 + decltype(more)::value) * (uint32_t)LPT;
+        // Waits until at most `pairs` of this wave's newest pairs of V and K are in flight, and its LDS reads are done.
+        auto wait = [](auto pairs) {
+            constexpr uint32_t vm = (uint32_t)decltype(pairs)::value * 2u * (uint32_t)LPT;
             __builtin_amdgcn_s_waitcnt((short)((vm & 15u) | ((vm >> 4) << 14) | (7u << 4))); // vmcnt(vm), lgkmcnt(0)
         };
         // Step i of K sits in buffer i % BUFS of K, of V likewise.  While step i is worked, V of
-        // i and K of i + 1 are read, and V up to i + BUFS - 1 and K up to i + BUFS are on the
-        // way: loads are issued in pairs (V of i + BUFS - 1, K of i + BUFS) once every wave has
-        // read what was there.
+        // i and K of i + 1 are read, and the pair (V of i + BUFS - 1, K of i + BUFS) is loaded
+        // into what every wave has read before.
         auto pass = [&](auto split) {
             using I0 = std::integral_constant<int, 0>;
             m_run = -INFINITY;
             l_run = 0.0f;
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) oacc[nb] = (float16_t)0.0f;
-            held = 0;
-            refv = refs_from(0);
-            refn = refs_from(1);
+            ref_cur = 0;
+            ok_cur = 0;
+            ref_next = refs_from(0);
+            take(0);
             float16_t s0[TB], s1[TB];
-            load_k(0, 0);
 #pragma unroll
-            for (int i = 1; i < BUFS; ++i)
-                if (i - 1 < steps) {
-                    load_v((uint32_t)(i - 1));
-                    if (i < steps) load_k(i, (uint32_t)i);
-                }
-            if (steps >= BUFS) wait(std::integral_constant<int, BUFS - 1>{}, I0{});
-            else wait(I0{}, I0{});
+            for (int v = -1; v < BUFS - 1; ++v) {
+                vrefs = ref_cur; // BUFS steps lie in the first run
+#pragma unroll
+                for (int x = 0; x < 2 * LPT; ++x) load_pair(std::false_type{}, x, v, (uint32_t)(v + BUFS) % BUFS, (uint32_t)(v + 1));
+            }
+            if (steps >= BUFS) wait(std::integral_constant<int, BUFS - 1>{});
+            else wait(I0{});
             barrier();
 #pragma unroll
             for (int tb = 0; tb < TB; ++tb) s0[tb] = (float16_t)0.0f;
@@ -524,25 +521,36 @@ struct PrefixTile {
 #pragma unroll
                 for (int x = 0; x < NS; ++x)
                     s0[x % TB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kfrag(lds, x), qop[x / TB], s0[x % TB], 0, 0, 0);
-            uint32_t cur = 0, nxt = BUFS > 1 ? 1u : 0u, old = BUFS - 1; // buffers i, i + 1, i - 1 (mod BUFS)
-            auto step = [&](int i, float16_t (&sc)[TB], float16_t (&sn)[TB]) {
-                if (i - 1 + BUFS < steps) wait(std::integral_constant<int, BUFS - 2>{}, I0{}); // every pair so far was a whole one
-                else wait(I0{}, I0{});
+            uint32_t cur = 0, nxt = 1, old = BUFS - 1; // buffers of i, i + 1, i - 1
+            // INNER: the pair that this step loads is whole, and not of the part's last step.
+            auto step = [&](auto inner, int i, float16_t (&sc)[TB], float16_t (&sn)[TB]) {
+                if (decltype(inner)::value || i - 1 + BUFS < steps) wait(std::integral_constant<int, BUFS - 2>{}); // every pair so far was whole
+                else wait(I0{});
                 barrier();
-                if (i + BUFS - 1 < steps) {
-                    load_v(old);
-                    if (i + BUFS < steps) load_k(i + BUFS, cur);
+                ready(i + BUFS - 1);
+                auto load_x = [&](int x) { load_pair(inner, x, i + BUFS - 1, old, cur); };
+                if (wave_rows) {
+                    process(split, i, lds + nxt * OP, lds + (BUFS + cur) * OP, sc, sn, load_x);
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 2 * LPT; ++x) load_x(x);
                 }
-                if (wave_rows) process(split, i, lds + nxt * OP, lds + (BUFS + cur) * OP, sc, sn);
                 old = cur;
                 cur = nxt;
                 nxt = nxt + 1u == (uint32_t)BUFS ? 0u : nxt + 1u;
             };
-            for (int i = 0; i < steps; i += 2) {
-                step(i, s0, s1);
-                if (i + 1 < steps) step(i + 1, s1, s0);
+            int i = 0;
+            if constexpr (!decltype(split)::value)
+                for (; i + 2 + BUFS < steps; i += 2) {
+                    step(std::true_type{}, i, s0, s1);
+                    step(std::true_type{}, i + 1, s1, s0);
+                }
+#pragma unroll 1
+            for (; i < steps; i += 2) {
+                step(std::false_type{}, i, s0, s1);
+                if (i + 1 < steps) step(std::false_type{}, i + 1, s1, s0);
             }
-            wait(I0{}, I0{});
+            wait(I0{});
             barrier(); // every step has been read
         };
         pass(std::false_type{});
