@@ -31,10 +31,10 @@ struct PrefixArgs {
     uint32_t batch, queries, q_heads, kv_heads, gqa, causal;
     uint32_t rows, own_rows;    // query rows per kv head: of all sequences, of one
     uint32_t prefix_tokens, own_max, refs_stride;
-    uint32_t prefix_splits, own_splits, splits; // splits = prefix_splits + own_splits
-    uint32_t prefix_span, own_span;             // tokens of a split, a multiple of 32
+    uint32_t prefix_splits, own_splits, splits; // splits = prefix_splits + own_splits, or 0: no parts to join
+    uint32_t prefix_span, own_span;             // tokens of a split, a multiple of 64
     uint32_t prefix_wgs, work_groups;           // work-groups of PrefixTile parts, all
-    uint32_t prefix_units, own_units;           // one-wave parts, kv_heads each
+    uint32_t prefix_units, own_units;           // 16 rows x a part of a table, kv_heads work-groups each
     uint32_t prefix_tiles, own_tiles;
     uint64_t blocks;
     float scale_log2;           // > 0
@@ -50,181 +50,230 @@ __device__ __forceinline__ half8_t prefix_query(const PrefixArgs& a, const uint1
 }
 
 // Few rows to a table (a sequence's own pages; a prefix that at most kPrefixFewRows rows
-// see): 16 query rows of one kv head x the tokens [t0, t1), one wave, as in the decode
-// over hot blocks: S^T = K Q^T and O^T += V^T P^T on 16 x 16 x 32 MFMAs, 32 tokens a
-// step, the next step's rows loading while this one is multiplied, V read back from LDS
-// transposed.  A row's softmax keeps its running maximum and sum in fp32; weights are f16
-// operands of the second product (each off by 2^-12 of itself, independently: less than
-// the f16 store of the output).  Bound: HBM, the pages' bytes.
-// Tokens past `end` and tokens of a bad ref count as zeros that score -inf.
+// see): a work-group takes 16 query rows of one kv head x a run of pages, its 4 waves the
+// pages in turn, each on its own until the waves' sums meet in LDS.  A page's K and V go
+// from memory straight into LDS, 256 bytes (128 dims) of a row side by side, kPageBufs
+// pages a wave.
+//   S^T = K Q^T on v_mfma_f32_16x16x32_f16 (lane li + 16 lg): A = K (token li, dims 32 j
+//     + 8 lg ..), B = Q^T from registers; a lane ends with tokens 4 lg .. + 3 of row li;
+//   O^T += V^T P^T on v_mfma_f32_16x16x16_f16: B = P^T from the same registers, A = V^T
+//     (dim 16 nb + li, tokens 4 lg ..) by transposing LDS reads.
+// A row's softmax keeps its running maximum and sum in fp32; weights are f16 operands of
+// the second product (each off by 2^-12 of itself on average, independently: less than
+// the f16 store of the output).  Staged rows are HD / 8 16-byte chunks, chunk c of K row
+// r at c ^ r, of V row r at c ^ vsw(r): no bank conflict at 128 dims.
+// Bound: HBM, the pages' bytes.
 constexpr uint32_t kPrefixFewRows = 32;
+constexpr int kPageBufs = 2;
+constexpr size_t pages_lds_bytes(int HD) {
+    const size_t ring = (size_t)4 * kPageBufs * 2 * 16 * HD * 2, sums = (size_t)4 * 16 * (HD + 4) * 4 + 4 * 16 * 2 * 4;
+    return ring > sums ? ring : sums;
+}
+
+// A stretch of one table for 16 rows: pages [p0, p1) of it, tokens below `end`, of which
+// this lane's row sees those below `lim`.
+struct PageRun {
+    const uint32_t* table;
+    uint32_t p0, p1, end, lim;
+};
 
 template <int HD>
-struct PrefixWave {
-    static constexpr int KS = HD / 32, NB = HD / 16, P = HD + 16;
+struct PrefixPages {
+    static constexpr int CH = HD / 8, KS = HD / 32, NB = HD / 16, P = HD + 4;
+    static constexpr int LPP = CH / 4;                     // loads of a wave for a page of K (or V)
+    static constexpr uint32_t OP = 16 * HD;                // halves of a staged page operand
     half8_t qop[KS];
     float m_run, l_run;
     float4_t oacc[NB];
     bool bad;
 
-    // SPLIT: the products take the values' finite part; tokens whose values hold an inf or
-    // NaN are then added one by one, in fp32, to the rows that see them.
-    template <bool SPLIT>
-    __device__ __forceinline__ void pass(const PrefixArgs& a, const uint32_t* table, uint32_t g, uint32_t t0, uint32_t t1,
-                                         uint32_t end, uint32_t lim, _Float16* lds, int lane) {
+    static __device__ __forceinline__ uint32_t ksw(uint32_t row) { return row & (uint32_t)(CH - 1); }
+    static __device__ __forceinline__ uint32_t vsw(uint32_t row) {
+        return CH == 16 ? ((row & 3u) << 2) | ((row >> 2) & 3u) : ((row >> 1) & 1u) << 2;
+    }
+
+    // This wave's pages of the runs.  SPLIT: the products take the values' finite part;
+    // tokens whose values hold an inf or NaN are then added one by one, in fp32, to the
+    // rows that see them.
+    template <bool SPLIT, int RUNS>
+    __device__ __forceinline__ void pass(const PrefixArgs& a, const PageRun (&runs)[RUNS], uint32_t g, _Float16* lds, int lane, uint32_t wave) {
         const int li = lane & 15, lg = lane >> 4;
         m_run = -INFINITY;
         l_run = 0.0f;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) oacc[nb] = (float4_t)0.0f;
-        if (t0 >= t1) return;
-        // Refs of 64 blocks, one in each lane, and of the next 64.
-        const uint32_t last = (end - 1u) / kBlockTokens, first = t0 / kBlockTokens;
-        uint32_t held = 0;
-        uint32_t refv = table[min(first + (uint32_t)lane, last)] & kRefMask;
-        uint32_t refn = table[min(first + 64u + (uint32_t)lane, last)] & kRefMask;
-        // The 32 tokens from c0 on: this lane's pieces of K and V (loads that nothing masks:
-        // a bad ref reads block 0), and whether each block counts.
-        auto load = [&](uint32_t c0, uint4_t (&kr)[2][KS], uint4_t (&vr)[2][KS], bool (&ok)[2]) {
-            const uint32_t b0 = c0 / kBlockTokens - first;
-            if (b0 / 64u != held) { // a step's two blocks lie in one run of 64
-                held = b0 / 64u;
-                refv = refn;
-                refn = table[min(first + (held + 1u) * 64u + (uint32_t)lane, last)] & kRefMask;
+        const uint32_t n0 = runs[0].p1 - runs[0].p0, n = n0 + (RUNS > 1 ? runs[RUNS - 1].p1 - runs[RUNS - 1].p0 : 0u);
+        if (wave >= n) return; // wave-uniform
+        const uint32_t mine = (n - wave + 3u) / 4u; // pages wave, wave + 4, ..
+        // Page i of this wave: its run and its place there.
+        auto place = [&](uint32_t i, uint32_t& p) -> const PageRun& {
+            p = wave + 4u * i;
+            if (RUNS > 1 && p >= n0) {
+                p = runs[RUNS - 1].p0 + (p - n0);
+                return runs[RUNS - 1];
             }
-#pragma unroll
-            for (int tb = 0; tb < 2; ++tb) {
-                const uint32_t ref = (uint32_t)__builtin_amdgcn_readlane((int)refv, (int)((b0 + (uint32_t)tb) & 63u));
-                const bool in = c0 + 16u * tb < end;
-                ok[tb] = in && ref < a.blocks;
-                bad |= in && !ok[tb];
-                const uint64_t at = (((uint64_t)(ok[tb] ? ref : 0u) * kBlockTokens + li) * a.kv_heads + g) * HD + 8 * lg;
-#pragma unroll
-                for (int j = 0; j < KS; ++j) kr[tb][j] = *(const uint4_t*)(a.k + at + 32 * j);
-#pragma unroll
-                for (int j = 0; j < KS; ++j) vr[tb][j] = *(const uint4_t*)(a.v + at + 32 * j);
-            }
+            p += runs[0].p0;
+            return runs[0];
         };
-        auto process = [&](uint32_t c0, uint4_t (&kr)[2][KS], uint4_t (&vr)[2][KS], const bool (&ok)[2]) {
-#pragma unroll
-            for (int tb = 0; tb < 2; ++tb)
-                if (!ok[tb] || c0 + 16u * tb + (uint32_t)li >= end)
-#pragma unroll
-                    for (int j = 0; j < KS; ++j) kr[tb][j] = vr[tb][j] = (uint4_t)0u;
-            float4_t sacc[2];
-#pragma unroll
-            for (int tb = 0; tb < 2; ++tb) {
-                sacc[tb] = (float4_t)0.0f;
-#pragma unroll
-                for (int j = 0; j < KS; ++j) sacc[tb] = mfma16x16x32(as_h8(kr[tb][j]), qop[j], sacc[tb]);
+        // Refs of this wave's pages, 64 at a time, one in each lane, and of the next 64.
+        auto refs_from = [&](uint32_t from) {
+            uint32_t p;
+            const uint32_t i = min(from + (uint32_t)lane, mine - 1u), q = wave + 4u * i;
+            const bool second = RUNS > 1 && q >= n0;
+            p = second ? runs[RUNS - 1].p0 + (q - n0) : runs[0].p0 + q;
+            return (second ? runs[RUNS - 1].table : runs[0].table)[p] & kRefMask;
+        };
+        uint32_t held = 0, ref_cur = 0, ref_next = refs_from(0);
+        uint64_t ok_cur = 0, ok_old = 0;
+        auto take = [&] {
+            const bool ok = ref_next < a.blocks;
+            ref_cur = ok ? ref_next : 0u;
+            ok_old = ok_cur;
+            ok_cur = __ballot(ok);
+            bad |= !ok;
+        };
+        take();
+        ref_next = refs_from(64u);
+        // Staging: load j of a page fills slots lane + 64 j (slot -> row, chunk).
+        const uint32_t rstride = a.kv_heads * (uint32_t)HD;
+        _Float16* ring = lds + wave * (uint32_t)(kPageBufs * 2) * OP;
+        auto load = [&](uint32_t i) {
+            if (i / 64u != held) {
+                held = i / 64u;
+                take();
+                ref_next = refs_from((held + 1u) * 64u);
             }
-            wave_lds_order(); // the reads of the last step
+            uint32_t p;
+            const PageRun& r = place(i, p);
+            const uint32_t ref = (uint32_t)__builtin_amdgcn_readlane((int)ref_cur, (int)(i & 63u));
+            const uint32_t rows = min(16u, r.end - p * 16u); // rows past the end load the last one (and count for nothing)
+            const uint64_t at = (uint64_t)ref * (16u * rstride) + (uint64_t)g * HD;
+            _Float16* dst = ring + (i % (uint32_t)kPageBufs) * 2u * OP;
 #pragma unroll
-            for (int tb = 0; tb < 2; ++tb)
+            for (int o = 0; o < 2; ++o)
 #pragma unroll
-                for (int j = 0; j < KS; ++j) *(uint4_t*)(lds + (16 * tb + li) * P + 32 * j + 8 * lg) = vr[tb][j];
-            wave_lds_order();
-            float pf[8], mx = -INFINITY;
-#pragma unroll
-            for (int tb = 0; tb < 2; ++tb)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const bool see = ok[tb] && c0 + (uint32_t)(16 * tb + 4 * lg + e) < lim;
-                    pf[4 * tb + e] = see ? sacc[tb][e] * a.scale_log2 : -INFINITY;
-                    mx = fmaxf(mx, pf[4 * tb + e]);
+                for (int j = 0; j < LPP; ++j) {
+                    const uint32_t slot = (uint32_t)(lane + 64 * j), row = slot / CH, c = slot % CH;
+                    const uint16_t* src = (o ? a.v : a.k) + at + min(row, rows - 1u) * rstride + 8u * (c ^ (o ? vsw(row) : ksw(row)));
+                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                                     (__attribute__((address_space(3))) void*)(dst + (uint32_t)o * OP + 512u * j), 16, 0, 0);
                 }
+        };
+        auto wait = [](auto pages) {
+            constexpr uint32_t vm = (uint32_t)decltype(pages)::value * 2u * (uint32_t)LPP;
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_waitcnt((short)((vm & 15u) | ((vm >> 4) << 14) | (7u << 4) | (15u << 8))); // vmcnt(vm)
+            __asm__ volatile("" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+        };
+#pragma unroll
+        for (int i = 0; i < kPageBufs - 1; ++i)
+            if ((uint32_t)i < mine) load((uint32_t)i);
+        for (uint32_t i = 0; i < mine; ++i) {
+            __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the page before has been read
+            if (i + (uint32_t)kPageBufs - 1u < mine) {
+                load(i + (uint32_t)kPageBufs - 1u);
+                wait(std::integral_constant<int, kPageBufs - 1>{});
+            } else {
+                wait(std::integral_constant<int, 0>{});
+            }
+            uint32_t p;
+            const PageRun& r = place(i, p);
+            const bool ok = ((i / 64u == held ? ok_cur : ok_old) >> (i & 63u)) & 1u;
+            const _Float16 *sk = ring + (i % (uint32_t)kPageBufs) * 2u * OP, *sv = sk + OP;
+            float4_t sacc = (float4_t)0.0f;
+#pragma unroll
+            for (int j = 0; j < KS; ++j)
+                sacc = mfma16x16x32(*(const half8_t*)(sk + li * HD + 8 * ((4 * j + lg) ^ (int)ksw((uint32_t)li))), qop[j], sacc);
+            const uint32_t rlim = ok ? min(r.lim, r.end) : 0u;
+            float pf[4], mx = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                pf[e] = p * 16u + (uint32_t)(4 * lg + e) < rlim ? sacc[e] * a.scale_log2 : -INFINITY;
+                mx = fmaxf(mx, pf[e]);
+            }
             mx = fmaxf(mx, __shfl_xor(mx, 16));
             mx = fmaxf(mx, __shfl_xor(mx, 32));
             const float mnew = fmaxf(m_run, mx), mref = mnew == -INFINITY ? 0.0f : mnew;
             const float alpha = mnew == -INFINITY ? 1.0f : fast_exp2(m_run - mnew);
-            half8_t pop;
+            half4_t pop;
             float psum = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
+            for (int e = 0; e < 4; ++e) {
                 pf[e] = fast_exp2(pf[e] - mref);
                 psum += pf[e];
                 pop[e] = (_Float16)pf[e];
             }
             l_run = l_run * alpha + psum;
             m_run = mnew;
-            const _Float16* vrow = lds + (4 * lg + (li >> 2)) * P + 4 * (li & 3);
+            const uint32_t vr = 4u * (uint32_t)lg + ((uint32_t)li >> 2), vc = ((uint32_t)li & 3u) >> 1, vlo = 4u * ((uint32_t)li & 1u);
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-                half8_t vop = __builtin_bit_cast(
-                    half8_t, __builtin_shufflevector(lds_read_tr16(vrow + 16 * nb), lds_read_tr16(vrow + 16 * P + 16 * nb), 0,
-                                                     1, 2, 3, 4, 5, 6, 7));
-                if constexpr (SPLIT) vop = finite_part(vop);
-                oacc[nb] = mfma16x16x32(vop, pop, oacc[nb] * alpha);
+                half4_t v = __builtin_bit_cast(half4_t, lds_read_tr16_waited(sv + vr * HD + 8u * ((2u * nb + vc) ^ vsw(vr)) + vlo));
+                if constexpr (SPLIT) v = finite_part4(v);
+                oacc[nb] = __builtin_amdgcn_mfma_f32_16x16x16f16(v, pop, oacc[nb] * alpha, 0, 0, 0);
             }
             if constexpr (SPLIT) {
-                bool any[2] = {false, false};
+                bool any = false; // token li, a quarter of its chunks
 #pragma unroll
-                for (int tb = 0; tb < 2; ++tb)
+                for (int j = 0; j < LPP; ++j) {
+                    const uint4_t w = *(const uint4_t*)(sv + li * HD + 8 * (LPP * lg + j));
 #pragma unroll
-                    for (int j = 0; j < KS; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            any[tb] |= (vr[tb][j][e] & 0x7C00u) == 0x7C00u || (vr[tb][j][e] & 0x7C000000u) == 0x7C000000u;
-#pragma unroll
-                for (int tb = 0; tb < 2; ++tb) {
-                    uint64_t todo = __ballot(any[tb]); // lane li + 16 lg: token li
-                    todo = (todo | todo >> 16 | todo >> 32 | todo >> 48) & 0xFFFFu;
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t x = w[e];
+                        any |= (x & 0x7C00u) == 0x7C00u || (x & 0x7C000000u) == 0x7C000000u;
+                    }
+                }
+                uint64_t todo = __ballot(any);
+                todo = (todo | todo >> 16 | todo >> 32 | todo >> 48) & 0xFFFFu;
 #pragma unroll 1
-                    for (; todo; todo &= todo - 1u) {
-                        const int tok = __builtin_ctzll(todo);
-                        float p = 0.0f;
+                for (; todo; todo &= todo - 1u) {
+                    const int tok = __builtin_ctzll(todo);
+                    float w = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = __shfl(pf[e], li + 16 * (tok >> 2));
+                        if (e == (tok & 3)) w = x;
+                    }
+                    const bool see = p * 16u + (uint32_t)tok < rlim;
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) {
+                        const half4_t x = *(const half4_t*)(sv + tok * HD + 8 * ((2 * nb + (lg >> 1)) ^ (int)vsw((uint32_t)tok)) + 4 * (lg & 1));
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const float x = __shfl(pf[4 * tb + e], li + 16 * (tok >> 2));
-                            if (e == (tok & 3)) p = x;
-                        }
-                        const bool see = c0 + (uint32_t)(16 * tb + tok) < lim;
-#pragma unroll
-                        for (int nb = 0; nb < NB; ++nb) {
-                            const half4_t x = *(const half4_t*)(lds + (16 * tb + tok) * P + 16 * nb + 4 * lg);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const float f = (float)x[e];
-                                if (see && !(fabsf(f) < INFINITY)) oacc[nb][e] = fmaf(p, f, oacc[nb][e]);
-                            }
+                            const float f = (float)x[e];
+                            if (see && !(fabsf(f) < INFINITY)) oacc[nb][e] = fmaf(w, f, oacc[nb][e]);
                         }
                     }
                 }
             }
-        };
-        // Two sets of registers in turn.
-        uint4_t k0[2][KS], v0[2][KS], k1[2][KS], v1[2][KS];
-        bool ok0[2], ok1[2];
-        load(t0, k0, v0, ok0);
-        for (uint32_t c0 = t0; c0 < t1; c0 += 64u) {
-            const bool more = c0 + 32u < t1;
-            if (more) load(c0 + 32u, k1, v1, ok1);
-            process(c0, k0, v0, ok0);
-            if (!more) break;
-            if (c0 + 64u < t1) load(c0 + 64u, k0, v0, ok0);
-            process(c0 + 32u, k1, v1, ok1);
         }
         l_run += __shfl_xor(l_run, 16);
         l_run += __shfl_xor(l_run, 32);
     }
 
-    // LDS that one wave alone uses is written and read in order by the hardware; this keeps the compiler to it.
-    static __device__ __forceinline__ void wave_lds_order() {
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    // x with its infinities and NaNs replaced by zeros.
+    static __device__ __forceinline__ half4_t finite_part4(half4_t x) {
+        uint2_t w = __builtin_bit_cast(uint2_t, x);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const uint32_t v = w[e];
+            w[e] = ((v & 0x7C00u) == 0x7C00u ? 0u : v & 0xFFFFu) | ((v & 0x7C000000u) == 0x7C000000u ? 0u : v & 0xFFFF0000u);
+        }
+        return __builtin_bit_cast(half4_t, w);
     }
 
-    __device__ __forceinline__ void run(const PrefixArgs& a, const uint32_t* table, uint32_t g, uint32_t row, bool valid,
-                                        uint32_t t0, uint32_t t1, uint32_t end, uint32_t lim, uint32_t slot, _Float16* lds,
-                                        int lane) {
-        const int lg = lane >> 4;
+    // `row` of all rows is this lane's (clamped), row0 + i < row_end the work-group's.
+    template <int RUNS>
+    __device__ __forceinline__ void run(const PrefixArgs& a, const PageRun (&runs)[RUNS], uint32_t g, uint32_t row, uint32_t row0,
+                                        uint32_t row_end, uint32_t slot, _Float16* lds, int lane, uint32_t wave) {
+        const int li = lane & 15, lg = lane >> 4;
         const uint32_t head = g * a.gqa + row % a.gqa;
         const uint16_t* p = a.q + ((uint64_t)(row / a.gqa) * a.q_heads + head) * HD;
 #pragma unroll
         for (int j = 0; j < KS; ++j) qop[j] = prefix_query(a, p + 32 * j + 8 * lg);
         bad = false;
-        pass<false>(a, table, g, t0, t1, end, lim, lds, lane);
+        pass<false>(a, runs, g, lds, lane, wave);
         // An inf or NaN among the sums under finite weights comes from the values, and may
         // have reached rows that do not see it (0 * inf): once more, split.
         float chk = 0.0f;
@@ -232,18 +281,57 @@ struct PrefixWave {
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int e = 0; e < 4; ++e) chk = fmaf(oacc[nb][e], 0.0f, chk);
-        if (__any(chk != 0.0f && l_run * 0.0f == 0.0f)) pass<true>(a, table, g, t0, t1, end, lim, lds, lane);
-        if (bad) flag_error(a.err, kErrHotRef);
-        if (!valid) return;
-        const uint64_t at = ((uint64_t)g * a.splits + slot) * a.rows + row;
-        if (lg == 0) {
-            a.part_m[at] = m_run;
-            a.part_l[at] = l_run;
-        }
-        if (l_run == 0.0f) return; // nothing seen: the merge takes no value of it
-        float* po = a.part_o + at * HD;
+        if (__any(chk != 0.0f && l_run * 0.0f == 0.0f)) pass<true>(a, runs, g, lds, lane, wave);
+        if (__any(bad) && lane == 0) flag_error(a.err, kErrHotRef);
+        // The waves' sums, joined as prefix_merge_kernel joins the parts'.
+        float *so = (float*)lds, *sm = so + 4 * 16 * P, *sl = sm + 64; // [wave][row]
+        __syncthreads(); // every page has been read
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) *(float4_t*)(po + 16 * nb + 4 * lg) = oacc[nb];
+        for (int nb = 0; nb < NB; ++nb) *(float4_t*)(so + (wave * 16u + (uint32_t)li) * P + 16 * nb + 4 * lg) = oacc[nb];
+        if (lg == 0) {
+            sm[wave * 16u + (uint32_t)li] = l_run != 0.0f ? m_run : -INFINITY;
+            sl[wave * 16u + (uint32_t)li] = l_run;
+        }
+        __syncthreads();
+        const uint32_t t = wave * 64u + (uint32_t)lane, i = t >> 4, d = 4u * (t & 15u); // row, dims d .. + 3 (and d + 64 .. at 128)
+        if (row0 + i >= row_end) return;
+        const float M = fmaxf(fmaxf(sm[i], sm[16 + i]), fmaxf(sm[32 + i], sm[48 + i]));
+        float L = 0.0f;
+        float4_t o[HD / 64];
+#pragma unroll
+        for (int h = 0; h < HD / 64; ++h) o[h] = (float4_t)0.0f;
+#pragma unroll
+        for (uint32_t w = 0; w < 4; ++w) {
+            const float l = sl[w * 16u + i], f = l != 0.0f ? fast_exp2(sm[w * 16u + i] - M) : 0.0f;
+            L = fmaf(f, l, L);
+            if (f != 0.0f)
+#pragma unroll
+                for (int h = 0; h < HD / 64; ++h) {
+                    const float4_t x = *(const float4_t*)(so + (w * 16u + i) * P + 64 * h + d);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[h][e] = fmaf(f, x[e], o[h][e]);
+                }
+        }
+        const uint32_t r = row0 + i;
+        if (a.splits == 0) { // the request in one part: its rows
+            uint16_t* out = a.out + ((uint64_t)(r / a.gqa) * a.q_heads + g * a.gqa + r % a.gqa) * HD + d;
+#pragma unroll
+            for (int h = 0; h < HD / 64; ++h) {
+                half4_t y;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = (_Float16)(L == 0.0f ? 0.0f : o[h][e] / L);
+                *(half4_t*)(out + 64 * h) = y;
+            }
+            return;
+        }
+        const uint64_t at = ((uint64_t)g * a.splits + slot) * a.rows + r;
+        if (d == 0) {
+            a.part_m[at] = M;
+            a.part_l[at] = L;
+        }
+        if (L == 0.0f) return; // nothing seen: the merge takes no value of it
+#pragma unroll
+        for (int h = 0; h < HD / 64; ++h) *(float4_t*)(a.part_o + at * HD + 64 * h + d) = o[h];
     }
 };
 
@@ -275,7 +363,7 @@ struct PrefixTile {
     static constexpr int NS = TB * KS, NV = 2 * TB * NB;  // MFMAs of a step's scores, of its output
     static constexpr int EXP = 16 * TB / NS;              // weights worked out beside one MFMA of the scores
     static constexpr int AHEAD = 4;                       // fragments read ahead of their MFMAs
-    static_assert(prefix_lds_bytes(HD) >= (size_t)4 * 32 * (HD + 16) * 2, "the one-wave parts' LDS");
+    static_assert(prefix_lds_bytes(HD) >= pages_lds_bytes(HD), "the other parts' LDS");
     static_assert(BUFS >= 2 && EXP % 2 == 0 && 16 * TB % NS == 0 && NS >= 2 * LPT && NS >= AHEAD && NV >= AHEAD, "");
 
     static __device__ __forceinline__ uint32_t ksw(uint32_t row) { return row & (uint32_t)(CH - 1); }
@@ -591,14 +679,11 @@ struct PrefixTile {
     }
 };
 
-// Work-groups 0 .. prefix_wgs - 1 take the prefix, the others four one-wave parts each.
-// TILES: the prefix in PrefixTile's parts; else in one-wave parts too.
-// Work-group b runs on XCD b % 8.  A head's rows lie kv_heads * HD apart, so an XCD that
-// read one head alone would use a few of its L2's channels: each XCD takes all heads of
-// what it reads, the parts of one stretch of tokens after another (tiles: a run of
-// parts, each part's row tiles side by side, so that its pages come from memory once;
-// one-wave parts: the heads of four units, a unit one sequence's part, in turn over the
-// XCDs, since sequences differ in length).
+// Work-groups 0 .. prefix_wgs - 1 take the prefix in PrefixTile's parts (TILES), the others
+// a unit's kv head each: 16 rows x a part of one table, or (splits == 0: small requests)
+// all that they see, the prefix and their own pages, without a merge.
+// Work-group b runs on XCD b % 8: the row tiles of one part of the prefix follow one
+// another on one XCD, so its pages come from memory once, and so do the heads of a unit.
 template <int HD, bool TILES>
 __global__ __launch_bounds__(kPrefixThreads) __attribute__((amdgpu_waves_per_eu(2))) void prefix_kernel(PrefixArgs a) {
     extern __shared__ __attribute__((aligned(16))) _Float16 prefix_lds[];
@@ -617,40 +702,42 @@ __global__ __launch_bounds__(kPrefixThreads) __attribute__((amdgpu_waves_per_eu(
         }
         j -= a.prefix_wgs >> 3;
     }
-    const uint32_t chunk = uniform(j / a.kv_heads), item = (j - chunk * a.kv_heads) * 4u + wave; // of a chunk's 4 kv_heads items
-    uint32_t unit = (chunk * 8u + xcd) * 4u + uniform(item / a.kv_heads);
-    const uint32_t g = uniform(item % a.kv_heads);
-    _Float16* lds = prefix_lds + wave * 32 * (HD + 16);
-    const uint32_t li = (uint32_t)lane & 15u;
-    PrefixWave<HD> w;
+    const uint32_t eight = uniform(j / a.kv_heads), g = j - eight * a.kv_heads, li = (uint32_t)lane & 15u;
+    uint32_t unit = eight * 8u + xcd;
+    PrefixPages<HD> w;
     if constexpr (!TILES) {
         if (unit < a.prefix_units) {
-            const uint32_t s = uniform(unit / a.prefix_tiles), r = (unit - s * a.prefix_tiles) * 16u + li;
+            const uint32_t s = uniform(unit / a.prefix_tiles), row0 = (unit - s * a.prefix_tiles) * 16u;
             const uint32_t t0 = s * a.prefix_span, t1 = min(t0 + a.prefix_span, a.prefix_tokens);
-            w.run(a, a.prefix_refs, g, min(r, a.rows - 1u), r < a.rows, t0, t1, a.prefix_tokens, a.prefix_tokens, s, lds, lane);
+            const PageRun runs[1] = {{a.prefix_refs, t0 / 16u, (t1 + 15u) / 16u, a.prefix_tokens, a.prefix_tokens}};
+            w.run(a, runs, g, min(row0 + li, a.rows - 1u), row0, a.rows, s, prefix_lds, lane, wave);
             return;
         }
         unit -= a.prefix_units;
     }
     if (unit >= a.own_units) return;
     const uint32_t s = uniform(unit / (a.batch * a.own_tiles)), bt = unit - s * a.batch * a.own_tiles, b = uniform(bt / a.own_tiles);
-    const uint32_t r = (bt - b * a.own_tiles) * 16u + li, rc = min(r, a.own_rows - 1u);
+    const uint32_t r0 = (bt - b * a.own_tiles) * 16u, rc = min(r0 + li, a.own_rows - 1u);
     uint32_t n = a.seq_own ? a.seq_own[b] : a.own_max;
     if (n > a.own_max) {
         n = a.own_max;
-        if (lane == 0) flag_error(a.err, aw_engine_internal::kErrSeqBit);
+        if (threadIdx.x == 0) flag_error(a.err, aw_engine_internal::kErrSeqBit);
     }
+    n = uniform(n);
     const uint32_t i = rc / a.gqa; // query of the row: it sees n - queries + 1 + i tokens
     const uint32_t lim = a.causal ? (n + 1u + i > a.queries ? n + 1u + i - a.queries : 0u) : n;
-    const uint32_t t0 = s * a.own_span, t1 = min(t0 + a.own_span, n);
-    w.run(a, a.refs + (uint64_t)b * a.refs_stride, g, b * a.own_rows + rc, r < a.own_rows, t0, t1, n, lim,
-          a.prefix_splits + s, lds, lane);
-}
-
-// A batch that sees no token at all: rows of zeros, 4 halves a lane.
-__global__ __launch_bounds__(256) void prefix_zero_kernel(uint16_t* out, uint64_t n4) {
-    for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < n4; i += (uint64_t)gridDim.x * 256u)
-        ((half4_t*)out)[i] = (half4_t)(_Float16)0;
+    const uint32_t* table = a.refs + (uint64_t)b * a.refs_stride;
+    const uint32_t base = b * a.own_rows;
+    if constexpr (!TILES) {
+        if (a.splits == 0) {
+            const PageRun runs[2] = {{a.prefix_refs, 0, (a.prefix_tokens + 15u) / 16u, a.prefix_tokens, a.prefix_tokens}, {table, 0, (n + 15u) / 16u, n, lim}};
+            w.run(a, runs, g, base + rc, base + r0, base + a.own_rows, 0, prefix_lds, lane, wave);
+            return;
+        }
+    }
+    const uint32_t t0 = s * a.own_span, p0 = t0 / 16u; // a sequence may end before this part
+    const PageRun runs[1] = {{table, p0, t0 < n ? (min(t0 + a.own_span, n) + 15u) / 16u : p0, n, lim}};
+    w.run(a, runs, g, base + rc, base + r0, base + a.own_rows, a.prefix_splits + s, prefix_lds, lane, wave);
 }
 
 // Joins a row's parts: the largest maximum, each part's sums times 2^(its maximum -

@@ -1010,17 +1010,19 @@ int launch_prefill(aw_engine* e, const aw_decode_desc* d, uint32_t n, uint32_t k
 
 // ---- a batch that shares a prefix ------------------------------------------------
 
-// Parts of `tokens` tokens so that `items` work items of one part each become about
-// `want`: at most `most` parts of at least `least` tokens, a multiple of 32.
-void prefix_parts(uint64_t items, uint64_t want, uint32_t tokens, uint32_t least, uint32_t most, uint32_t* parts, uint32_t* span) {
+// Parts of `tokens` tokens (multiples of 64) so that `items` work-groups for each part
+// become about `want`, and no part is longer than `longest` where `most` parts allow it.
+void prefix_parts(uint64_t items, uint64_t want, uint32_t tokens, uint32_t longest, uint32_t most, uint32_t* parts, uint32_t* span) {
     *parts = *span = 0;
     if (tokens == 0) return;
-    const uint64_t n = std::max<uint64_t>(1, std::min<uint64_t>({want / std::max<uint64_t>(items, 1), most, cdiv(tokens, least)}));
-    *span = (uint32_t)align_up(cdiv(tokens, n), 32);
+    uint64_t n = std::max<uint64_t>({1, want / std::max<uint64_t>(items, 1), cdiv(tokens, longest)});
+    n = std::min<uint64_t>({n, most, cdiv(tokens, 64)});
+    *span = (uint32_t)align_up(cdiv(tokens, n), 64);
     *parts = cdiv(tokens, *span);
 }
 
 constexpr uint64_t kPrefixTilesPerCu = 1;
+constexpr uint32_t kPrefixOneTokens = 512;
 
 // Checks a request and fills its kernel arguments but for addresses of scratch.
 int prefix_plan(const aw_prefix_desc* d, uint32_t n_cu, aw::PrefixArgs* out, aw_prefix_plan_info* info, char* msg, size_t len) {
@@ -1074,23 +1076,27 @@ int prefix_plan(const aw_prefix_desc* d, uint32_t n_cu, aw::PrefixArgs* out, aw_
     a.q_and = d->scale == 0.0f ? 0u : ~0u;
     a.q_xor = d->scale < 0.0f ? 0x80008000u : 0u;
     a.scale_log2 = d->scale == 0.0f ? 1.0f : std::fabs(d->scale) * aw::kLog2e;
-    const bool tiles = rows > aw::kPrefixFewRows;
+    const bool tiles = rows > aw::kPrefixFewRows && d->prefix_tokens > 0;
     a.prefix_tiles = cdiv(rows, tiles ? aw::kPrefixRows : 16);
     a.own_tiles = cdiv(a.own_rows, 16);
-    const uint64_t own_parts = (uint64_t)d->batch * d->kv_heads * a.own_tiles, prefix_parts_n = (uint64_t)a.prefix_tiles * d->kv_heads;
-    if (tiles) prefix_parts(prefix_parts_n, kPrefixTilesPerCu * n_cu, a.prefix_tokens, 128, 48, &a.prefix_splits, &a.prefix_span);
-    else prefix_parts(prefix_parts_n, 8ull * n_cu, a.prefix_tokens, 128, 48, &a.prefix_splits, &a.prefix_span);
-    prefix_parts(own_parts, 8ull * n_cu, a.own_max, 128, 16, &a.own_splits, &a.own_span);
-    a.splits = a.prefix_splits + a.own_splits;
-    const uint64_t wgs = tiles ? (uint64_t)cdiv((uint64_t)d->kv_heads * a.prefix_splits, 8) * 8 * a.prefix_tiles : 0;
-    const uint64_t prefix_units = tiles ? 0 : (uint64_t)a.prefix_tiles * a.prefix_splits;
-    const uint64_t own_units = (uint64_t)d->batch * a.own_tiles * a.own_splits;
-    const uint64_t wave_wgs = (uint64_t)cdiv(prefix_units + own_units, 32) * 8 * d->kv_heads; // chunks of 4 units, in eights
-    if (wgs + wave_wgs > 0x7FFFFFFFull || prefix_units + own_units > 0x7FFFFFFFull) return refuse(AW_E_UNSUPPORTED, "grid too large");
+    const uint64_t own_wgs = (uint64_t)d->batch * d->kv_heads * a.own_tiles, prefix_wgs = (uint64_t)a.prefix_tiles * d->kv_heads;
+    uint64_t wgs = 0, prefix_units = 0, own_units = (uint64_t)d->batch * a.own_tiles;
+    const uint32_t tokens = a.prefix_tokens + a.own_max;
+    const bool one = tokens == 0 || (tokens <= kPrefixOneTokens && own_wgs <= 2ull * n_cu);
+    if (!one) {
+        prefix_parts(prefix_wgs, (tiles ? kPrefixTilesPerCu : 2) * n_cu, a.prefix_tokens, ~0u, 48, &a.prefix_splits, &a.prefix_span);
+        prefix_parts(own_wgs, 2ull * n_cu, a.own_max, 512, 16, &a.own_splits, &a.own_span);
+        a.splits = a.prefix_splits + a.own_splits;
+        own_units *= a.own_splits;
+        if (tiles) wgs = (uint64_t)cdiv((uint64_t)d->kv_heads * a.prefix_splits, 8) * 8 * a.prefix_tiles;
+        else prefix_units = (uint64_t)a.prefix_tiles * a.prefix_splits;
+    }
+    const uint64_t unit_wgs = (uint64_t)cdiv(prefix_units + own_units, 8) * 8 * d->kv_heads;
+    if (wgs + unit_wgs > 0x7FFFFFFFull) return refuse(AW_E_UNSUPPORTED, "grid too large");
     a.prefix_wgs = (uint32_t)wgs;
     a.prefix_units = (uint32_t)prefix_units;
     a.own_units = (uint32_t)own_units;
-    a.work_groups = (uint32_t)(wgs + wave_wgs);
+    a.work_groups = (uint32_t)(wgs + unit_wgs);
     if (info) {
         *info = aw_prefix_plan_info{};
         info->prefix_splits = a.prefix_splits;
@@ -1107,20 +1113,15 @@ int prefix_plan(const aw_prefix_desc* d, uint32_t n_cu, aw::PrefixArgs* out, aw_
 template <int HD>
 int launch_prefix(aw_engine* e, aw::PrefixArgs& a, hipStream_t st) {
     const dim3 grid(a.work_groups), block(aw::kPrefixThreads);
-    if (a.splits) {
+    {
         StageTimer t(e, AW_STAGE_HOT, st);
         if (a.prefix_wgs)
             hipLaunchKernelGGL((aw::prefix_kernel<HD, true>), grid, block, aw::prefix_lds_bytes(HD), st, a);
         else
-            hipLaunchKernelGGL((aw::prefix_kernel<HD, false>), grid, block, (size_t)4 * 32 * (HD + 16) * 2, st, a);
+            hipLaunchKernelGGL((aw::prefix_kernel<HD, false>), grid, block, aw::pages_lds_bytes(HD), st, a);
         AW_HIP(e, hipGetLastError());
     }
-    if (!a.splits) { // nothing to see
-        hipLaunchKernelGGL(aw::prefix_zero_kernel, dim3(std::min<uint32_t>(cdiv((uint64_t)a.batch * a.queries * a.q_heads * HD, 1024), 4096)),
-                           dim3(256), 0, st, a.out, (uint64_t)a.batch * a.queries * a.q_heads * HD / 4);
-        AW_HIP(e, hipGetLastError());
-        return AW_OK;
-    }
+    if (!a.splits) return AW_OK;
     StageTimer t(e, AW_STAGE_MERGE, st);
     const uint64_t all = (uint64_t)a.kv_heads * a.rows;
     // Fewer rows than waves that the CUs hold: four waves a row.
@@ -1356,6 +1357,8 @@ int aw_engine_create(int device, aw_engine** out) {
         set_lds((const void*)aw::prefill_kernel<64>);
         set_lds((const void*)aw::prefill_kernel<128>);
         set_lds((const void*)aw::prefix_kernel<64, true>);
+        set_lds((const void*)aw::prefix_kernel<64, false>);
+        set_lds((const void*)aw::prefix_kernel<128, false>);
         set_lds((const void*)aw::prefix_kernel<128, true>);
         if (!aw_engine_internal::ops_set_lds_limits(e->max_lds)) attr_ok = false;
     }
@@ -1568,7 +1571,7 @@ int aw_shared_prefix_attention_device(aw_engine* e, const aw_prefix_desc* d, voi
     if (rc) return fail(e, rc, "%s", msg);
     AW_HIP(e, hipSetDevice(e->device));
     hipStream_t st = (hipStream_t)stream; // NULL is HIP's null stream
-    if ((rc = ensure_keep(e->ws, info.workspace_bytes, e->retired_ws, e->last_error, st))) return rc;
+    if (a.splits && (rc = ensure_keep(e->ws, info.workspace_bytes, e->retired_ws, e->last_error, st))) return rc;
     char* ws = (char*)e->ws.ptr;
     const size_t stat = align_up((uint64_t)a.kv_heads * a.splits * a.rows * 4, kAlign);
     a.part_m = (float*)ws;

@@ -348,7 +348,8 @@ typedef struct aw_prefix_desc {
     uint16_t*       out;
 } aw_prefix_desc;
 
-/* How a request is split; filled by aw_shared_prefix_plan. */
+/* How a request is split; filled by aw_shared_prefix_plan.  Small requests are not
+ * (no parts of either kind, no workspace). */
 typedef struct aw_prefix_plan_info {
     uint32_t prefix_splits, prefix_tokens_per_split; /* parts of the prefix (0: none) */
     uint32_t own_splits, own_tokens_per_split;       /* parts of each sequence's own tokens (0: none) */

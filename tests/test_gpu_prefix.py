@@ -298,8 +298,10 @@ def test_capture_refuses_workspace_growth():
     from aether_nexus_amd.weaver import WeaverError
     fresh = OpsEngine()
     try:
-        c = Case(43, 2, 1, 8, 2, 64, 100, [20, 3])
+        c = Case(43, 2, 1, 8, 2, 64, 1000, [20, 3])
         d = c.desc()
+        small = Case(45, 2, 1, 8, 2, 64, 100, [20, 3])  # in one part: no workspace
+        d2 = small.desc()
         s = torch.cuda.Stream()
         s.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(s):
@@ -311,6 +313,14 @@ def test_capture_refuses_workspace_growth():
             del g
             torch.cuda.synchronize()
             assert np.isnan(host(c.out)).all()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                fresh.shared_prefix_attention(d2, stream=torch.cuda.current_stream().cuda_stream)
+            for _ in range(2):
+                small.out.fill_(float("nan"))
+                g.replay()
+                small.check("a small request captured at once")
+            del g
             fresh.shared_prefix_attention(d)
         c.check("after the refusal")
     finally:
