@@ -351,8 +351,8 @@ struct PrefixPages {
 constexpr uint32_t kPrefixRows = 128;
 constexpr float kPrefixGrow = 8.0f;
 constexpr int kPrefixThreads = 256;
-constexpr int kPrefixTok = 64, kPrefixBufs = 2; // tokens a step, steps of K (and of V) in LDS
-constexpr size_t prefix_lds_bytes(int HD) { return (size_t)kPrefixBufs * 2 * kPrefixTok * HD * 2; }
+constexpr int kPrefixTok = 64, kPrefixBufs = 5; // tokens a step, steps of K or of V in LDS: two work-groups fill a CU's
+constexpr size_t prefix_lds_bytes(int HD) { return (size_t)kPrefixBufs * kPrefixTok * HD * 2; }
 
 template <int HD>
 struct PrefixTile {
@@ -364,7 +364,7 @@ struct PrefixTile {
     static constexpr int EXP = 16 * TB / NS;              // weights worked out beside one MFMA of the scores
     static constexpr int AHEAD = 4;                       // fragments read ahead of their MFMAs
     static_assert(prefix_lds_bytes(HD) >= pages_lds_bytes(HD), "the other parts' LDS");
-    static_assert(BUFS >= 2 && EXP % 2 == 0 && 16 * TB % NS == 0 && NS >= 2 * LPT && NS >= AHEAD && NV >= AHEAD, "");
+    static_assert(BUFS == 5 && EXP % 2 == 0 && 16 * TB % NS == 0 && NS >= 2 * LPT && NS >= AHEAD && NV >= AHEAD, "");
 
     static __device__ __forceinline__ uint32_t ksw(uint32_t row) { return row & (uint32_t)(CH - 1); }
     static __device__ __forceinline__ uint32_t vsw(uint32_t row) {
@@ -429,18 +429,19 @@ struct PrefixTile {
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
                                              (__attribute__((address_space(3))) void*)(dst + ((uint32_t)wave * 512u + (uint32_t)(kPrefixThreads * 8 * j))), 16, 0, 0);
         };
-        // The pair (V of step v into its buffer vbuf, K of step v + 1 into kbuf): 2 LPT loads, x < LPT of V.  ready() first.
+        // The loads that step i issues, V of step i + 1 and K of step i + 3, into the buffers
+        // vbuf and kbuf: 2 LPT, x < LPT of V.  ready(i) first.
         uint32_t vrefs;
-        auto ready = [&](int v) {
-            if (v + 1 < steps && (uint32_t)(v + 1) * (uint32_t)PAGES / 64u != held) take(held + 1u); // a step's pages lie in one run of 64
-            vrefs = (uint32_t)v * (uint32_t)PAGES / 64u == held ? ref_cur : ref_old;
+        auto ready = [&](int i) {
+            if (i + 3 < steps && (uint32_t)(i + 3) * (uint32_t)PAGES / 64u != held) take(held + 1u); // a step's pages lie in one run of 64
+            vrefs = (uint32_t)(i + 1) * (uint32_t)PAGES / 64u == held ? ref_cur : ref_old;
         };
-        auto load_pair = [&](auto inner, int x, int v, uint32_t vbuf, uint32_t kbuf) {
+        auto load_pair = [&](auto inner, int x, int i, uint32_t vbuf, uint32_t kbuf) {
             constexpr bool INNER = decltype(inner)::value;
             if (x < LPT) {
-                if (INNER || (v >= 0 && v < steps)) load(inner, vfrom, vrefs, v, lds + (BUFS + vbuf) * OP, x);
-            } else if (INNER || v + 1 < steps) {
-                load(inner, kfrom, ref_cur, v + 1, lds + kbuf * OP, x - LPT);
+                if (INNER || (i >= -1 && i + 1 < steps)) load(inner, vfrom, vrefs, i + 1, lds + vbuf * OP, x);
+            } else if (INNER || i + 3 < steps) {
+                load(inner, kfrom, ref_cur, i + 3, lds + kbuf * OP, x - LPT);
             }
         };
 
@@ -467,7 +468,7 @@ struct PrefixTile {
         float16_t oacc[NB];
         // One step: the weights of `sc` (this step's scores), this step's output, and beside
         // the weights the next step's scores into `sn`.  SPLIT: as in PrefixWave.
-        auto process = [&](auto split, int step, const _Float16* sk, const _Float16* sv, float16_t (&sc)[TB], float16_t (&sn)[TB], auto load_x) {
+        auto process = [&](auto split, int step, const _Float16* sk, const _Float16* sv, float16_t (&sc)[TB], float16_t (&sn)[TB], auto load_x, auto v_there) {
             constexpr bool SPLIT = decltype(split)::value;
             const uint32_t c0 = t0 + (uint32_t)step * (uint32_t)TOK, b0 = (uint32_t)step * (uint32_t)PAGES;
             const uint32_t ok4 = (uint32_t)((b0 / 64u == held ? ok_cur : ok_old) >> (b0 & 63u)) & ((1u << PAGES) - 1u);
@@ -509,6 +510,7 @@ struct PrefixTile {
 #pragma unroll
             for (int x = 0; x < NS; ++x) {
                 sn[x % TB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[x % AHEAD], qop[x / TB], sn[x % TB], 0, 0, 0);
+                if (x == NS - AHEAD) v_there();
                 if (x + AHEAD < NS) kf[x % AHEAD] = kfrag(sk, x + AHEAD);
                 else vf[x + AHEAD - NS] = vfrag(sv, x + AHEAD - NS);
                 if (x < 2 * LPT) load_x(x);
@@ -575,16 +577,20 @@ struct PrefixTile {
             }
         };
 
-        // Waits until at most `pairs` of this wave's newest pairs of V and K are in flight, and its LDS reads are done.
-        auto wait = [](auto pairs) {
-            constexpr uint32_t vm = (uint32_t)decltype(pairs)::value * 2u * (uint32_t)LPT;
-            __builtin_amdgcn_s_waitcnt((short)((vm & 15u) | ((vm >> 4) << 14) | (7u << 4))); // vmcnt(vm), lgkmcnt(0)
+        // Waits until at most `n` of this wave's newest steps of V or K are in flight.
+        auto wait = [](auto n) {
+            constexpr uint32_t vm = (uint32_t)decltype(n)::value * (uint32_t)LPT;
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_waitcnt((short)((vm & 15u) | ((vm >> 4) << 14) | (7u << 4) | (15u << 8))); // vmcnt(vm)
         };
-        // Step i of K sits in buffer i % BUFS of K, of V likewise.  While step i is worked, V of
-        // i and K of i + 1 are read, and the pair (V of i + BUFS - 1, K of i + BUFS) is loaded
-        // into what every wave has read before.
+        // Steps of K and V share a ring of 5 buffers in the order of their loads: K 0, K 1,
+        // V 0, K 2, V 1, K 3, ..  While step i is worked, K of i + 1 is read, then V of i, and V
+        // of i + 1 and K of i + 3 are loaded into what every wave read in step i - 1: K is
+        // loaded almost two steps before its use, V one and a half.
         auto pass = [&](auto split) {
             using I0 = std::integral_constant<int, 0>;
+            using I2 = std::integral_constant<int, 2>;
+            using I3 = std::integral_constant<int, 3>;
             m_run = -INFINITY;
             l_run = 0.0f;
 #pragma unroll
@@ -593,14 +599,13 @@ struct PrefixTile {
             ok_cur = 0;
             ref_next = refs_from(0);
             take(0);
+            vrefs = ref_cur; // 4 steps lie in the first run
             float16_t s0[TB], s1[TB];
 #pragma unroll
-            for (int v = -1; v < BUFS - 1; ++v) {
-                vrefs = ref_cur; // BUFS steps lie in the first run
+            for (int i = -3; i < 0; ++i)
 #pragma unroll
-                for (int x = 0; x < 2 * LPT; ++x) load_pair(std::false_type{}, x, v, (uint32_t)(v + BUFS) % BUFS, (uint32_t)(v + 1));
-            }
-            if (steps >= BUFS) wait(std::integral_constant<int, BUFS - 1>{});
+                for (int x = 0; x < 2 * LPT; ++x) load_pair(std::false_type{}, x, i, 2u, (uint32_t)(i < -1 ? i + 3 : 3));
+            if (steps >= 3) wait(I3{});
             else wait(I0{});
             barrier();
 #pragma unroll
@@ -609,27 +614,36 @@ struct PrefixTile {
 #pragma unroll
                 for (int x = 0; x < NS; ++x)
                     s0[x % TB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kfrag(lds, x), qop[x / TB], s0[x % TB], 0, 0, 0);
-            uint32_t cur = 0, nxt = 1, old = BUFS - 1; // buffers of i, i + 1, i - 1
-            // INNER: the pair that this step loads is whole, and not of the part's last step.
+            uint32_t kb = 1, vb = 2; // buffers of K i + 1 and V i; V i + 1 takes kb + 3, K i + 3 vb + 3 (mod 5)
+            auto ring = [](uint32_t b) { return b >= 5u ? b - 5u : b; };
+            // INNER: the steps that this one loads are there, and K's is not the part's last.
             auto step = [&](auto inner, int i, float16_t (&sc)[TB], float16_t (&sn)[TB]) {
-                if (decltype(inner)::value || i - 1 + BUFS < steps) wait(std::integral_constant<int, BUFS - 2>{}); // every pair so far was whole
+                const bool whole = decltype(inner)::value || i + 2 < steps; // what step i - 1 loaded is whole
+                if (whole) wait(I2{});
                 else wait(I0{});
+                __builtin_amdgcn_s_waitcnt((short)0xC07F); // lgkmcnt(0): what this wave read of step i - 1 is there
                 barrier();
-                ready(i + BUFS - 1);
-                auto load_x = [&](int x) { load_pair(inner, x, i + BUFS - 1, old, cur); };
+                ready(i);
+                const uint32_t vnext = ring(kb + 3u), knext = ring(vb + 3u);
+                auto load_x = [&](int x) { load_pair(inner, x, i, vnext, knext); };
+                auto v_there = [&] {
+                    if (decltype(inner)::value || i + 3 < steps) wait(I3{}); // this step's loads are whole too
+                    else wait(I0{});
+                    barrier();
+                };
                 if (wave_rows) {
-                    process(split, i, lds + nxt * OP, lds + (BUFS + cur) * OP, sc, sn, load_x);
+                    process(split, i, lds + kb * OP, lds + vb * OP, sc, sn, load_x, v_there);
                 } else {
 #pragma unroll
                     for (int x = 0; x < 2 * LPT; ++x) load_x(x);
+                    v_there();
                 }
-                old = cur;
-                cur = nxt;
-                nxt = nxt + 1u == (uint32_t)BUFS ? 0u : nxt + 1u;
+                kb = ring(kb + 2u);
+                vb = ring(vb + 2u);
             };
             int i = 0;
             if constexpr (!decltype(split)::value)
-                for (; i + 2 + BUFS < steps; i += 2) {
+                for (; i + 5 < steps; i += 2) {
                     step(std::true_type{}, i, s0, s1);
                     step(std::true_type{}, i + 1, s1, s0);
                 }
