@@ -361,10 +361,8 @@ struct PrefixTile {
     static constexpr int LPT = TOK * CH / kPrefixThreads; // loads per thread, operand and step
     static constexpr uint32_t OP = TOK * HD;              // halves per staged operand
     static constexpr int NS = TB * KS, NV = 2 * TB * NB;  // MFMAs of a step's scores, of its output
-    static constexpr int EXP = 16 * TB / NS;              // weights worked out beside one MFMA of the scores
-    static constexpr int AHEAD = 4;                       // fragments read ahead of their MFMAs
     static_assert(prefix_lds_bytes(HD) >= pages_lds_bytes(HD), "the other parts' LDS");
-    static_assert(BUFS == 5 && EXP % 2 == 0 && 16 * TB % NS == 0 && NS >= 2 * LPT && NS >= AHEAD && NV >= AHEAD, "");
+    static_assert(BUFS == 5 && NS - 4 >= 2 * LPT, "this step's loads are out before v_there");
 
     static __device__ __forceinline__ uint32_t ksw(uint32_t row) { return row & (uint32_t)(CH - 1); }
     static __device__ __forceinline__ uint32_t vsw(uint32_t row) {
@@ -466,16 +464,21 @@ struct PrefixTile {
 
         float m_run, l_run;
         float16_t oacc[NB];
-        // One step: the weights of `sc` (this step's scores), this step's output, and beside
-        // the weights the next step's scores into `sn`.  SPLIT: as in PrefixWave.
+        // One step: the weights of `sc` (this step's scores) and its output, and beside them the
+        // next step's scores into `sn`: NS products of the scores, then NV of the output, the
+        // weights worked out beside the first NS + NV / 2 of them, those of the first 32 tokens
+        // done before their products.  Operands are read four products ahead, in fours: with
+        // loads into LDS under way the compiler waits for every LDS read before it uses one, so
+        // reads are issued right after such a wait.  SPLIT: as in PrefixPages.
         auto process = [&](auto split, int step, const _Float16* sk, const _Float16* sv, float16_t (&sc)[TB], float16_t (&sn)[TB], auto load_x, auto v_there) {
             constexpr bool SPLIT = decltype(split)::value;
             const uint32_t c0 = t0 + (uint32_t)step * (uint32_t)TOK, b0 = (uint32_t)step * (uint32_t)PAGES;
             const uint32_t ok4 = (uint32_t)((b0 / 64u == held ? ok_cur : ok_old) >> (b0 & 63u)) & ((1u << PAGES) - 1u);
             __asm__ volatile("" : "+v"(kat), "+v"(va), "+v"(vb)); // their other forms are made in each step, not kept: no spills
-            half8_t kf[AHEAD], vf[AHEAD];
+            half8_t fr[8];
+            auto read = [&](int z) { fr[z % 8] = z < NS ? kfrag(sk, z) : vfrag(sv, z - NS); };
 #pragma unroll
-            for (int x = 0; x < AHEAD; ++x) kf[x] = kfrag(sk, x);
+            for (int z = 0; z < 4; ++z) read(z);
             if (c0 + (uint32_t)TOK > t1 || ok4 != (1u << PAGES) - 1u) { // wave-uniform
                 int see = (int)(t1 - c0) - 4 * hf;
                 __asm__ volatile("" : "+v"(see)); // compared with constants here, not as 32 values kept over the loop
@@ -487,9 +490,7 @@ struct PrefixTile {
             }
             float mx = -INFINITY;
 #pragma unroll
-            for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[tb][i]);
+            for (int at = 0; at < 32; ++at) mx = fmaxf(mx, sc[at / 16][at % 16]);
             const auto sw = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, mx), __builtin_bit_cast(uint32_t, mx), false, false);
             const uint32_t sw0 = sw[0], sw1 = sw[1]; // the row's two halves
             mx = fmaxf(__builtin_bit_cast(float, sw0), __builtin_bit_cast(float, sw1)) * a.scale_log2;
@@ -506,34 +507,37 @@ struct PrefixTile {
             float ps[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int tb = 0; tb < TB; ++tb) sn[tb] = (float16_t)0.0f;
+            constexpr int SLOTS = NS + NV / 2;
+            static_assert(TB == 2 && NS * 32 / SLOTS >= 16 && NS % 4 == 0, "");
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int x = 0; x < NS; ++x) {
-                sn[x % TB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[x % AHEAD], qop[x / TB], sn[x % TB], 0, 0, 0);
-                if (x == NS - AHEAD) v_there();
-                if (x + AHEAD < NS) kf[x % AHEAD] = kfrag(sk, x + AHEAD);
-                else vf[x + AHEAD - NS] = vfrag(sv, x + AHEAD - NS);
-                if (x < 2 * LPT) load_x(x);
-#pragma unroll
-                for (int e = 0; e < EXP; ++e) {
-                    const int at = x * EXP + e, tb = at / 16, i = at % 16;
-                    const float p = fast_exp2(fmaf(sc[tb][i], a.scale_log2, -mref));
-                    ps[e % 2] += p;
-                    pop[tb][i / 8][i % 8] = (_Float16)p;
-                    if constexpr (SPLIT) sc[tb][i] = p;
+            for (int z = 0; z < NS + NV; ++z) {
+                if (z < NS) {
+                    sn[z % TB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fr[z % 8], qop[z / TB], sn[z % TB], 0, 0, 0);
+                } else {
+                    const int y = z - NS;
+                    half8_t v = fr[z % 8];
+                    if constexpr (SPLIT) v = finite_part(v);
+                    oacc[y % NB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pop[y / (2 * NB)][(y / NB) % 2], oacc[y % NB], 0, 0, 0);
                 }
+                __builtin_amdgcn_sched_barrier(0);
+                if (z == NS - 4) v_there();
+                if (z % 4 == 0)
+#pragma unroll
+                    for (int r = z + 4; r < z + 8 && r < NS + NV; ++r) read(r);
+                if (z < 2 * LPT) load_x(z);
+                if (z < SLOTS)
+#pragma unroll
+                    for (int at = z * 32 / SLOTS; at < (z + 1) * 32 / SLOTS; ++at) {
+                        const int tb = at / 16, i = at % 16;
+                        const float p = fast_exp2(fmaf(sc[tb][i], a.scale_log2, -mref));
+                        ps[at % 2] += p;
+                        pop[tb][i / 8][i % 8] = (_Float16)p;
+                        if constexpr (SPLIT) sc[tb][i] = p;
+                    }
                 __builtin_amdgcn_sched_barrier(0);
             }
             l_run += ps[0] + ps[1];
-#pragma unroll
-            for (int x = 0; x < NV; ++x) {
-                const int nb = x % NB;
-                half8_t v = vf[x % AHEAD];
-                if constexpr (SPLIT) v = finite_part(v);
-                oacc[nb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pop[x / (2 * NB)][(x / NB) % 2], oacc[nb], 0, 0, 0);
-                if (x + AHEAD < NV) vf[x % AHEAD] = vfrag(sv, x + AHEAD);
-                __builtin_amdgcn_sched_barrier(0);
-            }
             if constexpr (SPLIT) {
                 auto nonfinite = [&](uint32_t r, uint32_t c) -> bool { // slot c of V row r
                     const uint4_t w = *(const uint4_t*)(sv + r * HD + 8u * c);
@@ -553,6 +557,7 @@ struct PrefixTile {
                 for (uint64_t todo = __ballot(any); todo; todo &= todo - 1u) {
                     const uint32_t at = (uint32_t)__builtin_ctzll(todo);
                     const uint32_t slots = (uint32_t)__ballot(lane < CH && nonfinite(at, (uint32_t)lane % (uint32_t)CH));
+                    const bool counts = c0 + at < t1 && ((ok4 >> (at / 16u)) & 1u);
                     float p = 0.0f; // token `at`'s weight: register (at / 8 % 4) 4 + at % 4 of the half at / 4 % 2
 #pragma unroll
                     for (int tb = 0; tb < TB; ++tb)
@@ -565,7 +570,7 @@ struct PrefixTile {
 #pragma unroll
                         for (int i = 0; i < 16; i += 4) {
                             const uint32_t slot = (uint32_t)(4 * nb + i / 4) ^ vsw(at);
-                            if (!((slots >> slot) & 1u) || c0 + at >= t1 || !((ok4 >> (at / 16u)) & 1u)) continue; // uniform
+                            if (!((slots >> slot) & 1u) || !counts) continue; // uniform
                             const half4_t v = *(const half4_t*)(sv + at * HD + 8u * slot + 4 * hf);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
