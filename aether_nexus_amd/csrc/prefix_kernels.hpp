@@ -49,8 +49,8 @@ __device__ __forceinline__ half8_t prefix_query(const PrefixArgs& a, const uint1
     return as_h8(w);
 }
 
-// Few rows to a table (a sequence's own pages; a prefix that at most kPrefixFewRows rows
-// see): a work-group takes 16 query rows of one kv head x a run of pages, its 4 waves the
+// Few rows to a table (a sequence's own pages; a prefix that few rows see, or a short
+// one): a work-group takes 16 query rows of one kv head x a run of pages, its 4 waves the
 // pages in turn, each on its own until the waves' sums meet in LDS.  A page's K and V go
 // from memory straight into LDS, 256 bytes (128 dims) of a row side by side, kPageBufs
 // pages a wave.
@@ -63,7 +63,6 @@ __device__ __forceinline__ half8_t prefix_query(const PrefixArgs& a, const uint1
 // the f16 store of the output).  Staged rows are HD / 8 16-byte chunks, chunk c of K row
 // r at c ^ r, of V row r at c ^ vsw(r): no bank conflict at 128 dims.
 // Bound: HBM, the pages' bytes.
-constexpr uint32_t kPrefixFewRows = 32;
 constexpr int kPageBufs = 2;
 constexpr size_t pages_lds_bytes(int HD) {
     const size_t ring = (size_t)4 * kPageBufs * 2 * 16 * HD * 2, sums = (size_t)4 * 16 * (HD + 4) * 4 + 4 * 16 * 2 * 4;

@@ -1021,8 +1021,18 @@ void prefix_parts(uint64_t items, uint64_t want, uint32_t tokens, uint32_t longe
     *parts = cdiv(tokens, *span);
 }
 
-constexpr uint64_t kPrefixTilesPerCu = 1;
+// Up to this many tokens (prefix and own) a request runs in one part for each sequence,
+// head and 16 rows, without a merge, where its work-groups all fit the CUs at once.
+// Measured, us, in one part and in several: 64 sequences of 32 / 8 heads x 128, 200 shared
+// and up to 200 own tokens 12.2, 15.3; 16 of 300 and 200 11.2, 10.8; 1 of 600 and 100 14.0,
+// 7.3; 8 of 600 and 100 13.7, 8.2.
 constexpr uint32_t kPrefixOneTokens = 512;
+// Up to this many values of K for all 16-row tiles that read the prefix, it is read in
+// PrefixPages' parts, once for each of them, else in PrefixTile's.  Measured, us, pages
+// and tiles: 32 rows x 128 dims of 8 heads, 600 tokens 8.2, 9.2; 1000 tokens 9.7, 9.7;
+// 8192 tokens 20.8, 16.1; 64 rows, 600 tokens 14.0, 11.4; 56 rows x 64 dims of 2 heads,
+// 4000 tokens 8.3, 9.2; 112 rows, 1500 tokens 8.0, 9.0.
+constexpr uint64_t kPrefixPagesValues = 2u << 20;
 
 // Checks a request and fills its kernel arguments but for addresses of scratch.
 int prefix_plan(const aw_prefix_desc* d, uint32_t n_cu, aw::PrefixArgs* out, aw_prefix_plan_info* info, char* msg, size_t len) {
@@ -1076,7 +1086,8 @@ int prefix_plan(const aw_prefix_desc* d, uint32_t n_cu, aw::PrefixArgs* out, aw_
     a.q_and = d->scale == 0.0f ? 0u : ~0u;
     a.q_xor = d->scale < 0.0f ? 0x80008000u : 0u;
     a.scale_log2 = d->scale == 0.0f ? 1.0f : std::fabs(d->scale) * aw::kLog2e;
-    const bool tiles = rows > aw::kPrefixFewRows && d->prefix_tokens > 0;
+    const uint64_t page_tiles = cdiv(rows, 16);
+    const bool tiles = page_tiles > 1 && page_tiles * d->kv_heads * d->head_dim * d->prefix_tokens > kPrefixPagesValues;
     a.prefix_tiles = cdiv(rows, tiles ? aw::kPrefixRows : 16);
     a.own_tiles = cdiv(a.own_rows, 16);
     const uint64_t own_wgs = (uint64_t)d->batch * d->kv_heads * a.own_tiles, prefix_wgs = (uint64_t)a.prefix_tiles * d->kv_heads;
@@ -1084,8 +1095,11 @@ int prefix_plan(const aw_prefix_desc* d, uint32_t n_cu, aw::PrefixArgs* out, aw_
     const uint32_t tokens = a.prefix_tokens + a.own_max;
     const bool one = tokens == 0 || (tokens <= kPrefixOneTokens && own_wgs <= 2ull * n_cu);
     if (!one) {
-        prefix_parts(prefix_wgs, (tiles ? kPrefixTilesPerCu : 2) * n_cu, a.prefix_tokens, ~0u, 48, &a.prefix_splits, &a.prefix_span);
-        prefix_parts(own_wgs, 2ull * n_cu, a.own_max, 512, 16, &a.own_splits, &a.own_span);
+        // The prefix: one work-group a CU (tiles; 64 sequences behind 8192 tokens 28 us, two a
+        // CU 37: their sums), or two.  Own tokens: at most 512 a part, so that long sequences
+        // are no longer than the rest (96 of up to 1500 tokens beside a prefix 110 us).
+        prefix_parts(prefix_wgs, (tiles ? 1ull : 2ull) * n_cu, a.prefix_tokens, ~0u, a.own_max ? 48 : 64, &a.prefix_splits, &a.prefix_span);
+        prefix_parts(own_wgs, 2ull * n_cu, a.own_max, 512, aw::kMaxSplits - a.prefix_splits, &a.own_splits, &a.own_span);
         a.splits = a.prefix_splits + a.own_splits;
         own_units *= a.own_splits;
         if (tiles) wgs = (uint64_t)cdiv((uint64_t)d->kv_heads * a.prefix_splits, 8) * 8 * a.prefix_tiles;
