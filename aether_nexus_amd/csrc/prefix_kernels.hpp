@@ -677,7 +677,7 @@ struct PrefixTile {
             pass(std::true_type{});
             l = l_run + __shfl_xor(l_run, 32);
         }
-        if (bad && lane == 0 && wave == 0) flag_error(a.err, kErrHotRef);
+        if (wave == 0 && __any(bad) && lane == 0) flag_error(a.err, kErrHotRef);
         uint32_t ro = row;
         __asm__ volatile("" : "+v"(ro)); // its addresses are made here, not kept over the loops
         if (ro >= a.rows) return;

@@ -1117,7 +1117,7 @@ int prefix_plan(const aw_prefix_desc* d, uint32_t n_cu, aw::PrefixArgs* out, aw_
         info->prefix_tokens_per_split = a.prefix_span;
         info->own_splits = a.own_splits;
         info->own_tokens_per_split = a.own_span;
-        info->row_tile = tiles ? aw::kPrefixRows : 16;
+        info->row_tile = tiles && !one ? aw::kPrefixRows : 16;
         const uint64_t parts = (uint64_t)d->kv_heads * a.splits * a.rows;
         info->workspace_bytes = 2 * align_up(parts * 4, kAlign) + parts * d->head_dim * 4;
     }

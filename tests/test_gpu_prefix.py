@@ -38,6 +38,11 @@ def host(t):
     return t.contiguous().cpu().view(torch.int16).numpy().view(np.float16)
 
 
+def plan(c):
+    from aether_nexus_amd import ops as O
+    return O.prefix_plan(c.desc())
+
+
 class Case:
     """Inputs of one request: pages in a mixed order, stale rows (NaN, inf) wherever no token is."""
 
@@ -206,6 +211,70 @@ def test_infinities_reach_only_the_rows_that_see_them(ops, hd):
         assert np.all((np.abs(got - want) <= tol)[~bad])
 
 
+# Requests whose prefix is read by work-groups of 128 rows: parts of one step and of several, both widths, partial last pages
+TILES = [(33, 1, 8, 2, 128, 1700), (20, 2, 16, 16, 64, 1030), (9, 16, 4, 2, 64, 3500), (40, 1, 32, 32, 128, 777),
+         (70, 1, 64, 64, 64, 389), (12, 8, 24, 8, 128, 3001), (33, 1, 16, 16, 64, 2900), (40, 1, 32, 32, 128, 2000),
+         (18, 2, 32, 32, 128, 2500), (40, 1, 64, 64, 64, 1500)]
+
+
+@pytest.mark.parametrize("case", TILES, ids=["-".join(map(str, c)) for c in TILES])
+def test_many_rows_behind_a_prefix(ops, engine, case):
+    """Stale rows of the last page, keys as the values, scales of either sign, infinities and NaNs in keys and values."""
+    batch, queries, hq, hk, hd, prefix = case
+    own = [queries + b % 5 for b in range(batch)]
+    c = Case(60, *case, own)
+    p = plan(c)
+    assert p.row_tile == 128 and p.prefix_splits > 1
+    ops.shared_prefix_attention(c.desc())
+    c.check("random")
+    ops.shared_prefix_attention(c.desc(scale=-0.05))
+    c.check("a negative scale", scale=-0.05)
+    ops.shared_prefix_attention(c.desc(hot_v=None))
+    c.check("K rows as values", values=c.k)
+    # values: an inf and a NaN in the prefix, each in one dim of one head, in a full page and in the last row of all
+    at, last = c.prefix_refs[(prefix - 1) // 32] & P.REF_MASK, c.prefix_refs[(prefix - 1) // 16] & P.REF_MASK
+    values = c.v.copy()
+    values[at, 7, 0, 9], values[last, (prefix - 1) % 16, hk - 1, hd - 1] = -np.inf, np.nan
+    c.v, c.dv = values, dev(values)
+    ops.shared_prefix_attention(c.desc())
+    engine.check_device_errors()
+    got = host(c.out).astype(np.float64)
+    want, absolute = c.want(values=np.where(np.isfinite(values), values, 0).astype(np.float16))
+    bad = np.zeros(got.shape, dtype=bool)
+    g = hq // hk
+    bad[:, :, :g, 9] = bad[:, :, hq - g:, hd - 1] = True
+    assert np.array_equal(~np.isfinite(got), bad)
+    assert np.all(np.isneginf(got[:, :, :g, 9])) and np.all(np.isnan(got[:, :, hq - g:, hd - 1]))
+    tol = 2.0 ** -11 * np.abs(want) + 1.5 * 2.0 ** -11 * absolute + (prefix + 40) * 6 * 2.0 ** -25
+    assert np.all((np.abs(got - want) <= tol)[~bad])
+    k = c.k.copy()  # a NaN in a key: every row of its head
+    k[at, 7, 0, 5] = np.nan
+    c.dk = dev(k)
+    ops.shared_prefix_attention(c.desc())
+    nan = np.zeros(got.shape, dtype=bool)
+    nan[:, :, :g] = nan[:, :, hq - g:, hd - 1] = True
+    assert np.array_equal(np.isnan(host(c.out)), nan)
+
+
+def test_rising_scores_beside_many_rows(ops, engine):
+    """Scores that rise along the prefix, by steps below and above what the running maximum lets pass (2^8), up to
+    weights that span far more than f16 does."""
+    batch, hq, hk, hd, prefix = 40, 8, 2, 128, 4100
+    for slope in (0.01, 0.2, -0.2):
+        c = Case(61, batch, 1, hq, hk, hd, prefix, [2] * batch, stale=False, qscale=0.5)
+        c.q[..., 0] = 1.0
+        t = np.arange(prefix)
+        c.k[c.prefix_refs[t // 16] & P.REF_MASK, t % 16, :, 0] = (slope * t)[:, None].astype(np.float16)
+        c.dq, c.dk = dev(c.q), dev(c.k)
+        assert plan(c).row_tile == 128
+        ops.shared_prefix_attention(c.desc(scale=1.0))
+        # scores up to 820 + 12 6: fp32 sums off by 128 2^-24 900 = 0.007 in an exponent at most, 14 2^-11 in a weight
+        want, absolute = c.want(scale=1.0)
+        d = np.abs(host(c.out).astype(np.float64) - want)
+        assert np.all(d <= 2.0 ** -11 * np.abs(want) + 30 * 2.0 ** -11 * absolute + prefix * 6 * 2.0 ** -25), slope
+    engine.check_device_errors()
+
+
 def test_nan_keys_make_nan_rows(ops):
     """A NaN in a key that a row sees makes the row NaN, whichever part it lies in; other rows and heads stay."""
     for where in ("prefix", "own"):
@@ -247,6 +316,83 @@ def test_bad_refs_and_counts(ops, engine):
     ops.shared_prefix_attention(c.desc(seq_own=dev(np.array([33, 32]))))
     error("sequence length")
     c.check("count past the table")
+
+
+@pytest.mark.parametrize("page", [5, 70, 93])
+def test_bad_ref_beside_many_rows(ops, engine, page):
+    """A bad ref anywhere in a long prefix that many rows read: reported, its tokens hidden, whatever page 0 holds."""
+    from aether_nexus_amd.types import AW_E_OOB
+    from aether_nexus_amd.weaver import WeaverError
+    c = Case(33, 40, 1, 8, 2, 128, 2600, [3] * 40)
+    c.prefix_refs[page] = c.blocks + 7
+    for table in (c.prefix_refs, c.refs):  # no one's page 0: its stale rows, NaNs among them, are what a bad ref could show
+        table[(table & P.REF_MASK) == 0] = c.blocks - 1
+    c.k[0], c.v[0] = np.nan, np.inf
+    c.k[c.blocks - 1], c.v[c.blocks - 1] = 0.5, 0.25
+    c.dk, c.dv, c.drefs, c.dprefix = dev(c.k), dev(c.v), dev(c.refs), dev(c.prefix_refs)
+    assert plan(c).row_tile == 128
+    ops.shared_prefix_attention(c.desc())
+    with pytest.raises(WeaverError) as e:
+        engine.check_device_errors()
+    assert e.value.status == AW_E_OOB and "hot block ref" in str(e.value)
+    c.check(f"bad page {page}")
+
+
+# batch, queries, q heads, kv heads, head_dim, prefix, own tokens, rows to a tile, least tokens of a part of (prefix, own)
+LONG = [(20, 1, 2, 2, 64, 70001, [1] * 20, 128, (1024, 0)), (1, 2, 4, 1, 64, 300007, [2], 16, (4096, 0)),
+        (2, 2, 2, 1, 64, 3, [300003, 40], 16, (0, 4096))]
+
+
+@pytest.mark.parametrize("case", LONG, ids=["many-rows", "few-rows", "own"])
+def test_parts_of_many_pages(ops, engine, case):
+    """Parts longer than the 64 pages whose refs a wave holds at once: random scores; and equal ones, where every
+    token counts once: the output's dim d is 60000 / n for the one token t[d] that holds 60000 there (60000 and the
+    count n < 2^24 are sums that fp32 holds)."""
+    *shape, tile, (least_prefix, least_own) = case
+    c = Case(34, *shape)
+    p = plan(c)
+    assert p.row_tile == tile and p.prefix_tokens_per_split > least_prefix and p.own_tokens_per_split > least_own
+    ops.shared_prefix_attention(c.desc())
+    c.check("random scores")
+    queries, hd, prefix = shape[1], shape[4], shape[5]
+    c = Case(35, *shape, qscale=0.0, causal=False)
+    c.v[:] = 0
+    n = prefix + int(c.own[0])
+    table = np.concatenate([(c.prefix_refs & P.REF_MASK)[t // 16:t // 16 + 1] * 16 + t % 16 if t < prefix else
+                            c.refs[0, (t - prefix) // 16:(t - prefix) // 16 + 1] * 16 + (t - prefix) % 16
+                            for t in np.linspace(0, n - 1, hd).astype(int)])
+    c.v.reshape(-1, shape[3], hd)[table, :, np.arange(hd)] = 60000.0
+    c.dv = dev(c.v)
+    ops.shared_prefix_attention(c.desc())
+    engine.check_device_errors()
+    got = host(c.out).astype(np.float64)[0]
+    want = 60000.0 / n
+    assert np.all(np.abs(got - want) <= want * (2.0 ** -11 + 2.0 ** -20) + 2.0 ** -25), (got.min(), got.max(), want)
+
+
+def test_pages_past_32_bits(ops, engine):
+    """Pages whose addresses lie more than 2^32 bytes into the pool, written by append_paged and read back."""
+    import torch
+    from aether_nexus_amd import ops as O
+    hk, hd, blocks = 8, 128, 140000  # 4.6 GB
+    pool = torch.empty(blocks, 16, hk, hd, dtype=torch.float16, device="cuda:0")
+    assert pool.numel() * 2 > 2 ** 32
+    for batch, prefix in ((1, 40), (40, 900)):  # read by few rows, and by many
+        c = Case(37, batch, 1, 8, hk, hd, prefix, [5] * batch, stale=False)
+        assert plan(c).row_tile == (128 if batch > 1 else 16)
+        high = c.blocks
+        rows = torch.arange(blocks - high, blocks, device="cuda:0")
+        pool[rows] = 0
+        x = dev(c.k.reshape(-1, hk, hd))
+        ops.append_paged(O.make_append_desc(
+            batch=1, num_tokens=high * 16, q_heads=0, kv_heads=hk, head_dim=hd, k=x, v=None, hot_k=pool, hot_v=None,
+            refs=rows.to(torch.int32).view(1, -1), seq_hot=torch.tensor([high * 16], dtype=torch.int32, device="cuda:0")))
+        engine.check_device_errors()
+        assert torch.equal(pool[rows].view(torch.int16), c.dk.view(torch.int16).view(high, 16, hk, hd))
+        up = lambda t: dev(np.where((t & P.REF_MASK) == P.REF_MASK, t, (t & P.REF_MASK) + blocks - high))  # noqa: E731
+        ops.shared_prefix_attention(c.desc(hot_k=pool, hot_v=None, prefix_refs=up(c.prefix_refs), refs=up(c.refs)))
+        engine.check_device_errors()
+        c.check(f"high pages, {batch} sequences", values=c.k)
 
 
 def test_results_do_not_depend_on_the_batch_order_or_run(ops):
