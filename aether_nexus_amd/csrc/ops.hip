@@ -217,12 +217,26 @@ int launch_products(aw_engine* e, const char* what, const uint16_t* a, const Pro
     return AW_OK;
 }
 
-// Whether rows [tokens][heads * hd] at `p` share an element with those at `o`, other
-// than by being the same rows.
-bool rows_clash(const uint16_t* p, uint64_t stride, const uint16_t* o, uint64_t o_stride, uint64_t tokens, uint64_t row) {
-    if (tokens == 0 || (p == o && (stride == o_stride || tokens == 1))) return false;
-    return p < o + (tokens - 1) * o_stride + row && o < p + (tokens - 1) * stride + row;
+// Rows [tokens][row] of a call, `stride` elements apart; none at a null address.
+struct Rows {
+    const uint16_t* at;
+    uint64_t stride, row, tokens;
+    bool none() const { return !at || row == 0 || tokens == 0; }
+    uintptr_t begin() const { return (uintptr_t)at; }
+    uintptr_t end() const { return (uintptr_t)at + 2 * ((tokens - 1) * stride + row); }
+};
+
+// Whether two such sets share an element: parts of one fused buffer, rows of the same
+// stride, lie at a fixed distance within it; with strides of their own the whole
+// stretches count.
+bool rows_meet(const Rows& p, const Rows& o) {
+    if (p.none() || o.none() || p.begin() >= o.end() || o.begin() >= p.end()) return false;
+    if (p.stride != o.stride) return true;
+    const Rows &lo = p.begin() < o.begin() ? p : o, &hi = p.begin() < o.begin() ? o : p;
+    const uint64_t stride = 2 * p.stride, d = (hi.begin() - lo.begin()) % stride;
+    return d < 2 * lo.row || d + 2 * hi.row > stride;
 }
+bool rows_same(const Rows& p, const Rows& o) { return p.at == o.at && (p.stride == o.stride || p.tokens == 1); }
 
 int refuse(char* msg, size_t len, int code, const char* fmt, ...) __attribute__((format(printf, 4, 5)));
 int refuse(char* msg, size_t len, int code, const char* fmt, ...) {
@@ -236,6 +250,7 @@ int refuse(char* msg, size_t len, int code, const char* fmt, ...) {
 }
 
 constexpr uint64_t kRotaryWaves = 8; // waves per CU that a token's heads are cut for
+constexpr uint32_t kMostTokens = 1u << 24; // a call's work-groups of 256 threads stay below 2^32 threads
 constexpr uint64_t kMostStride = 1ull << 30; // elements: tokens * stride * 2 bytes stays below 2^63
 
 // The checks that the three rotary calls share, and their kernel arguments.
@@ -254,7 +269,7 @@ int rotary_args(const char* what, const aw_rotary_desc* d, bool append, awo::Rot
     if (d->rotary_dim && !std::isfinite(d->magnitude)) return bad("magnitude must be finite");
     if ((d->q_norm || d->k_norm) && !(d->eps >= 0.0f && std::isfinite(d->eps))) return bad("eps must be finite and not negative");
     if ((d->q_heads && (!d->q || !d->q_out)) || (d->kv_heads && (!d->k || (!append && !d->k_out)))) return bad("null pointer");
-    if (d->num_tokens > 0x7FFFFFFFu || d->q_heads > 0xFFFFu || d->kv_heads > 0xFFFFu)
+    if (d->num_tokens > kMostTokens || d->q_heads > 0xFFFFu || d->kv_heads > 0xFFFFu)
         return refuse(msg, len, AW_E_UNSUPPORTED, "%s: too many tokens or heads", what);
     awo::RotaryArgs& a = *out;
     a = awo::RotaryArgs{};
@@ -267,9 +282,11 @@ int rotary_args(const char* what, const aw_rotary_desc* d, bool append, awo::Rot
         return bad("a stride is shorter than a token's heads");
     if (std::max(std::max(a.q_stride, a.q_out_stride), std::max(a.k_stride, a.k_out_stride)) > kMostStride)
         return refuse(msg, len, AW_E_UNSUPPORTED, "%s: a stride exceeds 2^30 elements", what);
-    if ((d->q_heads && rows_clash(d->q, a.q_stride, d->q_out, a.q_out_stride, d->num_tokens, q_row)) ||
-        (d->kv_heads && !append && rows_clash(d->k, a.k_stride, d->k_out, a.k_out_stride, d->num_tokens, k_row)))
+    const Rows q{d->q, a.q_stride, q_row, d->num_tokens}, q_out{d->q_out, a.q_out_stride, q_row, d->num_tokens};
+    const Rows k{d->k, a.k_stride, k_row, d->num_tokens}, k_out{append ? nullptr : d->k_out, a.k_out_stride, k_row, d->num_tokens};
+    if ((!rows_same(q, q_out) && rows_meet(q, q_out)) || (!rows_same(k, k_out) && rows_meet(k, k_out)))
         return bad("the output overlaps its input, and is not the input itself");
+    if (rows_meet(q, k_out) || rows_meet(k, q_out) || rows_meet(q_out, k_out)) return bad("rows of q and k overlap, and one is an output");
     a.q = d->q;
     a.k = d->k;
     a.q_out = d->q_out;
@@ -322,6 +339,14 @@ int append_args(const aw_append_desc* d, awo::RotaryArgs* a, char* msg, size_t l
     a->v_stride = d->v_stride ? d->v_stride : row;
     if (a->v_stride < row) return bad("a stride is shorter than a token's heads");
     if (a->v_stride > kMostStride) return refuse(msg, len, AW_E_UNSUPPORTED, "append_paged: a stride exceeds 2^30 elements");
+    const uint64_t pool = d->hot_blocks * awo::kPageTokens * row, n = d->rows.num_tokens;
+    const Rows hot[2] = {{d->hot_k, pool, pool, 1}, {d->hot_v, pool, pool, 1}}, v{d->v, a->v_stride, row, n};
+    const Rows q{d->rows.q, a->q_stride, (uint64_t)a->q_heads * a->hd, n}, q_out{d->rows.q_out, a->q_out_stride, q.row, n};
+    const Rows k{d->rows.k, a->k_stride, row, n};
+    if (rows_meet(q_out, v)) return bad("rows of q_out and v overlap");
+    for (const Rows& h : hot)
+        if (rows_meet(h, q) || rows_meet(h, q_out) || rows_meet(h, k) || rows_meet(h, v)) return bad("a pool overlaps the rows");
+    if (rows_meet(hot[0], hot[1])) return bad("hot_k and hot_v overlap");
     a->v = d->v;
     a->k_out = d->hot_k;
     a->v_out = d->hot_v;
@@ -349,9 +374,7 @@ int launch_rotary(aw_engine* e, awo::RotaryArgs& a, hipStream_t st) {
     const uint64_t steps = cdiv64(heads, 64u >> a.lanes_log);
     // Few tokens: a token's heads over several waves.
     a.slices = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(steps, cdiv64(kRotaryWaves * (uint64_t)ei::compute_units(e), a.tokens)));
-    const uint64_t groups = cdiv64((uint64_t)a.tokens * a.slices, 4);
-    if (groups > 0x20000000ull) return ei::fail(e, AW_E_UNSUPPORTED, "rotary: grid too large");
-    const dim3 grid((uint32_t)groups), block(256);
+    const dim3 grid((uint32_t)cdiv64((uint64_t)a.tokens * a.slices, 4)), block(256);
     const bool norm = a.q_norm || a.k_norm;
     if (norm && a.interleaved) hipLaunchKernelGGL((awo::rotary_rows_kernel<APPEND, true, true>), grid, block, 0, st, a);
     else if (norm) hipLaunchKernelGGL((awo::rotary_rows_kernel<APPEND, true, false>), grid, block, 0, st, a);

@@ -129,7 +129,7 @@ template <bool APPEND, bool NORM, bool INTER>
 __global__ __launch_bounds__(256) void rotary_rows_kernel(RotaryArgs a) {
     __shared__ float2 s_turns[4][kRotaryMaxDim / 2];
     const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const uint32_t id = blockIdx.x * 4u + wave; // below 2^31 + 4
+    const uint32_t id = blockIdx.x * 4u + wave; // below 2^26
     const uint32_t t = (uint32_t)__builtin_amdgcn_readfirstlane((int)(id / a.slices)), slice = id - t * a.slices;
     if (t >= a.tokens) return; // no barrier follows
     const uint32_t n = a.rotary_dim, half = n / 2, hd = a.hd;

@@ -1046,11 +1046,11 @@ int prefix_plan(const aw_prefix_desc* d, uint32_t n_cu, aw::PrefixArgs* out, aw_
         return refuse(AW_E_INVALID_ARG, "q_heads must be a positive multiple of kv_heads");
     if (!supported_head_dim(d->head_dim)) return refuse(AW_E_UNSUPPORTED, "head_dim must be 64 or 128");
     if (d->flags & ~AW_F_CAUSAL) return refuse(AW_E_INVALID_ARG, "unknown flags");
-    if (!std::isfinite(d->scale)) return refuse(AW_E_INVALID_ARG, "scale must be finite");
+    if (!std::isfinite(d->scale * aw::kLog2e)) return refuse(AW_E_INVALID_ARG, "scale must be finite, and times log2 e too");
     if (d->refs_stride < d->own_count) return refuse(AW_E_INVALID_ARG, "refs_stride is less than own_count");
     const uint64_t gqa = d->q_heads / d->kv_heads, rows = (uint64_t)d->batch * d->queries * gqa;
     if (d->prefix_tokens > 1u << 26 || d->own_count > 1u << 18) return refuse(AW_E_UNSUPPORTED, "too many tokens");
-    if (rows > 1u << 26 || (uint64_t)d->batch * d->queries > 1u << 26 || gqa > 1u << 16 || rows * d->kv_heads > 1u << 28)
+    if (rows > 1u << 26 || (uint64_t)d->batch * d->queries > 1u << 26 || gqa > 1u << 16 || rows * d->kv_heads > 1u << 25)
         return refuse(AW_E_UNSUPPORTED, "too many query rows");
     if ((uint64_t)d->kv_heads * d->head_dim > 1u << 16) return refuse(AW_E_UNSUPPORTED, "too many kv heads");
     if (!d->q || !d->out) return refuse(AW_E_INVALID_ARG, "q and out are required");
@@ -1062,6 +1062,8 @@ int prefix_plan(const aw_prefix_desc* d, uint32_t n_cu, aw::PrefixArgs* out, aw_
     if (((uintptr_t)d->q | (uintptr_t)d->hot_k | (uintptr_t)d->hot_v) & 15u)
         return refuse(AW_E_ALIGN, "q, hot_k and hot_v must be 16-byte aligned");
     if ((uintptr_t)d->out & 7u) return refuse(AW_E_ALIGN, "out must be 8-byte aligned");
+    const uintptr_t q = (uintptr_t)d->q, o = (uintptr_t)d->out, bytes = rows * d->kv_heads * d->head_dim * 2;
+    if (q != o && q < o + bytes && o < q + bytes) return refuse(AW_E_INVALID_ARG, "out overlaps q, and is not q");
     aw::PrefixArgs& a = *out;
     a = aw::PrefixArgs{};
     a.q = d->q;
@@ -1106,7 +1108,7 @@ int prefix_plan(const aw_prefix_desc* d, uint32_t n_cu, aw::PrefixArgs* out, aw_
         else prefix_units = (uint64_t)a.prefix_tiles * a.prefix_splits;
     }
     const uint64_t unit_wgs = (uint64_t)cdiv(prefix_units + own_units, 8) * 8 * d->kv_heads;
-    if (wgs + unit_wgs > 0x7FFFFFFFull) return refuse(AW_E_UNSUPPORTED, "grid too large");
+    if (wgs + unit_wgs > 0xFFFFFFull) return refuse(AW_E_UNSUPPORTED, "too many query rows"); // 256 threads each, below 2^32
     a.prefix_wgs = (uint32_t)wgs;
     a.prefix_units = (uint32_t)prefix_units;
     a.own_units = (uint32_t)own_units;

@@ -65,6 +65,13 @@ _u32 = _checker("int32")
 _f64 = _checker("float64")
 
 
+def _counts(**values) -> None:
+    """Numbers that a descriptor holds in 32 unsigned bits."""
+    for name, v in values.items():
+        if not 0 <= v < 2 ** 32:
+            raise WeaverError(f"{name} {v} is not within [0, 2^32)", AW_E_INVALID_ARG)
+
+
 def _token_rows(t, tokens: int, heads: int, head_dim: int, what: str) -> int:
     """Token stride (elements) of rows [tokens][heads][head_dim]: a contiguous tensor, a
     raw pointer to one, or a view with contiguous heads whose rows lie further apart
@@ -135,6 +142,7 @@ class Rotary:
 def _rotary_rows(r: RotaryDesc, *, num_tokens, q_heads, kv_heads, head_dim, rotary, q, k, q_out, k_out, positions,
                  start_position, q_norm, k_norm, eps) -> list:
     """Fills the descriptor of the rows; returns the tensors behind it."""
+    _counts(num_tokens=num_tokens, q_heads=q_heads, kv_heads=kv_heads, head_dim=head_dim, start_position=start_position)
     r.num_tokens, r.q_heads, r.kv_heads, r.head_dim = num_tokens, q_heads, kv_heads, head_dim
     r.start_position, r.eps, r.magnitude = start_position, eps, 1.0
     for t, heads, name in ((q, q_heads, "q"), (k, kv_heads, "k"), (q_out, q_heads, "q_out"), (k_out, kv_heads, "k_out")):
@@ -205,6 +213,7 @@ def make_append_desc(*, batch: int, num_tokens: int, q_heads: int, kv_heads: int
         if not hasattr(hot_k, "numel"):
             raise WeaverError("append_paged: hot_blocks is required for a raw pool pointer", AW_E_INVALID_ARG)
         hot_blocks = hot_k.numel() // max(page, 1)
+    _counts(batch=batch, hot_count=hot_count, hot_blocks=hot_blocks, refs_stride=refs_stride or 0)
     for t, name in ((hot_k, "hot_k"), (hot_v, "hot_v")):
         _f16(t, hot_blocks * page, name)
         setattr(d, name, _ptr(t))
@@ -225,9 +234,11 @@ def make_prefix_desc(*, batch: int, queries: int, q_heads: int, kv_heads: int, h
     """An ``aw_prefix_desc`` from device tensors (or raw device pointers), for
     ``shared_prefix_attention``: q and out [batch][queries][q_heads][head_dim], the prefix'
     pages in ``prefix_refs``, each sequence's own in its row of ``refs`` and their number of
-    tokens in ``seq_own``.  ``scale`` defaults to 1 / sqrt(head_dim), ``hot_blocks`` to the
+    tokens in ``seq_own`` (``out`` may be q).  ``scale`` defaults to 1 / sqrt(head_dim), ``hot_blocks`` to the
     pool tensor's pages."""
     d = PrefixDesc()
+    _counts(batch=batch, queries=queries, q_heads=q_heads, kv_heads=kv_heads, head_dim=head_dim, prefix_tokens=prefix_tokens,
+            own_count=own_count, refs_stride=refs_stride or 0, hot_blocks=hot_blocks or 0)
     d.batch, d.queries, d.q_heads, d.kv_heads, d.head_dim = batch, queries, q_heads, kv_heads, head_dim
     d.prefix_tokens, d.own_count, d.flags = prefix_tokens, own_count, AW_F_CAUSAL if causal else 0
     d.scale = head_dim ** -0.5 if scale is None else scale

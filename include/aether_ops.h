@@ -161,7 +161,7 @@ int aw_rotary_frequencies(const aw_rotary_scaling* scaling, double* inv_freq);
  * head_dim; the heads of a token are contiguous.  Rows of any alignment are taken.
  * Rows, frequencies, positions and weights are device memory. */
 typedef struct aw_rotary_desc {
-    uint32_t num_tokens, q_heads, kv_heads, head_dim; /* head_dim <= 1024; either head count may be 0 */
+    uint32_t num_tokens, q_heads, kv_heads, head_dim; /* <= 2^24 tokens; head_dim <= 1024; either head count may be 0 */
     uint32_t rotary_dim;            /* even, <= head_dim: dims [0, rotary_dim) turn, the others pass */
     uint32_t layout;                /* AW_ROTARY_HALF or AW_ROTARY_INTERLEAVED */
     uint32_t start_position;        /* of token 0, where positions is NULL */
@@ -171,7 +171,7 @@ typedef struct aw_rotary_desc {
     uint64_t q_stride, k_stride, q_out_stride, k_out_stride;
     const uint16_t* q;              /* [num_tokens][q_heads][head_dim] */
     const uint16_t* k;              /* [num_tokens][kv_heads][head_dim] */
-    uint16_t*       q_out;          /* may be q (same stride: in place); no other overlap with an input */
+    uint16_t*       q_out;          /* may be q (same stride: in place); shares no element with other rows */
     uint16_t*       k_out;          /* likewise k; NULL in an append */
     const uint16_t* q_norm;         /* [head_dim] weights */
     const uint16_t* k_norm;
@@ -204,7 +204,8 @@ int aw_ops_qk_norm_rotary(aw_engine* engine, const aw_rotary_desc* desc, void* h
  * sets the device error "hot block ref": that token's k and v are not written.  A
  * sequence with more new tokens than seq_hot, or offsets that descend, set "sequence
  * length": nothing of those tokens is written (aw_engine_check_device_errors).  Two
- * tokens must not share a row of the pools: which is kept is then undefined. */
+ * tokens must not share a row of the pools: which is kept is then undefined.  The pools
+ * overlap neither each other nor the rows. */
 typedef struct aw_append_desc {
     aw_rotary_desc rows;            /* k_out NULL; q may be absent (q_heads 0) */
     uint32_t batch, hot_count, refs_stride, reserved;

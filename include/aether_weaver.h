@@ -317,7 +317,7 @@ int aw_multihead_attention_device(aw_engine* engine, const uint16_t* q, const ui
  * batch instead of once for each sequence (aw_decode_device with the prefix'
  * refs in every row of its table), each sequence's own pages beside them, and
  * the parts are joined by their log-sum-exp.  Device pointers, f16:
- *   q, out       [batch][queries][q_heads][head_dim]; q 16-byte, out 8-byte aligned
+ *   q, out       [batch][queries][q_heads][head_dim]; q 16-byte, out 8-byte aligned; out may be q
  *   hot_k, hot_v [hot_blocks][16][kv_heads][head_dim], 16-byte aligned; hot_v NULL: V is the K row
  *   prefix_refs  [ceil(prefix_tokens / 16)]: the prefix may end inside its last page, whose other rows are not used
  *   refs         [batch][refs_stride]: the pages of a sequence's tokens behind the prefix, which begin a page of their own
@@ -328,7 +328,8 @@ int aw_multihead_attention_device(aw_engine* engine, const uint16_t* q, const ui
  * device error "hot block ref", a seq_own over own_count * 16 is taken as that and
  * sets "sequence length" (aw_engine_check_device_errors).  Values of tokens that a
  * row does not see never reach it, infinities and NaNs neither.
- * Any number of queries; head_dim 64 or 128; up to 2^26 prefix and 2^22 own tokens.
+ * Any number of queries; head_dim 64 or 128; up to 2^25 rows of q, 2^26 prefix and
+ * 2^22 own tokens.
  * Scratch is the engine's workspace, as in aw_decode_device, also under capture. */
 typedef struct aw_prefix_desc {
     uint32_t batch, queries;

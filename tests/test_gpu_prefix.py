@@ -140,6 +140,15 @@ def test_own_pages_only_and_prefix_only(ops, engine):
     engine.check_device_errors()
 
 
+@pytest.mark.parametrize("case", [(3, 2, 8, 2, 128, 100, [5, 40, 17]), (40, 1, 8, 2, 64, 5000, [3] * 40)], ids=["small", "tiles"])
+def test_output_in_place_of_the_queries(ops, case):
+    c = Case(12, *case)
+    out = c.dq.clone()
+    ops.shared_prefix_attention(c.desc(q=out, out=out))
+    c.out = out
+    c.check("in place")
+
+
 def test_keys_that_are_the_values(ops):
     c = Case(5, 3, 1, 8, 2, 128, 100, [5, 40, 17])
     ops.shared_prefix_attention(c.desc(hot_v=None))

@@ -13,7 +13,7 @@ from aether_nexus_amd.types import (AW_E_ALIGN, AW_E_INVALID_ARG, AW_E_UNSUPPORT
                                     PrefixPlanInfo)
 from aether_nexus_amd.weaver import WeaverError
 
-A = {n: 0x100000 * (i + 1) for i, n in enumerate(("q", "out", "hot_k", "hot_v", "prefix_refs", "refs", "seq_own"))}
+A = {n: (i + 1) << 36 for i, n in enumerate(("q", "out", "hot_k", "hot_v", "prefix_refs", "refs", "seq_own"))}
 
 
 def desc(**kw):
@@ -33,7 +33,8 @@ def test_struct_sizes_match():
 @pytest.mark.parametrize("kw", [dict(), dict(hot_v=0), dict(seq_own=0), dict(prefix_tokens=0, prefix_refs=0),
                                 dict(own_count=0, refs=0, refs_stride=0), dict(flags=0), dict(head_dim=64), dict(queries=500),
                                 dict(prefix_tokens=0, own_count=0, hot_k=0, hot_v=0, hot_blocks=0), dict(q_heads=2 * 70),
-                                dict(prefix_tokens=1 << 26, own_count=1 << 18, refs_stride=1 << 18), dict(hot_blocks=1 << 31)])
+                                dict(prefix_tokens=1 << 26, own_count=1 << 18, refs_stride=1 << 18), dict(hot_blocks=1 << 31),
+                                dict(out=A["q"]), dict(scale=2e38)])
 def test_accepted_requests_are_covered_by_their_parts(kw):
     d = desc(**kw)
     for cus in (0, 1, 64, 304):
@@ -54,7 +55,7 @@ def test_accepted_requests_are_covered_by_their_parts(kw):
 @pytest.mark.parametrize("kw", [dict(batch=0), dict(queries=0), dict(kv_heads=0), dict(q_heads=7), dict(q_heads=0), dict(flags=2),
                                 dict(flags=AW_F_CAUSAL | 8), dict(scale=math.inf), dict(scale=math.nan), dict(refs_stride=2),
                                 dict(q=0), dict(out=0), dict(prefix_refs=0), dict(refs=0), dict(hot_k=0), dict(hot_blocks=0),
-                                dict(hot_blocks=(1 << 31) + 1)])
+                                dict(hot_blocks=(1 << 31) + 1), dict(scale=3e38), dict(out=A["q"] + 16), dict(q=A["out"] + 16)])
 def test_invalid(kw):
     with pytest.raises(WeaverError) as e:
         O.prefix_plan(desc(**kw))
@@ -63,7 +64,8 @@ def test_invalid(kw):
 
 @pytest.mark.parametrize("kw", [dict(head_dim=96), dict(head_dim=256), dict(prefix_tokens=(1 << 26) + 1),
                                 dict(own_count=(1 << 18) + 1, refs_stride=1 << 19), dict(kv_heads=1024, q_heads=1024),
-                                dict(batch=1 << 20, queries=1 << 10), dict(batch=1 << 26, queries=1 << 26)])
+                                dict(batch=1 << 20, queries=1 << 10), dict(batch=1 << 26, queries=1 << 26),
+                                dict(batch=1 << 23, queries=1)])
 def test_unsupported(kw):
     with pytest.raises(WeaverError) as e:
         O.prefix_plan(desc(**kw))
@@ -91,3 +93,12 @@ def test_descriptors_take_gpu_tensors_only():
         O.make_prefix_desc(batch=4, queries=2, q_heads=8, kv_heads=2, head_dim=128, prefix_tokens=0, q=A["q"], out=A["out"],
                            hot_k=A["hot_k"])
     assert "hot_blocks" in str(e.value)
+
+
+@pytest.mark.parametrize("kw", [dict(batch=-1), dict(queries=-1), dict(prefix_tokens=-1), dict(own_count=1 << 32), dict(hot_blocks=-1)])
+def test_numbers_that_do_not_fit_are_refused(kw):
+    base = dict(batch=1, queries=1, q_heads=8, kv_heads=2, head_dim=128, prefix_tokens=16, q=A["q"], out=A["out"],
+                hot_k=A["hot_k"], hot_blocks=4, prefix_refs=A["hot_v"])
+    with pytest.raises(WeaverError) as e:
+        O.make_prefix_desc(**{**base, **kw})
+    assert e.value.status == AW_E_INVALID_ARG and "within" in str(e.value)

@@ -111,14 +111,27 @@ def test_rows_accepted():
     (dict(k_out_stride=1), "stride"), (dict(q_norm=A["w"]), "norm"), (dict(k_norm=A["w"]), "norm"),
     (dict(q_out=A["q"] + 2), "overlaps"), (dict(q_out=A["q"], q_stride=512), "overlaps"),
     (dict(k_out=A["k"] + 2 * (4 * 128 + 127)), "overlaps"), (dict(k=A["k"] + 2 * 639, k_out=A["k"]), "overlaps"),
+    (dict(k_out=A["q"] + 2 * 500), "overlap"), (dict(q_out=A["k"] + 2 * 100), "overlap"), (dict(k_out=A["q_out"]), "overlap"),
+    (dict(q=A["q"], k=A["q"] + 2 * 255, q_out=A["q"], k_out=A["k_out"], q_stride=500, k_stride=500, q_out_stride=500), "overlap"),
 ])
 def test_rows_refused(kw, word):
     rc, msg = check_rows(rows(**kw))
     assert rc == AW_E_INVALID_ARG and word in msg, msg
 
 
+def test_parts_of_one_buffer_are_accepted():
+    """q, k and both outputs side by side in rows of one buffer: no element twice."""
+    part = dict(q=A["q"], k=A["q"] + 2 * 256, q_out=A["q"] + 2 * 384, k_out=A["q"] + 2 * 640,
+                q_stride=768, k_stride=768, q_out_stride=768, k_out_stride=768)
+    assert check_rows(rows(**part))[0] == 0, check_rows(rows(**part))
+    assert check_rows(rows(**{**part, "q_out": part["q"], "k_out": part["k"]}))[0] == 0  # in place
+    assert check_rows(rows(**{**part, "q_out": part["q_out"] + 2 * 768}))[0] == 0  # a row further
+    for n, by in (("q_out", -2), ("k_out", -2), ("k_out", 2), ("k_out", 2 * 768 - 2), ("k_out", 2 * 768 + 2)):
+        assert check_rows(rows(**{**part, n: part[n] + by}))[0] == AW_E_INVALID_ARG, (n, by)
+
+
 def test_rows_unsupported():
-    for kw in (dict(head_dim=1026), dict(num_tokens=1 << 31), dict(q_heads=1 << 16), dict(q_stride=(1 << 30) + 1)):
+    for kw in (dict(head_dim=1026), dict(num_tokens=1 << 31), dict(num_tokens=(1 << 24) + 1), dict(q_heads=1 << 16), dict(q_stride=(1 << 30) + 1)):
         assert check_rows(rows(**kw))[0] == AW_E_UNSUPPORTED, kw
     assert check_rows(None)[0] == AW_E_INVALID_ARG
 
@@ -146,7 +159,7 @@ def check_append(d):
 def test_append_accepted():
     for d in (append(), append(dict(rotary_dim=0, inv_freq=0)), append(dict(q_heads=0, q=0, q_out=0)),
               append(v=0, hot_v=0), append(dict(num_tokens=6), token_offsets=0), append(batch=0),
-              append(dict(k_norm=A["w"])), append(hot_blocks=1 << 31)):
+              append(dict(k_norm=A["w"])), append(hot_blocks=1 << 31, hot_v=1 << 50)):
         assert check_append(d)[0] == 0, check_append(d)
 
 
@@ -156,6 +169,9 @@ def test_append_accepted():
     ({}, dict(refs=0), "null"), ({}, dict(seq_hot=0), "null"), ({}, dict(hot_blocks=0), "hot_blocks"),
     ({}, dict(hot_blocks=(1 << 31) + 1), "hot_blocks"), ({}, dict(hot_count=0), "hot_count"),
     ({}, dict(refs_stride=2), "refs_stride"), ({}, dict(token_offsets=0), "token_offsets"), ({}, dict(v_stride=127), "stride"),
+    ({}, dict(hot_v=A["hot_k"]), "overlap"), ({}, dict(hot_v=A["hot_k"] + 7 * 16 * 128 * 2 - 2), "overlap"),
+    ({}, dict(hot_k=A["k"] - 2), "overlaps"), ({}, dict(hot_v=A["v"] + 2 * 639), "overlaps"), ({}, dict(hot_k=A["q_out"] - 64), "overlaps"),
+    (dict(q_out=A["v"]), {}, "overlap"),
 ])
 def test_append_refused(rows_kw, kw, word):
     rc, msg = check_append(append(rows_kw, **kw))
@@ -183,3 +199,13 @@ def test_descriptors_take_gpu_tensors_only():
     d = O.make_append_desc(batch=1, num_tokens=5, q_heads=0, kv_heads=2, head_dim=64, k=A["k"], v=A["v"], hot_k=A["hot_k"],
                            hot_v=A["hot_v"], hot_blocks=4, hot_count=1, refs=A["refs"], seq_hot=A["seq"])
     assert check_append(d)[0] == 0
+
+
+@pytest.mark.parametrize("kw", [dict(batch=-1), dict(num_tokens=-5), dict(q_heads=-1), dict(start_position=-1),
+                                dict(start_position=1 << 32), dict(hot_count=-1), dict(hot_blocks=-1), dict(refs_stride=-4)])
+def test_numbers_that_do_not_fit_are_refused(kw):
+    base = dict(batch=1, num_tokens=5, q_heads=0, kv_heads=2, head_dim=64, k=A["k"], v=A["v"], hot_k=A["hot_k"], hot_v=A["hot_v"],
+                hot_blocks=4, hot_count=1, refs=A["refs"], seq_hot=A["seq"], token_offsets=A["off"], q=A["q"])
+    with pytest.raises(WeaverError) as e:
+        O.make_append_desc(**{**base, **kw})
+    assert e.value.status == AW_E_INVALID_ARG and "within" in str(e.value)
