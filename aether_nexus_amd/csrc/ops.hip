@@ -304,6 +304,7 @@ int rotary_args(const char* what, const aw_rotary_desc* d, bool append, awo::Rot
     a.start = d->start_position;
     a.magnitude = d->magnitude;
     a.eps = d->eps;
+    a.inv_hd = 1.0f / (float)d->head_dim;
     return AW_OK;
 }
 

@@ -26,7 +26,7 @@ struct RotaryArgs {
     const uint32_t* positions;    // [tokens], or null: start + (append: the token's place in its sequence, else its index)
     const double* inv_freq;       // [rotary_dim / 2] radians per position
     uint32_t tokens, q_heads, kv_heads, hd, rotary_dim, interleaved, start;
-    float magnitude, eps;
+    float magnitude, eps, inv_hd; // inv_hd = 1 / hd
     // append
     uint32_t batch, hot_count, refs_stride;
     uint64_t hot_blocks;
@@ -91,6 +91,13 @@ __device__ inline float2 turn_of(const RotaryArgs& a, uint32_t p, uint32_t posit
 // 16 bytes at an element's alignment: one access on gfx950.
 typedef uint32_t uint4_el_t __attribute__((ext_vector_type(4), aligned(2)));
 
+// Two values rounded to f16, the first in the low half.
+__device__ inline uint32_t f2h_pair(float x, float y) {
+    typedef float float2_v __attribute__((ext_vector_type(2)));
+    typedef _Float16 half2_v __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2_v){x, y}, half2_v));
+}
+
 // Sum over the 2^log lanes of a head, in each of them: quad permutes and row mirrors up
 // to 16 lanes (a mirror meets a lane of the other half, whose lanes hold equal sums).
 __device__ inline float lanes_sum(float x, uint32_t log) {
@@ -116,8 +123,6 @@ __device__ inline float lanes_sum(float x, uint32_t log) {
 // waves, each a token or a slice of its heads, none waiting for another: a wave works its
 // token's cosines and sines out once, a pair a lane, into LDS of its own, while its
 // first kStep steps of rows are on the way.
-constexpr int kRotaryStep = 2;
-
 __host__ __device__ inline bool rotary_rows_take(uint32_t hd, uint32_t n) {
     return (n == 0 || n >= 16) && (hd == n || hd - n >= 8);
 }
@@ -127,6 +132,10 @@ __host__ __device__ inline uint32_t rotary_pass_lanes(uint32_t hd, uint32_t n) {
 
 template <bool APPEND, bool NORM, bool INTER>
 __global__ __launch_bounds__(256) void rotary_rows_kernel(RotaryArgs a) {
+    // Steps whose rows are loaded together.  Measured, us, 1 and 2, heads of 128 dims: 6000
+    // tokens of 12 / 2 heads with norms 9.6, 10.9; 12288 tokens of 32 / 8 heads appended with
+    // norms 36.7, 35.1; 8192 of them turned alone 34.6, 34.1; 3, 4 and 6 no better.
+    constexpr int kStep = NORM && !APPEND ? 1 : 2;
     __shared__ float2 s_turns[4][kRotaryMaxDim / 2];
     const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t id = blockIdx.x * 4u + wave; // below 2^26
@@ -151,14 +160,15 @@ __global__ __launch_bounds__(256) void rotary_rows_kernel(RotaryArgs a) {
         skip0 = d - at0;
         skip1 = d + 8u - at1;
     }
+    const bool whole = n % 16u == 0u && (hd - n) % 16u == 0u; // no value is held twice
     const uint32_t heads = a.q_heads + a.kv_heads + (APPEND && a.v_out ? a.kv_heads : 0u);
     const uint32_t steps = (heads + per - 1u) / per;
     const uint32_t s1 = (uint32_t)((uint64_t)steps * (slice + 1u) / a.slices);
     uint32_t s = (uint32_t)((uint64_t)steps * slice / a.slices);
-    uint4_el_t x0[kRotaryStep], x1[kRotaryStep];
+    uint4_el_t x0[kStep] = {}, x1[kStep] = {}; // zeros where a lane has no dims
     auto load = [&] {
 #pragma unroll
-        for (int j = 0; j < kRotaryStep; ++j) {
+        for (int j = 0; j < kStep; ++j) {
             const uint32_t h = (s + (uint32_t)j) * per + slot;
             if (s + (uint32_t)j >= s1 || h >= heads || !used) continue;
             const bool is_q = h < a.q_heads, is_v = APPEND && h >= a.q_heads + a.kv_heads;
@@ -201,7 +211,7 @@ __global__ __launch_bounds__(256) void rotary_rows_kernel(RotaryArgs a) {
     auto half_of = [](const uint4_el_t& v, int e) { return (uint16_t)(v[e / 2] >> (16 * (e % 2))); };
     for (;;) {
 #pragma unroll
-        for (int j = 0; j < kRotaryStep; ++j) {
+        for (int j = 0; j < kStep; ++j) {
             if (s + (uint32_t)j >= s1) break; // wave-uniform
             const uint32_t h = (s + (uint32_t)j) * per + slot;
             const bool is_q = h < a.q_heads, is_v = APPEND && h >= a.q_heads + a.kv_heads;
@@ -213,14 +223,19 @@ __global__ __launch_bounds__(256) void rotary_rows_kernel(RotaryArgs a) {
             }
             if constexpr (NORM) {
                 float sum = 0.0f;
+                if (whole) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    sum += used && (uint32_t)e >= skip0 ? f0[e] * f0[e] : 0.0f;
-                    sum += used && (uint32_t)e >= skip1 ? f1[e] * f1[e] : 0.0f;
+                    for (int e = 0; e < 8; ++e) sum = fmaf(f1[e], f1[e], fmaf(f0[e], f0[e], sum));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        sum = (uint32_t)e >= skip0 ? fmaf(f0[e], f0[e], sum) : sum;
+                        sum = (uint32_t)e >= skip1 ? fmaf(f1[e], f1[e], sum) : sum;
+                    }
                 }
                 sum = lanes_sum(sum, a.lanes_log);
                 if (is_q ? a.q_norm != nullptr : a.k_norm != nullptr) {
-                    const float inv = 1.0f / sqrtf(sum / (float)hd + a.eps);
+                    const float inv = rsqrtf(fmaf(sum, a.inv_hd, a.eps));
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         f0[e] = f0[e] * inv * h2f(half_of(is_q ? w0[0] : w0[1], e));
@@ -249,11 +264,11 @@ __global__ __launch_bounds__(256) void rotary_rows_kernel(RotaryArgs a) {
                         float(&f)[8] = e < 4 ? f0 : f1;
                         float(&g)[8] = e < 4 ? g0 : g1;
                         const int i = 2 * (e % 4);
-                        g[i] = f[i] * c[e] - f[i + 1] * sn[e];
-                        g[i + 1] = f[i] * sn[e] + f[i + 1] * c[e];
+                        g[i] = fmaf(f[i], c[e], -(f[i + 1] * sn[e]));
+                        g[i + 1] = fmaf(f[i], sn[e], f[i + 1] * c[e]);
                     } else {
-                        g0[e] = f0[e] * c[e] - f1[e] * sn[e];
-                        g1[e] = f0[e] * sn[e] + f1[e] * c[e];
+                        g0[e] = fmaf(f0[e], c[e], -(f1[e] * sn[e]));
+                        g1[e] = fmaf(f0[e], sn[e], f1[e] * c[e]);
                     }
                 }
 #pragma unroll
@@ -265,14 +280,14 @@ __global__ __launch_bounds__(256) void rotary_rows_kernel(RotaryArgs a) {
             if (turn || (NORM && !is_v && (is_q ? a.q_norm != nullptr : a.k_norm != nullptr))) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    r0[i] = (uint32_t)f2h(f0[2 * i]) | ((uint32_t)f2h(f0[2 * i + 1]) << 16);
-                    r1[i] = (uint32_t)f2h(f1[2 * i]) | ((uint32_t)f2h(f1[2 * i + 1]) << 16);
+                    r0[i] = f2h_pair(f0[2 * i], f0[2 * i + 1]);
+                    r1[i] = f2h_pair(f1[2 * i], f1[2 * i + 1]);
                 }
             }
             *(uint4_el_t*)(y + at0) = r0;
             *(uint4_el_t*)(y + at1) = r1;
         }
-        s += (uint32_t)kRotaryStep;
+        s += (uint32_t)kStep;
         if (s >= s1) return;
         load();
     }
@@ -316,15 +331,15 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
             float sum = 0.0f;
             for (uint32_t d = lane; d < a.hd; d += 64u) sum += h2f(x[d]) * h2f(x[d]);
             for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-            inv = 1.0f / sqrtf(sum / (float)a.hd + a.eps);
+            inv = rsqrtf(fmaf(sum, a.inv_hd, a.eps));
         }
         auto value = [&](uint32_t d) { return w ? h2f(x[d]) * inv * h2f(w[d]) : h2f(x[d]); };
         for (uint32_t p = lane; p < half; p += 64u) {
             const uint32_t d0 = a.interleaved ? 2u * p : p, d1 = a.interleaved ? 2u * p + 1u : p + half;
             const float x0 = value(d0), x1 = value(d1);
             const float2 cs = s_turn[p];
-            y[d0] = f2h(x0 * cs.x - x1 * cs.y);
-            y[d1] = f2h(x0 * cs.y + x1 * cs.x);
+            y[d0] = f2h(fmaf(x0, cs.x, -(x1 * cs.y)));
+            y[d1] = f2h(fmaf(x0, cs.y, x1 * cs.x));
         }
         for (uint32_t d = a.rotary_dim + lane; d < a.hd; d += 64u) y[d] = w ? f2h(value(d)) : x[d];
     }

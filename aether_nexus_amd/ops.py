@@ -12,6 +12,7 @@ anything is enqueued (the C ABI takes raw pointers).
 from __future__ import annotations
 
 import ctypes
+import sys
 from typing import Optional
 
 import numpy as np
@@ -438,9 +439,15 @@ class OpsEngine:
     # -- rotary positions, head norms, paged appends (no reference counterpart): a call's descriptor
     # holds its tensors and may be used again for as long as they are the call's
     def _request(self, name: str, desc, stream: Optional[int]) -> None:
-        if desc._device is not None and desc._device != self.engine.device:
-            raise WeaverError(f"{name}: tensors on GPU {desc._device}, the engine on {self.engine.device}", AW_E_INVALID_ARG)
-        self._call(name, ctypes.byref(desc), _stream(stream))
+        device = desc._device
+        if device is not None and device != self.engine.device:
+            raise WeaverError(f"{name}: tensors on GPU {device}, the engine on {self.engine.device}", AW_E_INVALID_ARG)
+        if stream is None:  # of the tensors' GPU, whichever torch's current one is
+            stream = _stream(None) if device is None else \
+                sys.modules["torch"]._C._cuda_getCurrentRawStream(device) or None
+        rc = getattr(self._lib, name)(self.engine._h, ctypes.byref(desc), stream)
+        if rc:
+            self.engine._check(rc, name.removeprefix("aw_ops_"))
 
     def rotary(self, desc: RotaryDesc, stream: Optional[int] = None) -> None:
         """q and k heads turned by their positions (``make_rotary_desc``)."""
