@@ -13,6 +13,7 @@
 #include <cstdint>
 #include <cstdio>
 #include <tuple>
+#include <type_traits>
 
 #include "../../include/aether_ops.h"
 #include "engine_internal.hpp"
@@ -376,11 +377,20 @@ int launch_rotary(aw_engine* e, awo::RotaryArgs& a, hipStream_t st) {
     // Few tokens: a token's heads over several waves.
     a.slices = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(steps, cdiv64(kRotaryWaves * (uint64_t)ei::compute_units(e), a.tokens)));
     const dim3 grid((uint32_t)cdiv64((uint64_t)a.tokens * a.slices, 4)), block(256);
-    const bool norm = a.q_norm || a.k_norm;
-    if (norm && a.interleaved) hipLaunchKernelGGL((awo::rotary_rows_kernel<APPEND, true, true>), grid, block, 0, st, a);
-    else if (norm) hipLaunchKernelGGL((awo::rotary_rows_kernel<APPEND, true, false>), grid, block, 0, st, a);
-    else if (a.interleaved) hipLaunchKernelGGL((awo::rotary_rows_kernel<APPEND, false, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((awo::rotary_rows_kernel<APPEND, false, false>), grid, block, 0, st, a);
+    auto launch = [&](auto norm, auto inter, auto odd) {
+        hipLaunchKernelGGL((awo::rotary_rows_kernel<APPEND, decltype(norm)::value, decltype(inter)::value, decltype(odd)::value>),
+                           grid, block, 0, st, a);
+    };
+    auto odd = [&](auto norm, auto inter) {
+        if (awo::rotary_rows_odd(a.hd, a.rotary_dim)) launch(norm, inter, std::true_type{});
+        else launch(norm, inter, std::false_type{});
+    };
+    auto inter = [&](auto norm) {
+        if (a.interleaved) odd(norm, std::true_type{});
+        else odd(norm, std::false_type{});
+    };
+    if (a.q_norm || a.k_norm) inter(std::true_type{});
+    else inter(std::false_type{});
     OPS_HIP(e, hipGetLastError());
     return AW_OK;
 }

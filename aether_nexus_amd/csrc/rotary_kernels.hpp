@@ -113,29 +113,50 @@ __device__ inline float lanes_sum(float x, uint32_t log) {
     return x;
 }
 
-// Heads whose turned dims are none or at least 16 and whose passing dims are none or at
-// least 8 (rotary_rows_take): 16 dims of a head in a lane, as two 16-byte pieces, the
-// heads of a wave's step side by side.  A turned lane holds 8 pairs from p0 on: dims p0
-// .. and rotary_dim / 2 + p0 .. (half), or 2 p0 .. 2 p0 + 15 (interleaved), so the same 8
-// cosines and sines serve every head of its token; a passing lane holds dims as they
-// lie.  Where the dims do not divide, the last lane starts earlier and makes some values
-// twice, the same bits (`skip` keeps them out of the norm's sum).  Work-group = 4
-// waves, each a token or a slice of its heads, none waiting for another: a wave works its
+// 16 dims of a head in a lane, as two 16-byte pieces, the heads of a wave's step side by
+// side.  A turned lane holds 8 pairs from p0 on: dims p0 .. and rotary_dim / 2 + p0 ..
+// (half), or 2 p0 .. 2 p0 + 15 (interleaved), so the same 8 cosines and sines serve every
+// head of its token; a passing lane holds dims as they lie.  Where the dims do not
+// divide, the last lane starts earlier and makes some values twice, the same bits (`skip`
+// keeps them out of the norm's sum).  ODD: fewer than 16 turned dims lie in one lane with
+// those behind them, 1 to 7 passing dims are stored one by one (8192 tokens of 32 / 8 heads
+// x 128, 10 turned dims 38 us, 122 63 us; in rotary_kernel 93 and 87).  Work-group = 4 waves,
+// each a token or a slice of its heads, none waiting for another: a wave works its
 // token's cosines and sines out once, a pair a lane, into LDS of its own, while its
 // first kStep steps of rows are on the way.
-__host__ __device__ inline bool rotary_rows_take(uint32_t hd, uint32_t n) {
-    return (n == 0 || n >= 16) && (hd == n || hd - n >= 8);
+// Bound: HBM, each row read and written once (8192 tokens of 32 / 8 heads x 128, 168 MB:
+// 33 us, 5.0 TB/s, the rate of a large copy); a token or two: the launch.
+// Dims of a head that the turned lanes hold: rotary_dim, or 16 where it is less.
+__host__ __device__ inline uint32_t rotary_turn_dims(uint32_t n) { return n ? (n < 16u ? 16u : n) : 0u; }
+__host__ __device__ inline bool rotary_rows_odd(uint32_t hd, uint32_t n) {
+    return rotary_turn_dims(n) != n || (hd > n && hd - rotary_turn_dims(n) < 8u);
 }
-// Lanes of turned and of passing dims of a head.
+// Lanes of a head that hold turned dims, passing ones.
 __host__ __device__ inline uint32_t rotary_turn_lanes(uint32_t n) { return (n + 15u) / 16u; }
-__host__ __device__ inline uint32_t rotary_pass_lanes(uint32_t hd, uint32_t n) { return (hd - n + 15u) / 16u; }
+__host__ __device__ inline uint32_t rotary_pass_lanes(uint32_t hd, uint32_t n) { return (hd - rotary_turn_dims(n) + 15u) / 16u; }
+// Heads of at least 16 dims (8 where none turn) that the lanes of a wave hold.
+__host__ __device__ inline bool rotary_rows_take(uint32_t hd, uint32_t n) {
+    return hd >= 8u && hd >= rotary_turn_dims(n) && rotary_turn_lanes(n) + rotary_pass_lanes(hd, n) <= 64u;
+}
 
-template <bool APPEND, bool NORM, bool INTER>
+// The pairs (p, p + H) of the 16 dims of a lane.
+template <int H>
+__device__ __forceinline__ void turn_few(float (&f)[16], const float (&c)[8], const float (&sn)[8]) {
+#pragma unroll
+    for (int p = 0; p < H; ++p) {
+        const float x = f[p], y = f[p + H];
+        f[p] = fmaf(x, c[p], -(y * sn[p]));
+        f[p + H] = fmaf(x, sn[p], y * c[p]);
+    }
+}
+
+template <bool APPEND, bool NORM, bool INTER, bool ODD>
 __global__ __launch_bounds__(256) void rotary_rows_kernel(RotaryArgs a) {
     // Steps whose rows are loaded together.  Measured, us, 1 and 2, heads of 128 dims: 6000
     // tokens of 12 / 2 heads with norms 9.6, 10.9; 12288 tokens of 32 / 8 heads appended with
-    // norms 36.7, 35.1; 8192 of them turned alone 34.6, 34.1; 3, 4 and 6 no better.
-    constexpr int kStep = NORM && !APPEND ? 1 : 2;
+    // norms 36.7, 35.1; 8192 of them turned alone 34.6, 34.1; 3, 4 and 6 no better.  (ODD: 2
+    // would take 180 registers.)
+    constexpr int kStep = ODD || (NORM && !APPEND) ? 1 : 2;
     __shared__ float2 s_turns[4][kRotaryMaxDim / 2];
     const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t id = blockIdx.x * 4u + wave; // below 2^26
@@ -145,8 +166,14 @@ __global__ __launch_bounds__(256) void rotary_rows_kernel(RotaryArgs a) {
     const uint32_t u = lane & ((1u << a.lanes_log) - 1u), slot = lane >> a.lanes_log, per = 64u >> a.lanes_log;
     const uint32_t turn_lanes = rotary_turn_lanes(n), unit = u - turn_lanes;
     const bool turning = u < turn_lanes, used = u < turn_lanes + rotary_pass_lanes(hd, n);
+    const uint32_t m = ODD ? rotary_turn_dims(n) : n;
+    const bool few = ODD && m != n;                 // the turned dims lie in one lane, as they lie
+    const bool tail = ODD && hd - m < 8u && hd > m; // 1 to 7 passing dims
     uint32_t at0, at1, p0 = 0, skip0, skip1; // dims of the pieces, leading values that another lane holds too
-    if (turning) {
+    if (few && turning) {
+        at0 = skip0 = skip1 = 0;
+        at1 = 8;
+    } else if (turning) {
         p0 = min(8u * u, half - 8u);
         at0 = INTER ? 2u * p0 : p0;
         at1 = INTER ? 2u * p0 + 8u : half + p0;
@@ -154,13 +181,13 @@ __global__ __launch_bounds__(256) void rotary_rows_kernel(RotaryArgs a) {
         skip0 = INTER ? min(2u * twice, 8u) : twice;
         skip1 = INTER ? 2u * twice - skip0 : twice;
     } else {
-        const uint32_t d = n + 16u * unit;
+        const uint32_t d = m + 16u * unit;
         at0 = min(d, hd - 8u);
         at1 = min(d + 8u, hd - 8u);
         skip0 = d - at0;
         skip1 = d + 8u - at1;
     }
-    const bool whole = n % 16u == 0u && (hd - n) % 16u == 0u; // no value is held twice
+    const bool whole = m % 16u == 0u && (hd - m) % 16u == 0u; // no value is held twice
     const uint32_t heads = a.q_heads + a.kv_heads + (APPEND && a.v_out ? a.kv_heads : 0u);
     const uint32_t steps = (heads + per - 1u) / per;
     const uint32_t s1 = (uint32_t)((uint64_t)steps * (slice + 1u) / a.slices);
@@ -215,6 +242,7 @@ __global__ __launch_bounds__(256) void rotary_rows_kernel(RotaryArgs a) {
             if (s + (uint32_t)j >= s1) break; // wave-uniform
             const uint32_t h = (s + (uint32_t)j) * per + slot;
             const bool is_q = h < a.q_heads, is_v = APPEND && h >= a.q_heads + a.kv_heads;
+            const bool normed = NORM && !is_v && (is_q ? a.q_norm != nullptr : a.k_norm != nullptr);
             float f0[8], f1[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -234,7 +262,7 @@ __global__ __launch_bounds__(256) void rotary_rows_kernel(RotaryArgs a) {
                     }
                 }
                 sum = lanes_sum(sum, a.lanes_log);
-                if (is_q ? a.q_norm != nullptr : a.k_norm != nullptr) {
+                if (normed) {
                     const float inv = rsqrtf(fmaf(sum, a.inv_hd, a.eps));
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
@@ -258,12 +286,36 @@ __global__ __launch_bounds__(256) void rotary_rows_kernel(RotaryArgs a) {
             const bool turn = turning && !is_v;
             if (turn) {
                 float g0[8], g1[8];
+                if (ODD && few && !INTER) {
+                    float f[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) f[e] = e < 8 ? f0[e] : f1[e - 8];
+                    switch (half) { // wave-uniform
+                    case 1: turn_few<1>(f, c, sn); break;
+                    case 2: turn_few<2>(f, c, sn); break;
+                    case 3: turn_few<3>(f, c, sn); break;
+                    case 4: turn_few<4>(f, c, sn); break;
+                    case 5: turn_few<5>(f, c, sn); break;
+                    case 6: turn_few<6>(f, c, sn); break;
+                    default: turn_few<7>(f, c, sn); break;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        g0[e] = f[e];
+                        g1[e] = f[e + 8];
+                    }
+                } else
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     if constexpr (INTER) { // pairs of neighbours: e and e + 1 of one piece
                         float(&f)[8] = e < 4 ? f0 : f1;
                         float(&g)[8] = e < 4 ? g0 : g1;
                         const int i = 2 * (e % 4);
+                        if (few && (uint32_t)e >= half) { // these pass
+                            g[i] = f[i];
+                            g[i + 1] = f[i + 1];
+                            continue;
+                        }
                         g[i] = fmaf(f[i], c[e], -(f[i + 1] * sn[e]));
                         g[i + 1] = fmaf(f[i], sn[e], f[i + 1] * c[e]);
                     } else {
@@ -277,12 +329,22 @@ __global__ __launch_bounds__(256) void rotary_rows_kernel(RotaryArgs a) {
                     f1[e] = g1[e];
                 }
             }
-            if (turn || (NORM && !is_v && (is_q ? a.q_norm != nullptr : a.k_norm != nullptr))) {
+            if (turn || normed) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     r0[i] = f2h_pair(f0[2 * i], f0[2 * i + 1]);
                     r1[i] = f2h_pair(f1[2 * i], f1[2 * i + 1]);
+                    if (few && !normed) { // dims that pass keep their bits
+                        if (2u * (uint32_t)i >= n) r0[i] = x0[j][i];
+                        if (2u * (uint32_t)i + 8u >= n) r1[i] = x1[j][i];
+                    }
                 }
+            }
+            if (tail && !turning) { // its other dims are the turned lanes'
+#pragma unroll
+                for (int e = 1; e < 8; ++e)
+                    if ((uint32_t)e >= skip0) y[at0 + (uint32_t)e] = half_of(r0, e);
+                continue;
             }
             *(uint4_el_t*)(y + at0) = r0;
             *(uint4_el_t*)(y + at1) = r1;
@@ -293,9 +355,8 @@ __global__ __launch_bounds__(256) void rotary_rows_kernel(RotaryArgs a) {
     }
 }
 
-// The other heads (fewer than 16 turned dims, fewer than 8 passing ones): work-group =
-// one token, a wave per head in turn, lanes over the pairs and then over the dims that
-// pass.
+// The other heads (of fewer than 16 dims, of 65 lanes): work-group = one token, a wave per head in
+// turn, lanes over the pairs and then over the dims that pass.
 template <bool APPEND>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
     __shared__ float2 s_turn[kRotaryMaxDim / 2];

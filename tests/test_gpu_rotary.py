@@ -87,6 +87,12 @@ SHAPES = [(1, 14, 2, 64, 64), (1, 32, 8, 128, 128), (3, 32, 8, 128, 64), (16, 4,
           (6, 3, 1, 112, 62), (130, 8, 2, 192, 128), (11, 2, 1, 2, 2), (3, 2, 2, 48, 16), (700, 5, 3, 32, 32), (8, 2, 1, 512, 96)]
 
 
+# Fewer than 16 turned dims, 1 to 7 passing ones, both, heads of fewer than 16
+SHAPES += [(300, 5, 3, 64, 2), (9, 4, 2, 128, 14), (5, 3, 1, 16, 8), (6, 3, 1, 16, 2), (7, 2, 2, 17, 12), (3, 2, 1, 23, 6), (4, 2, 2, 24, 10),
+           (9, 3, 2, 65, 64), (5, 32, 8, 128, 122), (8, 2, 1, 67, 60), (3, 2, 1, 17, 16), (2, 3, 2, 15, 14), (4, 1, 1, 12, 4), (3, 2, 2, 39, 32),
+           (2, 2, 1, 1023, 4), (2, 1, 2, 1024, 1018), (2, 2, 1, 1024, 1000), (2, 2, 1, 1023, 1010), (2, 2, 1, 1024, 1008)]
+
+
 @pytest.mark.parametrize("rows", ["plain", "fused", "odd"])
 @pytest.mark.parametrize("interleaved", [False, True], ids=["half", "interleaved"])
 @pytest.mark.parametrize("norm", [False, True], ids=["rotary", "norm"])
@@ -117,6 +123,24 @@ def test_rows(ops, shape, norm, interleaved, rows):
     call(d)
     assert np.array_equal(bits(q).reshape(before[0].shape), before[0])
     assert np.array_equal(bits(k).reshape(before[1].shape), before[1])
+
+
+@pytest.mark.parametrize("interleaved", [False, True], ids=["half", "interleaved"])
+@pytest.mark.parametrize("hd,n", [(64, 2), (16, 14), (23, 6), (65, 64), (128, 122), (128, 32), (12, 4)])
+def test_passing_dims_keep_their_bits(ops, hd, n, interleaved):
+    """Infinities and NaNs of any payload in dims that pass, none of which reach the turned ones."""
+    import torch
+    from aether_nexus_amd import ops as O
+    rng = np.random.default_rng(hd + n)
+    x = f16(rng, 5, 3, hd)
+    x[..., n:] = rng.choice(np.array([0x7C00, 0xFC00, 0x7E00, 0x7D01, 0xFC05, 0x0001, 0x8000], dtype=np.uint16), x[..., n:].shape).view(np.float16)
+    q, r = dev(x), O.Rotary(n, 10000.0, interleaved=interleaved)
+    out = torch.zeros_like(q)
+    ops.rotary(O.make_rotary_desc(num_tokens=5, q_heads=3, kv_heads=0, head_dim=hd, rotary=r, q=q, k=None, q_out=out, start_position=9))
+    got = host(out).reshape(5, 3, hd)
+    assert np.array_equal(got[..., n:].view(np.uint16), x[..., n:].view(np.uint16))
+    want, scale = turned(np.where(np.arange(hd) < n, x, 0).astype(np.float16), 9 + np.arange(5), r, None)
+    close(got[..., :n], want[..., :n], scale[..., :n], f"{hd} {n}")
 
 
 def test_positions_of_their_own(ops):
@@ -280,6 +304,19 @@ def test_append(ops, engine, held, new, heads, rows):
     ops.append_paged(b.desc(r, start_position=11))
     engine.check_device_errors()
     b.check(r, f"append {len(new)} sequences", start=11)
+
+
+@pytest.mark.parametrize("norms", ["none", "k", "both"])
+@pytest.mark.parametrize("hd,n", [(64, 10), (128, 2), (72, 66), (31, 30), (33, 14), (13, 6)])
+@pytest.mark.parametrize("interleaved", [False, True], ids=["half", "interleaved"])
+def test_append_of_few_turned_or_passing_dims(ops, engine, hd, n, norms, interleaved):
+    from aether_nexus_amd import ops as O
+    b = Batch(hd + n, [5, 0, 40, 15], [3, 0, 17, 2], 6, 3, hd, rows="fused", pad=1)
+    r = O.Rotary(n, 10000.0, interleaved=interleaved)
+    qw, kw = f16(b.rng, hd, scale=1.0) if norms == "both" else None, f16(b.rng, hd, scale=1.0) if norms != "none" else None
+    ops.append_paged(b.desc(r, start_position=3, q_norm=None if qw is None else dev(qw), k_norm=None if kw is None else dev(kw)))
+    engine.check_device_errors()
+    b.check(r, f"append {hd} {n} {norms}", start=3, q_norm=qw, k_norm=kw)
 
 
 def test_append_forms(ops, engine):
