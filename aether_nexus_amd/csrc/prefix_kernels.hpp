@@ -62,7 +62,9 @@ __device__ __forceinline__ half8_t prefix_query(const PrefixArgs& a, const uint1
 // the second product (each off by 2^-12 of itself on average, independently: less than
 // the f16 store of the output).  Staged rows are HD / 8 16-byte chunks, chunk c of K row
 // r at c ^ r, of V row r at c ^ vsw(r): no bank conflict at 128 dims.
-// Bound: HBM, the pages' bytes.
+// Bound: HBM, the pages' bytes (96 sequences of up to 1500 own tokens of 8 heads x 128,
+// 290 MB: 4.2 to 4.4 TB/s); few pages: a chain of refs, pages, products, sums (2
+// sequences behind 117 tokens 5 us, half of it the launch).
 constexpr int kPageBufs = 2;
 constexpr size_t pages_lds_bytes(int HD) {
     const size_t ring = (size_t)4 * kPageBufs * 2 * 16 * HD * 2, sums = (size_t)4 * 16 * (HD + 4) * 4 + 4 * 16 * 2 * 4;
@@ -347,7 +349,17 @@ struct PrefixPages {
 //     (j < 4) or 8 + 4 hf + j - 4; A = V^T by transposing LDS reads.
 // Staged rows are HD / 8 16-byte chunks, chunk c of K row r at c ^ (r % chunks), of V
 // row r at c ^ 4 (r % 4) ^ (r / 4) % 4 (128 dims): no bank conflict at 128 dims.
+// Measured, 96 sequences of 32 / 8 heads x 128 behind 32768 tokens, 51.5 GFLOP: 81 us
+// alone, 636 TFLOP/s; its loads alone take 60 to 76 us,
+// its products and softmax alone 58 to 70, so it is bound by both at once.  32 or 128
+// tokens a step, 3 or 4 buffers, 256 rows of 8 waves, two of these work-groups a CU: each
+// slower there or for 64 sequences behind 8192 tokens.
 constexpr uint32_t kPrefixRows = 128;
+// A row's sums are rescaled when its maximum grows by more than this (in powers of two), so
+// weights reach 2^8: f16 rounds them by as much of themselves, and its subnormals are as
+// far below the largest as with 0 or further.  Measured, us, 8 and 0: the same with own
+// tokens 113.9, 115.8; 64 sequences behind 8192 26.7, 28.0; 16 of 8 drafts behind 4099 x 64
+// dims 19.9, 20.9.
 constexpr float kPrefixGrow = 8.0f;
 constexpr int kPrefixThreads = 256;
 constexpr int kPrefixTok = 64, kPrefixBufs = 5; // tokens a step, steps of K or of V in LDS: two work-groups fill a CU's
@@ -687,13 +699,15 @@ struct PrefixTile {
             a.part_l[at] = l;
         }
         if (l == 0.0f) return;
+        // Past the L2, whose dirty lines would be written when the kernel ends: 64 sequences
+        // behind 8192 tokens 28.1 us, through it 29.1; whole rows by way of LDS no better.
         float* po = a.part_o + at * HD;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
-                *(float4_t*)(po + 32 * nb + 2 * i + 4 * hf) =
-                    (float4_t){oacc[nb][i], oacc[nb][i + 1], oacc[nb][i + 2], oacc[nb][i + 3]};
+                __builtin_nontemporal_store((float4_t){oacc[nb][i], oacc[nb][i + 1], oacc[nb][i + 2], oacc[nb][i + 3]},
+                                            (float4_t*)(po + 32 * nb + 2 * i + 4 * hf));
     }
 };
 

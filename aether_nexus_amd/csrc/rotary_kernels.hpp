@@ -153,8 +153,8 @@ __device__ __forceinline__ void turn_few(float (&f)[16], const float (&c)[8], co
 template <bool APPEND, bool NORM, bool INTER, bool ODD>
 __global__ __launch_bounds__(256) void rotary_rows_kernel(RotaryArgs a) {
     // Steps whose rows are loaded together.  Measured, us, 1 and 2, heads of 128 dims: 6000
-    // tokens of 12 / 2 heads with norms 9.6, 10.9; 12288 tokens of 32 / 8 heads appended with
-    // norms 36.7, 35.1; 8192 of them turned alone 34.6, 34.1; 3, 4 and 6 no better.  (ODD: 2
+    // tokens of 12 / 2 heads with norms 9.6, 10.9; 6147 tokens of 32 / 8 heads appended with
+    // norms 36.7, 35.1; 8192 tokens of those turned alone 34.6, 34.1; 3, 4 and 6 no better.  (ODD: 2
     // would take 180 registers.)
     constexpr int kStep = ODD || (NORM && !APPEND) ? 1 : 2;
     __shared__ float2 s_turns[4][kRotaryMaxDim / 2];
