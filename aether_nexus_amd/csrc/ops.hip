@@ -1,10 +1,11 @@
 // ops.hip — C ABI of the dense transformer ops (include/aether_ops.h).
 //
 // Replaces the dispatch methods of the reference's Ops engine
-// (nexus-core/src/ops.rs:166-462); the kernels are in ops_kernels.hpp.  Every
-// entry point validates its arguments on the host, picks the 16-byte vector
-// variant of a kernel when the pointers and sizes allow it, and enqueues on the
-// caller's stream.  There is no CPU fallback.
+// (nexus-core/src/ops.rs:166-462); the kernels are in ops_kernels.hpp.  Beside them the
+// rows of a batch over pages, which the reference does not have: rotary positions, head
+// norms and appends (rotary_kernels.hpp).  Every entry point validates its arguments on
+// the host, picks the 16-byte vector variant of a kernel when the pointers and sizes allow
+// it, and enqueues on the caller's stream.  There is no CPU fallback.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -272,7 +273,8 @@ int rotary_args(const char* what, const aw_rotary_desc* d, bool append, awo::Rot
     if (d->rotary_dim && !d->inv_freq) return bad("inv_freq is required");
     if (d->rotary_dim && !std::isfinite(d->magnitude)) return bad("magnitude must be finite");
     if ((d->q_norm || d->k_norm) && !(d->eps >= 0.0f && std::isfinite(d->eps))) return bad("eps must be finite and not negative");
-    if ((d->q_heads && (!d->q || !d->q_out)) || (d->kv_heads && (!d->k || (!append && !d->k_out)))) return bad("null pointer");
+    if (d->num_tokens && ((d->q_heads && (!d->q || !d->q_out)) || (d->kv_heads && (!d->k || (!append && !d->k_out)))))
+        return bad("null pointer");
     if (d->num_tokens > kMostTokens || d->q_heads > 0xFFFFu || d->kv_heads > 0xFFFFu)
         return refuse(msg, len, AW_E_UNSUPPORTED, "%s: too many tokens or heads", what);
     awo::RotaryArgs& a = *out;
@@ -332,7 +334,8 @@ int append_args(const aw_append_desc* d, awo::RotaryArgs* a, char* msg, size_t l
     if (d->rows.kv_heads == 0) return bad("kv_heads is 0");
     if (d->rows.k_out) return bad("k_out must be NULL (k goes to hot_k)");
     if (d->v && !d->hot_v) return bad("v given without hot_v");
-    if (!d->hot_k || !d->refs || !d->seq_hot || (d->hot_v && !d->v)) return bad("null pointer");
+    if (!d->hot_k || (d->rows.num_tokens && (d->hot_v && !d->v)) || (d->rows.num_tokens && d->batch && (!d->refs || !d->seq_hot)))
+        return bad("null pointer");
     if (d->hot_blocks == 0 || d->hot_count == 0) return bad("hot_blocks and hot_count must be >= 1");
     if (d->hot_blocks > 1ull << 31) return bad("hot_blocks exceeds 2^31, the refs' range");
     if (d->refs_stride < d->hot_count)

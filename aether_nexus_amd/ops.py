@@ -8,6 +8,11 @@ HIP stream, torch's current stream by default: the reference's batch mode
 forward pass) is the stream itself, and ``end_batch`` waits for it.  With
 tensors the wrapper also checks their dtype, device and element counts before
 anything is enqueued (the C ABI takes raw pointers).
+
+Beside them, without a counterpart in the reference, what a batch over pages needs:
+``rotary``, ``qk_norm_rotary``, ``append_paged`` and ``shared_prefix_attention``, each
+of a descriptor (``make_rotary_desc``, ``make_append_desc``, ``make_prefix_desc``) that
+is checked once and may be used again.
 """
 from __future__ import annotations
 

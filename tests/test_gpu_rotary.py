@@ -306,6 +306,22 @@ def test_append(ops, engine, held, new, heads, rows):
     b.check(r, f"append {len(new)} sequences", start=11)
 
 
+def test_no_tokens(ops, engine):
+    """Empty tensors, whose address is null: nothing happens."""
+    import torch
+    from aether_nexus_amd import ops as O
+    q, k = (torch.empty(0, h, 64, dtype=torch.float16, device="cuda:0") for h in (4, 2))
+    pool = torch.full((3, 16, 2, 64), 5.0, dtype=torch.float16, device="cuda:0")
+    r = O.Rotary(64)
+    ops.rotary(O.make_rotary_desc(num_tokens=0, q_heads=4, kv_heads=2, head_dim=64, rotary=r, q=q, k=k))
+    for batch in (0, 2):
+        ops.append_paged(O.make_append_desc(
+            batch=batch, num_tokens=0, q_heads=4, kv_heads=2, head_dim=64, q=q, k=k, v=k, hot_k=pool, hot_v=pool.clone(), rotary=r,
+            refs=torch.zeros(batch, 3, dtype=torch.int32, device="cuda:0"), seq_hot=torch.zeros(batch, dtype=torch.int32, device="cuda:0")))
+    engine.check_device_errors()
+    assert bool((pool == 5).all())
+
+
 @pytest.mark.parametrize("norms", ["none", "k", "both"])
 @pytest.mark.parametrize("hd,n", [(64, 10), (128, 2), (72, 66), (31, 30), (33, 14), (13, 6)])
 @pytest.mark.parametrize("interleaved", [False, True], ids=["half", "interleaved"])

@@ -119,6 +119,14 @@ def test_rows_refused(kw, word):
     assert rc == AW_E_INVALID_ARG and word in msg, msg
 
 
+def test_no_tokens_need_no_rows():
+    """An empty tensor's address is null."""
+    assert check_rows(rows(num_tokens=0, q=0, k=0, q_out=0, k_out=0))[0] == 0
+    assert check_append(append(dict(num_tokens=0, q=0, k=0, q_out=0), v=0))[0] == 0
+    assert check_append(append(dict(num_tokens=0, q=0, k=0, q_out=0), v=0, batch=0, refs=0, seq_hot=0, token_offsets=0))[0] == 0
+    assert check_append(append(dict(num_tokens=0), hot_k=0))[0] == AW_E_INVALID_ARG
+
+
 def test_parts_of_one_buffer_are_accepted():
     """q, k and both outputs side by side in rows of one buffer: no element twice."""
     part = dict(q=A["q"], k=A["q"] + 2 * 256, q_out=A["q"] + 2 * 384, k_out=A["q"] + 2 * 640,
