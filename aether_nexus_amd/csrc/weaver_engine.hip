@@ -1098,8 +1098,9 @@ int prefix_plan(const aw_prefix_desc* d, uint32_t n_cu, aw::PrefixArgs* out, aw_
     const bool one = tokens == 0 || (tokens <= kPrefixOneTokens && own_wgs <= 2ull * n_cu);
     if (!one) {
         // The prefix: one work-group a CU (tiles; 64 sequences behind 8192 tokens 27 us, two a
-        // CU 37: their sums; three for four CUs 30, one for two 33), or two.  Own tokens: at most 512 a part, so that long sequences
-        // are no longer than the rest (96 of up to 1500 tokens beside a prefix 110 us).
+        // CU 37: their sums; three for four CUs 30, one for two 33), or two.  Own tokens: at
+        // most 512 a part, so that long sequences are no longer than the rest (1024: 64 of up
+        // to 257 beside that prefix 28.3 for 27.3, no other change).
         prefix_parts(prefix_wgs, (tiles ? 1ull : 2ull) * n_cu, a.prefix_tokens, ~0u, a.own_max ? 48 : 64, &a.prefix_splits, &a.prefix_span);
         prefix_parts(own_wgs, 2ull * n_cu, a.own_max, 512, aw::kMaxSplits - a.prefix_splits, &a.own_splits, &a.own_span);
         a.splits = a.prefix_splits + a.own_splits;
