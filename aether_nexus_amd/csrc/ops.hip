@@ -256,6 +256,7 @@ int refuse(char* msg, size_t len, int code, const char* fmt, ...) {
 // tokens 4.2 each.
 constexpr uint64_t kRotaryWaves = 16;
 constexpr uint32_t kMostTokens = 1u << 24; // a call's work-groups of 256 threads stay below 2^32 threads
+constexpr uint32_t kMostSequences = 1u << 24; // of an append: a search of its offsets in four steps, in 32 bits
 constexpr uint64_t kMostStride = 1ull << 30; // elements: tokens * stride * 2 bytes stays below 2^63
 
 // The checks that the three rotary calls share, and their kernel arguments.
@@ -340,6 +341,7 @@ int append_args(const aw_append_desc* d, awo::RotaryArgs* a, char* msg, size_t l
     if (d->hot_blocks > 1ull << 31) return bad("hot_blocks exceeds 2^31, the refs' range");
     if (d->refs_stride < d->hot_count)
         return refuse(msg, len, AW_E_INVALID_ARG, "append_paged: refs_stride %u < hot_count %u", d->refs_stride, d->hot_count);
+    if (d->batch > kMostSequences) return refuse(msg, len, AW_E_UNSUPPORTED, "append_paged: batch %u exceeds 2^24", d->batch);
     if (!d->token_offsets && d->batch && d->rows.num_tokens % d->batch)
         return refuse(msg, len, AW_E_INVALID_ARG, "append_paged: %u tokens over %u sequences need token_offsets",
                       d->rows.num_tokens, d->batch);

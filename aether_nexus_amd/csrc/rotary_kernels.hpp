@@ -47,16 +47,22 @@ struct Place {
 
 // Token t of an append: the sequence whose tokens hold it, its place behind the tokens
 // that the sequence had, the page of the block table.  Every lane of a wave asks for
-// the same token; the offsets are read 64 at a time, so the search is one or two round
-// trips to L2, not a chain of them.
+// the same token; the offsets ascend, so it is found among 64 equal stretches of them at
+// a time: a round trip to L2 up to 64 sequences, two up to 4096, four up to 2^24, the
+// most that the host lets through.  Offsets that descend end the search as well, at
+// some sequence, and the checks below see that the token is not its own.
 __device__ inline Place find_place(const RotaryArgs& a, uint32_t t, uint32_t lane, bool report) {
     uint32_t b, first, end;
     if (a.token_offsets) {
+        uint32_t n = a.batch; // the sequences that end at or before t are the first b .. b + n
         b = 0;
-        for (uint32_t i = 0; i < a.batch; i += 64u) {
-            const uint32_t at = i + lane;
-            b += (uint32_t)__popcll(__ballot(at < a.batch && a.token_offsets[min(at, a.batch - 1u) + 1u] <= t));
+        while (n > 64u) {
+            const uint32_t stretch = (n + 63u) / 64u, at = (lane + 1u) * stretch - 1u;
+            const uint32_t skip = stretch * (uint32_t)__popcll(__ballot(at < n && a.token_offsets[b + min(at, n - 1u) + 1u] <= t));
+            b += skip;
+            n = min(n - skip, stretch);
         }
+        if (n) b += (uint32_t)__popcll(__ballot(lane < n && a.token_offsets[b + min(lane, n - 1u) + 1u] <= t));
         if (b >= a.batch) return {false, false, 0, 0}; // behind the last sequence
         first = a.token_offsets[b];
         end = a.token_offsets[b + 1u];

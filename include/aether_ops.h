@@ -208,7 +208,7 @@ int aw_ops_qk_norm_rotary(aw_engine* engine, const aw_rotary_desc* desc, void* h
  * overlap neither each other nor the rows. */
 typedef struct aw_append_desc {
     aw_rotary_desc rows;            /* k_out NULL; q may be absent (q_heads 0) */
-    uint32_t batch, hot_count, refs_stride, reserved;
+    uint32_t batch, hot_count, refs_stride, reserved; /* batch <= 2^24 */
     uint64_t v_stride, hot_blocks;
     const uint16_t* v;              /* [num_tokens][kv_heads][head_dim], NULL with hot_v */
     uint16_t* hot_k;                /* [hot_blocks][16][kv_heads][head_dim] */

@@ -366,6 +366,29 @@ def test_append_forms(ops, engine):
     engine.check_device_errors()
 
 
+@pytest.mark.parametrize("batch", [64, 65, 128, 4096, 4097, 5000, 70000])
+def test_append_of_many_sequences(ops, engine, batch):
+    """Each token finds its sequence among any number of them: sequences without new tokens wherever a search of 64
+    stretches at a time cuts the batch, at both ends, and in runs longer than a stretch; rows behind the last one."""
+    from aether_nexus_amd import ops as O
+    r = O.Rotary(16, 10000.0)
+    rng = np.random.default_rng(batch)
+    new, held = rng.integers(0, 3, batch), rng.integers(0, 20, batch)
+    n = batch
+    while n > 1:
+        stretch = -(-n // 64)
+        for cut in range(0, batch, stretch if stretch > 1 else 7):
+            new[cut:cut + 2] = 0
+        n = stretch
+    new[batch // 3:batch // 3 + batch // 50 + 2] = new[-3:] = 0
+    new[batch // 2] = 40
+    assert 0 < np.count_nonzero(new) < batch
+    b = Batch(9, held.tolist(), new.tolist(), 1, 1, 16, pad=3)
+    ops.append_paged(b.desc(r))
+    engine.check_device_errors()
+    b.check(r, f"{batch} sequences")
+
+
 def test_append_bad_pages_and_lengths(ops, engine):
     """A ref past the pool, a page past the table, a sequence with more new tokens than it has, offsets that
     descend: the tokens are left out as described, everything else is written, and the error is reported."""

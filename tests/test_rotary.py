@@ -186,6 +186,14 @@ def test_append_refused(rows_kw, kw, word):
     assert rc == AW_E_INVALID_ARG and word in msg, msg
 
 
+@pytest.mark.parametrize("batch", [(1 << 24) + 1, (1 << 32) - 63, (1 << 32) - 1])
+def test_append_of_too_many_sequences(batch):
+    """The search of the offsets counts them in 32 bits: a batch near 2^32 is refused, not searched."""
+    rc, msg = check_append(append(batch=batch))
+    assert rc == AW_E_UNSUPPORTED and "batch" in msg
+    assert check_append(append(batch=1 << 24))[0] == 0
+
+
 def test_append_refuses_k_out():
     d = append()
     d.rows.k_out = A["k_out"]
