@@ -255,7 +255,7 @@ int refuse(char* msg, size_t len, int code, const char* fmt, ...) {
 // 128: 1024 tokens appended with norms 6.85, 6.32, 6.08; 2048 turned 9.06, 9.06, 8.67; 509
 // tokens 4.2 each.
 constexpr uint64_t kRotaryWaves = 16;
-constexpr uint32_t kMostTokens = 1u << 24; // a call's work-groups of 256 threads stay below 2^32 threads
+constexpr uint32_t kMostTokens = 1u << 24; // waves of a call, and threads of a grid's row, stay below 2^32
 constexpr uint32_t kMostSequences = 1u << 24; // of an append: a search of its offsets in four steps, in 32 bits
 constexpr uint64_t kMostStride = 1ull << 30; // elements: tokens * stride * 2 bytes stays below 2^63
 
@@ -374,7 +374,8 @@ template <bool APPEND>
 int launch_rotary(aw_engine* e, awo::RotaryArgs& a, hipStream_t st) {
     a.err = ei::error_word(e);
     if (!awo::rotary_rows_take(a.hd, a.rotary_dim)) {
-        hipLaunchKernelGGL(awo::rotary_kernel<APPEND>, dim3(a.tokens), dim3(256), 0, st, a);
+        const dim3 tokens(std::min(a.tokens, awo::kRotaryGridRow), (uint32_t)cdiv64(a.tokens, awo::kRotaryGridRow));
+        hipLaunchKernelGGL(awo::rotary_kernel<APPEND>, tokens, dim3(256), 0, st, a);
         OPS_HIP(e, hipGetLastError());
         return AW_OK;
     }

@@ -362,11 +362,15 @@ __global__ __launch_bounds__(256) void rotary_rows_kernel(RotaryArgs a) {
 }
 
 // The other heads (of fewer than 16 dims, of 65 lanes): work-group = one token, a wave per head in
-// turn, lanes over the pairs and then over the dims that pass.
+// turn, lanes over the pairs and then over the dims that pass.  Tokens past a grid row's
+// kRotaryGridRow go to further rows: a row of 2^24 work-groups would be 2^32 threads, one
+// more than a launch takes.
+constexpr uint32_t kRotaryGridRow = 1u << 20;
 template <bool APPEND>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
     __shared__ float2 s_turn[kRotaryMaxDim / 2];
-    const uint32_t t = blockIdx.x, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+    const uint32_t t = blockIdx.y * kRotaryGridRow + blockIdx.x, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+    if (t >= a.tokens) return; // the whole work-group
     Place place{true, true, t, 0};
     if constexpr (APPEND) place = find_place(a, t, lane, wave == 0);
     if (!place.rows) return; // the same in every wave

@@ -125,6 +125,29 @@ def test_rows(ops, shape, norm, interleaved, rows):
     assert np.array_equal(bits(k).reshape(before[1].shape), before[1])
 
 
+@pytest.mark.parametrize("tokens", [1 << 20, (1 << 20) + 1, 1 << 24])
+def test_as_many_tokens_as_a_call_takes(ops, engine, tokens):
+    """Heads of 2 dims, a work-group a token: more of them than one row of a grid takes, up to the most that is
+    accepted; turned alone, and into pages in the opposite order."""
+    import torch
+    from aether_nexus_amd import ops as O
+    rng = np.random.default_rng(3)
+    x = f16(rng, tokens, 1, 2)
+    r = O.Rotary(2, 10000.0)
+    q, out = dev(x), torch.full((tokens, 1, 2), 7.0, dtype=torch.float16, device="cuda:0")
+    ops.rotary(O.make_rotary_desc(num_tokens=tokens, q_heads=1, kv_heads=0, head_dim=2, rotary=r, q=q, q_out=out, k=None))
+    want = turned(x, np.arange(tokens), r)
+    close(host(out), *want, f"{tokens} tokens")
+    pages = -(-tokens // 16)
+    pool = torch.full((pages, 16, 1, 2), 7.0, dtype=torch.float16, device="cuda:0")
+    refs = torch.arange(pages - 1, -1, -1, dtype=torch.int32, device="cuda:0").view(1, pages)
+    ops.append_paged(O.make_append_desc(batch=1, num_tokens=tokens, q_heads=0, kv_heads=1, head_dim=2, rotary=r, k=q, v=None,
+                                        hot_k=pool, hot_v=None, refs=refs,
+                                        seq_hot=torch.tensor([tokens], dtype=torch.int32, device="cuda:0")))
+    engine.check_device_errors()
+    assert np.array_equal(bits(pool)[::-1].reshape(-1, 1, 2)[:tokens], bits(out))
+
+
 @pytest.mark.parametrize("interleaved", [False, True], ids=["half", "interleaved"])
 @pytest.mark.parametrize("hd,n", [(64, 2), (16, 14), (23, 6), (65, 64), (128, 122), (128, 32), (12, 4)])
 def test_passing_dims_keep_their_bits(ops, hd, n, interleaved):
