@@ -1064,6 +1064,10 @@ int prefix_plan(const aw_prefix_desc* d, uint32_t n_cu, aw::PrefixArgs* out, aw_
     if ((uintptr_t)d->out & 7u) return refuse(AW_E_ALIGN, "out must be 8-byte aligned");
     const uintptr_t q = (uintptr_t)d->q, o = (uintptr_t)d->out, bytes = rows * d->kv_heads * d->head_dim * 2;
     if (q != o && q < o + bytes && o < q + bytes) return refuse(AW_E_INVALID_ARG, "out overlaps q, and is not q");
+    if (d->prefix_tokens || d->own_count)
+        for (const uintptr_t pool : {(uintptr_t)d->hot_k, (uintptr_t)d->hot_v})
+            if (pool && o < pool + d->hot_blocks * kBlock * d->kv_heads * d->head_dim * 2 && pool < o + bytes)
+                return refuse(AW_E_INVALID_ARG, "out overlaps a pool");
     aw::PrefixArgs& a = *out;
     a = aw::PrefixArgs{};
     a.q = d->q;

@@ -317,7 +317,8 @@ int aw_multihead_attention_device(aw_engine* engine, const uint16_t* q, const ui
  * batch instead of once for each sequence (aw_decode_device with the prefix'
  * refs in every row of its table), each sequence's own pages beside them, and
  * the parts are joined by their log-sum-exp.  Device pointers, f16:
- *   q, out       [batch][queries][q_heads][head_dim]; q 16-byte, out 8-byte aligned; out may be q
+ *   q, out       [batch][queries][q_heads][head_dim]; q 16-byte, out 8-byte aligned; out may be q, and overlaps
+ *                neither it otherwise nor a pool
  *   hot_k, hot_v [hot_blocks][16][kv_heads][head_dim], 16-byte aligned; hot_v NULL: V is the K row
  *   prefix_refs  [ceil(prefix_tokens / 16)]: the prefix may end inside its last page, whose other rows are not used
  *   refs         [batch][refs_stride]: the pages of a sequence's tokens behind the prefix, which begin a page of their own

@@ -62,6 +62,19 @@ def test_invalid(kw):
     assert e.value.status == AW_E_INVALID_ARG and "shared_prefix_attention" in str(e.value)
 
 
+@pytest.mark.parametrize("pool", ["hot_k", "hot_v"])
+def test_out_over_a_pool(pool):
+    """Rows written into pages that other work-groups still read."""
+    size = 50 * 16 * 2 * 128 * 2
+    for at in (0, 16, size - 8, -16, 8 - 4 * 2 * 8 * 128 * 2):
+        with pytest.raises(WeaverError) as e:
+            O.prefix_plan(desc(out=A[pool] + at))
+        assert e.value.status == AW_E_INVALID_ARG and "pool" in str(e.value)
+    for at in (size, -4 * 2 * 8 * 128 * 2):  # right behind it, right before it
+        O.prefix_plan(desc(out=A[pool] + at))
+    O.prefix_plan(desc(out=A["hot_k"], prefix_tokens=0, own_count=0))  # no token: the pool is not read
+
+
 @pytest.mark.parametrize("kw", [dict(head_dim=96), dict(head_dim=256), dict(prefix_tokens=(1 << 26) + 1),
                                 dict(own_count=(1 << 18) + 1, refs_stride=1 << 19), dict(kv_heads=1024, q_heads=1024),
                                 dict(batch=1 << 20, queries=1 << 10), dict(batch=1 << 26, queries=1 << 26),
