@@ -1034,6 +1034,14 @@ constexpr uint32_t kPrefixOneTokens = 512;
 // 4000 tokens 8.3, 9.2; 112 rows, 1500 tokens 8.0, 9.0.
 constexpr uint64_t kPrefixPagesValues = 2u << 20;
 
+// Bytes of parts' sums that more than one part of the own tokens may take: the parts of a
+// request with many query rows (which fill the GPU without them) or a wide table go down
+// to as many as this holds, at the least to one beside the prefix'.  Then they are about
+// twice 4 bytes for each 2 of q.  (16 sequences x 2048 queries of 32 / 8 heads x 128 with
+// tables of 32768 tokens: 57 parts were 31.6 GB; now 1.1 GB.)  A step of few queries keeps
+// its parts: 128 sequences with such tables 128 MB.
+constexpr uint64_t kPrefixPartBytes = 128u << 20;
+
 // Checks a request and fills its kernel arguments but for addresses of scratch.
 int prefix_plan(const aw_prefix_desc* d, uint32_t n_cu, aw::PrefixArgs* out, aw_prefix_plan_info* info, char* msg, size_t len) {
     auto refuse = [&](int code, const char* why) {
@@ -1106,7 +1114,8 @@ int prefix_plan(const aw_prefix_desc* d, uint32_t n_cu, aw::PrefixArgs* out, aw_
         // most 512 a part, so that long sequences are no longer than the rest (1024: 64 of up
         // to 257 beside that prefix 28.3 for 27.3, no other change).
         prefix_parts(prefix_wgs, (tiles ? 1ull : 2ull) * n_cu, a.prefix_tokens, ~0u, a.own_max ? 48 : 64, &a.prefix_splits, &a.prefix_span);
-        prefix_parts(own_wgs, 2ull * n_cu, a.own_max, 512, aw::kMaxSplits - a.prefix_splits, &a.own_splits, &a.own_span);
+        const uint64_t most = std::min<uint64_t>(aw::kMaxSplits, kPrefixPartBytes / ((uint64_t)d->kv_heads * rows * d->head_dim * 4));
+        prefix_parts(own_wgs, 2ull * n_cu, a.own_max, 512, (uint32_t)std::max<int64_t>(1, (int64_t)most - a.prefix_splits), &a.own_splits, &a.own_span);
         a.splits = a.prefix_splits + a.own_splits;
         own_units *= a.own_splits;
         if (tiles) wgs = (uint64_t)cdiv((uint64_t)d->kv_heads * a.prefix_splits, 8) * 8 * a.prefix_tiles;

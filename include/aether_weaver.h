@@ -331,7 +331,8 @@ int aw_multihead_attention_device(aw_engine* engine, const uint16_t* q, const ui
  * row does not see never reach it, infinities and NaNs neither.
  * Any number of queries; head_dim 64 or 128; up to 2^25 rows of q, 2^26 prefix and
  * 2^22 own tokens.
- * Scratch is the engine's workspace, as in aw_decode_device, also under capture. */
+ * Scratch is the engine's workspace, as in aw_decode_device, also under capture:
+ * at most 133 MiB, or 4.2 times q's bytes where that is more. */
 typedef struct aw_prefix_desc {
     uint32_t batch, queries;
     uint32_t q_heads, kv_heads, head_dim;

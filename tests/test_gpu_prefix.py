@@ -379,6 +379,40 @@ def test_parts_of_many_pages(ops, engine, case):
     assert np.all(np.abs(got - want) <= want * (2.0 ** -11 + 2.0 ** -20) + 2.0 ** -25), (got.min(), got.max(), want)
 
 
+@pytest.mark.parametrize("shape", [(2, 1100, 32, 8, 128, 300, [1400, 4096]), (1, 2600, 14, 2, 64, 1000, [2700])], ids=["two", "one"])
+def test_many_queries(ops, engine, shape):
+    """Prompt pieces behind a prefix, whose parts' sums are bounded: against float64 on the GPU, causal, over each
+    sequence's tokens end to end."""
+    import torch
+    batch, queries, hq, hk, hd, prefix, own = shape
+    c = Case(36, *shape, stale=False, spare=300)
+    p = plan(c)
+    assert p.own_tokens_per_split > 512 and p.workspace_bytes <= 133 << 20
+    ops.shared_prefix_attention(c.desc())
+    engine.check_device_errors()
+    got, group = c.out.double(), hq // hk
+    worst = 0.0
+    for b in range(batch):
+        at = torch.from_numpy(np.concatenate([c.prefix_refs & P.REF_MASK, c.refs[b, :-(-own[b] // 16)]])).cuda()
+        n0 = -(-prefix // 16) * 16
+        rows = torch.cat([torch.arange(prefix), n0 + torch.arange(own[b])]).cuda()
+        last = prefix + own[b] - queries + torch.arange(queries, device="cuda:0").repeat_interleave(group)
+        hidden = torch.arange(len(rows), device="cuda:0") > last[:, None]
+        for g in range(hk):
+            k, v = (x[at][:, :, g].flatten(0, 1)[rows].double() for x in (c.dk, c.dv))
+            q = c.dq[b, :, g * group:(g + 1) * group].double().flatten(0, 1)
+            s = (q @ k.t().contiguous() * hd ** -0.5).masked_fill(hidden, -float("inf"))
+            w = (s - s.amax(1, keepdim=True)).exp()
+            total = w.sum(1, keepdim=True)
+            want, absolute = w @ v / total, w @ v.abs() / total
+            # the head's tolerance, its subnormal weights over the row's sum of weights (its largest is 1)
+            tol = 2.0 ** -11 * want.abs() + 1.5 * 2.0 ** -11 * absolute + len(rows) * 6.0 * 2.0 ** -25 / total + 2.0 ** -25
+            d = (got[b, :, g * group:(g + 1) * group].flatten(0, 1) - want).abs()
+            worst = max(worst, float((d / tol).max()))
+    print(f"many queries: worst error over tolerance {worst:.3f}", flush=True)
+    assert worst <= 1.0
+
+
 def test_pages_past_32_bits(ops, engine):
     """Pages whose addresses lie more than 2^32 bytes into the pool, written by append_paged and read back."""
     import torch

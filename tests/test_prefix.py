@@ -52,6 +52,32 @@ def test_accepted_requests_are_covered_by_their_parts(kw):
         assert floats * (d.head_dim + 2) * 4 <= p.workspace_bytes + 1024
 
 
+@pytest.mark.parametrize("batch,queries,own_count", [
+    (64, 512, 160), (1, 4096, 512), (16, 2048, 2048), (8, 2048, 256), (32, 2048, 512), (1, 8192, 2048), (64, 1, 2048),
+    (256, 1, 2048), (1, 64, 2048), (4, 16, 1 << 18), (1, 1 << 20, 1 << 10)])
+@pytest.mark.parametrize("heads", [(32, 8, 128), (14, 2, 64)], ids=str)
+def test_workspace_of_many_queries_and_wide_tables(batch, queries, own_count, heads):
+    """Parts are for filling the GPU: their sums stay within 128 MiB (and two numbers a row: 1 / 32 of 64 dims), or,
+    where the queries are many, one part of the prefix and one of the own tokens, 4 bytes for each 2 of q."""
+    hq, hk, hd = heads
+    for prefix in (0, 2048, 32768):
+        for cus in (256, 304):
+            d = desc(batch=batch, queries=queries, q_heads=hq, kv_heads=hk, head_dim=hd, prefix_tokens=prefix,
+                     own_count=own_count, refs_stride=own_count, q=1 << 50, out=2 << 50)
+            p = O.prefix_plan(d, cus)
+            q_bytes = 2 * batch * queries * hq * hd
+            assert p.workspace_bytes <= max(133 << 20, 4.2 * q_bytes)
+            if 4 * q_bytes > 128 << 20:
+                assert p.own_splits == 1 and p.prefix_splits == (prefix > 0)
+
+
+@pytest.mark.parametrize("batch,own_count,splits", [(64, 17, 1), (64, 256, 8), (64, 1024, 32), (96, 94, 3)])
+def test_parts_of_few_queries(batch, own_count, splits):
+    """A step of few queries is cut as its own tokens ask for: at most 512 a part."""
+    d = desc(batch=batch, queries=1, q_heads=32, kv_heads=8, prefix_tokens=8192, own_count=own_count, refs_stride=own_count)
+    assert O.prefix_plan(d, 256).own_splits == splits
+
+
 @pytest.mark.parametrize("kw", [dict(batch=0), dict(queries=0), dict(kv_heads=0), dict(q_heads=7), dict(q_heads=0), dict(flags=2),
                                 dict(flags=AW_F_CAUSAL | 8), dict(scale=math.inf), dict(scale=math.nan), dict(refs_stride=2),
                                 dict(q=0), dict(out=0), dict(prefix_refs=0), dict(refs=0), dict(hot_k=0), dict(hot_blocks=0),
