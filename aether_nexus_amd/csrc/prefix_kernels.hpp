@@ -355,12 +355,19 @@ struct PrefixPages {
 // tokens a step, 3 or 4 buffers, 256 rows of 8 waves, two of these work-groups a CU: each
 // slower there or for 64 sequences behind 8192 tokens.
 constexpr uint32_t kPrefixRows = 128;
-// A row's sums are rescaled when its maximum grows by more than this (in powers of two), so
-// weights reach 2^8: f16 rounds them by as much of themselves, and its subnormals are as
-// far below the largest as with 0 or further.  Measured, us, 8 and 0: the same with own
-// tokens 113.9, 115.8; 64 sequences behind 8192 26.7, 28.0; 16 of 8 drafts behind 4099 x 64
-// dims 19.9, 20.9.
-constexpr float kPrefixGrow = 8.0f;
+// A row's sums are rescaled whenever its maximum grows: its largest weight so far is exactly
+// 1, as in the decode kernel, and its bits do not depend on the rows beside it (their
+// growth multiplies its sums by 1).  Error against 64 bits, this and the decode kernel's
+// on the same tokens (f16 outputs alone 2.1e-4): random scores 2.4e-4, 2.5e-4 at 8192
+// tokens, 2.6e-4, 2.7e-4 at 32768; rows where a late token takes most of the weight
+// 2.1e-4 to 2.5e-4, no more than the decode kernel's; two such tokens in the two halves of one
+// step 2.3e-4 to 2.5e-4, up to 6% above it (its groups are of 32 tokens).  Measured, us: 64
+// sequences behind 8192 tokens 27.4, 96 behind 32768 and their own 118.  Not taken: rescaling only
+// after a growth of 2^8, 26.7 and 115, but errors up to 33% above the decode kernel's (the
+// largest weight rounded, not its part of the sum) and a row's bits by its neighbours'
+// growth; a second f16 term for what is left of the weights of a step's first 32 tokens,
+// 2.0e-4 to 2.4e-4 but 29.6 and 127, or of all of them, f16 outputs' own error but 34.1
+// and 167.
 constexpr int kPrefixThreads = 256;
 constexpr int kPrefixTok = 64, kPrefixBufs = 5; // tokens a step, steps of K or of V in LDS: two work-groups fill a CU's
 constexpr size_t prefix_lds_bytes(int HD) { return (size_t)kPrefixBufs * kPrefixTok * HD * 2; }
@@ -505,7 +512,7 @@ struct PrefixTile {
             const auto sw = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, mx), __builtin_bit_cast(uint32_t, mx), false, false);
             const uint32_t sw0 = sw[0], sw1 = sw[1]; // the row's two halves
             mx = fmaxf(__builtin_bit_cast(float, sw0), __builtin_bit_cast(float, sw1)) * a.scale_log2;
-            if (__any(mx > m_run + kPrefixGrow)) {
+            if (__any(mx > m_run)) { // wave-uniform; a row whose maximum stays is multiplied by 1
                 const float mnew = fmaxf(m_run, mx);
                 const float alpha = mnew == -INFINITY ? 1.0f : fast_exp2(m_run - mnew);
                 m_run = mnew;

@@ -447,6 +447,73 @@ def test_results_do_not_depend_on_the_batch_order_or_run(ops):
         assert np.array_equal(host(c.out).view(np.int16), first.view(np.int16))
 
 
+@pytest.mark.parametrize("growth", [3.0, 7.75])
+@pytest.mark.parametrize("case", [(64, 1, 16, 4, 128, 8192), (40, 2, 12, 4, 64, 6000), (5, 1, 8, 2, 128, 1104)],
+                         ids=["tiles-128", "tiles-64", "pages"])
+def test_peaked_rows_beside_the_decode(ops, engine, case, growth):
+    """Rows whose maximum grows in a later step, by a token that then takes most of the weight: every 64th token has
+    2^0, one in the second half of the second step and one in the first half of the last 2^growth, the others 2^-14.
+    The error against 64 bits is no larger than aw_decode_device's over the same tokens (its rounding of the weights
+    is the reference: a row's largest is exactly 1); 5% for the two orders of sums, whose effect on the root mean
+    square of thousands of values is below 1%."""
+    import torch
+    from aether_nexus_amd.weaver import make_desc
+    batch, queries, hq, hk, hd, prefix = case
+    c = Case(47, *case, [queries + b % 20 for b in range(batch)], stale=False)
+    assert plan(c).row_tile == (128 if batch > 8 else 16)
+    scores = np.full(prefix, -14.0)
+    scores[::64] = 0.0
+    for i, at in enumerate((64 + 45, 64 * (prefix // 64 - 1) + 10)):
+        scores[at] = growth - 0.25 * i
+    t, unit = np.arange(prefix), np.sqrt(hd) / (8.0 * np.log2(np.e))
+    c.q[..., 0] = 8.0
+    c.k[..., 1:] *= np.float16(0.01)
+    c.k[..., 0] = -14.0 * unit
+    c.k[c.prefix_refs[t // 16] & P.REF_MASK, t % 16, :, 0] = (scores * unit)[:, None].astype(np.float16)
+    c.dq, c.dk = dev(c.q), dev(c.k)
+    ops.shared_prefix_attention(c.desc())
+    count = prefix // 16 + c.count  # the prefix fills its pages: a sequence's tokens are one table's
+    table = np.concatenate([np.repeat(c.prefix_refs[None] & P.REF_MASK, batch, 0), np.where(c.refs < c.blocks, c.refs, 0)], axis=1)
+    few = torch.empty_like(c.out)
+    engine.decode_device(make_desc(layers=1, batch=batch, queries=queries, q_heads=hq, kv_heads=hk, head_dim=hd, dict_size=0,
+                                   dict_heads=1, hot_count=count, cold_count=0, refs_stride=count, hot_blocks=c.blocks,
+                                   cold_blocks=0, q=c.dq, out=few, hot_k=c.dk, hot_v=c.dv, refs=dev(table),
+                                   seq_hot=dev(prefix + c.own), seq_hot_tokens=True, causal=True, scale=hd ** -0.5))
+    engine.check_device_errors()
+    want = P.shared_prefix_attention(c.q, c.k, c.v, c.prefix_refs, prefix, c.refs, c.own, hd ** -0.5, True)
+    rel = [float(np.linalg.norm(host(x).astype(np.float64) - want) / np.linalg.norm(want)) for x in (c.out, few)]
+    print(f"peaked rows {case} growth {growth}: rel-L2 {rel[0]:.3e}, decode {rel[1]:.3e}", flush=True)
+    c.check("peaked rows")
+    assert rel[0] <= 1.05 * rel[1], rel
+
+
+@pytest.mark.parametrize("case", [(64, 1, 32, 8, 128, 2600), (33, 2, 32, 8, 64, 1500)], ids=["128", "64"])
+def test_results_do_not_depend_on_the_neighbours(ops, case):
+    """Rows of many sequences share a work-group's wave; each keeps its bits when the sequences change places, and when
+    the others' queries change.  Scores of standard deviation 9: their maxima keep growing, by less and by more than 2^8,
+    in other steps for each row."""
+    batch, queries = case[:2]
+    c = Case(46, *case, [queries + b % 40 for b in range(batch)], qscale=9.0)
+    p = plan(c)
+    assert p.row_tile == 128 and p.prefix_tokens_per_split > 2 * 64 and p.prefix_splits > 1
+    ops.shared_prefix_attention(c.desc())
+    first = host(c.out).view(np.int16).copy()
+    assert np.isfinite(first.view(np.float16)).all()
+    q, refs, own = c.q.copy(), c.refs.copy(), c.own.copy()
+    for turn in range(3):
+        order = c.rng.permutation(batch)
+        c.dq, c.drefs, c.down = dev(q[order]), dev(refs[order]), dev(own[order])
+        ops.shared_prefix_attention(c.desc())
+        assert np.array_equal(host(c.out).view(np.int16), first[order]), f"order {turn}"
+    c.drefs, c.down = dev(refs), dev(own)
+    for keep in (0, batch // 2, batch - 1):
+        other = (c.rng.standard_normal(q.shape) * 3.0).astype(np.float16)
+        other[keep] = q[keep]
+        c.dq = dev(other)
+        ops.shared_prefix_attention(c.desc())
+        assert np.array_equal(host(c.out)[keep].view(np.int16), first[keep]), f"sequence {keep}"
+
+
 def test_another_stream_and_graph_replays(ops, engine):
     """Captured once, replayed while counts grow in device memory, with eager calls of another shape between:
     every replay gives the eager call's bits."""
