@@ -305,7 +305,7 @@ struct PrefixPages {
         for (uint32_t w = 0; w < 4; ++w) {
             const float l = sl[w * 16u + i], f = l != 0.0f ? fast_exp2(sm[w * 16u + i] - M) : 0.0f;
             L = fmaf(f, l, L);
-            if (f != 0.0f)
+            if (l != 0.0f) // also where f is 0: an inf or NaN among the sums stays
 #pragma unroll
                 for (int h = 0; h < HD / 64; ++h) {
                     const float4_t x = *(const float4_t*)(so + (w * 16u + i) * P + 64 * h + d);
@@ -781,7 +781,7 @@ __global__ __launch_bounds__(kPrefixThreads) __attribute__((amdgpu_waves_per_eu(
 
 // Joins a row's parts: the largest maximum, each part's sums times 2^(its maximum -
 // that), added in an order of their own; zeros where no part saw a token.  An inf or NaN
-// in a part's sum stays in the result.  W waves a row (4 where rows are few, their sums
+// in a part's sum stays in the result, as NaN where the part's factor is 0.  W waves a row (4 where rows are few, their sums
 // added in the order of the waves); a row of a part is HD / 4 lanes' float4, U loads in
 // flight before the parts' factors are known.
 template <int HD, int U, int W>
@@ -806,6 +806,7 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a) {
     load(0);
     if (lane >= S) l = 0.0f;
     if (l == 0.0f) m = -INFINITY;
+    const uint64_t held = __ballot(l != 0.0f); // a part that saw nothing holds no sums
     const float M = wave_max(m);
     const float f = l != 0.0f ? fast_exp2(m - M) : 0.0f;
     const float L = wave_sum(f * l);
@@ -816,7 +817,7 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a) {
         for (int j = 0; j < U; ++j) {
             const uint32_t p = part(p0, j);
             const float fp = __shfl(f, (int)min(p, S - 1u));
-            if (p < S && fp != 0.0f) // a part that saw nothing holds no sums
+            if (p < S && ((held >> p) & 1u))
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[e] = fmaf(fp, v[j][e], acc[e]);
         }

@@ -265,6 +265,35 @@ def test_many_rows_behind_a_prefix(ops, engine, case):
     assert np.array_equal(np.isnan(host(c.out)), nan)
 
 
+@pytest.mark.parametrize("case,tile,parts", [
+    ((2, 1, 8, 2, 128, 100), 16, False), ((1, 1, 8, 2, 64, 480), 16, False), ((2, 1, 8, 2, 64, 1500), 16, True),
+    ((33, 1, 8, 2, 128, 1700), 128, True)], ids=["waves-128", "waves-64", "merged-pages", "merged-tiles"])
+def test_infinities_whose_weight_is_below_fp32(ops, engine, case, tile, parts):
+    """A token that every row sees, whose weight 2^-240 is 0 in fp32, holds an inf in one dim: that dim is not finite
+    (0 times inf, as in any fp32 softmax), wherever the token and the one that takes all of the weight lie."""
+    batch, queries, hq, hk, hd, prefix = case
+    own = [queries + b % 5 for b in range(batch)]
+    for heavy, far in ((3, 17), (3, prefix - 1), (prefix - 1, 3), (prefix - 1, prefix // 2)):
+        c = Case(62, *case, own, stale=False)
+        p = plan(c)
+        assert (p.prefix_splits > 1) == parts and p.row_tile == tile
+        at = lambda t: (c.prefix_refs[t // 16] & P.REF_MASK, t % 16)  # noqa: E731
+        c.k[:] = 0
+        c.q[..., 0] = 8.0
+        c.k[at(heavy)][:, 0] = 240.0 / 8.0 / np.log2(np.e) * hd ** 0.5
+        c.v[at(far)][:, 9] = np.inf
+        c.dq, c.dk, c.dv = dev(c.q), dev(c.k), dev(c.v)
+        ops.shared_prefix_attention(c.desc())
+        engine.check_device_errors()
+        got = host(c.out)
+        bad = np.zeros(got.shape, dtype=bool)
+        bad[..., 9] = True
+        assert np.array_equal(~np.isfinite(got), bad), (heavy, far)
+        want = np.broadcast_to(c.v[at(heavy)].repeat(hq // hk, axis=0), got.shape)
+        # the other weights together are below prefix 2^-240
+        assert np.array_equal(got[~bad], want[~bad]), (heavy, far)
+
+
 def test_rising_scores_beside_many_rows(ops, engine):
     """Scores that rise along the prefix, by steps below and above what the running maximum lets pass (2^8), up to
     weights that span far more than f16 does."""
