@@ -63,15 +63,12 @@ def places(tokens: int, batch: int, seq_hot, offsets, refs, hot_count: int, hot_
     return seq, place, row
 
 
-def shared_prefix_attention(q, hot_k, hot_v, prefix_refs, prefix_tokens: int, refs, seq_own, scale: float, causal: bool):
-    """q [batch][queries][q_heads][head_dim], pools [blocks][16][kv_heads][head_dim]; query i of Q sees
-    every prefix token and own tokens p < seq_own - Q + 1 + i (all of them where not causal).  Rows that
-    see nothing are zeros.  Out-of-range refs (>= blocks) hide their tokens."""
+def _seen_scores(q, hot_k, hot_v, prefix_refs, prefix_tokens: int, refs, seq_own, scale: float, causal: bool):
+    """((sequence, query, kv head), its heads' exp(score - largest), the values), of what each query sees."""
     q = np.asarray(q, dtype=np.float64)
     blocks, _, kv_heads, hd = hot_k.shape
     batch, queries, q_heads, _ = q.shape
     group = q_heads // kv_heads
-    out = np.zeros_like(q)
 
     def gather(table, tokens):
         at = np.asarray([(int(table[t // PAGE]) & REF_MASK, t % PAGE) for t in range(tokens)], dtype=np.int64).reshape(-1, 2)
@@ -91,6 +88,22 @@ def shared_prefix_attention(q, hot_k, hot_v, prefix_refs, prefix_tokens: int, re
             k, v = np.concatenate([pk, ok_])[see], np.concatenate([pv, ov])[see]
             for g in range(kv_heads):
                 s = q[b, i, g * group:(g + 1) * group] @ k[:, g].T * scale
-                w = np.exp(s - s.max(1, keepdims=True))
-                out[b, i, g * group:(g + 1) * group] = (w / w.sum(1, keepdims=True)) @ v[:, g]
+                yield (b, i, slice(g * group, (g + 1) * group)), np.exp(s - s.max(1, keepdims=True)), v[:, g]
+
+
+def shared_prefix_attention(q, hot_k, hot_v, prefix_refs, prefix_tokens: int, refs, seq_own, scale: float, causal: bool):
+    """q [batch][queries][q_heads][head_dim], pools [blocks][16][kv_heads][head_dim]; query i of Q sees
+    every prefix token and own tokens p < seq_own - Q + 1 + i (all of them where not causal).  Rows that
+    see nothing are zeros.  Out-of-range refs (>= blocks) hide their tokens."""
+    out = np.zeros(np.shape(q))
+    for at, w, v in _seen_scores(q, hot_k, hot_v, prefix_refs, prefix_tokens, refs, seq_own, scale, causal):
+        out[at] = (w / w.sum(1, keepdims=True)) @ v
     return out
+
+
+def shared_prefix_weight_sums(q, hot_k, prefix_refs, prefix_tokens: int, refs, seq_own, scale: float, causal: bool):
+    """[batch][queries][q_heads]: the sum of a row's weights where its largest is 1 (0 for a row that sees nothing)."""
+    total = np.zeros(np.shape(q)[:3])
+    for at, w, _ in _seen_scores(q, hot_k, hot_k, prefix_refs, prefix_tokens, refs, seq_own, scale, causal):
+        total[at] = w.sum(1)
+    return total

@@ -13,6 +13,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
+from helpers import LONG_PREFIXES, PREFIX_REL_L2, prefix_errors
 from oracle import paged_oracle as P
 
 pytestmark = pytest.mark.gpu
@@ -406,6 +407,23 @@ def test_parts_of_many_pages(ops, engine, case):
     got = host(c.out).astype(np.float64)[0]
     want = 60000.0 / n
     assert np.all(np.abs(got - want) <= want * (2.0 ** -11 + 2.0 ** -20) + 2.0 ** -25), (got.min(), got.max(), want)
+
+
+@pytest.mark.parametrize("shape", LONG_PREFIXES, ids=["many-rows", "few-rows", "own"])
+def test_no_page_of_a_long_prefix_is_lost(ops, engine, shape):
+    """Scores of standard deviation 1 / 4 over the same long parts, so that every page counts: within bounds that a
+    single page left out exceeds (test_the_bounds_of_long_prefixes_see_what_is_lost)."""
+    c = Case(48, *shape, qscale=0.25)
+    assert max(plan(c).prefix_tokens_per_split, plan(c).own_tokens_per_split) > 1024
+    ops.shared_prefix_attention(c.desc())
+    engine.check_device_errors()
+    want, absolute = c.want()
+    total = P.shared_prefix_weight_sums(c.q, c.k, c.prefix_refs, c.prefix, c.refs, c.own, c.shape[4] ** -0.5, c.causal)
+    got = host(c.out)
+    largest = float(np.abs(c.v[np.isfinite(c.v) & (np.abs(c.v) < 65504)]).max())
+    worst, rel = prefix_errors(got, want, absolute, total, c.prefix + int(c.own.max()), largest)
+    print(f"{shape[:6]}: worst error over tolerance {worst:.3f}, worst rel-L2 of a sequence {rel:.2e}", flush=True)
+    assert np.isfinite(got).all() and worst <= 1.0 and rel <= PREFIX_REL_L2
 
 
 @pytest.mark.parametrize("shape", [(2, 1100, 32, 8, 128, 300, [1400, 4096]), (1, 2600, 14, 2, 64, 1000, [2700])], ids=["two", "one"])

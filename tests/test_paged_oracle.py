@@ -4,6 +4,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
+from helpers import LONG_PREFIXES, PREFIX_REL_L2, prefix_errors
 from oracle import paged_oracle as P
 
 
@@ -64,6 +65,57 @@ def test_shared_prefix_attention_is_attention_over_each_sequence(causal):
         want = torch.nn.functional.scaled_dot_product_attention(torch.from_numpy(q[b]).transpose(0, 1).contiguous(), k, v,
                                                                 attn_mask=mask, scale=0.3)
         np.testing.assert_allclose(got[b], want.transpose(0, 1).numpy(), rtol=0, atol=1e-12)
+
+
+def test_weight_sums():
+    rng = np.random.default_rng(6)
+    pools = rng.standard_normal((2, 4, 16, 1, 8))
+    q = rng.standard_normal((2, 1, 2, 8))
+    got = P.shared_prefix_weight_sums(q, pools[0], [2], 5, [[1], [0]], [4, 0], 0.5, True)
+    for b, n in ((0, 4), (1, 0)):
+        k = np.concatenate([pools[0][2, :5, 0], pools[0][1 - b, :n, 0]])
+        s = q[b, 0] @ k.T * 0.5
+        np.testing.assert_allclose(got[b, 0], [sum(np.exp(x - max(row)) for x in row) for row in s], rtol=1e-12)
+    assert not P.shared_prefix_weight_sums(q, pools[0], [], 0, [[1], [0]], [0, 0], 0.5, True).any()
+
+
+@pytest.mark.parametrize("shape", LONG_PREFIXES, ids=["many-rows", "few-rows", "own"])
+def test_the_bounds_of_long_prefixes_see_what_is_lost(shape):
+    """Zeros, half of the tokens, and any single page left out miss the bounds that the GPU's outputs over these many
+    tokens are held to."""
+    batch, queries, hq, hk, hd, prefix, own = shape
+    rng = np.random.default_rng(34)
+    pages = [-(-n // 16) for n in own]
+    shared = -(-prefix // 16)
+    blocks = shared + sum(pages)
+    order = rng.permutation(blocks)
+    refs = np.full((batch, max(pages)), blocks)
+    for b, n in enumerate(pages):
+        refs[b, :n] = order[shared + sum(pages[:b]):][:n]
+    q = (rng.standard_normal((batch, queries, hq, hd)) * 0.25).astype(np.float16)
+    k, v = (rng.standard_normal((blocks, 16, hk, hd)).astype(np.float16) for _ in range(2))
+    shape = (batch, queries, hq, hd)
+    want, absolute, half, total = np.zeros(shape), np.zeros(shape), np.zeros(shape), np.zeros(shape[:3])
+    lost = [0.0] * batch  # squared error of a sequence for each page left out
+    for at, w, x in P._seen_scores(q, k, v, order[:shared], prefix, refs, own, hd ** -0.5, True):
+        tokens = w.shape[1]
+        total[at] = w.sum(1)
+        want[at], absolute[at] = w @ x / total[at][:, None], w @ np.abs(x) / total[at][:, None]
+        half[at] = w[:, :tokens // 2] @ x[:tokens // 2] / w[:, :tokens // 2].sum(1, keepdims=True)
+        first = np.concatenate([np.arange(0, prefix, 16), np.arange(prefix, tokens, 16)])
+        for h in range(w.shape[0]):
+            sums = np.add.reduceat(w[h][:, None] * x, first, axis=0)
+            rest = total[at][h] - np.add.reduceat(w[h], first)
+            lost[at[0]] = lost[at[0]] + (((want[at][h] * total[at][h] - sums) / rest[:, None] - want[at][h]) ** 2).sum(1)
+    n, largest = prefix + max(own), float(np.abs(v).max())
+    for what, got in (("zeros", np.zeros(shape)), ("half", half)):
+        worst, rel = prefix_errors(got, want, absolute, total, n, largest)
+        assert worst > 1.0 and rel > 2 * PREFIX_REL_L2, what
+    assert prefix_errors(want.astype(np.float16), want, absolute, total, n, largest)[0] < 1.0
+    for b in range(batch):
+        rel = np.sqrt(lost[b]) / np.linalg.norm(want[b])
+        print(f"sequence {b}: a page left out is {rel.min():.2e} to {rel.max():.2e} of the output", flush=True)
+        assert rel.min() > 2 * PREFIX_REL_L2
 
 
 def test_shared_prefix_rows_that_see_nothing_are_zeros():
