@@ -349,9 +349,9 @@ struct PrefixPages {
 //     (j < 4) or 8 + 4 hf + j - 4; A = V^T by transposing LDS reads.
 // Staged rows are HD / 8 16-byte chunks, chunk c of K row r at c ^ (r % chunks), of V
 // row r at c ^ 4 (r % 4) ^ (r / 4) % 4 (128 dims): no bank conflict at 128 dims.
-// Measured, 96 sequences of 32 / 8 heads x 128 behind 32768 tokens, 51.5 GFLOP: 81 us
-// alone, 636 TFLOP/s; its loads alone take 60 to 76 us,
-// its products and softmax alone 58 to 70, so it is bound by both at once.  32 or 128
+// Measured, 96 sequences of 32 / 8 heads x 128 behind 32768 tokens, 51.5 GFLOP: 86 us
+// alone, 600 TFLOP/s (81 with sums rescaled seldom, see below; then its loads alone took 60
+// to 76 us, its products and softmax alone 58 to 70), so it is bound by both at once.  32 or 128
 // tokens a step, 3 or 4 buffers, 256 rows of 8 waves, two of these work-groups a CU: each
 // slower there or for 64 sequences behind 8192 tokens.
 constexpr uint32_t kPrefixRows = 128;

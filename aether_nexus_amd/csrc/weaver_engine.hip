@@ -1029,9 +1029,9 @@ void prefix_parts(uint64_t items, uint64_t want, uint32_t tokens, uint32_t longe
 constexpr uint32_t kPrefixOneTokens = 512;
 // Up to this many values of K for all 16-row tiles that read the prefix, it is read in
 // PrefixPages' parts, once for each of them, else in PrefixTile's.  Measured, us, pages
-// and tiles: 32 rows x 128 dims of 8 heads, 600 tokens 8.2, 9.2; 1000 tokens 9.7, 9.7;
-// 8192 tokens 20.8, 16.1; 64 rows, 600 tokens 14.0, 11.4; 56 rows x 64 dims of 2 heads,
-// 4000 tokens 8.3, 9.2; 112 rows, 1500 tokens 8.0, 9.0.
+// and tiles, a token of their own each: 32 rows x 128 dims of 8 heads, 600 tokens 8.4, 9.7;
+// 1000 tokens 9.5, 9.9; 8192 tokens 20.5, 16.3; 64 rows, 600 tokens 10.3, 10.7; 56 rows x 64
+// dims of 2 heads, 4000 tokens 8.6, 9.8; 112 rows, 1500 tokens 8.4, 9.5.
 constexpr uint64_t kPrefixPagesValues = 2u << 20;
 
 // Bytes of parts' sums that more than one part of the own tokens may take: the parts of a

@@ -110,7 +110,8 @@ def rotary_frequencies(rotary_dim: int, theta: float, scaling: str = "none", fac
     theta^(-2p / rotary_dim), scaled for contexts longer than a model was trained on.
     ``scaling``: "none"; "linear" (divided by ``factor``); "ntk" (theta raised by
     factor^(d / (d - 2))); "parts" (pairs that turn more than ``high`` times over
-    ``original_length`` kept, fewer than ``low`` times divided, a ramp between).  No GPU needed."""
+    ``original_length`` kept, fewer than ``low`` times divided, a ramp over the turns between; for a
+    ramp over the pair's index pass ``Rotary`` an ``inv_freq`` of its own).  No GPU needed."""
     if scaling not in ROTARY_SCALINGS:
         raise WeaverError(f"rotary scaling {scaling!r} (one of {', '.join(ROTARY_SCALINGS)})", AW_E_INVALID_ARG)
     if rotary_dim < 2 or rotary_dim % 2 or rotary_dim >= 2 ** 32:

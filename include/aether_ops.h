@@ -145,7 +145,9 @@ int aw_ops_matmul_qkv(aw_engine* engine, const uint16_t* a, const uint16_t* b_q,
 #define AW_ROTARY_SCALE_NTK    2u /* theta * factor^(rotary_dim / (rotary_dim - 2)) for theta; rotary_dim > 2 */
 #define AW_ROTARY_SCALE_PARTS  3u /* (1 - g) f_p / factor + g f_p with g = clamp((r_p - low) / (high - low), 0, 1),
                                      r_p = original_length * f_p / (2 pi) the pair's turns over that length: pairs
-                                     that turn often are kept, those that turn less than `low` times interpolated */
+                                     that turn often are kept, those that turn less than `low` times interpolated.
+                                     The ramp is over turns; models whose ramp is over the pair's index, between
+                                     rounded bounds, pass frequencies of their own as inv_freq */
 
 typedef struct aw_rotary_scaling {
     uint32_t rotary_dim, kind;            /* AW_ROTARY_SCALE_* */
@@ -164,7 +166,7 @@ typedef struct aw_rotary_desc {
     uint32_t num_tokens, q_heads, kv_heads, head_dim; /* <= 2^24 tokens; head_dim <= 1024; either head count may be 0 */
     uint32_t rotary_dim;            /* even, <= head_dim: dims [0, rotary_dim) turn, the others pass */
     uint32_t layout;                /* AW_ROTARY_HALF or AW_ROTARY_INTERLEAVED */
-    uint32_t start_position;        /* of token 0, where positions is NULL */
+    uint32_t start_position;        /* of token 0, where positions is NULL; positions are taken modulo 2^32 */
     float    magnitude;             /* cosines and sines are multiplied by it (1: a plain rotation) */
     float    eps;                   /* aw_ops_qk_norm_rotary and appends with norms */
     uint32_t reserved;              /* 0 */
