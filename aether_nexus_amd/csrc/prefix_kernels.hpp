@@ -781,9 +781,9 @@ __global__ __launch_bounds__(kPrefixThreads) __attribute__((amdgpu_waves_per_eu(
 
 // Joins a row's parts: the largest maximum, each part's sums times 2^(its maximum -
 // that), added in an order of their own; zeros where no part saw a token.  An inf or NaN
-// in a part's sum stays in the result, as NaN where the part's factor is 0.  W waves a row (4 where rows are few, their sums
-// added in the order of the waves); a row of a part is HD / 4 lanes' float4, U loads in
-// flight before the parts' factors are known.
+// in a part's sum stays in the result, as NaN where the part's factor is 0.  W waves a
+// row (4 where rows are few, their sums added in the order of the waves); a row of a part
+// is HD / 4 lanes' float4, U loads in flight before the parts' factors are known.
 template <int HD, int U, int W>
 __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a) {
     constexpr int LP = HD / 4, PG = 64 / LP; // lanes of a part's row, parts of one load

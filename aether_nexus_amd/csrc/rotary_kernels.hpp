@@ -50,7 +50,7 @@ struct Place {
 // the same token; the offsets ascend, so it is found among 64 equal stretches of them at
 // a time: a round trip to L2 up to 64 sequences, two up to 4096, four up to 2^24, the
 // most that the host lets through.  Offsets that descend end the search as well, at
-// some sequence, and the checks below see that the token is not its own.
+// some sequence, and a token that is not within its rows is reported below.
 __device__ inline Place find_place(const RotaryArgs& a, uint32_t t, uint32_t lane, bool report) {
     uint32_t b, first, end;
     if (a.token_offsets) {
