@@ -44,6 +44,9 @@ SIGNATURES = {
     "aw_shared_prefix_plan": (_c_int, [_vp, _u32, _vp, ctypes.c_char_p, _sz]),
     "aw_shared_prefix_attention_device": (_c_int, [_vp, _vp, _vp]),
     "aw_abi_prefix_sizes": (None, [ctypes.POINTER(_sz)]),
+    "aw_tree_plan": (_c_int, [_vp, _u32, _vp, ctypes.c_char_p, _sz]),
+    "aw_tree_attention_device": (_c_int, [_vp, _vp, _vp]),
+    "aw_abi_tree_sizes": (None, [ctypes.POINTER(_sz)]),
     "aw_engine_check_device_errors": (_c_int, [_vp, _vp]),
     "aw_debug_product_tile": (_c_int, [_u32, _u32, _vp, _u32, _u32, _vp]),
     "aw_debug_gather_codes": (_c_int, [_vp, _vp, _sz, _vp, _u32, _u32, _vp, _vp, _vp, _vp]),
@@ -99,6 +102,13 @@ SIGNATURES = {
     "aw_ops_check_rotary": (_c_int, [_vp, _c_int, ctypes.c_char_p, _sz]),
     "aw_ops_check_append": (_c_int, [_vp, ctypes.c_char_p, _sz]),
     "aw_abi_ops_desc_sizes": (None, [ctypes.POINTER(_sz)]),
+    "aw_ops_page_tables": (_c_int, [_vp, _vp, _vp]),
+    "aw_ops_adjust_logits": (_c_int, [_vp, _vp, _vp]),
+    "aw_ops_accept_tree": (_c_int, [_vp, _vp, _vp]),
+    "aw_ops_check_tables": (_c_int, [_vp, ctypes.c_char_p, _sz]),
+    "aw_ops_check_logits": (_c_int, [_vp, ctypes.c_char_p, _sz]),
+    "aw_ops_check_accept": (_c_int, [_vp, ctypes.c_char_p, _sz]),
+    "aw_abi_step_desc_sizes": (None, [ctypes.POINTER(_sz)]),
 }
 
 _cache: dict[str, ctypes.CDLL] = {}

@@ -16,7 +16,8 @@ PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 SOURCES = [PKG / "csrc" / "weaver_engine.hip", PKG / "csrc" / "fabric.hip", PKG / "csrc" / "ops.hip"]
 DEPS = [PKG / "csrc" / "weaver_kernels.hpp", PKG / "csrc" / "prefill_kernels.hpp", PKG / "csrc" / "prefix_kernels.hpp", PKG / "csrc" / "ops_kernels.hpp",
-        PKG / "csrc" / "gemm_kernels.hpp", PKG / "csrc" / "rotary_kernels.hpp", PKG / "csrc" / "engine_internal.hpp",
+        PKG / "csrc" / "gemm_kernels.hpp", PKG / "csrc" / "rotary_kernels.hpp", PKG / "csrc" / "step_kernels.hpp", PKG / "csrc" / "tree_kernels.hpp",
+        PKG / "csrc" / "engine_internal.hpp",
         ROOT / "include" / "aether_weaver.h", ROOT / "include" / "aether_fabric.h", ROOT / "include" / "aether_ops.h"]
 OUT = PKG / "libaether_weaver.so"
 ARCH = "gfx950"

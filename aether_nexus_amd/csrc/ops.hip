@@ -3,7 +3,8 @@
 // Replaces the dispatch methods of the reference's Ops engine
 // (nexus-core/src/ops.rs:166-462); the kernels are in ops_kernels.hpp.  Beside them the
 // rows of a batch over pages, which the reference does not have: rotary positions, head
-// norms and appends (rotary_kernels.hpp).  Every entry point validates its arguments on
+// norms and appends (rotary_kernels.hpp), and a step over trees of drafted tokens: tables,
+// logits, acceptance (step_kernels.hpp).  Every entry point validates its arguments on
 // the host, picks the 16-byte vector variant of a kernel when the pointers and sizes allow
 // it, and enqueues on the caller's stream.  There is no CPU fallback.
 #include <hip/hip_runtime.h>
@@ -21,10 +22,14 @@
 #include "gemm_kernels.hpp"
 #include "ops_kernels.hpp"
 #include "rotary_kernels.hpp"
+#include "step_kernels.hpp"
 
 namespace {
 
 namespace ei = aw_engine_internal;
+using ei::Rows;
+using ei::rows_meet;
+using ei::rows_same;
 
 uint64_t cdiv64(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 bool aligned(const void* p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
@@ -219,27 +224,6 @@ int launch_products(aw_engine* e, const char* what, const uint16_t* a, const Pro
     return AW_OK;
 }
 
-// Rows [tokens][row] of a call, `stride` elements apart; none at a null address.
-struct Rows {
-    const uint16_t* at;
-    uint64_t stride, row, tokens;
-    bool none() const { return !at || row == 0 || tokens == 0; }
-    uintptr_t begin() const { return (uintptr_t)at; }
-    uintptr_t end() const { return (uintptr_t)at + 2 * ((tokens - 1) * stride + row); }
-};
-
-// Whether two such sets share an element: parts of one fused buffer, rows of the same
-// stride, lie at a fixed distance within it; with strides of their own the whole
-// stretches count.
-bool rows_meet(const Rows& p, const Rows& o) {
-    if (p.none() || o.none() || p.begin() >= o.end() || o.begin() >= p.end()) return false;
-    if (p.stride != o.stride) return true;
-    const Rows &lo = p.begin() < o.begin() ? p : o, &hi = p.begin() < o.begin() ? o : p;
-    const uint64_t stride = 2 * p.stride, d = (hi.begin() - lo.begin()) % stride;
-    return d < 2 * lo.row || d + 2 * hi.row > stride;
-}
-bool rows_same(const Rows& p, const Rows& o) { return p.at == o.at && (p.stride == o.stride || p.tokens == 1); }
-
 int refuse(char* msg, size_t len, int code, const char* fmt, ...) __attribute__((format(printf, 4, 5)));
 int refuse(char* msg, size_t len, int code, const char* fmt, ...) {
     if (msg && len) {
@@ -401,6 +385,250 @@ int launch_rotary(aw_engine* e, awo::RotaryArgs& a, hipStream_t st) {
     if (a.q_norm || a.k_norm) inter(std::true_type{});
     else inter(std::false_type{});
     OPS_HIP(e, hipGetLastError());
+    return AW_OK;
+}
+
+// A stretch of memory that a call reads or writes.
+struct Span {
+    const void* at;
+    uint64_t bytes;
+};
+bool spans_meet(const Span& p, const Span& o) {
+    const uintptr_t x = (uintptr_t)p.at, y = (uintptr_t)o.at;
+    return p.at && o.at && p.bytes && o.bytes && x < y + o.bytes && y < x + p.bytes;
+}
+// Whether an output meets an input or another output.
+template <size_t N, size_t M>
+bool outputs_meet(const Span (&out)[N], const Span (&in)[M]) {
+    for (size_t i = 0; i < N; ++i) {
+        for (size_t j = 0; j < i; ++j)
+            if (spans_meet(out[i], out[j])) return true;
+        for (const Span& x : in)
+            if (spans_meet(out[i], x)) return true;
+    }
+    return false;
+}
+
+constexpr uint32_t kMostStepSequences = 1u << 20;
+
+// What the three calls of a step ask of their rows; `what` begins the text.
+int step_rows(const char* what, uint32_t batch, uint32_t tokens, const void* offsets, bool divide, char* msg, size_t len) {
+    if (tokens > kMostTokens) return refuse(msg, len, AW_E_UNSUPPORTED, "%s: num_tokens %u exceeds 2^24", what, tokens);
+    if (batch > kMostStepSequences) return refuse(msg, len, AW_E_UNSUPPORTED, "%s: batch %u exceeds 2^20", what, batch);
+    if (divide && !offsets && batch && tokens % batch)
+        return refuse(msg, len, AW_E_INVALID_ARG, "%s: %u tokens over %u sequences need token_offsets", what, tokens, batch);
+    return AW_OK;
+}
+
+int tables_args(const aw_tables_desc* d, awo::TablesArgs* a, char* msg, size_t len) {
+    auto bad = [&](const char* why) { return refuse(msg, len, AW_E_INVALID_ARG, "page_tables: %s", why); };
+    if (!d) return bad("null descriptor");
+    if (int rc = step_rows("page_tables", d->batch, d->num_tokens, nullptr, false, msg, len)) return rc;
+    if (d->hot_count > 1u << 26) return refuse(msg, len, AW_E_UNSUPPORTED, "page_tables: hot_count %u exceeds 2^26", d->hot_count);
+    if (d->refs_stride < d->hot_count)
+        return refuse(msg, len, AW_E_INVALID_ARG, "page_tables: refs_stride %u < hot_count %u", d->refs_stride, d->hot_count);
+    if (d->free_count > 1u << 30) return refuse(msg, len, AW_E_UNSUPPORTED, "page_tables: free_count %u exceeds 2^30", d->free_count);
+    if (d->mask_words > AW_MAX_NODES / 32) return refuse(msg, len, AW_E_UNSUPPORTED, "page_tables: mask_words %u exceeds 32", d->mask_words);
+    if (!d->parents != !d->mask_words || !d->parents != !d->tree_mask) return bad("parents, mask_words and tree_mask go together");
+    if (!d->token_offsets || (d->batch && (!d->seq_held || !d->seq_new || !d->seq_hot || (d->hot_count && !d->refs))) ||
+        (d->free_count && !d->free_pages))
+        return bad("null pointer");
+    const uint64_t b = 4ull * d->batch, t = d->num_tokens;
+    const Span out[] = {{d->refs, d->batch ? 4ull * ((uint64_t)(d->batch - 1) * d->refs_stride + d->hot_count) : 0}, {d->seq_hot, b},
+                        {d->pages_out, b}, {d->token_offsets, b + 4}, {d->free_next, 4}, {d->slots, 8 * t}, {d->positions, 4 * t},
+                        {d->tree_mask, 4 * t * d->mask_words}};
+    const Span in[] = {{d->seq_held, b}, {d->seq_new, b}, {d->seq_pages, b}, {d->free_pages, 4ull * d->free_count}, {d->free_first, 4},
+                       {d->parents, 4 * t}};
+    if (outputs_meet(out, in)) return bad("an output overlaps an input or another output");
+    *a = awo::TablesArgs{};
+    a->batch = d->batch;
+    a->tokens = d->num_tokens;
+    a->hot_count = d->hot_count;
+    a->refs_stride = d->refs_stride;
+    a->free_count = d->free_count;
+    a->mask_words = d->mask_words;
+    a->seq_held = d->seq_held;
+    a->seq_new = d->seq_new;
+    a->seq_pages = d->seq_pages;
+    a->free_pages = d->free_pages;
+    a->free_first = d->free_first;
+    a->parents = d->parents;
+    a->refs = d->refs;
+    a->seq_hot = d->seq_hot;
+    a->pages_out = d->pages_out;
+    a->token_offsets = d->token_offsets;
+    a->free_next = d->free_next;
+    a->slots = d->slots;
+    a->positions = d->positions;
+    a->tree_mask = d->tree_mask;
+    return AW_OK;
+}
+
+int logits_args(const aw_logits_desc* d, awo::LogitsArgs* a, char* msg, size_t len) {
+    auto bad = [&](const char* why) { return refuse(msg, len, AW_E_INVALID_ARG, "adjust_logits: %s", why); };
+    auto over = [&](const char* why) { return refuse(msg, len, AW_E_UNSUPPORTED, "adjust_logits: %s", why); };
+    if (!d) return bad("null descriptor");
+    if (int rc = step_rows("adjust_logits", d->batch, d->num_tokens, d->token_offsets, true, msg, len)) return rc;
+    if (d->flags & ~AW_LOGITS_F16) return bad("unknown flags");
+    if (d->vocab_size == 0) return bad("vocab_size is 0");
+    if (d->vocab_size > 1u << 24) return over("vocab_size exceeds 2^24");
+    if (d->history_stride > 1u << 20) return over("history_stride exceeds 2^20");
+    if (d->bias_stride > 1023) return over("bias_stride exceeds 1023");
+    if (d->mask_words > AW_MAX_NODES / 32) return over("mask_words exceeds 32");
+    if (!d->out && !d->best) return bad("neither out nor best is asked for");
+    if (!d->logits && d->num_tokens) return bad("null pointer");
+    if ((d->history || d->repetition || d->frequency || d->presence || d->bias_ids || d->node_tokens || d->token_offsets) && !d->batch &&
+        d->num_tokens)
+        return bad("batch is 0");
+    if (d->history && !d->history_count) return bad("history needs history_count");
+    if (d->prompt_count && !d->history) return bad("prompt_count without history");
+    if (!d->node_tokens != !d->tree_mask || !d->node_tokens != !d->mask_words) return bad("node_tokens, tree_mask and mask_words go together");
+    if (!d->bias_ids != !d->bias_values || (d->bias_count && !d->bias_ids)) return bad("bias_ids and bias_values go together");
+    if (d->allowed_index && !d->allowed) return bad("allowed_index without allowed");
+    const uint32_t size = d->flags & AW_LOGITS_F16 ? 2u : 4u;
+    const uint64_t words = cdiv64(d->vocab_size, 32);
+    const uint64_t stride = d->logits_stride ? d->logits_stride : d->vocab_size, out_stride = d->out_stride ? d->out_stride : d->vocab_size;
+    const uint64_t allowed = d->allowed_stride ? d->allowed_stride : words;
+    if (stride < d->vocab_size || out_stride < d->vocab_size || allowed < words) return bad("a stride is shorter than a row");
+    if (stride > kMostStride || out_stride > kMostStride || allowed > kMostStride) return over("a stride exceeds 2^30 elements");
+    if (((uintptr_t)d->logits | (uintptr_t)d->out) & (size - 1u)) return refuse(msg, len, AW_E_ALIGN, "adjust_logits: rows at their elements' alignment");
+    if (d->allowed && !d->allowed_index && d->allowed_rows < d->num_tokens) return bad("fewer allowed rows than rows");
+    const uint64_t t = d->num_tokens, b = 4ull * d->batch;
+    auto rows = [&](uint64_t n, uint64_t s, uint64_t row) { return n ? (n - 1) * s + row : 0; };
+    const Span out[] = {{d->out, size * rows(t, out_stride, d->vocab_size)}, {d->best, 4 * t}};
+    const Span in[] = {{d->token_offsets, b + 4}, {d->history, b * d->history_stride}, {d->history_count, b}, {d->prompt_count, b}, {d->repetition, b},
+                       {d->frequency, b}, {d->presence, b}, {d->node_tokens, 4 * t}, {d->tree_mask, 4 * t * d->mask_words},
+                       {d->bias_ids, b * d->bias_stride}, {d->bias_values, b * d->bias_stride}, {d->bias_count, b},
+                       {d->allowed, 4 * rows(d->allowed_rows, allowed, words)}, {d->allowed_index, 4 * t},
+                       {d->out == d->logits && stride == out_stride ? nullptr : d->logits, size * rows(t, stride, d->vocab_size)}};
+    if (outputs_meet(out, in) || spans_meet(out[1], {d->logits, size * rows(t, stride, d->vocab_size)}))
+        return bad("an output overlaps an input or another output");
+    *a = awo::LogitsArgs{};
+    a->rows = d->num_tokens;
+    a->vocab = d->vocab_size;
+    a->batch = d->batch;
+    a->mask_words = d->mask_words;
+    a->history_stride = d->history_stride;
+    a->bias_stride = d->bias_stride;
+    a->allowed_rows = d->allowed_rows;
+    a->logits_stride = stride;
+    a->out_stride = out_stride;
+    a->allowed_stride = allowed;
+    a->logits = d->logits;
+    a->out = d->out;
+    a->best = d->best;
+    a->token_offsets = d->token_offsets;
+    a->history = d->history_stride ? d->history : nullptr;
+    a->history_count = d->history_count;
+    a->prompt_count = d->prompt_count;
+    a->repetition = d->repetition;
+    a->frequency = d->frequency;
+    a->presence = d->presence;
+    a->node_tokens = d->node_tokens;
+    a->tree_mask = d->tree_mask;
+    a->bias_ids = d->bias_stride ? d->bias_ids : nullptr;
+    a->bias_values = d->bias_values;
+    a->bias_count = d->bias_count;
+    a->allowed = d->allowed;
+    a->allowed_index = d->allowed_index;
+    if (!a->history && !a->node_tokens && !a->bias_ids && !a->token_offsets) a->batch = 0; // nothing is counted: the rows stand for themselves
+    return AW_OK;
+}
+
+int accept_args(const aw_accept_desc* d, awo::AcceptArgs* a, char* msg, size_t len) {
+    auto bad = [&](const char* why) { return refuse(msg, len, AW_E_INVALID_ARG, "accept_tree: %s", why); };
+    auto over = [&](const char* why) { return refuse(msg, len, AW_E_UNSUPPORTED, "accept_tree: %s", why); };
+    if (!d) return bad("null descriptor");
+    if (int rc = step_rows("accept_tree", d->batch, d->num_tokens, d->token_offsets, true, msg, len)) return rc;
+    if (d->layers > 65535u) return over("layers exceed 65535");
+    if (d->history_stride > 1u << 30) return over("history_stride exceeds 2^30");
+    const uint64_t t = d->num_tokens, b = 4ull * d->batch, row = (uint64_t)d->kv_heads * d->head_dim;
+    if (d->batch && (!d->seq_held || !d->accepted || !d->next_token || !d->seq_hot)) return bad("null pointer");
+    if (d->batch && t && (!d->parents || !d->node_tokens || !d->targets || !d->path)) return bad("null pointer");
+    if (!d->history != !d->history_count || !d->history != !d->history_count_out) return bad("history and its two counts go together");
+    uint64_t ks = d->k_stride ? d->k_stride : row, vs = d->v_stride ? d->v_stride : row;
+    uint64_t kl = d->k_layer_stride ? d->k_layer_stride : t * ks, vl = d->v_layer_stride ? d->v_layer_stride : t * vs;
+    uint64_t hl = d->hot_layer_stride ? d->hot_layer_stride : d->hot_blocks * awo::kPageTokens * row;
+    Span k{}, v{}, hk{}, hv{};
+    if (d->layers) {
+        if (row == 0) return bad("kv_heads or head_dim is 0");
+        if (row > 1u << 20) return over("a token's row exceeds 2^20 values");
+        if (t && (!d->k || !d->hot_k || !d->slots)) return bad("null pointer");
+        if (!d->v != !d->hot_v) return bad("v and hot_v go together");
+        if (d->hot_blocks == 0) return bad("hot_blocks is 0");
+        if (d->hot_blocks > 1ull << 31) return bad("hot_blocks exceeds 2^31, the refs' range");
+        if (ks < row || vs < row || (d->layers > 1 && hl < d->hot_blocks * awo::kPageTokens * row)) return bad("a stride is shorter than what it steps over");
+        if (std::max(ks, vs) > kMostStride || std::max({kl, vl, hl}) > 1ull << 46) return over("a stride is too long");
+        const uint64_t rows = t ? (t - 1) : 0, pool = 2 * ((d->layers - 1) * hl + d->hot_blocks * awo::kPageTokens * row);
+        k = {d->k, t ? 2 * ((d->layers - 1) * kl + rows * ks + row) : 0};
+        v = {d->v, t ? 2 * ((d->layers - 1) * vl + rows * vs + row) : 0};
+        hk = {d->hot_k, pool};
+        hv = {d->hot_v, pool};
+    }
+    const uint64_t hist = b * d->history_stride;
+    const Span out[] = {hk, hv, {d->accepted, b}, {d->next_token, b}, {d->seq_hot, b}, {d->path, 4 * t}, {d->history, hist}, {d->history_count_out, b}};
+    const Span in[] = {k, v, {d->parents, 4 * t}, {d->node_tokens, 4 * t}, {d->targets, 4 * t}, {d->token_offsets, b + 4},
+                       {d->seq_held == d->seq_hot ? nullptr : d->seq_held, b}, {d->slots, 8 * t},
+                       {d->history_count == d->history_count_out ? nullptr : d->history_count, b}};
+    if (outputs_meet(out, in)) return bad("an output overlaps an input or another output");
+    // The two inputs that an output may be are nobody else's.
+    for (const Span& o : out)
+        if ((o.at != d->seq_hot && spans_meet(o, {d->seq_held, b})) || (o.at != d->history_count_out && spans_meet(o, {d->history_count, b})))
+            return bad("an output overlaps an input or another output");
+    *a = awo::AcceptArgs{};
+    a->batch = d->batch;
+    a->tokens = d->num_tokens;
+    a->layers = d->layers;
+    a->row = (uint32_t)row;
+    a->history_stride = d->history_stride;
+    a->hot_blocks = d->hot_blocks;
+    a->k_stride = ks;
+    a->v_stride = vs;
+    a->k_layer = kl;
+    a->v_layer = vl;
+    a->hot_layer = hl;
+    a->parents = d->parents;
+    a->node_tokens = d->node_tokens;
+    a->targets = d->targets;
+    a->token_offsets = d->token_offsets;
+    a->seq_held = d->seq_held;
+    a->slots = d->slots;
+    a->k = d->k;
+    a->v = d->v;
+    a->hot_k = d->hot_k;
+    a->hot_v = d->hot_v;
+    a->accepted = d->accepted;
+    a->next_token = d->next_token;
+    a->seq_hot = d->seq_hot;
+    a->path = d->path;
+    a->history = d->history;
+    a->history_count = d->history_count;
+    a->history_count_out = d->history_count_out;
+    return AW_OK;
+}
+
+template <typename T, int IT>
+int launch_logits(aw_engine* e, awo::LogitsArgs& a, hipStream_t st) {
+    const uint32_t slice = 256u * (16u / (uint32_t)sizeof(T)) * IT;
+    const bool words = a.history || a.node_tokens || a.bias_ids;
+    a.slices = (uint32_t)cdiv64(a.vocab, slice);
+    a.group = 1;
+    const uint64_t grid = cdiv64(a.rows, a.group) * a.slices;
+    if (grid > 0xFFFFFFull) return ei::fail(e, AW_E_UNSUPPORTED, "adjust_logits: too many rows"); // 256 threads each, below 2^32
+    if (a.best && a.slices > 1) {
+        void* keys = nullptr;
+        if (int rc = ei::workspace(e, 8ull * a.rows * a.slices, st, &keys)) return rc;
+        a.keys = (uint64_t*)keys;
+    }
+    if (words)
+        hipLaunchKernelGGL((awo::logits_kernel<T, IT, true>), dim3((uint32_t)grid), dim3(256), 0, st, a);
+    else
+        hipLaunchKernelGGL((awo::logits_kernel<T, IT, false>), dim3((uint32_t)grid), dim3(256), 0, st, a);
+    OPS_HIP(e, hipGetLastError());
+    if (a.best && a.slices > 1) {
+        hipLaunchKernelGGL(awo::logits_best_kernel, dim3((uint32_t)cdiv64(a.rows, 4)), dim3(256), 0, st, a);
+        OPS_HIP(e, hipGetLastError());
+    }
     return AW_OK;
 }
 
@@ -665,6 +893,73 @@ void aw_abi_ops_desc_sizes(size_t sizes[3]) {
     sizes[0] = sizeof(aw_rotary_scaling);
     sizes[1] = sizeof(aw_rotary_desc);
     sizes[2] = sizeof(aw_append_desc);
+}
+
+int aw_ops_check_tables(const aw_tables_desc* d, char* msg, size_t msg_len) {
+    awo::TablesArgs a;
+    return tables_args(d, &a, msg, msg_len);
+}
+
+int aw_ops_check_logits(const aw_logits_desc* d, char* msg, size_t msg_len) {
+    awo::LogitsArgs a;
+    return logits_args(d, &a, msg, msg_len);
+}
+
+int aw_ops_check_accept(const aw_accept_desc* d, char* msg, size_t msg_len) {
+    awo::AcceptArgs a;
+    return accept_args(d, &a, msg, msg_len);
+}
+
+int aw_ops_page_tables(aw_engine* e, const aw_tables_desc* d, void* stream) {
+    int rc = enter(e);
+    if (rc) return rc;
+    awo::TablesArgs a;
+    char msg[256] = {0};
+    if ((rc = tables_args(d, &a, msg, sizeof msg))) return ei::fail(e, rc, "%s", msg);
+    a.err = ei::error_word(e);
+    const dim3 grid((uint32_t)std::max<uint64_t>(1, cdiv64(a.tokens, awo::kTablesRows)));
+    if (a.parents)
+        hipLaunchKernelGGL(awo::tables_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, a);
+    else
+        hipLaunchKernelGGL(awo::tables_kernel<false>, grid, dim3(256), 0, (hipStream_t)stream, a);
+    OPS_HIP(e, hipGetLastError());
+    return AW_OK;
+}
+
+int aw_ops_adjust_logits(aw_engine* e, const aw_logits_desc* d, void* stream) {
+    int rc = enter(e);
+    if (rc) return rc;
+    awo::LogitsArgs a;
+    char msg[256] = {0};
+    if ((rc = logits_args(d, &a, msg, sizeof msg))) return ei::fail(e, rc, "%s", msg);
+    if (a.rows == 0) return AW_OK;
+    a.err = ei::error_word(e);
+    return d->flags & AW_LOGITS_F16 ? launch_logits<_Float16, 2>(e, a, (hipStream_t)stream) : launch_logits<float, 4>(e, a, (hipStream_t)stream);
+}
+
+int aw_ops_accept_tree(aw_engine* e, const aw_accept_desc* d, void* stream) {
+    int rc = enter(e);
+    if (rc) return rc;
+    awo::AcceptArgs a;
+    char msg[256] = {0};
+    if ((rc = accept_args(d, &a, msg, sizeof msg))) return ei::fail(e, rc, "%s", msg);
+    if (a.batch == 0) return AW_OK;
+    a.err = ei::error_word(e);
+    const dim3 grid(a.batch, std::max(a.layers, 1u));
+    const bool vec = aligned(a.k, 16) && aligned(a.v, 16) && aligned(a.hot_k, 16) && aligned(a.hot_v, 16) &&
+                     (a.row | a.k_stride | a.v_stride | a.k_layer | a.v_layer | a.hot_layer) % 8 == 0;
+    if (vec)
+        hipLaunchKernelGGL(awo::accept_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, a);
+    else
+        hipLaunchKernelGGL(awo::accept_kernel<false>, grid, dim3(256), 0, (hipStream_t)stream, a);
+    OPS_HIP(e, hipGetLastError());
+    return AW_OK;
+}
+
+void aw_abi_step_desc_sizes(size_t sizes[3]) {
+    sizes[0] = sizeof(aw_tables_desc);
+    sizes[1] = sizeof(aw_logits_desc);
+    sizes[2] = sizeof(aw_accept_desc);
 }
 
 int aw_debug_product_tile(uint32_t compute_units, uint32_t m, const uint32_t* n, uint32_t products, uint32_t k,

@@ -19,6 +19,7 @@
 #include "engine_internal.hpp"
 #include "prefill_kernels.hpp"
 #include "prefix_kernels.hpp"
+#include "tree_kernels.hpp"
 #include "weaver_kernels.hpp"
 
 static_assert(sizeof(aw_sparse_code) == 16, "SparseCode is 16 bytes (types.rs:227)");
@@ -1165,6 +1166,99 @@ int launch_prefix(aw_engine* e, aw::PrefixArgs& a, hipStream_t st) {
     return AW_OK;
 }
 
+// ---- trees of drafted tokens over pages --------------------------------------------
+
+using aw_engine_internal::rows_meet;
+using aw_engine_internal::rows_same;
+
+// Checks a request and fills its kernel arguments but for addresses of scratch.
+int tree_plan(const aw_tree_desc* d, uint32_t n_cu, aw::TreeArgs* out, aw_tree_plan_info* info, char* msg, size_t len) {
+    auto refuse = [&](int code, const char* why) {
+        put_msg(msg, len, "tree_attention: %s", why);
+        return code;
+    };
+    if (!d) return refuse(AW_E_INVALID_ARG, "null descriptor");
+    if (d->reserved) return refuse(AW_E_INVALID_ARG, "reserved must be 0");
+    if (d->batch == 0) return refuse(AW_E_INVALID_ARG, "batch must be >= 1");
+    if (d->kv_heads == 0 || d->q_heads == 0 || d->q_heads % d->kv_heads)
+        return refuse(AW_E_INVALID_ARG, "q_heads must be a positive multiple of kv_heads");
+    if (!supported_head_dim(d->head_dim)) return refuse(AW_E_UNSUPPORTED, "head_dim must be 64 or 128");
+    if (!std::isfinite(d->scale * aw::kLog2e)) return refuse(AW_E_INVALID_ARG, "scale must be finite, and times log2 e too");
+    if (d->batch > 1u << 20) return refuse(AW_E_UNSUPPORTED, "batch exceeds 2^20");
+    if (d->hot_count > 1u << 18) return refuse(AW_E_UNSUPPORTED, "too many tokens");
+    if (d->refs_stride < d->hot_count) return refuse(AW_E_INVALID_ARG, "refs_stride is less than hot_count");
+    if (d->mask_words > 32u) return refuse(AW_E_UNSUPPORTED, "mask_words exceeds 32");
+    if (!d->tree_mask != !d->mask_words) return refuse(AW_E_INVALID_ARG, "tree_mask and mask_words go together");
+    const uint64_t gqa = d->q_heads / d->kv_heads, n = d->num_tokens;
+    if (n > 1u << 24 || gqa > 1u << 16 || n * d->q_heads > 1u << 25) return refuse(AW_E_UNSUPPORTED, "too many query rows");
+    if ((uint64_t)d->kv_heads * d->head_dim > 1u << 16) return refuse(AW_E_UNSUPPORTED, "too many kv heads");
+    if (!d->token_offsets && d->num_tokens % d->batch) return refuse(AW_E_INVALID_ARG, "tokens that the sequences do not share equally need token_offsets");
+    if (n && (!d->q || !d->k || !d->out)) return refuse(AW_E_INVALID_ARG, "q, k and out are required");
+    if (d->hot_count && (!d->refs || !d->hot_k || !d->seq_held || d->hot_blocks == 0))
+        return refuse(AW_E_INVALID_ARG, "refs, seq_held, hot_k and hot_blocks are required");
+    if (d->hot_count ? !d->v != !d->hot_v : d->hot_v && !d->v) return refuse(AW_E_INVALID_ARG, "v and hot_v go together");
+    if (d->hot_blocks > 1ull << 31) return refuse(AW_E_INVALID_ARG, "hot_blocks exceeds 2^31, the refs' range");
+    const uint64_t q_row = (uint64_t)d->q_heads * d->head_dim, k_row = (uint64_t)d->kv_heads * d->head_dim;
+    aw::TreeArgs& a = *out;
+    a = aw::TreeArgs{};
+    a.q_stride = d->q_stride ? d->q_stride : q_row;
+    a.k_stride = d->k_stride ? d->k_stride : k_row;
+    a.v_stride = d->v_stride ? d->v_stride : k_row;
+    a.out_stride = d->out_stride ? d->out_stride : q_row;
+    if (a.q_stride < q_row || a.k_stride < k_row || a.v_stride < k_row || a.out_stride < q_row)
+        return refuse(AW_E_INVALID_ARG, "a stride is shorter than a token's heads");
+    if (std::max(std::max(a.q_stride, a.k_stride), std::max(a.v_stride, a.out_stride)) > 1ull << 30)
+        return refuse(AW_E_UNSUPPORTED, "a stride exceeds 2^30 elements");
+    if ((((uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v | (uintptr_t)d->hot_k | (uintptr_t)d->hot_v) & 15u) ||
+        ((a.q_stride | a.k_stride | a.v_stride) & 7u))
+        return refuse(AW_E_ALIGN, "q, k, v and the pools must be 16-byte aligned, their strides multiples of 8 elements");
+    if (((uintptr_t)d->out & 7u) || (a.out_stride & 3u)) return refuse(AW_E_ALIGN, "out must be 8-byte aligned, its stride a multiple of 4 elements");
+    const aw_engine_internal::Rows q{d->q, a.q_stride, q_row, n}, o{d->out, a.out_stride, q_row, n};
+    const aw_engine_internal::Rows k{d->k, a.k_stride, k_row, n}, v{d->v, a.v_stride, k_row, n};
+    if ((!rows_same(q, o) && rows_meet(q, o)) || rows_meet(o, k) || rows_meet(o, v)) return refuse(AW_E_INVALID_ARG, "out overlaps q, k or v, and is not q");
+    if (d->hot_count) {
+        const uint64_t pool = d->hot_blocks * kBlock * k_row;
+        for (const uint16_t* p : {d->hot_k, d->hot_v})
+            if (rows_meet(o, {p, pool, pool, 1})) return refuse(AW_E_INVALID_ARG, "out overlaps a pool");
+    }
+    const uintptr_t ob = o.begin(), oe = n ? o.end() : ob;
+    auto meets = [&](const void* p, uint64_t bytes) { return p && bytes && (uintptr_t)p < oe && ob < (uintptr_t)p + bytes; };
+    if (meets(d->refs, d->hot_count ? 4ull * ((uint64_t)(d->batch - 1) * d->refs_stride + d->hot_count) : 0) || meets(d->seq_held, 4ull * d->batch) ||
+        meets(d->token_offsets, 4ull * d->batch + 4) || meets(d->tree_mask, 4ull * n * d->mask_words))
+        return refuse(AW_E_INVALID_ARG, "out overlaps a table");
+    a.q = d->q;
+    a.k = d->k;
+    a.v = d->v ? d->v : d->k;
+    a.hk = d->hot_k;
+    a.hv = d->hot_v ? d->hot_v : d->hot_k;
+    a.refs = d->refs;
+    a.seq_held = d->hot_count ? d->seq_held : nullptr;
+    a.token_offsets = d->token_offsets;
+    a.mask = d->tree_mask;
+    a.out = d->out;
+    a.blocks = d->hot_blocks;
+    a.batch = d->batch;
+    a.tokens = d->num_tokens;
+    a.q_heads = d->q_heads;
+    a.kv_heads = d->kv_heads;
+    a.gqa = (uint32_t)gqa;
+    a.hot_count = d->hot_count;
+    a.refs_stride = d->refs_stride;
+    a.mask_words = d->mask_words;
+    a.scale_log2 = d->scale * aw::kLog2e;
+    (void)n_cu;
+    if (info) *info = aw_tree_plan_info{};
+    return AW_OK;
+}
+
+template <int HD>
+int launch_tree(aw_engine* e, aw::TreeArgs& a, hipStream_t st) {
+    StageTimer t(e, AW_STAGE_HOT, st);
+    hipLaunchKernelGGL(aw::tree_row_kernel<HD>, dim3(a.tokens, a.q_heads), dim3(256), 0, st, a);
+    AW_HIP(e, hipGetLastError());
+    return AW_OK;
+}
+
 template <typename F>
 int check_kernel(aw_engine* e, F* fn, const char* name) {
     hipFuncAttributes attr;
@@ -1616,6 +1710,30 @@ void aw_abi_prefix_sizes(size_t sizes[2]) {
     sizes[1] = sizeof(aw_prefix_plan_info);
 }
 
+int aw_tree_plan(const aw_tree_desc* d, uint32_t compute_units, aw_tree_plan_info* info, char* msg, size_t mlen) {
+    aw::TreeArgs a;
+    return tree_plan(d, compute_units ? compute_units : 256, &a, info, msg, mlen);
+}
+
+int aw_tree_attention_device(aw_engine* e, const aw_tree_desc* d, void* stream) {
+    if (!e) return AW_E_INVALID_ARG;
+    aw::TreeArgs a;
+    aw_tree_plan_info info;
+    char msg[256] = {0};
+    int rc = tree_plan(d, e->n_cu, &a, &info, msg, sizeof msg);
+    if (rc) return fail(e, rc, "%s", msg);
+    if (!a.tokens) return AW_OK;
+    AW_HIP(e, hipSetDevice(e->device));
+    a.err = e->err;
+    hipStream_t st = (hipStream_t)stream; // NULL is HIP's null stream
+    return d->head_dim == 64 ? launch_tree<64>(e, a, st) : launch_tree<128>(e, a, st);
+}
+
+void aw_abi_tree_sizes(size_t sizes[2]) {
+    sizes[0] = sizeof(aw_tree_desc);
+    sizes[1] = sizeof(aw_tree_plan_info);
+}
+
 int aw_engine_check_device_errors(aw_engine* e, void* stream) {
     if (!e) return AW_E_INVALID_ARG;
     AW_HIP(e, hipSetDevice(e->device));
@@ -1626,11 +1744,12 @@ int aw_engine_check_device_errors(aw_engine* e, void* stream) {
     if (!word) return AW_OK;
     AW_HIP(e, hipMemsetAsync(e->err, 0, 4, st));
     AW_HIP(e, hipStreamSynchronize(st));
-    return fail(e, AW_E_OOB, "device saw out-of-range input:%s%s%s%s%s (the affected tokens or terms were skipped)",
+    return fail(e, AW_E_OOB, "device saw out-of-range input:%s%s%s%s%s%s (the affected tokens or terms were skipped)",
                 (word & aw::kErrHotRef) ? " hot block ref" : "", (word & aw::kErrColdRef) ? " cold block ref" : "",
                 (word & aw::kErrAtom) ? " atom index" : "",
                 (word & aw_engine_internal::kErrTokenBit) ? " token id" : "",
-                (word & aw_engine_internal::kErrSeqBit) ? " sequence length" : "");
+                (word & aw_engine_internal::kErrSeqBit) ? " sequence length" : "",
+                (word & aw_engine_internal::kErrFreeBit) ? " free pages" : "");
 }
 
 
@@ -1977,6 +2096,11 @@ int fail(aw_engine* e, int code, const char* fmt, ...) {
     va_end(ap);
     if (e) e->last_error = buf;
     return code;
+}
+int workspace(aw_engine* e, size_t bytes, void* stream, void** at) {
+    const int rc = ensure_keep(e->ws, bytes, e->retired_ws, e->last_error, (hipStream_t)stream);
+    *at = e->ws.ptr;
+    return rc;
 }
 
 } // namespace aw_engine_internal

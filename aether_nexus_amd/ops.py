@@ -12,7 +12,9 @@ anything is enqueued (the C ABI takes raw pointers).
 Beside them, without a counterpart in the reference, what a batch over pages needs:
 ``rotary``, ``qk_norm_rotary``, ``append_paged`` and ``shared_prefix_attention``, each
 of a descriptor (``make_rotary_desc``, ``make_append_desc``, ``make_prefix_desc``) that
-is checked once and may be used again.
+is checked once and may be used again; and a step over trees of drafted tokens, without the
+host in between: ``page_tables``, ``tree_attention``, ``adjust_logits`` and ``accept_tree``
+(``make_tables_desc``, ``make_tree_desc``, ``make_logits_desc``, ``make_accept_desc``).
 """
 from __future__ import annotations
 
@@ -23,8 +25,8 @@ from typing import Optional
 import numpy as np
 
 from . import _lib
-from .types import (AW_F_CAUSAL, BLOCK_SIZE, ROTARY_SCALINGS, AppendDesc, PrefixDesc, PrefixPlanInfo, RotaryDesc,
-                    RotaryScaling)
+from .types import (AW_F_CAUSAL, AW_LOGITS_F16, BLOCK_SIZE, ROTARY_SCALINGS, AcceptDesc, AppendDesc, LogitsDesc, PrefixDesc,
+                    PrefixPlanInfo, RotaryDesc, RotaryScaling, TablesDesc, TreeDesc, TreePlanInfo)
 from .weaver import WeaverEngine, WeaverError, _ptr, _stream
 
 AW_E_INVALID_ARG = -1
@@ -69,6 +71,7 @@ _f16 = _checker("float16", "int16")  # f16 values or their bit patterns
 _f32 = _checker("float32")
 _u32 = _checker("int32")
 _f64 = _checker("float64")
+_i64 = _checker("int64")
 
 
 def _counts(**values) -> None:
@@ -184,7 +187,7 @@ def make_rotary_desc(*, num_tokens: int, q_heads: int, kv_heads: int, head_dim: 
 def _table(refs, batch: int, count: int, stride: Optional[int], what: str) -> int:
     """Row stride of a block table [batch][>= count]."""
     if hasattr(refs, "dim") and refs.dim() == 2:
-        if refs.shape[0] < batch or refs.shape[1] < count or (refs.shape[1] > 1 and refs.stride(1) != 1) or \
+        if refs.shape[0] < batch or refs.shape[1] < count or (batch and refs.shape[1] > 1 and refs.stride(1) != 1) or \
                 (batch > 1 and refs.stride(0) < count):
             raise WeaverError(f"{what}: a table of [{batch}][{count}] entries is read, got shape {tuple(refs.shape)}, "
                               f"strides {tuple(refs.stride())}", AW_E_INVALID_ARG)
@@ -274,6 +277,205 @@ def prefix_plan(desc: PrefixDesc, compute_units: int = 0, lib_path=None) -> Pref
     if rc:
         raise WeaverError(msg.value.decode(), rc)
     return info
+
+
+def _columns(t, rows: int, given: Optional[int], what: str) -> int:
+    """Words of each of ``rows`` rows of a contiguous 2-D int32 tensor, or as given for a raw pointer."""
+    if t is None:
+        return 0
+    if given is None:
+        if not hasattr(t, "dim") or t.dim() != 2:
+            raise WeaverError(f"{what}: its row length is required without a 2-D tensor", AW_E_INVALID_ARG)
+        given = t.shape[1]
+    return given
+
+
+def make_tables_desc(*, batch: int, num_tokens: int, seq_held, seq_new, refs, seq_hot, token_offsets, free_pages=None,
+                     seq_pages=None, free_first=None, pages_out=None, free_next=None, slots=None, positions=None, parents=None,
+                     tree_mask=None, hot_count: Optional[int] = None, refs_stride: Optional[int] = None,
+                     free_count: Optional[int] = None, mask_words: Optional[int] = None) -> TablesDesc:
+    """An ``aw_tables_desc`` from device tensors (or raw device pointers), for ``page_tables``.
+    ``refs`` [batch][refs_stride] is continued in place; ``hot_count`` (entries of a row) defaults to a
+    2-D table's columns, ``free_count`` to the free list's length, ``mask_words`` to the columns of
+    ``tree_mask`` [num_tokens][mask_words].  ``slots`` is int64, everything else int32."""
+    d = TablesDesc()
+    if hot_count is None:
+        if not hasattr(refs, "dim") or refs.dim() != 2:
+            raise WeaverError("page_tables: hot_count is required without a 2-D table", AW_E_INVALID_ARG)
+        hot_count = refs.shape[1]
+    if free_count is None:
+        if free_pages is not None and not hasattr(free_pages, "numel"):
+            raise WeaverError("page_tables: free_count is required for a raw pointer", AW_E_INVALID_ARG)
+        free_count = 0 if free_pages is None else free_pages.numel()
+    words = _columns(tree_mask, num_tokens, mask_words, "page_tables tree_mask")
+    _counts(batch=batch, num_tokens=num_tokens, hot_count=hot_count, refs_stride=refs_stride or 0, free_count=free_count, mask_words=words)
+    d.batch, d.num_tokens, d.hot_count, d.free_count, d.mask_words = batch, num_tokens, hot_count, free_count, words
+    d.refs_stride = _table(refs, batch, hot_count, refs_stride, "refs")
+    tensors = dict(seq_held=(seq_held, batch), seq_new=(seq_new, batch), seq_pages=(seq_pages, batch), free_pages=(free_pages, free_count),
+                   free_first=(free_first, 1), parents=(parents, num_tokens), seq_hot=(seq_hot, batch), pages_out=(pages_out, batch),
+                   token_offsets=(token_offsets, batch + 1), free_next=(free_next, 1), positions=(positions, num_tokens),
+                   tree_mask=(tree_mask, num_tokens * words))
+    for name, (t, need) in tensors.items():
+        _u32(t, need, name)
+        setattr(d, name, _ptr(t))
+    _i64(slots, num_tokens, "slots")
+    d.refs, d.slots = _ptr(refs), _ptr(slots)
+    _one_device(d, [refs, slots] + [t for t, _ in tensors.values()])
+    return d
+
+
+def make_tree_desc(*, batch: int, num_tokens: int, q_heads: int, kv_heads: int, head_dim: int, q, k, out, v=None, hot_k=None,
+                   hot_v=None, refs=None, seq_held=None, token_offsets=None, tree_mask=None, mask_words: Optional[int] = None,
+                   hot_count: Optional[int] = None, refs_stride: Optional[int] = None, hot_blocks: Optional[int] = None,
+                   scale: Optional[float] = None) -> TreeDesc:
+    """An ``aw_tree_desc`` from device tensors (or raw device pointers to contiguous rows), for
+    ``tree_attention``: q, k, v and out are rows [num_tokens][heads][head_dim] (views of a fused product's
+    rows too), ``refs`` the block table of the ``seq_held`` tokens that each sequence has in pages,
+    ``tree_mask`` the bits of ``page_tables`` (None: a chain).  ``scale`` defaults to 1 / sqrt(head_dim)."""
+    d = TreeDesc()
+    if hot_count is None:
+        if refs is not None and (not hasattr(refs, "dim") or refs.dim() != 2):
+            raise WeaverError("tree_attention: hot_count is required without a 2-D table", AW_E_INVALID_ARG)
+        hot_count = 0 if refs is None else refs.shape[1]
+    page = BLOCK_SIZE * kv_heads * head_dim
+    if hot_blocks is None:
+        if hot_k is not None and not hasattr(hot_k, "numel"):
+            raise WeaverError("tree_attention: hot_blocks is required for a raw pool pointer", AW_E_INVALID_ARG)
+        hot_blocks = 0 if hot_k is None else hot_k.numel() // max(page, 1)
+    words = _columns(tree_mask, num_tokens, mask_words, "tree_attention tree_mask")
+    _counts(batch=batch, num_tokens=num_tokens, q_heads=q_heads, kv_heads=kv_heads, head_dim=head_dim, hot_count=hot_count,
+            refs_stride=refs_stride or 0, hot_blocks=hot_blocks, mask_words=words)
+    d.batch, d.num_tokens, d.q_heads, d.kv_heads, d.head_dim = batch, num_tokens, q_heads, kv_heads, head_dim
+    d.hot_count, d.hot_blocks, d.mask_words = hot_count, hot_blocks, words
+    d.scale = head_dim ** -0.5 if scale is None else scale
+    for t, heads, name in ((q, q_heads, "q"), (k, kv_heads, "k"), (v, kv_heads, "v"), (out, q_heads, "out")):
+        setattr(d, name, _ptr(t))
+        setattr(d, name + "_stride", _token_rows(t, num_tokens, heads, head_dim, name))
+    for t, name in ((hot_k, "hot_k"), (hot_v, "hot_v")):
+        _f16(t, hot_blocks * page, name)
+        setattr(d, name, _ptr(t))
+    d.refs_stride = _table(refs, batch, hot_count, refs_stride, "refs") if refs is not None else hot_count
+    d.refs = _ptr(refs)
+    for t, need, name in ((seq_held, batch, "seq_held"), (token_offsets, batch + 1, "token_offsets"),
+                          (tree_mask, num_tokens * words, "tree_mask")):
+        _u32(t, need, name)
+        setattr(d, name, _ptr(t))
+    _one_device(d, [q, k, v, out, hot_k, hot_v, refs, seq_held, token_offsets, tree_mask])
+    return d
+
+
+def tree_plan(desc: TreeDesc, compute_units: int = 0, lib_path=None) -> TreePlanInfo:
+    """Validate a ``tree_attention`` request and return how it is split (no GPU needed)."""
+    info, msg = TreePlanInfo(), ctypes.create_string_buffer(256)
+    rc = _lib.load(lib_path).aw_tree_plan(ctypes.byref(desc), compute_units, ctypes.byref(info), msg, 256)
+    if rc:
+        raise WeaverError(msg.value.decode(), rc)
+    return info
+
+
+def _vocab_rows(t, rows: int, vocab: int, dtype_check, what: str) -> int:
+    """Row stride of [rows][vocab]: contiguous, a raw pointer, or rows further apart."""
+    if t is None or isinstance(t, int) or not hasattr(t, "is_contiguous") or t.is_contiguous():
+        dtype_check(t, rows * vocab, what)
+        return vocab
+    if t.dim() != 2 or t.shape[0] < rows or t.shape[1] != vocab or (vocab > 1 and t.stride(1) != 1) or t.stride(0) < vocab:
+        raise WeaverError(f"{what}: a view must be [rows][{vocab}] with rows apart, got shape {tuple(t.shape)}, strides "
+                          f"{tuple(t.stride())}", AW_E_INVALID_ARG)
+    dtype_check(t[:0].contiguous(), 0, what)
+    return t.stride(0)
+
+
+def make_logits_desc(*, num_tokens: int, vocab_size: int, logits, out=None, best=None, batch: int = 0, token_offsets=None, history=None,
+                     history_count=None, prompt_count=None, repetition=None, frequency=None, presence=None, node_tokens=None,
+                     tree_mask=None, bias_ids=None, bias_values=None, bias_count=None, allowed=None, allowed_index=None,
+                     half: Optional[bool] = None, mask_words: Optional[int] = None, history_stride: Optional[int] = None,
+                     bias_stride: Optional[int] = None, allowed_rows: Optional[int] = None) -> LogitsDesc:
+    """An ``aw_logits_desc`` from device tensors (or raw device pointers to contiguous rows), for
+    ``adjust_logits``: ``logits`` and ``out`` [num_tokens][vocab_size] in fp32 or f16 (``half`` for raw
+    pointers; out may be logits, or None with ``best``), ``history`` [batch][stride] and ``bias_ids`` /
+    ``bias_values`` [batch][stride] with a count for each sequence, ``allowed`` [rows][ceil(vocab_size /
+    32)] bit words and ``allowed_index`` [num_tokens]."""
+    d = LogitsDesc()
+    if half is None:
+        half = hasattr(logits, "element_size") and logits.element_size() == 2
+    words = _columns(tree_mask, num_tokens, mask_words, "adjust_logits tree_mask")
+    past = _columns(history, batch, history_stride, "adjust_logits history")
+    biases = _columns(bias_ids, batch, bias_stride, "adjust_logits bias_ids")
+    states = allowed_rows if allowed_rows is not None else 0 if allowed is None else allowed.shape[0] if hasattr(allowed, "shape") else None
+    if states is None:
+        raise WeaverError("adjust_logits: allowed_rows is required for a raw pointer", AW_E_INVALID_ARG)
+    _counts(num_tokens=num_tokens, vocab_size=vocab_size, batch=batch, mask_words=words, history_stride=past, bias_stride=biases,
+            allowed_rows=states)
+    d.num_tokens, d.vocab_size, d.batch, d.flags = num_tokens, vocab_size, batch, AW_LOGITS_F16 if half else 0
+    d.mask_words, d.history_stride, d.bias_stride, d.allowed_rows = words, past, biases, states
+    check = _f16 if half else _f32
+    for t, name in ((logits, "logits"), (out, "out")):
+        setattr(d, name, _ptr(t))
+        setattr(d, name + "_stride", _vocab_rows(t, num_tokens, vocab_size, check, name))
+    d.allowed_stride = _vocab_rows(allowed, states, -(-vocab_size // 32), _u32, "allowed")
+    d.allowed = _ptr(allowed)
+    tensors = dict(best=(best, num_tokens, _u32), token_offsets=(token_offsets, batch + 1, _u32), history=(history, batch * past, _u32),
+                   history_count=(history_count, batch, _u32), prompt_count=(prompt_count, batch, _u32),
+                   repetition=(repetition, batch, _f32), frequency=(frequency, batch, _f32), presence=(presence, batch, _f32),
+                   node_tokens=(node_tokens, num_tokens, _u32), tree_mask=(tree_mask, num_tokens * words, _u32),
+                   bias_ids=(bias_ids, batch * biases, _u32), bias_values=(bias_values, batch * biases, _f32),
+                   bias_count=(bias_count, batch, _u32), allowed_index=(allowed_index, num_tokens, _u32))
+    for name, (t, need, chk) in tensors.items():
+        chk(t, need, name)
+        setattr(d, name, _ptr(t))
+    _one_device(d, [logits, out, allowed] + [t for t, _, _ in tensors.values()])
+    return d
+
+
+def _layer_rows(t, layers: int, tokens: int, heads: int, head_dim: int, what: str) -> tuple:
+    """(layer stride, token stride) of rows [layers][tokens][heads][head_dim], contiguous heads; 0, 0 for a raw pointer."""
+    if t is None or isinstance(t, int) or not hasattr(t, "is_contiguous") or t.is_contiguous():
+        _f16(t, layers * tokens * heads * head_dim, what)
+        return 0, 0
+    if t.dim() != 4 or tuple(t.shape) != (layers, tokens, heads, head_dim) or (head_dim > 1 and t.stride(3) != 1) or \
+            (heads > 1 and t.stride(2) != head_dim):
+        raise WeaverError(f"{what}: a view must be [{layers}][{tokens}][{heads}][{head_dim}] with contiguous heads, got shape "
+                          f"{tuple(t.shape)}, strides {tuple(t.stride())}", AW_E_INVALID_ARG)
+    _f16(t[:0].contiguous(), 0, what)
+    return t.stride(0), t.stride(1)
+
+
+def make_accept_desc(*, batch: int, num_tokens: int, parents, node_tokens, targets, seq_held, accepted, next_token, seq_hot, path,
+                     token_offsets=None, layers: int = 0, kv_heads: int = 0, head_dim: int = 0, k=None, v=None, hot_k=None,
+                     hot_v=None, slots=None, history=None, history_count=None, history_count_out=None,
+                     hot_blocks: Optional[int] = None, history_stride: Optional[int] = None) -> AcceptDesc:
+    """An ``aw_accept_desc`` from device tensors (or raw device pointers to contiguous rows), for
+    ``accept_tree``: ``k`` and ``v`` [layers][num_tokens][kv_heads][head_dim] (views with contiguous heads
+    too) go by ``slots`` (int64) into the pools [layers][hot_blocks][16][kv_heads][head_dim].  Without
+    ``layers`` no rows are moved.  ``seq_hot`` may be ``seq_held``, ``history_count_out``
+    ``history_count``."""
+    d = AcceptDesc()
+    page = BLOCK_SIZE * kv_heads * head_dim
+    if hot_blocks is None:
+        if hot_k is not None and not hasattr(hot_k, "numel"):
+            raise WeaverError("accept_tree: hot_blocks is required for a raw pool pointer", AW_E_INVALID_ARG)
+        hot_blocks = 0 if hot_k is None else hot_k.numel() // max(page * layers, 1)
+    past = _columns(history, batch, history_stride, "accept_tree history")
+    _counts(batch=batch, num_tokens=num_tokens, layers=layers, kv_heads=kv_heads, head_dim=head_dim, hot_blocks=hot_blocks,
+            history_stride=past)
+    d.batch, d.num_tokens, d.layers, d.kv_heads, d.head_dim = batch, num_tokens, layers, kv_heads, head_dim
+    d.history_stride, d.hot_blocks = past, hot_blocks
+    d.k_layer_stride, d.k_stride = _layer_rows(k, layers, num_tokens, kv_heads, head_dim, "k")
+    d.v_layer_stride, d.v_stride = _layer_rows(v, layers, num_tokens, kv_heads, head_dim, "v")
+    for t, name in ((hot_k, "hot_k"), (hot_v, "hot_v")):
+        _f16(t, layers * hot_blocks * page, name)
+    _i64(slots, num_tokens, "slots")
+    for t, name in ((k, "k"), (v, "v"), (hot_k, "hot_k"), (hot_v, "hot_v"), (slots, "slots")):
+        setattr(d, name, _ptr(t))
+    tensors = dict(parents=(parents, num_tokens), node_tokens=(node_tokens, num_tokens), targets=(targets, num_tokens),
+                   token_offsets=(token_offsets, batch + 1), seq_held=(seq_held, batch), accepted=(accepted, batch),
+                   next_token=(next_token, batch), seq_hot=(seq_hot, batch), path=(path, num_tokens), history=(history, batch * past),
+                   history_count=(history_count, batch), history_count_out=(history_count_out, batch))
+    for name, (t, need) in tensors.items():
+        _u32(t, need, name)
+        setattr(d, name, _ptr(t))
+    _one_device(d, [k, v, hot_k, hot_v, slots] + [t for t, _ in tensors.values()])
+    return d
 
 
 class OpsEngine:
@@ -472,6 +674,27 @@ class OpsEngine:
         """Attention over pages of a batch whose sequences share a prefix, read once for all
         (aw_shared_prefix_attention_device; ``make_prefix_desc``)."""
         self._request("aw_shared_prefix_attention_device", desc, stream)
+
+    # -- a step over trees of drafted tokens (no reference counterpart; agent.rs:337-410 verifies a chain on the host)
+    def page_tables(self, desc: TablesDesc, stream: Optional[int] = None) -> None:
+        """Row offsets, new pages, slots, positions and tree masks of a step, from lengths on the device
+        (``make_tables_desc``)."""
+        self._request("aw_ops_page_tables", desc, stream)
+
+    def tree_attention(self, desc: TreeDesc, stream: Optional[int] = None) -> None:
+        """Attention of each sequence's nodes over its pages, their ancestors and themselves
+        (aw_tree_attention_device; ``make_tree_desc``)."""
+        self._request("aw_tree_attention_device", desc, stream)
+
+    def adjust_logits(self, desc: LogitsDesc, stream: Optional[int] = None) -> None:
+        """Penalties for repeated tokens, biases and grammar masks on rows of logits, and the best token of
+        each (``make_logits_desc``)."""
+        self._request("aw_ops_adjust_logits", desc, stream)
+
+    def accept_tree(self, desc: AcceptDesc, stream: Optional[int] = None) -> None:
+        """The path of each tree that its targets take, its K and V rows into the pages of every layer
+        (``make_accept_desc``)."""
+        self._request("aw_ops_accept_tree", desc, stream)
 
     def multihead_attention(self, q, k_cache, v_cache, output, kv_len: int, head_dim: int, q_heads: int,
                             kv_heads: int, num_queries: int, cache_tokens: Optional[int] = None,

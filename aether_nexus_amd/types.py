@@ -239,6 +239,9 @@ class RotaryScaling(ctypes.Structure):
     ]
 
 
+#: AW_LOGITS_F16 (include/aether_ops.h).
+AW_LOGITS_F16 = 1
+
 #: AW_ROTARY_SCALE_* by name.
 ROTARY_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "parts": 3}
 
@@ -298,6 +301,67 @@ class PrefixPlanInfo(ctypes.Structure):
         ("prefix_splits", ctypes.c_uint32), ("prefix_tokens_per_split", ctypes.c_uint32),
         ("own_splits", ctypes.c_uint32), ("own_tokens_per_split", ctypes.c_uint32),
         ("row_tile", ctypes.c_uint32), ("reserved", ctypes.c_uint32), ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
+class TreeDesc(ctypes.Structure):
+    """``aw_tree_desc`` (include/aether_weaver.h): attention of trees of drafted tokens over pages."""
+
+    _device = None  # the GPU of the tensors behind it, where it was made from tensors
+
+    _fields_ = [
+        *((n, ctypes.c_uint32) for n in ("batch", "num_tokens", "q_heads", "kv_heads", "head_dim", "hot_count", "refs_stride",
+                                         "mask_words")),
+        ("scale", ctypes.c_float), ("reserved", ctypes.c_uint32),
+        *((n, ctypes.c_uint64) for n in ("hot_blocks", "q_stride", "k_stride", "v_stride", "out_stride")),
+        *((n, ctypes.c_void_p) for n in ("q", "k", "v", "hot_k", "hot_v", "refs", "seq_held", "token_offsets", "tree_mask", "out")),
+    ]
+
+
+class TreePlanInfo(ctypes.Structure):
+    """``aw_tree_plan_info``."""
+
+    _fields_ = [("work_groups", ctypes.c_uint32), ("row_tile", ctypes.c_uint32), ("workspace_bytes", ctypes.c_uint64)]
+
+
+class TablesDesc(ctypes.Structure):
+    """``aw_tables_desc`` (include/aether_ops.h): block tables, slots, positions and tree masks from lengths."""
+
+    _device = None
+
+    _fields_ = [
+        *((n, ctypes.c_uint32) for n in ("batch", "num_tokens", "hot_count", "refs_stride", "free_count", "mask_words")),
+        *((n, ctypes.c_void_p) for n in ("seq_held", "seq_new", "seq_pages", "free_pages", "free_first", "parents", "refs", "seq_hot",
+                                         "pages_out", "token_offsets", "free_next", "slots", "positions", "tree_mask")),
+    ]
+
+
+class LogitsDesc(ctypes.Structure):
+    """``aw_logits_desc`` (include/aether_ops.h): rows of logits before a token is chosen."""
+
+    _device = None
+
+    _fields_ = [
+        *((n, ctypes.c_uint32) for n in ("num_tokens", "vocab_size", "batch", "flags", "mask_words", "history_stride", "bias_stride",
+                                         "allowed_rows")),
+        *((n, ctypes.c_uint64) for n in ("logits_stride", "out_stride", "allowed_stride")),
+        *((n, ctypes.c_void_p) for n in ("logits", "out", "best", "token_offsets", "history", "history_count", "prompt_count",
+                                         "repetition", "frequency", "presence", "node_tokens", "tree_mask", "bias_ids", "bias_values",
+                                         "bias_count", "allowed", "allowed_index")),
+    ]
+
+
+class AcceptDesc(ctypes.Structure):
+    """``aw_accept_desc`` (include/aether_ops.h): the kept path of each tree and its rows into the pages."""
+
+    _device = None
+
+    _fields_ = [
+        *((n, ctypes.c_uint32) for n in ("batch", "num_tokens", "layers", "kv_heads", "head_dim", "history_stride")),
+        *((n, ctypes.c_uint64) for n in ("hot_blocks", "k_stride", "v_stride", "k_layer_stride", "v_layer_stride", "hot_layer_stride")),
+        *((n, ctypes.c_void_p) for n in ("parents", "node_tokens", "targets", "token_offsets", "seq_held", "slots", "k", "v", "hot_k",
+                                         "hot_v", "accepted", "next_token", "seq_hot", "path", "history", "history_count",
+                                         "history_count_out")),
     ]
 
 

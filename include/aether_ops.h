@@ -232,6 +232,166 @@ int aw_ops_check_append(const aw_append_desc* desc, char* msg, size_t msg_len);
 /* sizeof(aw_rotary_scaling), sizeof(aw_rotary_desc), sizeof(aw_append_desc), for bindings. */
 void aw_abi_ops_desc_sizes(size_t sizes[3]);
 
+/* ---- a step over trees of drafted tokens (no reference counterpart) ------------
+ * The reference drafts a chain and verifies it on the host (nexus-core/src/agent.rs:337-410).
+ * Here each sequence of a batch has a tree of `nodes` to verify: node 0 is its newest
+ * token, every other node continues its parent, an earlier node.  One step of the model
+ * checks all of them without the host in between:
+ *   aw_ops_page_tables            offsets, pages, slots, positions and the tree's mask, from the lengths
+ *   (products, aw_ops_rotary with those positions)
+ *   aw_tree_attention_device      each node over the sequence's pages, its ancestors and itself (aether_weaver.h)
+ *   (products, aw_ops_matmul_scaled)
+ *   aw_ops_adjust_logits          penalties, biases, grammar masks, the best token of each row
+ *   aw_ops_accept_tree            the path that the target's tokens take, its rows into the pages
+ * Rows are flat: sequence b's nodes are rows token_offsets[b] .. token_offsets[b + 1] - 1
+ * (token_offsets [batch + 1], ascending, from 0; NULL: num_tokens / batch rows each).  Rows
+ * behind the last sequence (a padded batch) belong to none.  A tree's mask is
+ * [num_tokens][mask_words] words: bit j of row i (bit j % 32 of word j / 32) says that node i
+ * sees node j of its own sequence.  Device pointers; outputs overlap neither inputs nor each
+ * other (but where a call says so).  Tokens and lengths out of range set the engine's device error
+ * (aw_engine_check_device_errors) and are taken as stated. */
+
+#define AW_MAX_NODES 1024u /* nodes of a sequence's tree: 32 mask words */
+
+/* Per sequence: seq_held tokens in pages before the step, seq_new new ones (nodes), seq_pages
+ * entries of its row of refs that name pages (NULL: as many as its tokens need; more where an
+ * earlier step left pages unfilled).  Where held + new tokens need more, the row is
+ * continued with free_pages[f], free_pages[f + 1], .., in the order of the sequences, f =
+ * *free_first (NULL: 0).  Outputs, each but refs, seq_hot and token_offsets may be NULL:
+ *   refs          [batch][refs_stride], its new entries alone; seq_pages + new pages in pages_out
+ *   seq_hot       held + new (what aw_ops_append_paged takes)
+ *   token_offsets [batch + 1]
+ *   free_next     [1] the place in free_pages behind the last page taken
+ *   slots         [num_tokens] the row of the pools of each new token, ref * 16 + place % 16
+ *   positions     [num_tokens] its place; with parents: held + its depth in the tree
+ *   tree_mask     [num_tokens][mask_words], required with parents: itself and its ancestors
+ * parents [num_tokens]: node numbers within the tree, < 0 for a root; one that is not an earlier node
+ * sets "sequence length" and makes a root.  Rows behind the last sequence: slot -1, position 0,
+ * mask 0.  New tokens past hot_count pages, past num_tokens rows or (with parents) past 32 mask_words
+ * nodes set "sequence length" and are left out; so do pages that seq_held needs and
+ * seq_pages lacks, which get none.  Where free_pages ends, entries become 0x7FFFFFFF (refused by the
+ * calls that read them), slots -1, and "free pages" is set. */
+typedef struct aw_tables_desc {
+    uint32_t batch, num_tokens;          /* batch <= 2^20, num_tokens <= 2^24 */
+    uint32_t hot_count, refs_stride;     /* entries of a row, <= 2^26; refs_stride >= hot_count */
+    uint32_t free_count, mask_words;     /* free_count <= 2^30; mask_words <= 32, 0 without parents */
+    const uint32_t* seq_held;
+    const uint32_t* seq_new;
+    const uint32_t* seq_pages;
+    const uint32_t* free_pages;          /* [free_count] */
+    const uint32_t* free_first;
+    const int32_t*  parents;
+    uint32_t* refs;
+    uint32_t* seq_hot;
+    uint32_t* pages_out;
+    uint32_t* token_offsets;
+    uint32_t* free_next;
+    int64_t*  slots;
+    uint32_t* positions;
+    uint32_t* tree_mask;
+} aw_tables_desc;
+
+int aw_ops_page_tables(aw_engine* engine, const aw_tables_desc* desc, void* hip_stream);
+
+#define AW_LOGITS_F16 1u /* logits and out are f16, else fp32 */
+
+/* Rows of logits before a token is chosen.  With c the times that token v stands among the
+ * sequence's history behind its first prompt_count tokens and among the tokens of the
+ * nodes that the row's mask names, and `seen` where c > 0 or v is in the prompt, in fp32, each step rounded:
+ *   x = seen ? (x > 0 ? x / repetition : x * repetition) : x
+ *   x = x - frequency * c;  c > 0: x = x - presence
+ *   x = x + bias of v;  v not allowed: x = -inf
+ * out (f16: rounded once; may be logits; NULL: best alone) and best, the lowest of the tokens of
+ * the largest x in fp32, -1 where no x is above -inf (a NaN is never the largest; NULL: none).
+ * history [batch][history_stride], of which history_count[b] tokens count (and bias_ids and
+ * bias_values [batch][bias_stride], bias_count); where bias_ids names a token twice the last entry
+ * holds.  allowed: bits [allowed_rows][allowed_stride words], 1 for a token that may follow; row t
+ * takes allowed row allowed_index[t], none where that is negative (NULL: row t); an index
+ * >= allowed_rows sets "token id" and allows nothing.  History, bias and node tokens >= vocab_size
+ * are passed over.  Each of the penalties, and each group of pointers, may be NULL.  Counts past their
+ * stride are taken as it and set "sequence length". */
+typedef struct aw_logits_desc {
+    uint32_t num_tokens, vocab_size;     /* rows <= 2^24, vocab_size <= 2^24 */
+    uint32_t batch, flags;               /* batch <= 2^20; 0 or AW_LOGITS_F16 */
+    uint32_t mask_words;                 /* <= 32, 0 without nodes */
+    uint32_t history_stride;             /* <= 2^20 */
+    uint32_t bias_stride;                /* <= 1023 */
+    uint32_t allowed_rows;
+    uint64_t logits_stride, out_stride;  /* elements from row to row, 0 for vocab_size */
+    uint64_t allowed_stride;             /* words, 0 for ceil(vocab_size / 32) */
+    const void* logits;                  /* at their elements' alignment */
+    void*       out;
+    int32_t*    best;                    /* [num_tokens] */
+    const uint32_t* token_offsets;
+    const uint32_t* history;
+    const uint32_t* history_count;
+    const uint32_t* prompt_count;        /* NULL: 0 each */
+    const float* repetition;             /* [batch] each */
+    const float* frequency;
+    const float* presence;
+    const uint32_t* node_tokens;         /* [num_tokens], with tree_mask */
+    const uint32_t* tree_mask;
+    const uint32_t* bias_ids;
+    const float*    bias_values;
+    const uint32_t* bias_count;
+    const uint32_t* allowed;
+    const int32_t*  allowed_index;
+} aw_logits_desc;
+
+/* `best` takes scratch of the engine's workspace, 8 bytes a row and 2048 tokens or more, as in
+ * aw_decode_device, also under capture. */
+int aw_ops_adjust_logits(aw_engine* engine, const aw_logits_desc* desc, void* hip_stream);
+
+/* From node 0 of each tree, whose token is kept, on: of the children of the node kept last
+ * the lowest whose token is targets[that node] is kept too, until there is none.
+ *   accepted   [batch] how many are kept (0 for a sequence without nodes)
+ *   next_token [batch] targets[the last one kept] (-1 without nodes): the next tree's node 0
+ *   seq_hot    [batch] seq_held + accepted; may be seq_held
+ *   path       [num_tokens] in the sequence's rows the kept nodes in order, then -1
+ *   history    [batch][history_stride] the kept tokens behind the history_count that were there, and
+ *              history_count_out; history_count_out may be history_count (all three NULL: none); past the
+ *              stride they are left out and "sequence length" is set
+ * and, for each of `layers` layers, K and V row of the j-th kept node to row slots[j-th row of the
+ * sequence] of the pool.  A slot past hot_blocks pages is left out and sets "hot block ref", a negative
+ * one is left out.  A tree of more than AW_MAX_NODES nodes sets "sequence length", its later nodes are
+ * not kept. */
+typedef struct aw_accept_desc {
+    uint32_t batch, num_tokens;          /* batch <= 2^20, num_tokens <= 2^24 */
+    uint32_t layers, kv_heads, head_dim; /* layers 0: no rows are moved; <= 65535 */
+    uint32_t history_stride;
+    uint64_t hot_blocks;
+    uint64_t k_stride, v_stride;         /* elements from node to node, 0 for kv_heads * head_dim */
+    uint64_t k_layer_stride, v_layer_stride; /* from layer to layer, 0 for num_tokens * stride */
+    uint64_t hot_layer_stride;           /* of the pools, 0 for hot_blocks * 16 * kv_heads * head_dim */
+    const int32_t*  parents;             /* [num_tokens] */
+    const uint32_t* node_tokens;
+    const uint32_t* targets;             /* [num_tokens]: best of aw_ops_adjust_logits, or sampled */
+    const uint32_t* token_offsets;
+    const uint32_t* seq_held;
+    const int64_t*  slots;               /* [num_tokens], of aw_ops_page_tables */
+    const uint16_t* k;                   /* [layers][num_tokens][kv_heads][head_dim] */
+    const uint16_t* v;                   /* likewise, NULL with hot_v */
+    uint16_t* hot_k;                     /* [layers][hot_blocks][16][kv_heads][head_dim] */
+    uint16_t* hot_v;
+    uint32_t* accepted;
+    int32_t*  next_token;
+    uint32_t* seq_hot;
+    int32_t*  path;
+    uint32_t* history;
+    const uint32_t* history_count;
+    uint32_t* history_count_out;
+} aw_accept_desc;
+
+int aw_ops_accept_tree(aw_engine* engine, const aw_accept_desc* desc, void* hip_stream);
+
+/* The host checks of the calls above, as aw_ops_check_rotary. */
+int aw_ops_check_tables(const aw_tables_desc* desc, char* msg, size_t msg_len);
+int aw_ops_check_logits(const aw_logits_desc* desc, char* msg, size_t msg_len);
+int aw_ops_check_accept(const aw_accept_desc* desc, char* msg, size_t msg_len);
+
+/* sizeof(aw_tables_desc), sizeof(aw_logits_desc), sizeof(aw_accept_desc), for bindings. */
+void aw_abi_step_desc_sizes(size_t sizes[3]);
+
 /* The tile that a call's product (matmul_qkv: 3, of n[0 .. products) weight rows)
  * of m > 64 rows with 16-byte aligned rows takes on a GPU of `compute_units`, for
  * testing: {activation rows, weight rows, LDS buffers of 64 k}.  Host only.

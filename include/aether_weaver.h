@@ -371,6 +371,63 @@ int aw_shared_prefix_attention_device(aw_engine* engine, const aw_prefix_desc* d
 /* sizeof(aw_prefix_desc) and sizeof(aw_prefix_plan_info), for bindings. */
 void aw_abi_prefix_sizes(size_t sizes[2]);
 
+/* ---- trees of drafted tokens over pages (no reference counterpart) -------------
+ * Attention of the nodes of each sequence's tree (aether_ops.h, aw_ops_page_tables): every
+ * node sees the sequence's seq_held tokens in pages and those nodes that its row of
+ * tree_mask names (NULL: those before it and itself, a chain or a piece of a prompt).
+ * The nodes' keys and values are rows of their own, not in pages yet: which of them go there
+ * is known after the step (aw_ops_accept_tree).  Device pointers, f16:
+ *   q, out       [num_tokens][q_heads][head_dim], *_stride elements from row to row (0: contiguous)
+ *   k, v         [num_tokens][kv_heads][head_dim], likewise; the parts of a fused q/k/v product's rows are taken
+ *   hot_k, hot_v [hot_blocks][16][kv_heads][head_dim]; v and hot_v NULL: V is the K row
+ *   refs         [batch][refs_stride]: a sequence's pages
+ *   seq_held     [batch] its tokens there
+ * q, k, v and the pools 16-byte aligned, with strides that are multiples of 8 elements; out 8-byte
+ * aligned, its stride a multiple of 4.  out may be q (same stride) and shares no element otherwise.
+ * A row that sees nothing is zeros; rows behind the last sequence are left as they are.  Bit 31 of a ref is masked; a ref >= hot_blocks
+ * hides its tokens and sets the device error "hot block ref"; a seq_held over hot_count * 16, offsets that
+ * descend or pass num_tokens, and nodes past 32 mask_words (which no row sees) set "sequence length".
+ * Values that a row does not see never reach it, infinities and NaNs neither.
+ * head_dim 64 or 128; up to 2^20 sequences, 2^22 tokens of each in pages, 2^25 rows of q.
+ * Scratch is the engine's workspace, as in aw_decode_device, also under capture. */
+typedef struct aw_tree_desc {
+    uint32_t batch, num_tokens;
+    uint32_t q_heads, kv_heads, head_dim;
+    uint32_t hot_count;                  /* table entries of a sequence (0: none has pages, refs NULL) */
+    uint32_t refs_stride;                /* >= hot_count */
+    uint32_t mask_words;                 /* <= 32; 0 without tree_mask */
+    float    scale;
+    uint32_t reserved;                   /* 0 */
+    uint64_t hot_blocks;
+    uint64_t q_stride, k_stride, v_stride, out_stride;
+    const uint16_t* q;
+    const uint16_t* k;
+    const uint16_t* v;
+    const uint16_t* hot_k;
+    const uint16_t* hot_v;
+    const uint32_t* refs;
+    const uint32_t* seq_held;            /* NULL: no tokens in pages */
+    const uint32_t* token_offsets;       /* NULL: num_tokens / batch rows each */
+    const uint32_t* tree_mask;           /* [num_tokens][mask_words] */
+    uint16_t*       out;
+} aw_tree_desc;
+
+/* How a request is split, filled by aw_tree_plan. */
+typedef struct aw_tree_plan_info {
+    uint32_t work_groups;                /* that share the work out equally */
+    uint32_t row_tile;                   /* query rows of a kv head that read a sequence's pages together */
+    uint64_t workspace_bytes;
+} aw_tree_plan_info;
+
+/* The host checks of the call below and its plan on a GPU of `compute_units` (0: 256),
+ * without an engine or a GPU; info and msg may be NULL. */
+int aw_tree_plan(const aw_tree_desc* desc, uint32_t compute_units, aw_tree_plan_info* info, char* msg, size_t msg_len);
+
+int aw_tree_attention_device(aw_engine* engine, const aw_tree_desc* desc, void* hip_stream);
+
+/* sizeof(aw_tree_desc) and sizeof(aw_tree_plan_info), for bindings. */
+void aw_abi_tree_sizes(size_t sizes[2]);
+
 /* Wait for `hip_stream` and report AW_E_OOB if any kernel since the last check
  * met an out-of-range block ref or atom index (then clears the record). */
 int aw_engine_check_device_errors(aw_engine* engine, void* hip_stream);
