@@ -41,11 +41,11 @@ struct PrefixArgs {
     uint32_t q_and, q_xor;      // of two halves of q: the sign of the scale, or all zero for a scale of 0
 };
 
-// 8 halves of a query row.
-__device__ __forceinline__ half8_t prefix_query(const PrefixArgs& a, const uint16_t* p) {
+// 8 halves of a query row, with the scale's sign.
+__device__ __forceinline__ half8_t prefix_query(const uint16_t* p, uint32_t q_and, uint32_t q_xor) {
     uint4_t w = *(const uint4_t*)p;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = (w[e] & a.q_and) ^ a.q_xor;
+    for (int e = 0; e < 4; ++e) w[e] = (w[e] & q_and) ^ q_xor;
     return as_h8(w);
 }
 
@@ -272,7 +272,7 @@ struct PrefixPages {
         const uint32_t head = g * a.gqa + row % a.gqa;
         const uint16_t* p = a.q + ((uint64_t)(row / a.gqa) * a.q_heads + head) * HD;
 #pragma unroll
-        for (int j = 0; j < KS; ++j) qop[j] = prefix_query(a, p + 32 * j + 8 * lg);
+        for (int j = 0; j < KS; ++j) qop[j] = prefix_query(p + 32 * j + 8 * lg, a.q_and, a.q_xor);
         bad = false;
         pass<false>(a, runs, g, lds, lane, wave);
         // An inf or NaN among the sums under finite weights comes from the values, and may
@@ -372,7 +372,29 @@ constexpr int kPrefixThreads = 256;
 constexpr int kPrefixTok = 64, kPrefixBufs = 5; // tokens a step, steps of K or of V in LDS: two work-groups fill a CU's
 constexpr size_t prefix_lds_bytes(int HD) { return (size_t)kPrefixBufs * kPrefixTok * HD * 2; }
 
-template <int HD>
+// One work-group's part: rows [row0, row0 + kPrefixRows) of `rows` x `tokens` tokens in
+// pages (and, NODES, after them nodes [node0, nodes) of a tree, each row those that its mask names).
+struct TilePart {
+    const uint16_t* q;          // row r: q_step * (r / gqa) + HD * (r % gqa) halves on
+    const uint16_t *k, *v;      // the pools at this kv head
+    const uint32_t* table;      // refs of the part's pages
+    uint64_t q_step, blocks;
+    uint32_t rstride;           // halves from token to token of a page
+    uint32_t gqa, rows, row0, tokens;
+    uint32_t q_and, q_xor;
+    float scale_log2;
+    float *m, *l, *o;           // sums of row 0 (and the rows after it)
+    uint32_t* err;
+    // NODES
+    const uint16_t *nk, *nv;    // node 0 at this kv head
+    uint64_t nk_step, nv_step;  // halves from node to node
+    const uint32_t* mask;       // [nodes][mask_words] or null: the nodes up to the row's own
+    uint32_t mask_words, node0, nodes; // node0 a multiple of the step
+    uint16_t* out;              // not null: the whole of what the rows see, normed and stored (as q, o_step)
+    uint64_t o_step;
+};
+
+template <int HD, bool NODES = false>
 struct PrefixTile {
     static constexpr int TOK = kPrefixTok, BUFS = kPrefixBufs, PAGES = TOK / 16, TB = TOK / 32;
     static constexpr int CH = HD / 8, KS = HD / 16, NB = HD / 32;
@@ -394,54 +416,60 @@ struct PrefixTile {
         __builtin_amdgcn_sched_barrier(0);
     }
 
-    static __device__ __forceinline__ void run(const PrefixArgs& a, uint32_t g, uint32_t tile, uint32_t s, _Float16* lds) {
+    static __device__ __forceinline__ void run(const TilePart& a, _Float16* lds) {
         const int tid = threadIdx.x, lane = tid & 63, li = lane & 31, hf = lane >> 5;
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-        const uint32_t t0 = s * a.prefix_span, t1 = min(t0 + a.prefix_span, a.prefix_tokens); // t0 < t1
-        const int steps = (int)((t1 - t0 + (uint32_t)TOK - 1u) / (uint32_t)TOK);
-        const uint32_t row = tile * kPrefixRows + 32u * (uint32_t)wave + (uint32_t)li;
-        const bool wave_rows = tile * kPrefixRows + 32u * (uint32_t)wave < a.rows;
+        const uint32_t t1 = a.tokens;
+        const int paged = (int)((t1 + (uint32_t)TOK - 1u) / (uint32_t)TOK); // steps over pages, > 0 without NODES
+        const int steps = paged + (NODES ? (int)((a.nodes - a.node0 + (uint32_t)TOK - 1u) / (uint32_t)TOK) : 0);
+        const uint32_t row = a.row0 + 32u * (uint32_t)wave + (uint32_t)li;
+        const bool wave_rows = a.row0 + 32u * (uint32_t)wave < a.rows;
 
         half8_t qop[KS];
         {
             const uint32_t r = min(row, a.rows - 1u);
-            const uint16_t* p = a.q + ((uint64_t)(r / a.gqa) * a.q_heads + g * a.gqa + r % a.gqa) * HD;
+            const uint16_t* p = a.q + (uint64_t)(r / a.gqa) * a.q_step + (r % a.gqa) * (uint32_t)HD;
 #pragma unroll
-            for (int j = 0; j < KS; ++j) qop[j] = prefix_query(a, p + 16 * j + 8 * hf);
+            for (int j = 0; j < KS; ++j) qop[j] = prefix_query(p + 16 * j + 8 * hf, a.q_and, a.q_xor);
         }
 
         // Staging: load j fills slots tid + 256 j of the operand (slot -> row, chunk); a wave's
         // slots of one load lie in one page, at the same place of it for every j.
-        const uint32_t rstride = a.kv_heads * (uint32_t)HD, page_halves = kBlockTokens * rstride; // halves
+        const uint32_t rstride = a.rstride, page_halves = kBlockTokens * rstride; // halves
         const uint32_t srow = ((uint32_t)tid / CH) & 15u, schunk = (uint32_t)tid % CH;
-        const uint16_t* kfrom = a.k + (uint64_t)g * HD + srow * rstride + 8u * (schunk ^ ksw(srow));
-        const uint16_t* vfrom = a.v + (uint64_t)g * HD + srow * rstride + 8u * (schunk ^ vsw(srow));
+        const uint16_t* kfrom = a.k + srow * rstride + 8u * (schunk ^ ksw(srow));
+        const uint16_t* vfrom = a.v + srow * rstride + 8u * (schunk ^ vsw(srow));
         // Rows past the part's last token load that token's (and count for nothing).
-        const uint32_t first = t0 / kBlockTokens, last = (t1 - 1u) / kBlockTokens - first;
+        const uint32_t last = paged ? (t1 - 1u) / kBlockTokens : 0u;
         const int back = ((int)min(srow, (t1 - 1u) % kBlockTokens) - (int)srow) * (int)rstride;
         // Refs of 64 pages, one in each lane, and which of them count: the run of the newest K
         // step, the one before it, and (refs alone) the next.
         uint32_t held, ref_cur, ref_old, ref_next;
         uint64_t ok_cur, ok_old;
         bool bad = false;
-        auto refs_from = [&](uint32_t run) { return a.prefix_refs[first + min(64u * run + (uint32_t)lane, last)] & kRefMask; };
+        auto refs_from = [&](uint32_t run) { return !NODES || paged ? a.table[min(64u * run + (uint32_t)lane, last)] & kRefMask : 0u; };
         auto take = [&](uint32_t run) {
             held = run;
             ref_old = ref_cur;
             ok_old = ok_cur;
-            const bool ok = ref_next < a.blocks;
+            const bool ok = ref_next < a.blocks || (NODES && !paged);
             ref_cur = ok ? ref_next : 0u;
             ok_cur = __ballot(ok);
             bad |= !ok;
             ref_next = refs_from(run + 1u);
         };
-        // Load j of a step of K or V; INNER: the step is not the part's last.
-        auto load = [&](auto inner, const uint16_t* from, uint32_t refs, int step, _Float16* dst, int j) {
+        // Load j of a step of K or (`v`) V; INNER: the step is not the last over pages.
+        auto load = [&](auto inner, bool v, uint32_t refs, int step, _Float16* dst, int j) {
             const uint32_t p = (uint32_t)(CH == 16 ? j : 2 * j + (wave >> 1)); // page: 16 rows a load, or 32
             const uint32_t b = (uint32_t)step * (uint32_t)PAGES + p, at = decltype(inner)::value ? b : min(b, last);
             const uint32_t ref = (uint32_t)__builtin_amdgcn_readlane((int)refs, (int)(at & 63u));
-            const uint16_t* src = from + (uint64_t)ref * page_halves;
+            const uint16_t* src = (v ? vfrom : kfrom) + (uint64_t)ref * page_halves;
             if constexpr (!decltype(inner)::value) src += b >= last ? back : 0;
+            if constexpr (NODES && !decltype(inner)::value)
+                if (step >= paged) { // uniform; rows past the last node load that one
+                    const uint32_t node = min(a.node0 + (uint32_t)(step - paged) * (uint32_t)TOK + 16u * p + srow, a.nodes - 1u);
+                    src = v ? a.nv + node * a.nv_step + 8u * (schunk ^ vsw(srow)) : a.nk + node * a.nk_step + 8u * (schunk ^ ksw(srow));
+                }
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
                                              (__attribute__((address_space(3))) void*)(dst + ((uint32_t)wave * 512u + (uint32_t)(kPrefixThreads * 8 * j))), 16, 0, 0);
         };
@@ -455,9 +483,9 @@ struct PrefixTile {
         auto load_pair = [&](auto inner, int x, int i, uint32_t vbuf, uint32_t kbuf) {
             constexpr bool INNER = decltype(inner)::value;
             if (x < LPT) {
-                if (INNER || (i >= -1 && i + 1 < steps)) load(inner, vfrom, vrefs, i + 1, lds + vbuf * OP, x);
+                if (INNER || (i >= -1 && i + 1 < steps)) load(inner, true, vrefs, i + 1, lds + vbuf * OP, x);
             } else if (INNER || i + 3 < steps) {
-                load(inner, kfrom, ref_cur, i + 3, lds + kbuf * OP, x - LPT);
+                load(inner, false, ref_cur, i + 3, lds + kbuf * OP, x - LPT);
             }
         };
 
@@ -490,14 +518,28 @@ struct PrefixTile {
         // reads are issued right after such a wait.  SPLIT: as in PrefixPages.
         auto process = [&](auto split, int step, const _Float16* sk, const _Float16* sv, float16_t (&sc)[TB], float16_t (&sn)[TB], auto load_x, auto v_there) {
             constexpr bool SPLIT = decltype(split)::value;
-            const uint32_t c0 = t0 + (uint32_t)step * (uint32_t)TOK, b0 = (uint32_t)step * (uint32_t)PAGES;
+            const uint32_t c0 = (uint32_t)step * (uint32_t)TOK, b0 = (uint32_t)step * (uint32_t)PAGES;
             const uint32_t ok4 = (uint32_t)((b0 / 64u == held ? ok_cur : ok_old) >> (b0 & 63u)) & ((1u << PAGES) - 1u);
             __asm__ volatile("" : "+v"(kat), "+v"(va), "+v"(vb)); // their other forms are made in each step, not kept: no spills
             half8_t fr[8];
             auto read = [&](int z) { fr[z % 8] = z < NS ? kfrag(sk, z) : vfrag(sv, z - NS); };
 #pragma unroll
             for (int z = 0; z < 4; ++z) read(z);
-            if (c0 + (uint32_t)TOK > t1 || ok4 != (1u << PAGES) - 1u) { // wave-uniform
+            uint32_t sees[TB]; // of the step's nodes, the row's
+            const bool at_nodes = NODES && step >= paged; // wave-uniform
+            if (at_nodes) {
+                const uint32_t n0 = a.node0 + (uint32_t)(step - paged) * (uint32_t)TOK, node = min(row, a.rows - 1u) / a.gqa;
+                auto low = [](uint32_t n, uint32_t from) { return n <= from ? 0u : n - from >= 32u ? ~0u : (1u << (n - from)) - 1u; };
+#pragma unroll
+                for (int tb = 0; tb < TB; ++tb) {
+                    const uint32_t from = n0 + 32u * tb;
+                    sees[tb] = !a.mask ? low(node + 1u, from) : from / 32u < a.mask_words ? a.mask[(uint64_t)node * a.mask_words + from / 32u] : 0u;
+                    sees[tb] &= low(a.nodes, from);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (!((sees[tb] >> (8 * (i / 4) + i % 4 + 4 * hf)) & 1u)) sc[tb][i] = -INFINITY;
+                }
+            } else if (c0 + (uint32_t)TOK > t1 || ok4 != (1u << PAGES) - 1u) { // wave-uniform
                 int see = (int)(t1 - c0) - 4 * hf;
                 __asm__ volatile("" : "+v"(see)); // compared with constants here, not as 32 values kept over the loop
 #pragma unroll
@@ -575,7 +617,8 @@ struct PrefixTile {
                 for (uint64_t todo = __ballot(any); todo; todo &= todo - 1u) {
                     const uint32_t at = (uint32_t)__builtin_ctzll(todo);
                     const uint32_t slots = (uint32_t)__ballot(lane < CH && nonfinite(at, (uint32_t)lane % (uint32_t)CH));
-                    const bool counts = c0 + at < t1 && ((ok4 >> (at / 16u)) & 1u);
+                    const bool counts = at_nodes || (c0 + at < t1 && ((ok4 >> (at / 16u)) & 1u));
+                    const bool see = !at_nodes || ((sees[at / 32u % TB] >> (at % 32u)) & 1u);
                     float p = 0.0f; // token `at`'s weight: register (at / 8 % 4) 4 + at % 4 of the half at / 4 % 2
 #pragma unroll
                     for (int tb = 0; tb < TB; ++tb)
@@ -593,7 +636,7 @@ struct PrefixTile {
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 const float f = (float)v[e];
-                                if (!(fabsf(f) < INFINITY)) oacc[nb][i + e] = fmaf(p, f, oacc[nb][i + e]);
+                                if (see && !(fabsf(f) < INFINITY)) oacc[nb][i + e] = fmaf(p, f, oacc[nb][i + e]);
                             }
                         }
                 }
@@ -666,7 +709,7 @@ struct PrefixTile {
             };
             int i = 0;
             if constexpr (!decltype(split)::value)
-                for (; i + 5 < steps; i += 2) {
+                for (; i + 5 < paged; i += 2) {
                     step(std::true_type{}, i, s0, s1);
                     step(std::true_type{}, i + 1, s1, s0);
                 }
@@ -700,15 +743,29 @@ struct PrefixTile {
         uint32_t ro = row;
         __asm__ volatile("" : "+v"(ro)); // its addresses are made here, not kept over the loops
         if (ro >= a.rows) return;
-        const uint64_t at = ((uint64_t)g * a.splits + s) * a.rows + ro;
+        if constexpr (NODES)
+            if (a.out) {
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                uint16_t* po = a.out + (uint64_t)(ro / a.gqa) * a.o_step + (ro % a.gqa) * (uint32_t)HD;
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        half4_t y;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) y[e] = (_Float16)(l == 0.0f ? 0.0f : oacc[nb][i + e] * inv);
+                        *(half4_t*)(po + 32 * nb + 2 * i + 4 * hf) = y;
+                    }
+                return;
+            }
         if (hf == 0) {
-            a.part_m[at] = m_run;
-            a.part_l[at] = l;
+            a.m[ro] = m_run;
+            a.l[ro] = l;
         }
         if (l == 0.0f) return;
         // Past the L2, whose dirty lines would be written when the kernel ends: 64 sequences
         // behind 8192 tokens 28.1 us, through it 29.1; whole rows by way of LDS no better.
-        float* po = a.part_o + at * HD;
+        float* po = a.o + (uint64_t)ro * HD;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -735,8 +792,29 @@ __global__ __launch_bounds__(kPrefixThreads) __attribute__((amdgpu_waves_per_eu(
             const uint32_t parts = a.kv_heads * a.prefix_splits, each = (parts + 7u) >> 3, i = uniform(j / a.prefix_tiles);
             const uint32_t part = xcd * each + i;
             if (part >= parts) return;
-            const uint32_t s = uniform(part / a.kv_heads);
-            PrefixTile<HD>::run(a, part - s * a.kv_heads, j - i * a.prefix_tiles, s, prefix_lds);
+            const uint32_t s = uniform(part / a.kv_heads), g = part - s * a.kv_heads;
+            const uint32_t t0 = s * a.prefix_span; // below prefix_tokens
+            const uint64_t at = ((uint64_t)g * a.splits + s) * a.rows;
+            TilePart w{};
+            w.q = a.q + (uint64_t)g * a.gqa * HD;
+            w.k = a.k + (uint64_t)g * HD;
+            w.v = a.v + (uint64_t)g * HD;
+            w.table = a.prefix_refs + t0 / kBlockTokens;
+            w.q_step = (uint64_t)a.q_heads * HD;
+            w.blocks = a.blocks;
+            w.rstride = a.kv_heads * (uint32_t)HD;
+            w.gqa = a.gqa;
+            w.rows = a.rows;
+            w.row0 = (j - i * a.prefix_tiles) * kPrefixRows;
+            w.tokens = min(a.prefix_span, a.prefix_tokens - t0);
+            w.q_and = a.q_and;
+            w.q_xor = a.q_xor;
+            w.scale_log2 = a.scale_log2;
+            w.m = a.part_m + at;
+            w.l = a.part_l + at;
+            w.o = a.part_o + at * HD;
+            w.err = a.err;
+            PrefixTile<HD>::run(w, prefix_lds);
             return;
         }
         j -= a.prefix_wgs >> 3;

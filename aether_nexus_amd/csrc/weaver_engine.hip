@@ -1245,16 +1245,29 @@ int tree_plan(const aw_tree_desc* d, uint32_t n_cu, aw::TreeArgs* out, aw_tree_p
     a.hot_count = d->hot_count;
     a.refs_stride = d->refs_stride;
     a.mask_words = d->mask_words;
-    a.scale_log2 = d->scale * aw::kLog2e;
-    (void)n_cu;
-    if (info) *info = aw_tree_plan_info{};
+    a.q_and = d->scale == 0.0f ? 0u : ~0u;
+    a.q_xor = d->scale < 0.0f ? 0x80008000u : 0u;
+    a.scale_log2 = d->scale == 0.0f ? 1.0f : std::fabs(d->scale) * aw::kLog2e;
+    a.work_groups = (uint32_t)align_up(n_cu, 8);
+    if (info) {
+        *info = aw_tree_plan_info{};
+        info->work_groups = a.work_groups;
+        info->row_tile = aw::kPrefixRows;
+        const uint64_t rows = 2ull * a.work_groups * aw::kPrefixRows;
+        info->workspace_bytes = align_up(rows * 4 * (d->head_dim + 2), kAlign) + a.work_groups * aw::kCutWords * 4;
+    }
     return AW_OK;
 }
 
 template <int HD>
 int launch_tree(aw_engine* e, aw::TreeArgs& a, hipStream_t st) {
-    StageTimer t(e, AW_STAGE_HOT, st);
-    hipLaunchKernelGGL(aw::tree_row_kernel<HD>, dim3(a.tokens, a.q_heads), dim3(256), 0, st, a);
+    {
+        StageTimer t(e, AW_STAGE_HOT, st);
+        hipLaunchKernelGGL(aw::tree_kernel<HD>, dim3(a.work_groups), dim3(aw::kPrefixThreads), aw::prefix_lds_bytes(HD), st, a);
+        AW_HIP(e, hipGetLastError());
+    }
+    StageTimer t(e, AW_STAGE_MERGE, st);
+    hipLaunchKernelGGL(aw::tree_merge_kernel<HD>, dim3(a.work_groups - 1, aw::kPrefixRows / aw::kTreeMergeRows), dim3(256), 0, st, a);
     AW_HIP(e, hipGetLastError());
     return AW_OK;
 }
@@ -1484,6 +1497,8 @@ int aw_engine_create(int device, aw_engine** out) {
         set_lds((const void*)aw::prefix_kernel<64, false>);
         set_lds((const void*)aw::prefix_kernel<128, false>);
         set_lds((const void*)aw::prefix_kernel<128, true>);
+        set_lds((const void*)aw::tree_kernel<64>);
+        set_lds((const void*)aw::tree_kernel<128>);
         if (!aw_engine_internal::ops_set_lds_limits(e->max_lds)) attr_ok = false;
     }
     if (!attr_ok) {
@@ -1724,8 +1739,14 @@ int aw_tree_attention_device(aw_engine* e, const aw_tree_desc* d, void* stream) 
     if (rc) return fail(e, rc, "%s", msg);
     if (!a.tokens) return AW_OK;
     AW_HIP(e, hipSetDevice(e->device));
-    a.err = e->err;
     hipStream_t st = (hipStream_t)stream; // NULL is HIP's null stream
+    if ((rc = ensure_keep(e->ws, info.workspace_bytes, e->retired_ws, e->last_error, st))) return rc;
+    const uint64_t rows = 2ull * a.work_groups * aw::kPrefixRows;
+    a.part_m = (float*)e->ws.ptr;
+    a.part_l = a.part_m + rows;
+    a.part_o = a.part_l + rows;
+    a.cuts = (uint32_t*)((char*)e->ws.ptr + align_up(rows * 4 * (d->head_dim + 2), kAlign));
+    a.err = e->err;
     return d->head_dim == 64 ? launch_tree<64>(e, a, st) : launch_tree<128>(e, a, st);
 }
 
