@@ -390,6 +390,7 @@ struct TilePart {
     uint64_t nk_step, nv_step;  // halves from node to node
     const uint32_t* mask;       // [nodes][mask_words] or null: the nodes up to the row's own
     uint32_t mask_words, node0, nodes; // node0 a multiple of the step
+    uint32_t turn;              // which wave has the first rows
     uint16_t* out;              // not null: the whole of what the rows see, normed and stored (as q, o_step)
     uint64_t o_step;
 };
@@ -417,13 +418,16 @@ struct PrefixTile {
     }
 
     static __device__ __forceinline__ void run(const TilePart& a, _Float16* lds) {
-        const int tid = threadIdx.x, lane = tid & 63, li = lane & 31, hf = lane >> 5;
+        int tid = threadIdx.x;
+        if constexpr (NODES) __asm__ volatile("" : "+v"(tid)); // what is made of it is made for each part, not kept between: no spills
+        const int lane = tid & 63, li = lane & 31, hf = lane >> 5;
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         const uint32_t t1 = a.tokens;
         const int paged = (int)((t1 + (uint32_t)TOK - 1u) / (uint32_t)TOK); // steps over pages, > 0 without NODES
         const int steps = paged + (NODES ? (int)((a.nodes - a.node0 + (uint32_t)TOK - 1u) / (uint32_t)TOK) : 0);
-        const uint32_t row = a.row0 + 32u * (uint32_t)wave + (uint32_t)li;
-        const bool wave_rows = a.row0 + 32u * (uint32_t)wave < a.rows;
+        const uint32_t wrow0 = a.row0 + 32u * (NODES ? ((uint32_t)wave + a.turn) & 3u : (uint32_t)wave); // the wave's rows
+        const uint32_t row = wrow0 + (uint32_t)li;
+        const bool wave_rows = wrow0 < a.rows;
 
         half8_t qop[KS];
         {
@@ -535,9 +539,10 @@ struct PrefixTile {
                     const uint32_t from = n0 + 32u * tb;
                     sees[tb] = !a.mask ? low(node + 1u, from) : from / 32u < a.mask_words ? a.mask[(uint64_t)node * a.mask_words + from / 32u] : 0u;
                     sees[tb] &= low(a.nodes, from);
+                    const uint32_t half = sees[tb] >> (4 * hf);
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
-                        if (!((sees[tb] >> (8 * (i / 4) + i % 4 + 4 * hf)) & 1u)) sc[tb][i] = -INFINITY;
+                        if (!(half & (1u << (8 * (i / 4) + i % 4)))) sc[tb][i] = -INFINITY;
                 }
             } else if (c0 + (uint32_t)TOK > t1 || ok4 != (1u << PAGES) - 1u) { // wave-uniform
                 int see = (int)(t1 - c0) - 4 * hf;

@@ -126,14 +126,24 @@ __global__ __launch_bounds__(kPrefixThreads) __attribute__((amdgpu_waves_per_eu(
     }
     __syncthreads(); // the sums have been read
     auto uniform = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); };
+    auto uniform64 = [&](uint64_t x) { return (uint64_t)uniform((uint32_t)(x >> 32)) << 32 | uniform((uint32_t)x); };
     b = uniform(b);
+    pos = uniform64(pos);
+    base = uniform64(base);
+    const uint64_t stop = uniform64(end), share = uniform64(each);
     uint32_t parts = 0, cut_rows = 0, cut_row0 = 0, cut_first = 0, cut_g = 0;
-    for (; pos < end; ++b) {
-        const TreeSeq s = tree_seq(a, b, false);
-        const uint64_t all = s.all(a.kv_heads);
-        while (pos < end && pos - base < all) {
+    for (; pos < stop; ++b) {
+        TreeSeq s = tree_seq(a, b, false);
+        s.first = uniform(s.first);
+        s.nodes = uniform(s.nodes);
+        s.held = uniform(s.held);
+        s.tiles = uniform(s.tiles);
+        s.paged = uniform(s.paged);
+        s.steps = uniform(s.steps);
+        const uint64_t all = uniform64(s.all(a.kv_heads));
+        while (pos < stop && pos - base < all) {
             const uint32_t unit = uniform((uint32_t)((pos - base) / s.steps)), s0 = uniform((uint32_t)((pos - base) - (uint64_t)unit * s.steps));
-            const uint32_t s1 = uniform((uint32_t)min((uint64_t)s.steps, s0 + (end - pos)));
+            const uint32_t s1 = uniform((uint32_t)min((uint64_t)s.steps, s0 + (stop - pos)));
             const uint32_t g = uniform(unit / s.tiles), row0 = (unit - g * s.tiles) * kPrefixRows;
             const bool whole = s0 == 0 && s1 == s.steps;
             const uint64_t slot = (2ull * w + (s0 == 0 ? 1u : 0u)) * kPrefixRows;
@@ -167,6 +177,7 @@ __global__ __launch_bounds__(kPrefixThreads) __attribute__((amdgpu_waves_per_eu(
             p.nodes = s1 > s.paged ? min((s1 - s.paged) * (uint32_t)kPrefixTok, s.nodes) : p.node0;
             p.out = whole ? a.out + s.first * a.out_stride + (uint64_t)g * a.gqa * HD : nullptr;
             p.o_step = a.out_stride;
+            p.turn = blockIdx.x >= a.work_groups / 2u ? 2u : 0u;
             PrefixTile<HD, true>::run(p, prefix_lds);
             __syncthreads(); // the tile's LDS has been read
             if (s0 == 0 && !whole) { // the last of this work-group
@@ -174,7 +185,7 @@ __global__ __launch_bounds__(kPrefixThreads) __attribute__((amdgpu_waves_per_eu(
                 cut_row0 = row0;
                 cut_first = s.first;
                 cut_g = g;
-                parts = 1u + (uint32_t)((s.steps - s1 + each - 1u) / each);
+                parts = 1u + (uint32_t)((s.steps - s1 + share - 1u) / share);
             }
             pos += s1 - s0;
         }

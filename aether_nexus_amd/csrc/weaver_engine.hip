@@ -1248,7 +1248,7 @@ int tree_plan(const aw_tree_desc* d, uint32_t n_cu, aw::TreeArgs* out, aw_tree_p
     a.q_and = d->scale == 0.0f ? 0u : ~0u;
     a.q_xor = d->scale < 0.0f ? 0x80008000u : 0u;
     a.scale_log2 = d->scale == 0.0f ? 1.0f : std::fabs(d->scale) * aw::kLog2e;
-    a.work_groups = (uint32_t)align_up(n_cu, 8);
+    a.work_groups = (uint32_t)align_up(2 * n_cu, 8);
     if (info) {
         *info = aw_tree_plan_info{};
         info->work_groups = a.work_groups;
