@@ -390,7 +390,6 @@ struct TilePart {
     uint64_t nk_step, nv_step;  // halves from node to node
     const uint32_t* mask;       // [nodes][mask_words] or null: the nodes up to the row's own
     uint32_t mask_words, node0, nodes; // node0 a multiple of the step
-    uint32_t turn;              // which wave has the first rows
     uint16_t* out;              // not null: the whole of what the rows see, normed and stored (as q, o_step)
     uint64_t o_step;
 };
@@ -425,7 +424,7 @@ struct PrefixTile {
         const uint32_t t1 = a.tokens;
         const int paged = (int)((t1 + (uint32_t)TOK - 1u) / (uint32_t)TOK); // steps over pages, > 0 without NODES
         const int steps = paged + (NODES ? (int)((a.nodes - a.node0 + (uint32_t)TOK - 1u) / (uint32_t)TOK) : 0);
-        const uint32_t wrow0 = a.row0 + 32u * (NODES ? ((uint32_t)wave + a.turn) & 3u : (uint32_t)wave); // the wave's rows
+        const uint32_t wrow0 = a.row0 + 32u * (uint32_t)wave; // the wave's rows
         const uint32_t row = wrow0 + (uint32_t)li;
         const bool wave_rows = wrow0 < a.rows;
 

@@ -1171,6 +1171,23 @@ int launch_prefix(aw_engine* e, aw::PrefixArgs& a, hipStream_t st) {
 using aw_engine_internal::rows_meet;
 using aw_engine_internal::rows_same;
 
+// Up to this many tokens (of the table's pages, and nodes) and this many work-groups a CU a
+// request runs in one launch, 16 rows of a kv head in one part.  Measured, us, in one part
+// and in several, behind 500, 900, 1400, 2000 tokens: 8 sequences x 4 nodes, 32 / 8 heads x 128, 10, 14, 17, 22 and
+// 16, 20, 23, 25; 32 x 4 19, 27, 37, 50 and 25, 30, 38, 45; 1 x 60 11, 15, 19, 23 and 18, 21, 25, 27; 2 x 5, 14 / 2
+// heads x 64, 8.9, 10.5, 12.6, 15.5 and 12.6 to 13.4.
+constexpr uint64_t kTreeOneTokens = 1500, kTreeOneGroups = 4;
+// Query rows of a unit, where a sequence has `rows` of a kv head; `values`: of K, read by all
+// 16-row units together.  Wide units read K and V less often, narrow ones share a short request out
+// to more work-groups.  Measured, us, 16, 32, 128 rows, heads x 128 (granite: 64): 64 sequences x 8 nodes x 4 heads a
+// kv head behind 4099 tokens (rows 18, 557 M values) 241, 181, 196; 16 x 64 behind 8192 (130) 435, 251, 135; 1 x 60 behind
+// 4000, 9000, 16000 (240; 65, 147, 262 M) 35, 33, 48; 59, 54, 59; 92, 96, 70; 4 x 30 behind 3000 (78, 60 M) 29, 33, 41; 32
+// x 4 behind 1100 (10) 34, 37, 42.
+uint32_t tree_row_tile(uint64_t rows, double values) {
+    if (rows <= 16 || values <= 96u << 20) return 16;
+    return rows <= 32 || values <= 128u << 20 ? 32 : aw::kPrefixRows;
+}
+
 // Checks a request and fills its kernel arguments but for addresses of scratch.
 int tree_plan(const aw_tree_desc* d, uint32_t n_cu, aw::TreeArgs* out, aw_tree_plan_info* info, char* msg, size_t len) {
     auto refuse = [&](int code, const char* why) {
@@ -1248,26 +1265,50 @@ int tree_plan(const aw_tree_desc* d, uint32_t n_cu, aw::TreeArgs* out, aw_tree_p
     a.q_and = d->scale == 0.0f ? 0u : ~0u;
     a.q_xor = d->scale < 0.0f ? 0x80008000u : 0u;
     a.scale_log2 = d->scale == 0.0f ? 1.0f : std::fabs(d->scale) * aw::kLog2e;
-    a.work_groups = (uint32_t)align_up(2 * n_cu, 8);
+    const uint64_t most = d->mask_words ? std::min<uint64_t>(n, 32ull * d->mask_words) : n; // nodes of a sequence
+    const uint64_t pages = align_up(n * gqa / 16 + d->batch, 8) * d->kv_heads;
+    // Steps of 16-row units, if every sequence filled its table, are counted in 32 bits.
+    auto steps = [&](uint32_t rows) {
+        return (double)d->kv_heads * ((double)n * gqa / rows + std::min<double>((double)n, d->batch)) * (d->hot_count / 4.0 + (double)most / 64 + 2);
+    };
+    if (steps(16) >= 4294967296.0) return refuse(AW_E_UNSUPPORTED, "too many rows over too many tokens");
+    const bool one = d->hot_count * (uint64_t)kBlock + most <= kTreeOneTokens && pages <= kTreeOneGroups * (uint64_t)n_cu;
+    const uint32_t rows = one ? 16u : tree_row_tile(n * gqa / d->batch, steps(16) * 64 * d->head_dim);
+    const double all = steps(rows);
+    a.work_groups = (uint32_t)(one ? pages : align_up((uint64_t)std::min<double>(all, (rows < aw::kPrefixRows && d->head_dim == 64 ? 4 : 2) * (double)n_cu), 8));
     if (info) {
         *info = aw_tree_plan_info{};
         info->work_groups = a.work_groups;
-        info->row_tile = aw::kPrefixRows;
-        const uint64_t rows = 2ull * a.work_groups * aw::kPrefixRows;
-        info->workspace_bytes = align_up(rows * 4 * (d->head_dim + 2), kAlign) + a.work_groups * aw::kCutWords * 4;
+        info->row_tile = rows;
+        const uint64_t slots = 2ull * a.work_groups * rows;
+        if (!one) info->workspace_bytes = align_up(slots * 4 * (d->head_dim + 2), kAlign) + a.work_groups * aw::kCutWords * 4;
     }
     return AW_OK;
 }
 
-template <int HD>
+template <int HD, int NR>
 int launch_tree(aw_engine* e, aw::TreeArgs& a, hipStream_t st) {
     {
         StageTimer t(e, AW_STAGE_HOT, st);
-        hipLaunchKernelGGL(aw::tree_kernel<HD>, dim3(a.work_groups), dim3(aw::kPrefixThreads), aw::prefix_lds_bytes(HD), st, a);
+        hipLaunchKernelGGL((aw::tree_kernel<HD, NR>), dim3(a.work_groups), dim3(aw::kPrefixThreads), aw::tree_lds(HD, NR), st, a);
         AW_HIP(e, hipGetLastError());
     }
     StageTimer t(e, AW_STAGE_MERGE, st);
-    hipLaunchKernelGGL(aw::tree_merge_kernel<HD>, dim3(a.work_groups - 1, aw::kPrefixRows / aw::kTreeMergeRows), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((aw::tree_merge_kernel<HD, NR>), dim3(a.work_groups - 1, cdiv(aw::tree_rows(NR), aw::kTreeMergeRows)), dim3(256), 0, st, a);
+    AW_HIP(e, hipGetLastError());
+    return AW_OK;
+}
+
+template <int HD>
+int launch_tree(aw_engine* e, aw::TreeArgs& a, const aw_tree_plan_info& info, hipStream_t st) {
+    if (info.workspace_bytes)
+        return info.row_tile == 16 ? launch_tree<HD, 1>(e, a, st) : info.row_tile == 32 ? launch_tree<HD, 2>(e, a, st) : launch_tree<HD, 0>(e, a, st);
+    StageTimer t(e, AW_STAGE_HOT, st);
+    constexpr int NW = HD == 64 ? 16 : 8; // 160 KB of LDS
+    if (a.work_groups <= e->n_cu)
+        hipLaunchKernelGGL((aw::tree_pages_kernel<HD, NW>), dim3(a.work_groups), dim3(NW * 64), aw::tree_pages_lds(HD, NW, 1), st, a);
+    else
+        hipLaunchKernelGGL((aw::tree_pages_kernel<HD, 4>), dim3(a.work_groups), dim3(256), aw::tree_pages_lds(HD, 4, 1), st, a);
     AW_HIP(e, hipGetLastError());
     return AW_OK;
 }
@@ -1497,8 +1538,13 @@ int aw_engine_create(int device, aw_engine** out) {
         set_lds((const void*)aw::prefix_kernel<64, false>);
         set_lds((const void*)aw::prefix_kernel<128, false>);
         set_lds((const void*)aw::prefix_kernel<128, true>);
-        set_lds((const void*)aw::tree_kernel<64>);
-        set_lds((const void*)aw::tree_kernel<128>);
+        const void* tree[] = {(const void*)aw::tree_kernel<64, 0>, (const void*)aw::tree_kernel<64, 1>, (const void*)aw::tree_kernel<64, 2>,
+                              (const void*)aw::tree_kernel<128, 0>, (const void*)aw::tree_kernel<128, 1>, (const void*)aw::tree_kernel<128, 2>};
+        for (const void* f : tree) set_lds(f);
+        set_lds((const void*)aw::tree_pages_kernel<64, 4>);
+        set_lds((const void*)aw::tree_pages_kernel<64, 16>);
+        set_lds((const void*)aw::tree_pages_kernel<128, 4>);
+        set_lds((const void*)aw::tree_pages_kernel<128, 8>);
         if (!aw_engine_internal::ops_set_lds_limits(e->max_lds)) attr_ok = false;
     }
     if (!attr_ok) {
@@ -1740,14 +1786,16 @@ int aw_tree_attention_device(aw_engine* e, const aw_tree_desc* d, void* stream) 
     if (!a.tokens) return AW_OK;
     AW_HIP(e, hipSetDevice(e->device));
     hipStream_t st = (hipStream_t)stream; // NULL is HIP's null stream
-    if ((rc = ensure_keep(e->ws, info.workspace_bytes, e->retired_ws, e->last_error, st))) return rc;
-    const uint64_t rows = 2ull * a.work_groups * aw::kPrefixRows;
-    a.part_m = (float*)e->ws.ptr;
-    a.part_l = a.part_m + rows;
-    a.part_o = a.part_l + rows;
-    a.cuts = (uint32_t*)((char*)e->ws.ptr + align_up(rows * 4 * (d->head_dim + 2), kAlign));
+    if (info.workspace_bytes) {
+        if ((rc = ensure_keep(e->ws, info.workspace_bytes, e->retired_ws, e->last_error, st))) return rc;
+        const uint64_t slots = 2ull * a.work_groups * info.row_tile;
+        a.part_m = (float*)e->ws.ptr;
+        a.part_l = a.part_m + slots;
+        a.part_o = a.part_l + slots;
+        a.cuts = (uint32_t*)((char*)e->ws.ptr + align_up(slots * 4 * (d->head_dim + 2), kAlign));
+    }
     a.err = e->err;
-    return d->head_dim == 64 ? launch_tree<64>(e, a, st) : launch_tree<128>(e, a, st);
+    return d->head_dim == 64 ? launch_tree<64>(e, a, info, st) : launch_tree<128>(e, a, info, st);
 }
 
 void aw_abi_tree_sizes(size_t sizes[2]) {
