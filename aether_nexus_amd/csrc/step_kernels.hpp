@@ -30,20 +30,6 @@ __device__ inline SeqRows seq_rows(const uint32_t* offsets, uint32_t tokens, uin
     return {first, end - first};
 }
 
-// The first sequence that ends behind row t (batch: none), as find_place searches.
-__device__ inline uint32_t seq_behind(const uint32_t* offsets, uint32_t tokens, uint32_t batch, uint32_t t, uint32_t lane) {
-    if (!offsets) return t / (tokens / batch);
-    uint32_t b = 0, n = batch;
-    while (n > 64u) {
-        const uint32_t stretch = (n + 63u) / 64u, at = (lane + 1u) * stretch - 1u;
-        const uint32_t skip = stretch * (uint32_t)__popcll(__ballot(at < n && offsets[b + min(at, n - 1u) + 1u] <= t));
-        b += skip;
-        n = n > skip ? min(n - skip, stretch) : 0u;
-    }
-    if (n) b += (uint32_t)__popcll(__ballot(lane < n && offsets[b + min(lane, n - 1u) + 1u] <= t));
-    return b;
-}
-
 // ------------------------------------------------------- block tables from lengths
 
 struct TablesArgs {
@@ -256,6 +242,25 @@ __device__ inline uint64_t wave_max64(uint64_t x) {
     }
     return x;
 }
+// The key of a wave's largest value and, of the lanes that have it, the lowest token: two
+// reductions by DPP (rows of 16 lanes, then broadcasts), the sum in lane 63.
+__device__ inline uint64_t wave_best(float top, uint32_t token) {
+#define AWO_DPP(id, v, ctrl, rmask) __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, id), __builtin_bit_cast(int, v), ctrl, rmask, 0xF, false)
+#define AWO_DPP_ALL(STEP) STEP(0x111, 0xF) STEP(0x112, 0xF) STEP(0x114, 0xF) STEP(0x118, 0xF) STEP(0x142, 0xA) STEP(0x143, 0xC)
+    float m = top;
+#define AWO_DPP_MAX(ctrl, rmask) m = fmaxf(m, __builtin_bit_cast(float, AWO_DPP(-INFINITY, m, ctrl, rmask)));
+    AWO_DPP_ALL(AWO_DPP_MAX)
+    m = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, m), 63));
+    uint32_t t = top == m ? token : ~0u;
+#define AWO_DPP_MIN(ctrl, rmask) t = min(t, (uint32_t)AWO_DPP(-1, t, ctrl, rmask));
+    AWO_DPP_ALL(AWO_DPP_MIN)
+    t = (uint32_t)__builtin_amdgcn_readlane((int)t, 63);
+#undef AWO_DPP_MIN
+#undef AWO_DPP_MAX
+#undef AWO_DPP_ALL
+#undef AWO_DPP
+    return best_key(m, t);
+}
 
 template <typename T>
 struct LogitsVec; // 16 bytes of logits at an element's alignment
@@ -268,162 +273,263 @@ struct LogitsVec<_Float16> {
     typedef _Float16 type __attribute__((ext_vector_type(8), aligned(2)));
 };
 
-// Work-group = `group` rows x a slice of 1024 IT (f16: 2048 IT) tokens.  The slice's
-// counts are a word a token in LDS: made once for a sequence from its history and
-// biases (integer atomics: no order shows in them), and for each row the tokens of its own
-// nodes are added and those of the row before taken off.  Logits go by in 16-byte pieces, read before the counts are
-// ready; tokens without a word take none of the arithmetic.
-// Bound: HBM, each logit read and written once.
+// Where the rows of a sequence lie: its number (batch: none), its rows.
+struct SeqAt {
+    uint32_t b, first, end;
+};
+// The sequence of row t, as find_place searches; both its offsets come with the search's last
+// round trip.
+__device__ inline SeqAt seq_at(const uint32_t* offsets, uint32_t tokens, uint32_t batch, uint32_t t, uint32_t lane) {
+    if (!offsets) {
+        const uint32_t each = tokens / batch, b = t / each;
+        return {b, b * each, b * each + each};
+    }
+    uint32_t b = 0, n = batch;
+    while (n > 64u) {
+        const uint32_t stretch = (n + 63u) / 64u, at = (lane + 1u) * stretch - 1u;
+        const uint32_t skip = stretch * (uint32_t)__popcll(__ballot(at < n && offsets[b + min(at, n - 1u) + 1u] <= t));
+        b += skip;
+        n = n > skip ? min(n - skip, stretch) : 0u;
+    }
+    if (n == 0u) return {batch, 0u, 0u};
+    const uint32_t at = b + min(lane, n - 1u), lo = offsets[at], hi = offsets[at + 1u];
+    const uint32_t k = (uint32_t)__popcll(__ballot(lane < n && hi <= t));
+    if (k >= n) return {batch, 0u, 0u};
+    return {b + k, (uint32_t)__builtin_amdgcn_readlane((int)lo, (int)k), (uint32_t)__builtin_amdgcn_readlane((int)hi, (int)k)};
+}
+
+// Work-group = `group` rows x a slice of 1024 IT (f16: 2048 IT) tokens.  The slice's counts
+// are a word a token in LDS: made once for a sequence from its history and biases (integer
+// atomics: no order shows in them), and for each row the tokens of its own nodes are added
+// and those of the row before taken off.  Logits go by in 16-byte pieces, the last of a slice
+// beginning earlier and making some values twice, from what was read before the row's first
+// write; the few tokens that have a word are taken one after another.  A row's logits, the
+// first 2048 tokens of the history and the biases are asked for before their counts are known
+// (history_stride and bias_stride entries are there whatever the counts), so a work-group
+// waits for memory two or three times.
+// Bound: HBM, each logit read and written once: 544 x 49155 f16 without words 18.3 us
+// (5.8 TB/s), with the best 21.3.  With words the vector unit is busy 60 % of the time:
+// 47.3 us with histories of 2048 tokens, tree nodes, a grammar and the best (44 to 51 as
+// one of them is left out: no part alone is what it waits for); 64 x 128256 f32 with
+// histories of 4096 and 300 biases 25.8 us, 2.6 TB/s.
 template <typename T, int IT, bool WORDS>
 __global__ __launch_bounds__(256) void logits_kernel(LogitsArgs a) {
     typedef typename LogitsVec<T>::type vec_t;
-    constexpr uint32_t VEC = 16 / sizeof(T), SLICE = 256u * VEC * IT;
+    constexpr uint32_t VEC = 16 / sizeof(T), SLICE = 256u * VEC * IT, HIST = 8, BIAS = WORDS ? 4 : 1;
     __shared__ __attribute__((aligned(16))) uint32_t s_word[WORDS ? SLICE : 1];
-    __shared__ uint64_t s_key[4];
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+    __shared__ float s_bias[WORDS ? 256 * BIAS : 1];
+    __shared__ uint64_t s_key[2][4];
+    uint32_t tid = threadIdx.x;
+    const uint32_t lane = tid & 63u, wave = tid >> 6;
     const uint32_t group = blockIdx.x / a.slices, slice = blockIdx.x - group * a.slices;
     const uint32_t v0 = slice * SLICE, len = min(SLICE, a.vocab - v0);
     const uint32_t r0 = group * a.group, r1 = min(r0 + a.group, a.rows);
-    uint32_t b = 0, first = 0, end = a.rows, before = ~0u; // the sequence and its rows; the row whose nodes are counted
-    const bool ragged = a.batch != 0u; // else the rows stand for themselves
-    if (ragged) {
-        b = (uint32_t)__builtin_amdgcn_readfirstlane((int)seq_behind(a.token_offsets, a.rows, a.batch, r0, lane));
-        end = r0; // looked up below
-    }
-    float rep = 1.0f, freq = 0.0f, pres = 0.0f;
-    auto count_nodes = [&](uint32_t r, uint32_t by) { // the tokens that row r's mask names
-        const uint32_t n = min(end - first, 32u * a.mask_words);
-        for (uint32_t j = tid; j < n; j += 256u)
-            if (a.tree_mask[(uint64_t)r * a.mask_words + j / 32u] >> (j % 32u) & 1u) {
-                const uint32_t id = a.node_tokens[first + j] - v0;
-                if (id < len) atomicAdd(&s_word[id], by);
-            }
+    const bool narrow = len < VEC; // a last slice shorter than a piece
+    // Where this thread's piece `it` begins (tokens of the slice).
+    auto place = [&](int it) { return min(((uint32_t)it * 256u + tid) * VEC, narrow ? 0u : len - VEC); };
+    auto within = [&](int it) { return ((uint32_t)it * 256u + tid) * VEC < len; };
+    vec_t x[IT];
+    auto fetch = [&](uint32_t r) {
+        const char* src = (const char*)a.logits + ((uint64_t)r * a.logits_stride + v0) * sizeof(T);
+        if (narrow) {
+#pragma unroll
+            for (uint32_t e = 0; e < VEC; ++e) x[0][e] = ((const T*)src)[min(e, len - 1u)];
+            return;
+        }
+#pragma unroll
+        for (int it = 0; it < IT; ++it)
+            if (within(it)) x[it] = *(const vec_t*)(src + place(it) * (uint32_t)sizeof(T));
     };
+    fetch(r0);
+    const bool ragged = a.batch != 0u; // else the rows stand for themselves
+    SeqAt seq{0, 0, a.rows};
+    if (ragged) seq.end = r0; // looked up below
+    float rep = 1.0f, freq = 0.0f, pres = 0.0f;
+    uint32_t node = 0, named = 0, nodes = 0; // token of node tid, whether the row before names it, nodes of the masks
     for (uint32_t r = r0; r < r1; ++r) {
-        if (ragged && r >= end) { // uniform
-            if (r != r0) ++b;
-            SeqRows at{0, 0};
-            for (; b < a.batch; ++b) {
-                at = seq_rows(a.token_offsets, a.rows, a.batch, b, a.err);
-                if (at.first + at.n > r) break;
-            }
-            if (b >= a.batch || r < at.first) { // rows of no sequence
+        __asm__ volatile("" : "+v"(tid)); // what is made of it is made in each row, not kept: 172 registers otherwise
+        if (ragged && r >= seq.end) { // uniform
+            seq = seq_at(a.token_offsets, a.rows, a.batch, r, lane);
+            seq = {(uint32_t)__builtin_amdgcn_readfirstlane((int)seq.b), (uint32_t)__builtin_amdgcn_readfirstlane((int)seq.first),
+                   (uint32_t)__builtin_amdgcn_readfirstlane((int)seq.end)};
+            const bool bad = seq.b < a.batch && (seq.first > r || seq.end <= r || seq.end > a.rows); // offsets that descend, or pass the rows
+            if (bad && tid == 0) flag(a.err, kErrSeq);
+            if (seq.b >= a.batch || bad) { // rows of no sequence
                 for (; r < r1; ++r)
                     if (tid == 0 && a.best && a.slices > 1u) a.keys[(uint64_t)r * a.slices + slice] = kNoRow;
                 return;
             }
-            first = at.first;
-            end = at.first + at.n;
-            before = ~0u;
-            if (a.repetition) rep = a.repetition[b];
-            if (a.frequency) freq = a.frequency[b];
-            if (a.presence) pres = a.presence[b];
+            if (a.repetition) rep = a.repetition[seq.b];
+            if (a.frequency) freq = a.frequency[seq.b];
+            if (a.presence) pres = a.presence[seq.b];
             if constexpr (WORDS) {
+                const uint32_t* hist = a.history + (uint64_t)seq.b * a.history_stride;
+                uint32_t h[HIST];
+                auto history = [&](uint32_t from) { // tokens from + tid + 256 k
+#pragma unroll
+                    for (uint32_t k = 0; k < HIST; ++k) h[k] = hist[min(from + tid + 256u * k, a.history_stride - 1u)];
+                };
+                uint32_t held = 0, prompt = 0, entries = 0, id[BIAS];
+                float value[BIAS];
+                if (a.history) {
+                    history(0);
+                    held = a.history_count[seq.b];
+                    if (a.prompt_count) prompt = a.prompt_count[seq.b];
+                }
+                if (a.bias_ids) {
+                    entries = a.bias_count ? a.bias_count[seq.b] : a.bias_stride;
+                    const uint32_t* ids = a.bias_ids + (uint64_t)seq.b * a.bias_stride;
+                    const float* values = a.bias_values + (uint64_t)seq.b * a.bias_stride;
+#pragma unroll
+                    for (uint32_t k = 0; k < BIAS; ++k)
+                        if (256u * k < a.bias_stride) { // uniform
+                            const uint32_t i = min(tid + 256u * k, a.bias_stride - 1u);
+                            id[k] = ids[i];
+                            value[k] = values[i];
+                        }
+                }
+                nodes = a.node_tokens ? min(seq.end - seq.first, 32u * a.mask_words) : 0u;
+                if (tid < nodes) node = a.node_tokens[seq.first + tid] - v0;
+                named = 0;
                 for (uint32_t i = 4u * tid; i < SLICE; i += 1024u) *(uint4_t*)(s_word + i) = (uint4_t)0u;
                 __syncthreads();
                 if (a.bias_ids) {
-                    const uint32_t n = a.bias_count ? a.bias_count[b] : a.bias_stride;
-                    if (n > a.bias_stride && tid == 0) flag(a.err, kErrSeq);
-                    for (uint32_t i = tid; i < min(n, a.bias_stride); i += 256u) {
-                        const uint32_t id = a.bias_ids[(uint64_t)b * a.bias_stride + i] - v0;
-                        if (id < len) atomicMax(&s_word[id], (i + 1u) << kCountBits); // the last entry holds
+                    if (entries > a.bias_stride && tid == 0) flag(a.err, kErrSeq);
+                    entries = min(entries, a.bias_stride);
+#pragma unroll
+                    for (uint32_t k = 0; k < BIAS; ++k) {
+                        const uint32_t i = tid + 256u * k, v = id[k] - v0;
+                        if (i < entries) {
+                            s_bias[i] = value[k];
+                            if (v < len) atomicMax(&s_word[v], (i + 1u) << kCountBits); // the last entry holds
+                        }
                     }
                     __syncthreads();
                 }
                 if (a.history) {
-                    const uint32_t n = a.history_count[b], prompt = a.prompt_count ? a.prompt_count[b] : 0u;
-                    if (n > a.history_stride && tid == 0) flag(a.err, kErrSeq);
-                    for (uint32_t i = tid; i < min(n, a.history_stride); i += 256u) {
-                        const uint32_t id = a.history[(uint64_t)b * a.history_stride + i] - v0;
-                        if (id < len) {
-                            if (i < prompt) atomicOr(&s_word[id], 1u << 31);
-                            else atomicAdd(&s_word[id], 1u);
+                    if (held > a.history_stride && tid == 0) flag(a.err, kErrSeq);
+                    held = min(held, a.history_stride);
+                    for (uint32_t from = 0;;) {
+#pragma unroll
+                        for (uint32_t k = 0; k < HIST; ++k) {
+                            const uint32_t i = from + tid + 256u * k, v = h[k] - v0;
+                            if (v < len && i < held) {
+                                if (i < prompt) atomicOr(&s_word[v], 1u << 31);
+                                else atomicAdd(&s_word[v], 1u);
+                            }
                         }
+                        from += 256u * HIST;
+                        if (from >= held) break; // uniform
+                        history(from);
                     }
                 }
             }
         }
-        const T* src = (const T*)a.logits + (uint64_t)r * a.logits_stride + v0;
-        vec_t x[IT];
+        // The grammar's row: none, one of the table, or (an index past it) nothing.
+        uint32_t may[IT];
+        {
+            int32_t at = -1;
+            if (a.allowed) at = a.allowed_index ? a.allowed_index[r] : (int32_t)r;
+            const bool nothing = at >= 0 && (uint32_t)at >= a.allowed_rows;
+            if (nothing && tid == 0) flag(a.err, kErrToken);
+            const char* bits = (const char*)(a.allowed + (uint64_t)(uint32_t)at * a.allowed_stride + v0 / 32u);
 #pragma unroll
-        for (int it = 0; it < IT; ++it) {
-            const uint32_t at = ((uint32_t)it * 256u + tid) * VEC;
-            if (at + VEC <= len) {
-                x[it] = *(const vec_t*)(src + at);
-            } else {
-#pragma unroll
-                for (uint32_t e = 0; e < VEC; ++e) x[it][e] = at + e < len ? src[at + e] : (T)0.0f;
+            for (int it = 0; it < IT; ++it) {
+                may[it] = nothing ? 0u : ~0u;
+                if (at >= 0 && !nothing) { // uniform; a piece may lie in two words
+                    const uint32_t t = place(it), k = t / 32u * 4u;
+                    may[it] = *(const uint32_t*)(bits + k) >> (t % 32u);
+                    if (t % 32u > 32u - VEC) may[it] |= *(const uint32_t*)(bits + min(k + 4u, (len - 1u) / 32u * 4u)) << (32u - t % 32u);
+                }
             }
         }
-        if (WORDS && a.node_tokens) {
-            if (before != ~0u) count_nodes(before, ~0u);
-            count_nodes(r, 1u);
-            before = r;
+        if (WORDS && nodes) { // uniform: the tokens that the row's mask names, but not the row's before, and the other way
+            const uint32_t* mask = a.tree_mask + (uint64_t)r * a.mask_words;
+            if (tid < nodes) {
+                const uint32_t now = mask[tid / 32u] >> (tid % 32u) & 1u;
+                if (now != named && node < len) atomicAdd(&s_word[node], now - named);
+                named = now;
+            }
+            for (uint32_t i = tid + 256u; i < nodes; i += 256u) { // wide trees: what the row before named is read again
+                const uint32_t now = mask[i / 32u] >> (i % 32u) & 1u;
+                const uint32_t was = r > r0 && r > seq.first ? mask[(int32_t)(i / 32u) - (int32_t)a.mask_words] >> (i % 32u) & 1u : 0u;
+                const uint32_t v = a.node_tokens[seq.first + i] - v0;
+                if (now != was && v < len) atomicAdd(&s_word[v], now - was);
+            }
         }
         if constexpr (WORDS) __syncthreads();
-        // The grammar's row: none, one of the table, or (an index past it) one that allows nothing.
-        const uint32_t* allowed = nullptr;
-        bool nothing = false;
-        if (a.allowed) {
-            const int32_t at = a.allowed_index ? a.allowed_index[r] : (int32_t)r;
-            nothing = at >= 0 && (uint32_t)at >= a.allowed_rows;
-            if (at >= 0 && !nothing) allowed = a.allowed + (uint64_t)at * a.allowed_stride + v0 / 32u;
-            if (nothing && tid == 0) flag(a.err, kErrToken);
-        }
         float top = -INFINITY;
         uint32_t token = 0;
+        char* dst = (char*)a.out + ((uint64_t)r * a.out_stride + v0) * sizeof(T);
 #pragma unroll
         for (int it = 0; it < IT; ++it) {
-            const uint32_t at = ((uint32_t)it * 256u + tid) * VEC;
-            if (at >= len) continue;
-            const uint32_t may = allowed ? allowed[at / 32u] >> (at % 32u) : (nothing ? 0u : ~0u);
+            if (!within(it)) continue;
+            const uint32_t at = place(it);
+            float f[VEC];
+#pragma unroll
+            for (uint32_t e = 0; e < VEC; ++e) f[e] = (float)x[it][e];
+            if constexpr (WORDS) {
+                uint32_t word[VEC], hit = 0; // tokens that have a word: few, taken one after another
+#pragma unroll
+                for (uint32_t e = 0; e < VEC; ++e) {
+                    word[e] = s_word[at + e];
+                    hit |= (word[e] ? 1u : 0u) << e;
+                }
+#pragma unroll 1
+                for (; hit; hit &= hit - 1u) {
+                    const uint32_t e = (uint32_t)__builtin_ctz(hit);
+                    uint32_t w = word[0];
+                    float y = f[0];
+#pragma unroll
+                    for (uint32_t k = 1; k < VEC; ++k) {
+                        w = e == k ? word[k] : w;
+                        y = e == k ? f[k] : y;
+                    }
+                    const uint32_t c = w & kCountMask, entry = w >> kCountBits & kBiasMask;
+                    if (c || w >> 31) y = y > 0.0f ? y / rep : y * rep;
+                    if (c) {
+                        y = y - freq * (float)c;
+                        y = y - pres;
+                    }
+                    if (entry) y = y + s_bias[entry - 1u];
+#pragma unroll
+                    for (uint32_t k = 0; k < VEC; ++k) f[k] = e == k ? y : f[k];
+                }
+            }
             vec_t y;
 #pragma unroll
             for (uint32_t e = 0; e < VEC; ++e) {
-                float f = (float)x[it][e];
-                if constexpr (WORDS) {
-                    const uint32_t w = s_word[at + e];
-                    if (w) {
-                        const uint32_t c = w & kCountMask, entry = w >> kCountBits & kBiasMask;
-                        if (c || w >> 31) f = f > 0.0f ? f / rep : f * rep;
-                        if (c) {
-                            f = f - freq * (float)c;
-                            f = f - pres;
-                        }
-                        if (entry) f = f + a.bias_values[(uint64_t)b * a.bias_stride + entry - 1u];
-                    }
-                }
-                if (!(may >> e & 1u)) f = -INFINITY;
-                if (at + e < len && f > top) {
-                    top = f;
+                if (!(may[it] >> e & 1u)) f[e] = -INFINITY;
+                if (f[e] > top && (!narrow || e < len)) {
+                    top = f[e];
                     token = v0 + at + e;
                 }
-                y[e] = (T)f;
+                y[e] = (T)f[e];
             }
             if (a.out) {
-                T* dst = (T*)a.out + (uint64_t)r * a.out_stride + v0 + at;
-                if (at + VEC <= len) {
-                    *(vec_t*)dst = y;
+                if (!narrow) {
+                    *(vec_t*)(dst + at * (uint32_t)sizeof(T)) = y;
                 } else {
 #pragma unroll
                     for (uint32_t e = 0; e < VEC; ++e)
-                        if (at + e < len) dst[e] = y[e];
+                        if (e < len) ((T*)dst)[e] = y[e];
                 }
             }
         }
+        if (r + 1u < r1) fetch(r + 1u); // while this row's best is found
+        uint64_t* keys = s_key[r & 1u]; // of the row before: thread 0 may still read them
         if (a.best) {
-            const uint64_t key = wave_max64(best_key(top, token));
-            if (lane == 0) s_key[wave] = key;
-            __syncthreads();
-            if (tid == 0) {
-                uint64_t k = s_key[0];
-#pragma unroll
-                for (int w = 1; w < 4; ++w) k = k > s_key[w] ? k : s_key[w];
-                if (a.slices > 1u) a.keys[(uint64_t)r * a.slices + slice] = k;
-                else a.best[r] = best_token(k);
-            }
+            const uint64_t key = wave_best(top, token);
+            if (lane == 0) keys[wave] = key;
         }
-        __syncthreads(); // words and keys have been read
+        __syncthreads(); // words have been read
+        if (a.best && tid == 0) {
+            uint64_t k = keys[0];
+#pragma unroll
+            for (int w = 1; w < 4; ++w) k = k > keys[w] ? k : keys[w];
+            if (a.slices > 1u) a.keys[(uint64_t)r * a.slices + slice] = k;
+            else a.best[r] = best_token(k);
+        }
     }
 }
 

@@ -338,7 +338,7 @@ typedef struct aw_logits_desc {
     const int32_t*  allowed_index;
 } aw_logits_desc;
 
-/* `best` takes scratch of the engine's workspace, 8 bytes a row and 2048 tokens or more, as in
+/* `best` takes scratch of the engine's workspace, 8 bytes a row and 1024 tokens or more, as in
  * aw_decode_device, also under capture. */
 int aw_ops_adjust_logits(aw_engine* engine, const aw_logits_desc* desc, void* hip_stream);
 
