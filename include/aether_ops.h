@@ -343,7 +343,8 @@ typedef struct aw_logits_desc {
 int aw_ops_adjust_logits(aw_engine* engine, const aw_logits_desc* desc, void* hip_stream);
 
 /* From node 0 of each tree, whose token is kept, on: of the children of the node kept last
- * the lowest whose token is targets[that node] is kept too, until there is none.
+ * the lowest whose token is targets[that node] is kept too, until there is none (a target of
+ * 0xFFFFFFFF, a best of -1, is no token).
  *   accepted   [batch] how many are kept (0 for a sequence without nodes)
  *   next_token [batch] targets[the last one kept] (-1 without nodes): the next tree's node 0
  *   seq_hot    [batch] seq_held + accepted; may be seq_held

@@ -192,7 +192,8 @@ def accept_tree(parents, tokens, targets, offsets) -> list:
         path = [0] if n else []
         while path:
             cur = path[-1]
-            child = [j for j in range(cur + 1, n) if int(parents[first + j]) == cur and int(tokens[first + j]) == int(targets[first + cur])]
+            target = int(targets[first + cur]) & 0xFFFFFFFF
+            child = [j for j in range(cur + 1, n) if int(parents[first + j]) == cur and int(tokens[first + j]) & 0xFFFFFFFF == target != 0xFFFFFFFF]
             if not child:
                 break
             path.append(child[0])

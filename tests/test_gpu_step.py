@@ -295,6 +295,26 @@ def test_logits_in_place_and_each_output_alone(ops, engine):
     c.check(out=c.src)
 
 
+# Rows of which a work-group takes 2, 4 or 16 of a sequence, or of two; a last slice of one token and of a piece less one.
+GROUPS = {"2": (40001, [7] * 60 + [0, 1, 90], False), "2_f16": (20481, [7] * 60 + [0, 1, 400], True), "4": (4099, [1] * 900 + [64] * 40, False),
+          "16": (1031, [33] * 990 + [1, 0, 2], False), "16_f16": (4101, [40] * 450 + [300, 2], True)}
+
+
+@pytest.mark.parametrize("name", sorted(GROUPS))
+def test_logits_of_many_rows(ops, engine, name):
+    vocab, counts, half = GROUPS[name]
+    c = Logits(11, vocab, counts, half=half, history=70, bias=9, allowed=0.8, pad=3)
+    d = c.desc()
+    ops.adjust_logits(d)
+    c.check()
+    d.out, d.out_stride = d.logits, d.logits_stride  # in place
+    c.best.fill_(-77)
+    ops.adjust_logits(d)
+    rows = int(c.offsets[-1])
+    assert np.array_equal(host(c.src)[:rows], host(c.out)[:rows]) and np.array_equal(host(c.src)[rows:], c.x[rows:])
+    assert error_of(engine) == ""
+
+
 def test_logits_penalties_left_out(ops):
     for name in ("repetition", "frequency", "presence", "prompt_count", "bias_count"):
         c = Logits(2, 2000, [3, 2], history=90, bias=12)
@@ -492,6 +512,15 @@ def test_accept_reports(ops, engine):
     c = Accept(4, [1500, 3], agree=1.0, shape="chain", layers=1, history=3000)
     ops.accept_tree(c.desc())
     assert "sequence length" in error_of(engine)
+    c.check()
+
+
+def test_accept_a_target_that_is_no_token(ops, engine):
+    c = Accept(5, [5, 9, 2, 33], agree=1.0)
+    c.tokens[[1, 2, 3, 6, 7, 17, 18]] = 0xFFFFFFFF
+    c.targets[[0, 5, 16]] = 0xFFFFFFFF  # a best of -1: nothing continues it, also not a token of the same bits
+    ops.accept_tree(c.desc())
+    assert error_of(engine) == ""
     c.check()
 
 
