@@ -461,18 +461,30 @@ __global__ __launch_bounds__(kPrefixThreads) __attribute__((amdgpu_waves_per_eu(
     // Work-group b runs on XCD b % 8: neighbours in the line, which read the same pages for
     // several tiles of rows, run on one XCD.
     const uint32_t w = (blockIdx.x & 7u) * (a.work_groups >> 3) + (blockIdx.x >> 3);
-    uint32_t* s_sum = (uint32_t*)prefix_lds; // [4] sums of waves; the sequence found: [5]
+    uint32_t* s_sum = (uint32_t*)prefix_lds; // [4] sums of waves, [5] the sequence found, [4] sums of waves in fp32
     // All steps; sequence tid of each 256.
     TreeSeq s{};
     uint32_t mine = 0;
+    // Counted in fp32 too: offsets that descend give rows to several sequences, or one has far more nodes than its
+    // mask names; steps that pass 32 bits by that (both are reported) are not taken.
+    float wide = 0.0f;
     for (uint32_t b = tid; b < a.batch; b += 256u) {
         s = tree_seq(a, b, blockIdx.x == 0);
-        mine += TreeWork<NR>(a, s).all(a.kv_heads);
+        const TreeWork<NR> work(a, s);
+        mine += work.all(a.kv_heads);
+        wide += (float)a.kv_heads * (float)work.tiles * (float)work.steps;
     }
     mine = lanes_scan(mine);
-    if (lane == 63u) s_sum[wave] = mine;
+    wide = wave_sum(wide);
+    if (lane == 63u) {
+        s_sum[wave] = mine;
+        s_sum[9u + wave] = __builtin_bit_cast(uint32_t, wide);
+    }
     __syncthreads();
-    const uint32_t total = uniform(s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]);
+    wide = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < 4u; ++i) wide += __builtin_bit_cast(float, s_sum[9u + i]);
+    const uint32_t total = uniform(wide >= 4294960000.0f ? 0u : s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]);
     const uint32_t each = uniform((total + a.work_groups - 1u) / a.work_groups);
     uint32_t pos = w * each;
     const uint32_t stop = min(pos + each, total);
@@ -583,7 +595,8 @@ __global__ __launch_bounds__(kPrefixThreads) __attribute__((amdgpu_waves_per_eu(
         }
         if (pos >= stop) break;
         base += all;
-        s = tree_seq(a, ++b, false); // there is one: its steps are among the total
+        if (++b >= a.batch) break; // not met: the steps left are a later sequence's
+        s = tree_seq(a, b, false);
         s = {uniform(s.first), uniform(s.nodes), uniform(s.held)};
     }
     if (tid == 0) {

@@ -386,7 +386,9 @@ void aw_abi_prefix_sizes(size_t sizes[2]);
  * aligned, its stride a multiple of 4.  out may be q (same stride) and shares no element otherwise.
  * A row that sees nothing is zeros; rows behind the last sequence are left as they are.  Bit 31 of a ref is masked; a ref >= hot_blocks
  * hides its tokens and sets the device error "hot block ref"; a seq_held over hot_count * 16, offsets that
- * descend or pass num_tokens, and nodes past 32 mask_words (which no row sees) set "sequence length".
+ * descend or pass num_tokens, and nodes past 32 mask_words (which no row sees) set "sequence length"; a
+ * sequence with such offsets has no rows; where the others then have more rows than num_tokens, or far more nodes than
+ * their masks name, none may be computed.
  * Values that a row does not see never reach it, infinities and NaNs neither.
  * head_dim 64 or 128; up to 2^20 sequences, 2^22 tokens of each in pages, 2^25 rows of q.
  * Scratch is the engine's workspace, as in aw_decode_device, also under capture. */

@@ -319,3 +319,49 @@ def test_a_lost_page_shows(ops, hd):
     want = (1500 - 16 + 16 * 65.0 + np.array([bin(int(c.mask[r, 0]) | int(c.mask[r, 1]) << 32).count("1") for r in range(40)])) / \
         (1500 + np.array([bin(int(c.mask[r, 0]) | int(c.mask[r, 1]) << 32).count("1") for r in range(40)]))
     assert np.abs(host(c.out)[:40].astype(np.float64) - want[:, None, None]).max() < 0.002
+
+
+# A table far wider than the lengths (spare) has the steps planned for it shared out, few of which there are.
+WAYS = [  # heads, nodes, held, entries of the table that no length reaches, query rows of a unit (0: one launch)
+    (32, 8, 64, [4] * 40, [50 + i for i in range(40)], 0, 0), (32, 8, 128, [4, 0, 9, 5] * 8, [3 * i for i in range(32)], 0, 0),
+    (32, 8, 128, [3, 5], [700, 64], 0, 0), (14, 2, 64, [30, 2], [900, 1], 0, 0),
+    (8, 2, 64, [3, 4, 1, 0, 5], [300, 0, 1025, 77, 64], 3000, 16), (8, 2, 128, [3, 4, 1, 0, 5], [300, 0, 1025, 77, 64], 3000, 16),
+    (8, 2, 64, [7, 8, 0, 9], [300, 0, 63, 1100], 8000, 32), (8, 2, 128, [7, 8, 1, 9], [300, 0, 63, 1100], 8000, 32),
+    (8, 2, 64, [40, 33, 64, 1], [300, 0, 1025, 77], 9000, 128), (8, 2, 128, [40, 33, 64, 1], [300, 0, 1025, 77], 9000, 128),
+    (6, 2, 64, [i % 3 for i in range(300)], [11 * i % 90 for i in range(300)], 500, 16),
+    (6, 2, 128, [8 + i % 3 for i in range(260)], [11 * i % 90 for i in range(260)], 400, 32),
+    (6, 2, 64, [16 + i % 3 for i in range(257)], [11 * i % 90 for i in range(257)], 400, 128),
+    (4, 1, 128, [1], [40000], 0, 16), (20, 1, 64, [1], [33333], 16900, 32), (5, 1, 64, [130], [20000], 60000, 128), (5, 1, 128, [130], [20000], 60000, 128),
+]
+
+
+@pytest.mark.parametrize("way", WAYS, ids=[f"{c[0]}-{c[1]}-{c[2]}-{len(c[3])}x{max(c[3])}-{c[6]}" for c in WAYS])
+def test_each_way_to_split(ops, engine, way):
+    import torch
+    from aether_nexus_amd import ops as O
+    hq, hk, hd, nodes, held, spare, tile = way
+    c = Case(31, hq, hk, hd, nodes, held, pad=3, spare=spare, qscale=1.0)
+    d = c.desc()
+    plan = O.tree_plan(d, torch.cuda.get_device_properties(0).multi_processor_count)
+    assert (plan.row_tile if plan.workspace_bytes else 0) == tile
+    ops.tree_attention(d)
+    assert error_of(engine) == ""
+    c.check("split")
+    first = host(c.out).copy()
+    c.out.fill_(7.0)
+    ops.tree_attention(d)
+    assert np.array_equal(host(c.out).view(np.int16), first.view(np.int16))  # parts are joined in one order
+
+
+@pytest.mark.parametrize("tile", [16, 128])
+def test_offsets_that_descend_where_steps_are_shared_out(ops, engine, tile):
+    from aether_nexus_amd import ops as O
+    nodes = [3, 0] * 150 if tile == 16 else [40, 0] * 6
+    c = Case(32, 8, 2, 64, nodes, [90] * len(nodes), spare=9000, pad=2)
+    n = c.rows
+    d = c.desc(token_offsets=dev(np.array([0, n] * (len(nodes) // 2) + [0])))  # every other sequence has all rows, the rest descend
+    assert O.tree_plan(d).row_tile == tile
+    ops.tree_attention(d)
+    assert "sequence length" in error_of(engine)
+    got = host(c.out)
+    assert np.isfinite(got[:sum(nodes)].astype(np.float64)).all()

@@ -177,7 +177,8 @@ def test_tree_invalid(kw):
 
 @pytest.mark.parametrize("kw", [
     dict(head_dim=96), dict(hot_count=(1 << 18) + 1, refs_stride=1 << 19), dict(kv_heads=1024, q_heads=1024), dict(num_tokens=1 << 23),
-    dict(batch=(1 << 20) + 1), dict(mask_words=33), dict(q_stride=(1 << 30) + 8), dict(num_tokens=(1 << 24) + 1, q_heads=2)])
+    dict(batch=(1 << 20) + 1), dict(mask_words=33), dict(q_stride=(1 << 30) + 8), dict(num_tokens=(1 << 24) + 1, q_heads=2),
+    dict(num_tokens=1 << 20, hot_count=1 << 16, refs_stride=1 << 16)])
 def test_tree_unsupported(kw):
     with pytest.raises(WeaverError) as e:
         O.tree_plan(tree(**kw))
