@@ -678,10 +678,10 @@ __global__ __launch_bounds__(NW * 64) void tree_pages_kernel(TreeArgs a) {
 
 // Joins the parts of the units that are cut, a wave a row: their largest maximum, each
 // part's sums times 2^(its maximum - that), in the order of the parts; zeros where no part saw a
-// token.  An inf or NaN in a part's sum stays, as in prefix_merge_kernel.  Bound: two round
-// trips (the cut's record; then factors and sums together), 9.6 us for 512 work-groups' 32-row units;
-// 128-row units of 128 dims 14.3, 44 MB of sums.
-constexpr uint32_t kTreeMergeRows = 16; // of a work-group
+// token.  An inf or NaN in a part's sum stays, as in prefix_merge_kernel.  Bound: round trips
+// (the cut's record; factors and sums together), so a row a wave: with four rows one after
+// another a request took 2 to 4 us more (182.7 for 180.8, 82.7 for 78.9).
+constexpr uint32_t kTreeMergeRows = 4; // of a work-group
 template <int HD, int NR>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
     constexpr uint32_t LP = HD / 4, PG = 64 / LP, U = 4; // lanes of a part's row, parts of one load, loads in flight
@@ -690,56 +690,56 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
     const uint32_t S = cut[0], rows = cut[1], row0 = cut[2], first = cut[3], g = cut[4];
     if (!S) return;
     const uint32_t sub = lane / LP, d = 4u * (lane % LP);
-    for (uint32_t r = blockIdx.y * kTreeMergeRows + wave; r < min(rows, (blockIdx.y + 1u) * kTreeMergeRows); r += 4u) {
-        auto slot = [&](uint32_t p) { return (p ? 2ull * (w + p) : 2ull * w + 1u) * tree_rows(NR) + r; };
-        float4_t v[U];
-        auto load = [&](uint32_t p0) {
+    const uint32_t r = blockIdx.y * kTreeMergeRows + wave;
+    if (r >= rows) return;
+    auto slot = [&](uint32_t p) { return (p ? 2ull * (w + p) : 2ull * w + 1u) * tree_rows(NR) + r; };
+    float4_t v[U];
+    auto load = [&](uint32_t p0) {
 #pragma unroll
-            for (uint32_t j = 0; j < U; ++j) v[j] = *(const float4_t*)(a.part_o + slot(min(p0 + j * PG + sub, S - 1u)) * HD + d);
-        };
-        float l = a.part_l[slot(min(lane, S - 1u))], m = a.part_m[slot(min(lane, S - 1u))];
-        load(0); // before the parts' factors are known
-        if (lane >= S || l == 0.0f) { // a part that saw nothing holds no sums
-            l = 0.0f;
-            m = -INFINITY;
-        }
-        float M = m;
-        for (uint32_t p = lane + 64u; p < S; p += 64u)
-            if (a.part_l[slot(p)] != 0.0f) M = fmaxf(M, a.part_m[slot(p)]);
-        M = wave_max(M);
-        float L = 0.0f;
-        float4_t acc = (float4_t)0.0f;
-        for (uint32_t c0 = 0; c0 < S; c0 += 64u) { // 64 parts' factors in the lanes
-            if (c0) {
-                l = c0 + lane < S ? a.part_l[slot(c0 + lane)] : 0.0f;
-                m = l != 0.0f ? a.part_m[slot(c0 + lane)] : -INFINITY;
-            }
-            const float f = l != 0.0f ? fast_exp2(m - M) : 0.0f;
-            const uint64_t saw = __ballot(l != 0.0f);
-            L += wave_sum(f * l);
-            for (uint32_t p0 = 0; p0 < min(S - c0, 64u); p0 += U * PG) {
-                if (c0 + p0) load(c0 + p0);
-#pragma unroll
-                for (uint32_t j = 0; j < U; ++j) {
-                    const uint32_t p = p0 + j * PG + sub; // < 64
-                    const float fp = __shfl(f, (int)p);
-                    if ((saw >> p) & 1u)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[e] = fmaf(fp, v[j][e], acc[e]);
-                }
-            }
-        }
-#pragma unroll
-        for (int o = LP; o < 64; o *= 2)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], o);
-        if (sub) continue;
-        const uint32_t R = row0 + r;
-        half4_t h;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) h[e] = (_Float16)(L == 0.0f ? 0.0f : acc[e] / L);
-        *(half4_t*)(a.out + (first + R / a.gqa) * a.out_stride + (g * a.gqa + R % a.gqa) * (uint64_t)HD + d) = h;
+        for (uint32_t j = 0; j < U; ++j) v[j] = *(const float4_t*)(a.part_o + slot(min(p0 + j * PG + sub, S - 1u)) * HD + d);
+    };
+    float l = a.part_l[slot(min(lane, S - 1u))], m = a.part_m[slot(min(lane, S - 1u))];
+    load(0); // before the parts' factors are known
+    if (lane >= S || l == 0.0f) { // a part that saw nothing holds no sums
+        l = 0.0f;
+        m = -INFINITY;
     }
+    float M = m;
+    for (uint32_t p = lane + 64u; p < S; p += 64u)
+        if (a.part_l[slot(p)] != 0.0f) M = fmaxf(M, a.part_m[slot(p)]);
+    M = wave_max(M);
+    float L = 0.0f;
+    float4_t acc = (float4_t)0.0f;
+    for (uint32_t c0 = 0; c0 < S; c0 += 64u) { // 64 parts' factors in the lanes
+        if (c0) {
+            l = c0 + lane < S ? a.part_l[slot(c0 + lane)] : 0.0f;
+            m = l != 0.0f ? a.part_m[slot(c0 + lane)] : -INFINITY;
+        }
+        const float f = l != 0.0f ? fast_exp2(m - M) : 0.0f;
+        const uint64_t saw = __ballot(l != 0.0f);
+        L += wave_sum(f * l);
+        for (uint32_t p0 = 0; p0 < min(S - c0, 64u); p0 += U * PG) {
+            if (c0 + p0) load(c0 + p0);
+#pragma unroll
+            for (uint32_t j = 0; j < U; ++j) {
+                const uint32_t p = p0 + j * PG + sub; // < 64
+                const float fp = __shfl(f, (int)p);
+                if ((saw >> p) & 1u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[e] = fmaf(fp, v[j][e], acc[e]);
+            }
+        }
+    }
+#pragma unroll
+    for (int o = LP; o < 64; o *= 2)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], o);
+    if (sub) return;
+    const uint32_t R = row0 + r;
+    half4_t h;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[e] = (_Float16)(L == 0.0f ? 0.0f : acc[e] / L);
+    *(half4_t*)(a.out + (first + R / a.gqa) * a.out_stride + (g * a.gqa + R % a.gqa) * (uint64_t)HD + d) = h;
 }
 
 } // namespace aw
