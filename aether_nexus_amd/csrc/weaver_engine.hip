@@ -1220,7 +1220,7 @@ int tree_plan(const aw_tree_desc* d, uint32_t n_cu, aw::TreeArgs* out, aw_tree_p
     a = aw::TreeArgs{};
     a.q_stride = d->q_stride ? d->q_stride : q_row;
     a.k_stride = d->k_stride ? d->k_stride : k_row;
-    a.v_stride = d->v_stride ? d->v_stride : k_row;
+    a.v_stride = !d->v ? a.k_stride : d->v_stride ? d->v_stride : k_row; // K rows as values lie where K lies
     a.out_stride = d->out_stride ? d->out_stride : q_row;
     if (a.q_stride < q_row || a.k_stride < k_row || a.v_stride < k_row || a.out_stride < q_row)
         return refuse(AW_E_INVALID_ARG, "a stride is shorter than a token's heads");

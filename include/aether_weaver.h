@@ -379,7 +379,8 @@ void aw_abi_prefix_sizes(size_t sizes[2]);
  * is known after the step (aw_ops_accept_tree).  Device pointers, f16:
  *   q, out       [num_tokens][q_heads][head_dim], *_stride elements from row to row (0: contiguous)
  *   k, v         [num_tokens][kv_heads][head_dim], likewise; the parts of a fused q/k/v product's rows are taken
- *   hot_k, hot_v [hot_blocks][16][kv_heads][head_dim]; v and hot_v NULL: V is the K row
+ *                (v NULL: V is the K row, and v_stride is not read)
+ *   hot_k, hot_v [hot_blocks][16][kv_heads][head_dim], hot_v NULL with v
  *   refs         [batch][refs_stride]: a sequence's pages
  *   seq_held     [batch] its tokens there
  * q, k, v and the pools 16-byte aligned, with strides that are multiples of 8 elements; out 8-byte
