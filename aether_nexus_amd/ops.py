@@ -373,16 +373,20 @@ def tree_plan(desc: TreeDesc, compute_units: int = 0, lib_path=None) -> TreePlan
     return info
 
 
-def _vocab_rows(t, rows: int, vocab: int, dtype_check, what: str) -> int:
-    """Row stride of [rows][vocab]: contiguous, a raw pointer, or rows further apart."""
-    if t is None or isinstance(t, int) or not hasattr(t, "is_contiguous") or t.is_contiguous():
-        dtype_check(t, rows * vocab, what)
-        return vocab
-    if t.dim() != 2 or t.shape[0] < rows or t.shape[1] != vocab or (vocab > 1 and t.stride(1) != 1) or t.stride(0) < vocab:
-        raise WeaverError(f"{what}: a view must be [rows][{vocab}] with rows apart, got shape {tuple(t.shape)}, strides "
+def _vocab_rows(t, rows: int, width: int, dtype_check, what: str) -> int:
+    """Row stride of [rows][width]: ``width`` of a flat tensor or a raw pointer, else the tensor's own, whose rows (all
+    dims but the last) may be longer than ``width`` (a padded vocabulary) or lie further apart."""
+    if t is None or isinstance(t, int) or not hasattr(t, "dim") or t.dim() < 2:
+        dtype_check(t, rows * width, what)
+        return width
+    whole, last = t.is_contiguous(), t.shape[-1]
+    stride = last if whole else t.stride(0)
+    if rows and (last < width or t.numel() // last < rows or (not whole and (t.dim() != 2 or (last > 1 and t.stride(1) != 1))) or
+                 (rows > 1 and stride < width)):
+        raise WeaverError(f"{what}: [{rows}][{width}] are read or written, rows of one stride, got shape {tuple(t.shape)}, strides "
                           f"{tuple(t.stride())}", AW_E_INVALID_ARG)
-    dtype_check(t[:0].contiguous(), 0, what)
-    return t.stride(0)
+    dtype_check(t if whole else t[:0].contiguous(), 0, what)
+    return stride if rows > 1 else width
 
 
 def make_logits_desc(*, num_tokens: int, vocab_size: int, logits, out=None, best=None, batch: int = 0, token_offsets=None, history=None,
@@ -392,7 +396,8 @@ def make_logits_desc(*, num_tokens: int, vocab_size: int, logits, out=None, best
                      bias_stride: Optional[int] = None, allowed_rows: Optional[int] = None) -> LogitsDesc:
     """An ``aw_logits_desc`` from device tensors (or raw device pointers to contiguous rows), for
     ``adjust_logits``: ``logits`` and ``out`` [num_tokens][vocab_size] in fp32 or f16 (``half`` for raw
-    pointers; out may be logits, or None with ``best``), ``history`` [batch][stride] and ``bias_ids`` /
+    pointers; out may be logits, or None with ``best``; their rows, and those of ``allowed``, may be longer than
+    that or lie apart), ``history`` [batch][stride] and ``bias_ids`` /
     ``bias_values`` [batch][stride] with a count for each sequence, ``allowed`` [rows][ceil(vocab_size /
     32)] bit words and ``allowed_index`` [num_tokens]."""
     d = LogitsDesc()

@@ -1,0 +1,41 @@
+"""Page tables, adjusted logits and accepted trees where tensors, lists or tables are at an edge, against oracle/step_oracle.py as
+test_gpu_step.py compares them, whose inputs it takes."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from oracle import step_oracle as S
+from test_gpu_step import Accept, Logits, Tables, dev, empty, error_of, host
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops(engine):
+    from aether_nexus_amd.ops import OpsEngine
+    return OpsEngine(engine)
+
+
+@pytest.mark.parametrize("half", [False, True], ids=["f32", "f16"])
+def test_logits_of_a_padded_vocabulary(ops, engine, half):
+    """Contiguous rows longer than the vocabulary, of logits, outputs and grammar words: what lies past it stays."""
+    import torch
+    c = Logits(21, 9001, [3, 0, 5], half=half, history=50, bias=5, allowed=0.5, pad=2)
+    d = c.desc()
+    rows, vocab = c.x.shape
+    src = torch.full((rows, 9216), 3.0, dtype=c.src.dtype, device="cuda:0")
+    src[:, :vocab] = c.src
+    out = torch.full_like(src, 7.0)
+    words = torch.full((c.kw["allowed"].shape[0], 288), -1, dtype=torch.int32, device="cuda:0")
+    words[:, :c.kw["allowed"].shape[1]] = dev(c.kw["allowed"])
+    ops.adjust_logits(c.desc(logits=src, out=out, allowed=words))
+    assert error_of(engine) == ""
+    c.out = out[:, :vocab]
+    c.check()
+    assert (host(out)[:, vocab:] == 7.0).all()
+    c.best.fill_(-77)
+    d = c.desc(logits=src, out=src, allowed=words)
+    ops.adjust_logits(d)
+    c.check(out=src[:, :vocab])
+    assert (host(src)[:, vocab:] == 3.0).all() and np.array_equal(host(src)[8:, :vocab], c.x[8:])

@@ -2,11 +2,64 @@
 from __future__ import annotations
 
 import pytest
+import torch
 
 from aether_nexus_amd import ops as O
+from aether_nexus_amd.types import AW_E_INVALID_ARG
+from aether_nexus_amd.weaver import WeaverError
 from test_step import A, tree
 
 
 @pytest.mark.parametrize("kw", [dict(v_stride=257), dict(v_stride=8), dict(v_stride=1 << 40), dict(k_stride=1536, k=A["q"] + 2 * 1024, q_stride=1536)])
 def test_v_stride_is_not_read_without_v(kw):
     assert O.tree_plan(tree(v=0, hot_v=0, **kw)).work_groups
+
+
+# ---------------------------------------------------------------- tensors of other shapes than the request's
+
+@pytest.fixture
+def on_cpu(monkeypatch):
+    """Descriptors of CPU tensors: every check of a tensor but that it is on the GPU."""
+    def check(t, need, what, dtypes):
+        if t is None or isinstance(t, int):
+            return
+        if t.dtype not in dtypes or not t.is_contiguous() or t.numel() < need:
+            raise WeaverError(f"{what}: dtype, contiguity or {t.numel()} < {need}", AW_E_INVALID_ARG)
+    monkeypatch.setattr(O, "_check_tensor", check)
+
+
+def i32(*shape):
+    return torch.zeros(shape, dtype=torch.int32)
+
+
+def refused(make, **kw):
+    with pytest.raises(WeaverError) as e:
+        make(**kw)
+    assert e.value.status == AW_E_INVALID_ARG
+    return str(e.value)
+
+
+def logits_of(rows=3, vocab=1000, **kw):
+    return O.make_logits_desc(**{**dict(num_tokens=rows, vocab_size=vocab, logits=torch.zeros(rows, vocab), best=i32(rows)), **kw})
+
+
+def test_logits_of_a_padded_vocabulary(on_cpu):
+    """Rows longer than the vocabulary are a tensor's own, contiguous or sliced; flat tensors are rows of the vocabulary."""
+    for wide in (torch.zeros(3, 1024), torch.zeros(3, 1024)[:, :1000], torch.zeros(5, 1024), torch.zeros(1, 3, 1024)):
+        d = logits_of(logits=wide, out=wide, allowed=i32(3, 40))
+        assert (d.logits_stride, d.out_stride, d.allowed_stride) == (1024, 1024, 40)
+    d = logits_of(logits=torch.zeros(3, 1000), out=torch.zeros(3000), allowed=i32(3 * 32), allowed_rows=3)
+    assert (d.logits_stride, d.out_stride, d.allowed_stride) == (1000, 1000, 32)
+    d = logits_of(allowed=i32(7, 64)[:, :32])
+    assert (d.allowed_stride, d.allowed_rows) == (64, 7)
+    assert logits_of(rows=1, logits=torch.zeros(1, 1000).expand(1, 1000)).logits_stride >= 1000
+    assert logits_of(rows=0, logits=torch.zeros(0, 1000)).num_tokens == 0
+
+
+@pytest.mark.parametrize("kw", [
+    dict(logits=torch.zeros(6, 500)), dict(logits=torch.zeros(1, 3000)), dict(logits=torch.zeros(2, 1024)), dict(logits=torch.zeros(2999)),
+    dict(logits=torch.zeros(3, 999)), dict(logits=torch.zeros(1, 1000).expand(3, 1000)), dict(logits=torch.zeros(1000, 3).t()),
+    dict(logits=torch.zeros(3, 2, 1000)[:, 0], out=torch.zeros(3, 1, 2, 1000)[:, :, 0]), dict(out=torch.zeros(3, 2000)[:, ::2]),
+    dict(allowed=i32(3, 31)), dict(allowed=i32(2, 40), allowed_rows=3), dict(allowed=i32(6, 16), allowed_rows=3)], ids=lambda d: None)
+def test_rows_of_another_shape_are_refused(on_cpu, kw):
+    refused(logits_of, **kw)
