@@ -280,13 +280,16 @@ def prefix_plan(desc: PrefixDesc, compute_units: int = 0, lib_path=None) -> Pref
 
 
 def _columns(t, rows: int, given: Optional[int], what: str) -> int:
-    """Words of each of ``rows`` rows of a contiguous 2-D int32 tensor, or as given for a raw pointer."""
+    """Words of each of ``rows`` rows of a contiguous 2-D int32 tensor, or as given for a raw pointer or a flat tensor."""
     if t is None:
         return 0
+    columns = t.shape[1] if hasattr(t, "dim") and t.dim() == 2 else None
     if given is None:
-        if not hasattr(t, "dim") or t.dim() != 2:
+        if columns is None:
             raise WeaverError(f"{what}: its row length is required without a 2-D tensor", AW_E_INVALID_ARG)
-        given = t.shape[1]
+        return columns
+    if columns is not None and columns != given:
+        raise WeaverError(f"{what}: rows of {given} words are read, got shape {tuple(t.shape)}", AW_E_INVALID_ARG)
     return given
 
 
@@ -406,6 +409,7 @@ def make_logits_desc(*, num_tokens: int, vocab_size: int, logits, out=None, best
     words = _columns(tree_mask, num_tokens, mask_words, "adjust_logits tree_mask")
     past = _columns(history, batch, history_stride, "adjust_logits history")
     biases = _columns(bias_ids, batch, bias_stride, "adjust_logits bias_ids")
+    _columns(bias_values, batch, biases, "adjust_logits bias_values")
     states = allowed_rows if allowed_rows is not None else 0 if allowed is None else allowed.shape[0] if hasattr(allowed, "shape") else None
     if states is None:
         raise WeaverError("adjust_logits: allowed_rows is required for a raw pointer", AW_E_INVALID_ARG)

@@ -63,3 +63,17 @@ def test_logits_of_a_padded_vocabulary(on_cpu):
     dict(allowed=i32(3, 31)), dict(allowed=i32(2, 40), allowed_rows=3), dict(allowed=i32(6, 16), allowed_rows=3)], ids=lambda d: None)
 def test_rows_of_another_shape_are_refused(on_cpu, kw):
     refused(logits_of, **kw)
+
+
+def test_row_lengths_that_differ_from_their_tensors_are_refused(on_cpu):
+    own = dict(batch=2, bias_count=i32(2), token_offsets=i32(3))
+    f32 = torch.zeros(2, 16)
+    assert logits_of(**own, bias_ids=i32(2, 16), bias_values=f32).bias_stride == 16
+    assert logits_of(**own, bias_ids=i32(2, 8), bias_values=torch.zeros(16)).bias_stride == 8  # flat: rows of the ids' length
+    assert "bias_values" in refused(logits_of, **own, bias_ids=i32(2, 8), bias_values=f32)
+    assert "bias_ids" in refused(logits_of, **own, bias_ids=i32(2, 16), bias_values=f32, bias_stride=8)
+    assert "history" in refused(logits_of, **own, history=i32(2, 64), history_count=i32(2), history_stride=32)
+    assert "tree_mask" in refused(logits_of, **own, node_tokens=i32(3), tree_mask=i32(3, 4), mask_words=1)
+    tables = dict(batch=2, num_tokens=3, seq_held=i32(2), seq_new=i32(2), refs=i32(2, 4), seq_hot=i32(2), token_offsets=i32(3), parents=i32(3))
+    assert O.make_tables_desc(**tables, tree_mask=i32(3, 2), mask_words=2).mask_words == 2
+    assert "tree_mask" in refused(O.make_tables_desc, **tables, tree_mask=i32(3, 2), mask_words=1)
