@@ -442,11 +442,11 @@ def _layer_rows(t, layers: int, tokens: int, heads: int, head_dim: int, what: st
         _f16(t, layers * tokens * heads * head_dim, what)
         return 0, 0
     if t.dim() != 4 or tuple(t.shape) != (layers, tokens, heads, head_dim) or (head_dim > 1 and t.stride(3) != 1) or \
-            (heads > 1 and t.stride(2) != head_dim):
-        raise WeaverError(f"{what}: a view must be [{layers}][{tokens}][{heads}][{head_dim}] with contiguous heads, got shape "
-                          f"{tuple(t.shape)}, strides {tuple(t.stride())}", AW_E_INVALID_ARG)
+            (heads > 1 and t.stride(2) != head_dim) or (layers > 1 and t.stride(0) == 0) or (tokens > 1 and t.stride(1) < heads * head_dim):
+        raise WeaverError(f"{what}: a view must be [{layers}][{tokens}][{heads}][{head_dim}] with contiguous heads and layers and "
+                          f"tokens apart, got shape {tuple(t.shape)}, strides {tuple(t.stride())}", AW_E_INVALID_ARG)
     _f16(t[:0].contiguous(), 0, what)
-    return t.stride(0), t.stride(1)
+    return t.stride(0) if layers > 1 else 0, t.stride(1) if tokens > 1 else 0  # of one, any stride
 
 
 def make_accept_desc(*, batch: int, num_tokens: int, parents, node_tokens, targets, seq_held, accepted, next_token, seq_hot, path,

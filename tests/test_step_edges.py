@@ -77,3 +77,25 @@ def test_row_lengths_that_differ_from_their_tensors_are_refused(on_cpu):
     tables = dict(batch=2, num_tokens=3, seq_held=i32(2), seq_new=i32(2), refs=i32(2, 4), seq_hot=i32(2), token_offsets=i32(3), parents=i32(3))
     assert O.make_tables_desc(**tables, tree_mask=i32(3, 2), mask_words=2).mask_words == 2
     assert "tree_mask" in refused(O.make_tables_desc, **tables, tree_mask=i32(3, 2), mask_words=1)
+
+
+def accept_of(layers=3, tokens=6, **kw):
+    own = {n: A[n] for n in ("parents", "node_tokens", "targets", "seq_held", "accepted", "next_token", "seq_hot", "path", "slots", "hot_k", "hot_v")}
+    return O.make_accept_desc(**{**dict(batch=2, num_tokens=tokens, layers=layers, kv_heads=2, head_dim=64, hot_blocks=9, v=A["v"], **own), **kw})
+
+
+def f16(*shape):
+    return torch.zeros(shape, dtype=torch.float16)
+
+
+def test_expanded_rows_are_refused(on_cpu):
+    """A stride of 0 would be taken for contiguous rows, layers or tokens times the memory that is there."""
+    refused(accept_of, k=f16(1, 6, 2, 64).expand(3, 6, 2, 64))
+    refused(accept_of, k=f16(3, 1, 2, 64).expand(3, 6, 2, 64))
+    refused(accept_of, k=f16(3, 6, 2, 64), v=f16(1, 6, 2, 64).expand(3, 6, 2, 64))
+    d = accept_of(k=f16(6, 3, 9, 64).transpose(0, 1)[:, :, 5:7])
+    assert (d.k_layer_stride, d.k_stride) == (9 * 64, 27 * 64)
+    d = accept_of(layers=1, k=f16(6, 9, 64)[None, :, 5:7])  # one layer, one token: no stride is taken
+    assert (d.k_layer_stride, d.k_stride) == (0, 9 * 64)
+    d = accept_of(tokens=1, k=f16(3, 1, 9, 64)[:, :, 5:7])
+    assert (d.k_layer_stride, d.k_stride) == (9 * 64, 0)
