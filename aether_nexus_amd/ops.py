@@ -437,16 +437,26 @@ def make_logits_desc(*, num_tokens: int, vocab_size: int, logits, out=None, best
 
 
 def _layer_rows(t, layers: int, tokens: int, heads: int, head_dim: int, what: str) -> tuple:
-    """(layer stride, token stride) of rows [layers][tokens][heads][head_dim], contiguous heads; 0, 0 for a raw pointer."""
-    if t is None or isinstance(t, int) or not hasattr(t, "is_contiguous") or t.is_contiguous():
-        _f16(t, layers * tokens * heads * head_dim, what)
+    """(layer stride, token stride) of rows [layers][tokens][heads][head_dim]: 0, 0 of a flat tensor or a raw pointer, else the
+    tensor's own, with contiguous heads, of at least as many layers and tokens.  [layers][tokens][row] and, of one layer or
+    of layers one after another, [tokens][heads][head_dim] and [tokens][row] are taken too."""
+    row = heads * head_dim
+    if t is None or isinstance(t, int) or not hasattr(t, "dim") or t.dim() < 2 or layers == 0:
+        _f16(t, layers * tokens * row, what)
         return 0, 0
-    if t.dim() != 4 or tuple(t.shape) != (layers, tokens, heads, head_dim) or (head_dim > 1 and t.stride(3) != 1) or \
-            (heads > 1 and t.stride(2) != head_dim) or (layers > 1 and t.stride(0) == 0) or (tokens > 1 and t.stride(1) < heads * head_dim):
-        raise WeaverError(f"{what}: a view must be [{layers}][{tokens}][{heads}][{head_dim}] with contiguous heads and layers and "
+    shape, strides, whole = tuple(t.shape), t.stride(), t.is_contiguous()
+    inner = next((n for n in (2, 1) if len(shape) in (n + 1, n + 2) and shape[-n:] == ((heads, head_dim) if n == 2 else (row,))), 0)
+    if inner and len(shape) == inner + 1:  # no axis of layers
+        if layers > 1 and whole and shape[0] >= layers * tokens:
+            _f16(t, 0, what)
+            return 0, 0
+        shape, strides = (1,) + shape, (0,) + strides
+    if not inner or shape[0] < layers or shape[1] < tokens or (head_dim > 1 and strides[-1] != 1) or \
+            (inner == 2 and heads > 1 and strides[-2] != head_dim) or (layers > 1 and strides[0] == 0) or (tokens > 1 and strides[1] < row):
+        raise WeaverError(f"{what}: rows must be [{layers}][{tokens}][{heads}][{head_dim}] with contiguous heads and layers and "
                           f"tokens apart, got shape {tuple(t.shape)}, strides {tuple(t.stride())}", AW_E_INVALID_ARG)
-    _f16(t[:0].contiguous(), 0, what)
-    return t.stride(0) if layers > 1 else 0, t.stride(1) if tokens > 1 else 0  # of one, any stride
+    _f16(t if whole else t[:0].contiguous(), 0, what)
+    return strides[0] if layers > 1 else 0, strides[1] if tokens > 1 else 0  # of one, any stride
 
 
 def make_accept_desc(*, batch: int, num_tokens: int, parents, node_tokens, targets, seq_held, accepted, next_token, seq_hot, path,

@@ -39,3 +39,14 @@ def test_logits_of_a_padded_vocabulary(ops, engine, half):
     ops.adjust_logits(d)
     c.check(out=src[:, :vocab])
     assert (host(src)[:, vocab:] == 3.0).all() and np.array_equal(host(src)[8:, :vocab], c.x[8:])
+
+
+def test_accept_rows_of_a_larger_buffer(ops, engine):
+    """K and V rows of a step in buffers of more tokens: each layer's own, not those behind the first one's."""
+    import torch
+    c = Accept(22, [7, 12, 1], layers=3, agree=1.0)
+    k, v = (torch.full((3, c.rows + 13, 2, 64), float("nan"), dtype=torch.float16, device="cuda:0") for _ in range(2))
+    k[:, :c.rows], v[:, :c.rows] = dev(c.k), dev(c.v)
+    ops.accept_tree(c.desc(k=k, v=v))
+    assert error_of(engine) == ""
+    c.check()

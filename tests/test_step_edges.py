@@ -99,3 +99,23 @@ def test_expanded_rows_are_refused(on_cpu):
     assert (d.k_layer_stride, d.k_stride) == (0, 9 * 64)
     d = accept_of(tokens=1, k=f16(3, 1, 9, 64)[:, :, 5:7])
     assert (d.k_layer_stride, d.k_stride) == (9 * 64, 0)
+
+
+def test_rows_of_a_larger_buffer(on_cpu):
+    """k and v of more tokens or layers than the step's: the buffer's own strides, contiguous or not."""
+    for k in (f16(3, 10, 2, 64), f16(5, 10, 2, 64), f16(3, 10, 128)):
+        d = accept_of(k=k, v=f16(3, 6, 2, 64))
+        assert (d.k_layer_stride, d.k_stride, d.v_layer_stride, d.v_stride) == (1280, 128, 768, 128)
+    for k in (f16(2, 64).expand(18, 2, 64).contiguous(), f16(20, 128), f16(3 * 6 * 128)):  # layers one after another
+        assert (lambda d: (d.k_layer_stride, d.k_stride))(accept_of(k=k)) == (0, 0)
+    for k in (f16(9, 2, 64), f16(9, 128), f16(1, 9, 2, 64), f16(7, 9, 2, 64)):
+        assert (lambda d: (d.k_layer_stride, d.k_stride))(accept_of(layers=1, k=k)) == (0, 128)
+    d = accept_of(layers=1, k=f16(9, 6, 64)[:, 2:4])
+    assert (d.k_layer_stride, d.k_stride) == (0, 384)
+    assert accept_of(layers=0, k=None, v=None, hot_k=None, hot_v=None).k_stride == 0
+
+
+@pytest.mark.parametrize("shape", [(3, 6, 3, 64), (3, 6, 2, 128), (3, 5, 2, 64), (2, 9, 2, 64), (2, 18, 2, 64), (17, 2, 64), (6, 3, 64), (3 * 6 * 128 - 1,),
+                                   (18, 64, 2), (1, 3, 6, 2, 64), (9, 256)])
+def test_rows_of_other_heads_are_refused(on_cpu, shape):
+    refused(accept_of, k=f16(*shape))
