@@ -459,30 +459,51 @@ def _layer_rows(t, layers: int, tokens: int, heads: int, head_dim: int, what: st
     return strides[0] if layers > 1 else 0, strides[1] if tokens > 1 else 0  # of one, any stride
 
 
+def _pool(t, layers: int, heads: int, head_dim: int, blocks: Optional[int], what: str) -> tuple:
+    """(blocks of a layer, elements from layer to layer) of a pool [layers][blocks][16][heads][head_dim], of at least as many
+    layers and blocks; a flat tensor or a raw pointer is taken for just that."""
+    page = BLOCK_SIZE * heads * head_dim
+    if t is None or isinstance(t, int) or not hasattr(t, "dim") or t.dim() < 5 or layers == 0:
+        if blocks is None:
+            if t is not None and not hasattr(t, "numel"):
+                raise WeaverError("accept_tree: hot_blocks is required for a raw pool pointer", AW_E_INVALID_ARG)
+            blocks = 0 if t is None else t.numel() // max(page * layers, 1)
+        if layers and hasattr(t, "dim") and t.dim() == 4 and tuple(t.shape[1:]) != (BLOCK_SIZE, heads, head_dim):
+            raise WeaverError(f"{what}: pages must be [{BLOCK_SIZE}][{heads}][{head_dim}], got shape {tuple(t.shape)}", AW_E_INVALID_ARG)
+        _f16(t, layers * blocks * page, what)
+        return blocks, blocks * page
+    if blocks is None:
+        blocks = t.shape[1]
+    if tuple(t.shape[-3:]) != (BLOCK_SIZE, heads, head_dim) or t.dim() > 5 or t.shape[0] < layers or t.shape[1] < blocks:
+        raise WeaverError(f"{what}: a pool must be [{layers}][{blocks}][{BLOCK_SIZE}][{heads}][{head_dim}], got shape {tuple(t.shape)}",
+                          AW_E_INVALID_ARG)
+    _f16(t, 0, what)
+    return blocks, t.shape[1] * page
+
+
 def make_accept_desc(*, batch: int, num_tokens: int, parents, node_tokens, targets, seq_held, accepted, next_token, seq_hot, path,
                      token_offsets=None, layers: int = 0, kv_heads: int = 0, head_dim: int = 0, k=None, v=None, hot_k=None,
                      hot_v=None, slots=None, history=None, history_count=None, history_count_out=None,
                      hot_blocks: Optional[int] = None, history_stride: Optional[int] = None) -> AcceptDesc:
     """An ``aw_accept_desc`` from device tensors (or raw device pointers to contiguous rows), for
     ``accept_tree``: ``k`` and ``v`` [layers][num_tokens][kv_heads][head_dim] (views with contiguous heads
-    too) go by ``slots`` (int64) into the pools [layers][hot_blocks][16][kv_heads][head_dim].  Without
+    too, and buffers of more layers and tokens) go by ``slots`` (int64) into the pools
+    [layers][hot_blocks][16][kv_heads][head_dim] (of more layers and blocks, too).  Without
     ``layers`` no rows are moved.  ``seq_hot`` may be ``seq_held``, ``history_count_out``
     ``history_count``."""
     d = AcceptDesc()
-    page = BLOCK_SIZE * kv_heads * head_dim
-    if hot_blocks is None:
-        if hot_k is not None and not hasattr(hot_k, "numel"):
-            raise WeaverError("accept_tree: hot_blocks is required for a raw pool pointer", AW_E_INVALID_ARG)
-        hot_blocks = 0 if hot_k is None else hot_k.numel() // max(page * layers, 1)
     past = _columns(history, batch, history_stride, "accept_tree history")
-    _counts(batch=batch, num_tokens=num_tokens, layers=layers, kv_heads=kv_heads, head_dim=head_dim, hot_blocks=hot_blocks,
+    _counts(batch=batch, num_tokens=num_tokens, layers=layers, kv_heads=kv_heads, head_dim=head_dim, hot_blocks=hot_blocks or 0,
             history_stride=past)
+    hot_blocks, apart = _pool(hot_k, layers, kv_heads, head_dim, hot_blocks, "hot_k")
+    if hot_v is not None and _pool(hot_v, layers, kv_heads, head_dim, hot_blocks, "hot_v")[1] != apart and layers > 1:
+        raise WeaverError("accept_tree: the layers of hot_k and hot_v lie differently far apart", AW_E_INVALID_ARG)
+    if layers > 1 and apart != hot_blocks * BLOCK_SIZE * kv_heads * head_dim:
+        d.hot_layer_stride = apart
     d.batch, d.num_tokens, d.layers, d.kv_heads, d.head_dim = batch, num_tokens, layers, kv_heads, head_dim
     d.history_stride, d.hot_blocks = past, hot_blocks
     d.k_layer_stride, d.k_stride = _layer_rows(k, layers, num_tokens, kv_heads, head_dim, "k")
     d.v_layer_stride, d.v_stride = _layer_rows(v, layers, num_tokens, kv_heads, head_dim, "v")
-    for t, name in ((hot_k, "hot_k"), (hot_v, "hot_v")):
-        _f16(t, layers * hot_blocks * page, name)
     _i64(slots, num_tokens, "slots")
     for t, name in ((k, "k"), (v, "v"), (hot_k, "hot_k"), (hot_v, "hot_v"), (slots, "slots")):
         setattr(d, name, _ptr(t))

@@ -50,3 +50,23 @@ def test_accept_rows_of_a_larger_buffer(ops, engine):
     ops.accept_tree(c.desc(k=k, v=v))
     assert error_of(engine) == ""
     c.check()
+
+
+def test_accept_into_pools_of_more_layers_and_blocks(ops, engine):
+    """The first layers and blocks of a larger pool: the rest stays."""
+    import torch
+    c = Accept(23, [7, 12, 1], layers=2, agree=1.0)
+    pools = [torch.full((4, c.blocks + 3, 16, 2, 64), 5.0, dtype=torch.float16, device="cuda:0") for _ in range(2)]
+    for p, x in zip(pools, (c.pool, -c.pool)):
+        p[:2, :c.blocks] = dev(x)
+    ops.accept_tree(c.desc(hot_k=pools[0], hot_v=pools[1], hot_blocks=c.blocks))
+    assert error_of(engine) == ""
+    c.hot_k, c.hot_v = (p[:2, :c.blocks].contiguous() for p in pools)
+    c.check()
+    for p in pools:
+        assert (host(p)[2:] == 5.0).all() and (host(p)[:, c.blocks:] == 5.0).all()
+    for p, x in zip(pools, (c.pool, -c.pool)):
+        p[:2, :c.blocks] = dev(x)
+    ops.accept_tree(c.desc(hot_k=pools[0], hot_v=pools[1]))
+    c.hot_k, c.hot_v = (p[:2, :c.blocks].contiguous() for p in pools)
+    c.check()

@@ -119,3 +119,29 @@ def test_rows_of_a_larger_buffer(on_cpu):
                                    (18, 64, 2), (1, 3, 6, 2, 64), (9, 256)])
 def test_rows_of_other_heads_are_refused(on_cpu, shape):
     refused(accept_of, k=f16(*shape))
+
+
+def test_pools_of_more_layers_or_blocks(on_cpu):
+    """A pool's own layers: not the elements of all of them shared out over the step's."""
+    def of(d):
+        return d.hot_blocks, d.hot_layer_stride
+    page, flat = 16 * 128, f16(3, 6, 2, 64)
+    kw = dict(k=flat, v=flat, hot_blocks=None)
+    for pool, want in ((f16(3, 9, 16, 2, 64), (9, 0)), (f16(5, 9, 16, 2, 64), (9, 0)), (f16(3 * 9 * page), (9, 0)), (f16(27, 16, 2, 64), (9, 0))):
+        assert of(accept_of(**kw, hot_k=pool, hot_v=pool)) == want
+    pool = f16(3, 12, 16, 2, 64)
+    assert of(accept_of(**{**kw, "hot_blocks": 9}, hot_k=pool, hot_v=pool)) == (9, 12 * page)
+    for layers in (1, 2):
+        d = accept_of(layers=layers, k=flat, v=flat, hot_k=pool, hot_v=pool, hot_blocks=None)
+        assert of(d) == (12, 0)
+    assert of(accept_of(layers=1, k=flat, v=flat, hot_k=f16(9, 16, 2, 64), hot_v=f16(1, 9, 16, 2, 64), hot_blocks=None)) == (9, 0)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(hot_k=f16(2, 30, 16, 2, 64)), dict(hot_k=f16(3, 9, 16, 3, 64)), dict(hot_k=f16(3, 9, 16, 1, 128)), dict(hot_k=f16(27, 16, 4, 32)),
+    dict(hot_k=f16(3, 9, 16, 2, 64), hot_blocks=10), dict(hot_k=f16(3, 9, 16, 2, 64), hot_v=f16(3, 8, 16, 2, 64)),
+    dict(hot_k=f16(3, 9, 16, 2, 64), hot_v=f16(3, 10, 16, 2, 64)), dict(hot_k=f16(3 * 9 * 16 * 128 - 1), hot_blocks=9),
+    dict(hot_k=f16(3, 12, 16, 2, 64)[:, :9])], ids=lambda d: None)
+def test_pools_of_other_pages_are_refused(on_cpu, kw):
+    rows = f16(3, 6, 2, 64)
+    refused(accept_of, **{**dict(k=rows, v=rows, hot_v=kw["hot_k"], hot_blocks=None), **kw})
