@@ -81,12 +81,19 @@ def _counts(**values) -> None:
             raise WeaverError(f"{name} {v} is not within [0, 2^32)", AW_E_INVALID_ARG)
 
 
-def _token_rows(t, tokens: int, heads: int, head_dim: int, what: str) -> int:
+def _token_rows(t, tokens: int, heads: int, head_dim: int, what: str, shaped: bool = False) -> int:
     """Token stride (elements) of rows [tokens][heads][head_dim]: a contiguous tensor, a
     raw pointer to one, or a view with contiguous heads whose rows lie further apart
-    (the q, k or v part of a fused product's output)."""
+    (the q, k or v part of a fused product's output).  ``shaped``: a contiguous tensor of several
+    dims has such rows; one of other heads is no flat memory."""
     row = heads * head_dim
     if t is None or isinstance(t, int) or not hasattr(t, "is_contiguous") or t.is_contiguous():
+        if shaped and tokens and hasattr(t, "dim") and t.dim() > 1:
+            inner = 1
+            for n in reversed(t.shape):
+                inner = inner * n if inner < row else inner
+            if inner != row:
+                raise WeaverError(f"{what}: rows must be [tokens][{heads}][{head_dim}] (or flat), got shape {tuple(t.shape)}", AW_E_INVALID_ARG)
         _f16(t, tokens * row, what)
         return row
     inner = ((heads, head_dim), (head_dim, 1)) if t.dim() == 3 else ((row,), (1,))
@@ -353,8 +360,10 @@ def make_tree_desc(*, batch: int, num_tokens: int, q_heads: int, kv_heads: int, 
     d.scale = head_dim ** -0.5 if scale is None else scale
     for t, heads, name in ((q, q_heads, "q"), (k, kv_heads, "k"), (v, kv_heads, "v"), (out, q_heads, "out")):
         setattr(d, name, _ptr(t))
-        setattr(d, name + "_stride", _token_rows(t, num_tokens, heads, head_dim, name))
+        setattr(d, name + "_stride", _token_rows(t, num_tokens, heads, head_dim, name, shaped=True))
     for t, name in ((hot_k, "hot_k"), (hot_v, "hot_v")):
+        if hasattr(t, "dim") and t.dim() >= 4 and tuple(t.shape[-3:]) != (BLOCK_SIZE, kv_heads, head_dim):
+            raise WeaverError(f"{name}: pages must be [{BLOCK_SIZE}][{kv_heads}][{head_dim}], got shape {tuple(t.shape)}", AW_E_INVALID_ARG)
         _f16(t, hot_blocks * page, name)
         setattr(d, name, _ptr(t))
     d.refs_stride = _table(refs, batch, hot_count, refs_stride, "refs") if refs is not None else hot_count

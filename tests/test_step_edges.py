@@ -145,3 +145,20 @@ def test_pools_of_more_layers_or_blocks(on_cpu):
 def test_pools_of_other_pages_are_refused(on_cpu, kw):
     rows = f16(3, 6, 2, 64)
     refused(accept_of, **{**dict(k=rows, v=rows, hot_v=kw["hot_k"], hot_blocks=None), **kw})
+
+
+def tree_of(rows=6, **kw):
+    return O.make_tree_desc(**{**dict(batch=2, num_tokens=rows, q_heads=4, kv_heads=2, head_dim=64, q=f16(rows, 4, 64), k=f16(rows, 2, 64),
+                                      v=f16(rows, 2, 64), out=f16(rows, 4, 64)), **kw})
+
+
+def test_tree_rows_of_other_heads_are_refused(on_cpu):
+    """A whole fused row, or a pool of other heads, where its part is asked for: no flat memory of the request's rows."""
+    for kw in (dict(q=f16(6, 8, 64)), dict(k=f16(6, 4, 64)), dict(v=f16(6, 3, 64)), dict(out=f16(6, 512)),
+               dict(hot_k=f16(9, 16, 4, 64), hot_v=A["hot_v"]), dict(hot_k=A["hot_k"], hot_v=f16(9, 16, 1, 128), hot_blocks=9)):
+        refused(tree_of, **kw)
+    for kw in (dict(q=f16(6, 256), k=f16(8, 128)), dict(q=f16(6, 2, 64, 2, 2)), dict(q=f16(6 * 256), out=f16(2, 3, 4, 64)), dict(k=f16(6, 8, 64)[:, 4:6]),
+               dict(hot_k=f16(9, 16, 2, 64), hot_v=f16(3, 3, 16, 2, 64)), dict(rows=0, q=f16(0, 8, 64)), dict(q=f16(1, 6, 4, 64))):
+        assert tree_of(**kw).q_stride == 256
+    one = dict(kv_heads=1, q_heads=4)
+    assert tree_of(**one, k=f16(6, 1, 64), v=f16(6, 64)).k_stride == 64
