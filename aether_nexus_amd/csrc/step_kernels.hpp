@@ -87,12 +87,14 @@ __global__ __launch_bounds__(256) void tables_kernel(TablesArgs a) {
     uint32_t tokens = 0, pages = a.free_first ? min(a.free_first[0], 1u << 30) : 0u; // before the chunk
     bool bad_seq = false, bad_free = false;
     for (uint32_t c0 = 0; c0 < a.batch; c0 += kTablesSeqs) {
-        uint32_t held[4], had[4], n[4], need[4];
+        uint32_t held[4], had[4], n[4], need[4], got[4];
+        bool lacks[4]; // pages for the tokens that it holds
         uint32_t sum = 0;
 #pragma unroll
         for (uint32_t j = 0; j < 4u; ++j) {
             const uint32_t s = c0 + 4u * tid + j;
             held[j] = had[j] = n[j] = 0;
+            lacks[j] = false;
             if (s < a.batch) {
                 held[j] = a.seq_held[s];
                 const uint32_t want = a.seq_new[s], most = held[j] < room ? room - held[j] : 0u;
@@ -101,8 +103,8 @@ __global__ __launch_bounds__(256) void tables_kernel(TablesArgs a) {
                 held[j] = min(held[j], 0xFFFFFFFFu - kPageTokens);
                 const uint32_t least = (held[j] + kPageTokens - 1u) / kPageTokens;
                 had[j] = a.seq_pages ? a.seq_pages[s] : least;
-                bad_seq |= had[j] < least;
-                had[j] = max(had[j], least);
+                lacks[j] = had[j] < least;
+                bad_seq |= lacks[j];
             }
             sum = min(sum + n[j], a.tokens);
         }
@@ -114,7 +116,7 @@ __global__ __launch_bounds__(256) void tables_kernel(TablesArgs a) {
             bad_seq |= end - off < n[j];
             n[j] = end - off;
             const uint32_t after = n[j] ? (held[j] + n[j] + kPageTokens - 1u) / kPageTokens : 0u;
-            need[j] = after > had[j] ? after - had[j] : 0u;
+            need[j] = after > had[j] && !lacks[j] ? after - had[j] : 0u;
             taken = min(taken + need[j], 1u << 30);
             s_off[4u * tid + j] = off;
             s_held[4u * tid + j] = held[j];
@@ -125,9 +127,10 @@ __global__ __launch_bounds__(256) void tables_kernel(TablesArgs a) {
         uint32_t from = min(pages + taken, 1u << 30);
 #pragma unroll
         for (uint32_t j = 0; j < 4u; ++j) {
-            s_start[4u * tid + j] = from;
+            s_start[4u * tid + j] = lacks[j] ? 1u << 30 : from; // past any list
+            got[j] = from < a.free_count ? min(need[j], a.free_count - from) : 0u;
             from = min(from + need[j], 1u << 30);
-            bad_free |= need[j] && from > a.free_count;
+            bad_free |= got[j] < need[j];
         }
         const uint32_t count = min(a.batch - c0, kTablesSeqs);
         tokens = min(tokens + all, a.tokens);
@@ -139,7 +142,7 @@ __global__ __launch_bounds__(256) void tables_kernel(TablesArgs a) {
                 const uint32_t s = c0 + 4u * tid + j;
                 if (s >= a.batch) continue;
                 a.seq_hot[s] = held[j] + n[j];
-                if (a.pages_out) a.pages_out[s] = had[j] + need[j];
+                if (a.pages_out) a.pages_out[s] = had[j] + got[j];
                 a.token_offsets[s] = s_off[4u * tid + j];
             }
         }
@@ -151,12 +154,13 @@ __global__ __launch_bounds__(256) void tables_kernel(TablesArgs a) {
             const uint32_t i = t - s_off[k], place = s_held[k] + i, page = place / kPageTokens;
             const uint64_t entry = (uint64_t)(c0 + k) * a.refs_stride + page;
             uint32_t ref;
-            if (page >= s_pages[k]) { // a page taken here, named by the row that begins it
+            if (page >= s_pages[k]) { // a page taken here, named by the row that begins it; or there is none
                 const uint32_t f = s_start[k] + (page - s_pages[k]);
                 ref = f < a.free_count ? a.free_pages[f] & kPageMask : kNoPage;
-                if (place % kPageTokens == 0u) a.refs[entry] = ref;
+                if (place % kPageTokens == 0u || i == 0u) a.refs[entry] = ref;
             } else {
                 ref = a.refs[entry] & kPageMask;
+                bad_free |= ref == kNoPage; // an entry that an earlier step found no page for
             }
             if (a.slots) a.slots[t] = ref == kNoPage ? -1 : (int64_t)ref * kPageTokens + place % kPageTokens;
             uint32_t position = place;

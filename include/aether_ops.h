@@ -258,7 +258,7 @@ void aw_abi_ops_desc_sizes(size_t sizes[3]);
  * earlier step left pages unfilled).  Where held + new tokens need more, the row is
  * continued with free_pages[f], free_pages[f + 1], .., in the order of the sequences, f =
  * *free_first (NULL: 0).  Outputs, each but refs, seq_hot and token_offsets may be NULL:
- *   refs          [batch][refs_stride], its new entries alone; seq_pages + new pages in pages_out
+ *   refs          [batch][refs_stride], its new entries alone; seq_pages + the pages taken in pages_out
  *   seq_hot       held + new (what aw_ops_append_paged takes)
  *   token_offsets [batch + 1]
  *   free_next     [1] the place in free_pages behind the last page taken
@@ -268,9 +268,11 @@ void aw_abi_ops_desc_sizes(size_t sizes[3]);
  * parents [num_tokens]: node numbers within the tree, < 0 for a root; one that is not an earlier node
  * sets "sequence length" and makes a root.  Rows behind the last sequence: slot -1, position 0,
  * mask 0.  New tokens past hot_count pages, past num_tokens rows or (with parents) past 32 mask_words
- * nodes set "sequence length" and are left out; so do pages that seq_held needs and
- * seq_pages lacks, which get none.  Where free_pages ends, entries become 0x7FFFFFFF (refused by the
- * calls that read them), slots -1, and "free pages" is set. */
+ * nodes set "sequence length" and are left out.  A sequence whose seq_held needs more pages than seq_pages
+ * sets "sequence length" and takes none.  New tokens without a page, there or where free_pages ends
+ * ("free pages"), get slot -1 and entries of 0x7FFFFFFF (refused by the calls that read them), which are
+ * not counted in pages_out: a later step with seq_held up to 16 * pages_out takes pages for them.  One
+ * of the seq_pages entries that is 0x7FFFFFFF sets "free pages" where a new token falls into it. */
 typedef struct aw_tables_desc {
     uint32_t batch, num_tokens;          /* batch <= 2^20, num_tokens <= 2^24 */
     uint32_t hot_count, refs_stride;     /* entries of a row, <= 2^26; refs_stride >= hot_count */

@@ -61,20 +61,25 @@ def page_tables(refs, held, new, pages, free, first: int, rows: int, hot_count: 
             errors.add("sequence length")
         least = -(-h // PAGE)
         p = least if pages is None else int(pages[b])
-        if p < least:
+        lacks = p < least
+        if lacks:
             errors.add("sequence length")
-            p = least
-        need = max(0, -(-(h + n) // PAGE) - p) if n else 0
-        for j in range(need):
-            if f + j < len(free):
-                refs[b, p + j] = int(free[f + j]) & REF_MASK
-            else:
-                refs[b, p + j] = REF_MASK
-                errors.add("free pages")
+        need = max(0, -(-(h + n) // PAGE) - p) if n and not lacks else 0
+        mine = [int(x) & REF_MASK for x in free[f:f + need]]
+        if len(mine) < need:
+            errors.add("free pages")
         f += need
         tree = None if parents is None else sees_of(parents[t:t + n])
         for i in range(n):
-            ref = int(refs[b, (h + i) // PAGE]) & REF_MASK
+            at = (h + i) // PAGE
+            if at >= p:
+                ref = mine[at - p] if at - p < len(mine) else REF_MASK
+                if i == 0 or (h + i) % PAGE == 0:
+                    refs[b, at] = ref
+            else:
+                ref = int(refs[b, at]) & REF_MASK
+                if ref == REF_MASK:
+                    errors.add("free pages")
             slots[t] = -1 if ref == REF_MASK else ref * PAGE + (h + i) % PAGE
             positions[t] = h + (i if tree is None else tree[i][1])
             for w in range(words):
@@ -82,7 +87,7 @@ def page_tables(refs, held, new, pages, free, first: int, rows: int, hot_count: 
             if tree is not None and int(parents[t]) >= i:
                 errors.add("sequence length")
             t += 1
-        got["seq_hot"][b], got["pages_out"][b] = h + n, p + need
+        got["seq_hot"][b], got["pages_out"][b] = h + n, p + len(mine)
         offsets.append(t)
     return {**got, "refs": refs, "token_offsets": np.array(offsets), "free_next": min(f, max(len(free), int(first))), "slots": slots,
             "positions": positions, "tree_mask": mask, "errors": errors}

@@ -70,3 +70,45 @@ def test_accept_into_pools_of_more_layers_and_blocks(ops, engine):
     ops.accept_tree(c.desc(hot_k=pools[0], hot_v=pools[1]))
     c.hot_k, c.hot_v = (p[:2, :c.blocks].contiguous() for p in pools)
     c.check()
+
+
+# ---------------------------------------------------------------- a list of free pages that ends
+
+@pytest.mark.parametrize("tree", [None, "random"], ids=["plain", "tree"])
+@pytest.mark.parametrize("short", [1, 3, 5])
+def test_tables_after_a_list_that_ended(ops, engine, tree, short):
+    """Only pages that a step took are counted: when the list is full again, the next step of the same lengths takes the rest."""
+    c = Tables(24, [3, 16, 0, 31, 48, 10], [14, 40, 2, 9, 33, 5], extra=[0, 0, 1, 0, 0, 0], tree=tree, free_short=short)
+    full = Tables(24, c.held, c.new, extra=[0, 0, 1, 0, 0, 0], tree=tree)
+    d = c.desc()
+    ops.page_tables(d)
+    want = c.want()
+    assert want["errors"] == {"free pages"} and "free pages" in error_of(engine)
+    c.check(want)
+    assert int((want["pages_out"] - c.pages).sum()) == len(c.free) - c.first
+    # The same lengths again, the pages that were taken, the rest of the list.
+    c.refs, c.pages, c.first = want["refs"], want["pages_out"], int(want["free_next"])
+    c.free = full.free
+    ops.page_tables(c.desc())
+    assert error_of(engine) == ""
+    want = c.want()
+    assert not want["errors"] and (want["slots"] >= 0).all()
+    c.check(want)
+
+
+def test_tables_of_held_tokens_without_pages(ops, engine):
+    """A sequence that holds more than its pages takes none: its new tokens have no slot, and their entries name no page."""
+    c = Tables(25, [20, 33, 16, 40], [14, 1, 0, 30], first=0)
+    c.pages = np.array([1, 3, 0, 2])
+    ops.page_tables(c.desc())
+    want = c.want()
+    assert want["errors"] == {"sequence length"} and "sequence length" in error_of(engine)
+    assert want["pages_out"].tolist() == [1, 3, 0, 2] and (want["slots"][:14] < 0).all() and (want["slots"][15:] < 0).all() and want["slots"][14] >= 0
+    c.check(want)
+    # An entry that is counted but names no page is reported whenever a new token falls into it.
+    c = Tables(26, [20, 33], [14, 1], first=0)
+    c.refs[0, 1] = 0xFFFFFFFF  # bit 31 masked: 0x7FFFFFFF
+    ops.page_tables(c.desc())
+    want = c.want()
+    assert want["errors"] == {"free pages"} and "free pages" in error_of(engine) and (want["slots"][:12] < 0).all()
+    c.check(want)

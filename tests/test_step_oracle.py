@@ -121,3 +121,18 @@ def test_acceptance_against_all_paths():
                 good.append(i)
         assert path == good
     assert S.accept_tree([], [], [], [0, 0]) == [[]]
+
+
+def test_tables_after_a_list_that_ended():
+    """What a step found no page for is not a page that a sequence has: the next step takes it."""
+    free, none = np.array([7, 8, 9]), np.array([], dtype=np.int64)
+    first = S.page_tables([[3, 0, 0]], [16], [4], [1], none, 0, 4, 3)
+    assert first["errors"] == {"free pages"} and first["pages_out"].tolist() == [1] and (first["slots"] < 0).all()
+    assert first["refs"].tolist() == [[3, S.REF_MASK, 0]]
+    again = S.page_tables(first["refs"], [16], [4], first["pages_out"], free, 0, 4, 3)
+    assert not again["errors"] and again["pages_out"].tolist() == [2] and again["slots"].tolist() == [7 * 16 + i for i in range(4)]
+    assert again["refs"].tolist() == [[3, 7, 0]] and again["free_next"] == 1
+    held = S.page_tables(first["refs"], [20], [14], first["pages_out"], free, 0, 14, 3)  # held without a page: none is taken behind it
+    assert held["errors"] == {"sequence length"} and held["pages_out"].tolist() == [1] and (held["slots"] < 0).all() and held["free_next"] == 0
+    hole = S.page_tables(first["refs"], [20], [14], [2], free, 0, 14, 3)  # counted as a page although it names none
+    assert hole["errors"] == {"free pages"} and hole["pages_out"].tolist() == [3] and (hole["slots"] < 0).sum() == 12
