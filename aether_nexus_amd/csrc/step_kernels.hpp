@@ -14,6 +14,7 @@ namespace awo {
 constexpr uint32_t kMaxNodes = 1024u;   // of a sequence's tree
 constexpr uint32_t kErrFree = aw_engine_internal::kErrFreeBit;
 constexpr uint32_t kNoPage = kPageMask; // an entry without a page
+constexpr int64_t kNoSlot = AW_NO_SLOT;
 
 // First row and number of rows of sequence b, uniform; offsets that descend or pass the
 // rows give none.
@@ -162,7 +163,7 @@ __global__ __launch_bounds__(256) void tables_kernel(TablesArgs a) {
                 ref = a.refs[entry] & kPageMask;
                 bad_free |= ref == kNoPage; // an entry that an earlier step found no page for
             }
-            if (a.slots) a.slots[t] = ref == kNoPage ? -1 : (int64_t)ref * kPageTokens + place % kPageTokens;
+            if (a.slots) a.slots[t] = ref == kNoPage ? kNoSlot : (int64_t)ref * kPageTokens + place % kPageTokens;
             uint32_t position = place;
             if constexpr (TREE) {
                 uint32_t* row = a.tree_mask + (uint64_t)t * a.mask_words;
@@ -589,12 +590,21 @@ __global__ __launch_bounds__(256) void accept_kernel(AcceptArgs a) {
         s_parent[i] = a.parents[rows.first + i];
         s_token[i] = a.node_tokens[rows.first + i];
         s_target[i] = a.targets[rows.first + i];
+        s_path[i] = a.slots && a.slots[rows.first + i] == kNoSlot; // until the walk: no page for the i-th kept node
     }
     __syncthreads();
     if (tid < 64u) {
-        uint32_t kept = n ? 1u : 0u, cur = 0;
+        uint32_t room = n; // nodes that may be kept
+        for (uint32_t c = 0; c < n; c += 64u) {
+            const uint64_t m = __ballot(c + lane < n && s_path[min(c + lane, n - 1u)] != 0);
+            if (m) {
+                room = c + (uint32_t)__builtin_ctzll(m);
+                break;
+            }
+        }
+        uint32_t kept = room ? 1u : 0u, cur = 0;
         if (lane == 0) s_path[0] = 0;
-        for (uint32_t c = 0; n && c < n;) { // nodes c .. of this step: each pass moves on, or to a later node
+        for (uint32_t c = 0; kept < room && c < n;) { // nodes c .. of this step: each pass moves on, or to a later node
             const uint32_t i = c + lane;
             const uint64_t m = __ballot(i < n && i > cur && s_parent[min(i, n - 1u)] == (int32_t)cur &&
                                         s_token[min(i, n - 1u)] == s_target[cur] && s_target[cur] != ~0u);
@@ -623,7 +633,7 @@ __global__ __launch_bounds__(256) void accept_kernel(AcceptArgs a) {
         }
         if (tid == 0) {
             a.accepted[b] = kept;
-            a.next_token[b] = kept ? (int32_t)s_target[s_path[kept - 1u]] : -1;
+            a.next_token[b] = kept ? (int32_t)s_target[s_path[kept - 1u]] : n ? (int32_t)s_token[0] : -1;
             a.seq_hot[b] = a.seq_held[b] + kept;
             if (rows.n > kMaxNodes) flag(a.err, kErrSeq);
         }

@@ -242,6 +242,9 @@ class RotaryScaling(ctypes.Structure):
 #: AW_LOGITS_F16 (include/aether_ops.h).
 AW_LOGITS_F16 = 1
 
+#: AW_NO_SLOT: the slot of a token that there was no page for.
+AW_NO_SLOT = -(1 << 63)
+
 #: AW_ROTARY_SCALE_* by name.
 ROTARY_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "parts": 3}
 

@@ -252,6 +252,7 @@ void aw_abi_ops_desc_sizes(size_t sizes[3]);
  * (aw_engine_check_device_errors) and are taken as stated. */
 
 #define AW_MAX_NODES 1024u /* nodes of a sequence's tree: 32 mask words */
+#define AW_NO_SLOT INT64_MIN /* the slot of a token that there was no page for */
 
 /* Per sequence: seq_held tokens in pages before the step, seq_new new ones (nodes), seq_pages
  * entries of its row of refs that name pages (NULL: as many as its tokens need; more where an
@@ -262,7 +263,7 @@ void aw_abi_ops_desc_sizes(size_t sizes[3]);
  *   seq_hot       held + new (what aw_ops_append_paged takes)
  *   token_offsets [batch + 1]
  *   free_next     [1] the place in free_pages behind the last page taken
- *   slots         [num_tokens] the row of the pools of each new token, ref * 16 + place % 16
+ *   slots         [num_tokens] the row of the pools of each new token, ref * 16 + place % 16, or AW_NO_SLOT
  *   positions     [num_tokens] its place; with parents: held + its depth in the tree
  *   tree_mask     [num_tokens][mask_words], required with parents: itself and its ancestors
  * parents [num_tokens]: node numbers within the tree, < 0 for a root; one that is not an earlier node
@@ -270,7 +271,7 @@ void aw_abi_ops_desc_sizes(size_t sizes[3]);
  * mask 0.  New tokens past hot_count pages, past num_tokens rows or (with parents) past 32 mask_words
  * nodes set "sequence length" and are left out.  A sequence whose seq_held needs more pages than seq_pages
  * sets "sequence length" and takes none.  New tokens without a page, there or where free_pages ends
- * ("free pages"), get slot -1 and entries of 0x7FFFFFFF (refused by the calls that read them), which are
+ * ("free pages"), get AW_NO_SLOT and entries of 0x7FFFFFFF (refused by the calls that read them), which are
  * not counted in pages_out: a later step with seq_held up to 16 * pages_out takes pages for them.  One
  * of the seq_pages entries that is 0x7FFFFFFF sets "free pages" where a new token falls into it. */
 typedef struct aw_tables_desc {
@@ -346,16 +347,18 @@ int aw_ops_adjust_logits(aw_engine* engine, const aw_logits_desc* desc, void* hi
 
 /* From node 0 of each tree, whose token is kept, on: of the children of the node kept last
  * the lowest whose token is targets[that node] is kept too, until there is none (a target of
- * 0xFFFFFFFF, a best of -1, is no token).
- *   accepted   [batch] how many are kept (0 for a sequence without nodes)
- *   next_token [batch] targets[the last one kept] (-1 without nodes): the next tree's node 0
+ * 0xFFFFFFFF, a best of -1, is no token).  Where slots are given a path ends before its j-th node if the
+ * sequence's j-th row has AW_NO_SLOT: a later step, with a page for it, takes that token again.
+ *   accepted   [batch] how many are kept (0 for a sequence without nodes, or without a page for node 0)
+ *   next_token [batch] targets[the last one kept] (node 0's own token where it has no page, -1 without
+ *              nodes): the next tree's node 0
  *   seq_hot    [batch] seq_held + accepted; may be seq_held
  *   path       [num_tokens] in the sequence's rows the kept nodes in order, then -1
  *   history    [batch][history_stride] the kept tokens behind the history_count that were there, and
  *              history_count_out; history_count_out may be history_count (all three NULL: none); past the
  *              stride they are left out and "sequence length" is set
  * and, for each of `layers` layers, K and V row of the j-th kept node to row slots[j-th row of the
- * sequence] of the pool.  A slot past hot_blocks pages is left out and sets "hot block ref", a negative
+ * sequence] of the pool.  A slot past hot_blocks pages is left out and sets "hot block ref", another negative
  * one is left out.  A tree of more than AW_MAX_NODES nodes sets "sequence length", its later nodes are
  * not kept. */
 typedef struct aw_accept_desc {
@@ -371,7 +374,7 @@ typedef struct aw_accept_desc {
     const uint32_t* targets;             /* [num_tokens]: best of aw_ops_adjust_logits, or sampled */
     const uint32_t* token_offsets;
     const uint32_t* seq_held;
-    const int64_t*  slots;               /* [num_tokens], of aw_ops_page_tables */
+    const int64_t*  slots;               /* [num_tokens], of aw_ops_page_tables; may be NULL without layers */
     const uint16_t* k;                   /* [layers][num_tokens][kv_heads][head_dim] */
     const uint16_t* v;                   /* likewise, NULL with hot_v */
     uint16_t* hot_k;                     /* [layers][hot_blocks][16][kv_heads][head_dim] */

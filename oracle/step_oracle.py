@@ -17,6 +17,7 @@ import numpy as np
 PAGE = 16
 REF_MASK = 0x7FFFFFFF
 MAX_NODES = 1024
+NO_SLOT = -(1 << 63)
 
 
 def offsets_of(counts) -> list:
@@ -80,7 +81,7 @@ def page_tables(refs, held, new, pages, free, first: int, rows: int, hot_count: 
                 ref = int(refs[b, at]) & REF_MASK
                 if ref == REF_MASK:
                     errors.add("free pages")
-            slots[t] = -1 if ref == REF_MASK else ref * PAGE + (h + i) % PAGE
+            slots[t] = NO_SLOT if ref == REF_MASK else ref * PAGE + (h + i) % PAGE
             positions[t] = h + (i if tree is None else tree[i][1])
             for w in range(words):
                 mask[t, w] = tree[i][0] >> (32 * w) & 0xFFFFFFFF
@@ -189,8 +190,8 @@ def adjust_logits(logits, offsets=None, history=None, history_count=None, prompt
     return out, best
 
 
-def accept_tree(parents, tokens, targets, offsets) -> list:
-    """The kept nodes of each sequence, in order."""
+def accept_tree(parents, tokens, targets, offsets, slots=None) -> list:
+    """The kept nodes of each sequence, in order; with slots, those before the first row without one."""
     paths = []
     for b in range(len(offsets) - 1):
         first, n = int(offsets[b]), min(int(offsets[b + 1]) - int(offsets[b]), MAX_NODES)
@@ -202,5 +203,7 @@ def accept_tree(parents, tokens, targets, offsets) -> list:
             if not child:
                 break
             path.append(child[0])
+        if slots is not None:
+            path = path[:next((j for j in range(n) if int(slots[first + j]) == NO_SLOT), n)]
         paths.append(path)
     return paths

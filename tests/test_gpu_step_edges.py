@@ -112,3 +112,62 @@ def test_tables_of_held_tokens_without_pages(ops, engine):
     want = c.want()
     assert want["errors"] == {"free pages"} and "free pages" in error_of(engine) and (want["slots"][:12] < 0).all()
     c.check(want)
+
+
+@pytest.mark.parametrize("layers", [0, 2])
+def test_accept_before_a_row_without_a_slot(ops, engine, layers):
+    """A path ends where its sequence has no page: nothing is kept, counted or written from there on."""
+    import torch
+    c = Accept(27, [5, 9, 2, 0, 130, 3], agree=1.0, shape="chain", history=400)
+    none = {1: 0, 2: 0, 4: 77}  # sequence: its first row without a slot
+    slots = c.slots.copy()
+    for b, j in none.items():
+        slots[c.offsets[b] + j:c.offsets[b + 1]] = S.NO_SLOT
+    slots[c.offsets[4] + 100:c.offsets[5]] = 7  # behind the first
+    rows = {} if layers else dict(layers=0, kv_heads=0, head_dim=0, k=None, v=None, hot_k=None, hot_v=None)
+    ops.accept_tree(c.desc(slots=torch.from_numpy(slots).cuda(), **rows))
+    assert error_of(engine) == ""
+    paths = S.accept_tree(c.parents, c.tokens, c.targets, c.offsets, slots)
+    assert [len(p) for p in paths] == [5, 0, 0, 0, 77, 3]
+    kept = np.array([len(p) for p in paths])
+    assert host(c.got["accepted"]).tolist() == kept.tolist()
+    assert host(c.got["seq_hot"]).tolist() == (c.held + kept).tolist()
+    assert host(c.got["history_count_out"]).tolist() == (c.count + kept).tolist()
+    k, history = c.pool.copy(), c.history.copy()
+    for b, p in enumerate(paths):
+        first, end = c.offsets[b], c.offsets[b + 1]
+        following = c.targets[first + p[-1]] if p else c.tokens[first] if end > first else -1
+        assert int(host(c.got["next_token"])[b]) & 0xFFFFFFFF == int(following) & 0xFFFFFFFF
+        assert host(c.got["path"])[first:end].tolist() == p + [-1] * (end - first - len(p))
+        for j, node in enumerate(p):
+            k[:, slots[first + j] // 16, slots[first + j] % 16] = c.k[:, first + node]
+            history[b, c.count[b] + j] = c.tokens[first + node]
+    assert np.array_equal(host(c.got["history"]).astype(np.int64) & 0xFFFFFFFF, history & 0xFFFFFFFF)
+    assert np.array_equal(host(c.hot_k).view(np.int16), (k if layers else c.pool).view(np.int16))
+
+
+def test_generation_over_a_list_that_ends_and_is_filled_again(ops, engine):
+    """While there is no page a sequence keeps nothing and takes its token again; what it keeps is in its pages."""
+    import torch
+    from test_gpu_step_run import HK, HQ, Run
+    run = Run(64)
+    whole = run.d_tables.free_count
+    run.d_tables.free_count = 3
+    held, errors = [], []
+    for i in range(14):
+        if i == 7:
+            run.d_tables.free_count = whole
+        run.step(ops)
+        errors.append(error_of(engine))
+        held.append(run.held.cpu().numpy().copy())
+    print(np.array(held), errors, flush=True)
+    assert all("free pages" in e for e in errors[4:7]) and not any(errors[7:])
+    assert (held[6] == held[5]).any() and (held[13] > held[6]).all()
+    pages, refs, history, count = (x.cpu().numpy() for x in (run.pages, run.refs, run.history, run.count))
+    assert np.array_equal(count, held[13])
+    for b in range(len(count)):
+        n = int(count[b])
+        assert n <= 16 * pages[b]
+        rows = (run.embed[:, torch.from_numpy(history[b, :n]).cuda().long()] * run.turn[:n]).half()
+        at = torch.from_numpy(refs[b, np.arange(n) // 16].astype(np.int64)).cuda(), torch.arange(n, device="cuda:0") % 16
+        assert torch.equal(run.hot_k[:, at[0], at[1]], rows[:, :, HQ:HQ + HK]) and torch.equal(run.hot_v[:, at[0], at[1]], rows[:, :, HQ + HK:])

@@ -136,3 +136,10 @@ def test_tables_after_a_list_that_ended():
     assert held["errors"] == {"sequence length"} and held["pages_out"].tolist() == [1] and (held["slots"] < 0).all() and held["free_next"] == 0
     hole = S.page_tables(first["refs"], [20], [14], [2], free, 0, 14, 3)  # counted as a page although it names none
     assert hole["errors"] == {"free pages"} and hole["pages_out"].tolist() == [3] and (hole["slots"] < 0).sum() == 12
+
+
+def test_acceptance_before_a_row_without_a_slot():
+    parents, tokens = [-1, 0, 1, 2, -1, 0], [5, 6, 7, 8, 3, 4]
+    targets, offsets = [6, 7, 8, 9, 4, 2], [0, 4, 6]
+    assert S.accept_tree(parents, tokens, targets, offsets, [9, -1, 2, 3, 4, 5]) == [[0, 1, 2, 3], [0, 1]]
+    assert S.accept_tree(parents, tokens, targets, offsets, [9, -1, S.NO_SLOT, 3, S.NO_SLOT, 5]) == [[0, 1], []]
