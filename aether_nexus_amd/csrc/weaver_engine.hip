@@ -1265,7 +1265,8 @@ int tree_plan(const aw_tree_desc* d, uint32_t n_cu, aw::TreeArgs* out, aw_tree_p
     a.q_and = d->scale == 0.0f ? 0u : ~0u;
     a.q_xor = d->scale < 0.0f ? 0x80008000u : 0u;
     a.scale_log2 = d->scale == 0.0f ? 1.0f : std::fabs(d->scale) * aw::kLog2e;
-    const uint64_t most = d->mask_words ? std::min<uint64_t>(n, 32ull * d->mask_words) : n; // nodes of a sequence
+    // Nodes of a sequence: all rows may be one's where only the device knows the offsets.
+    const uint64_t all_of = d->token_offsets ? n : n / d->batch, most = d->mask_words ? std::min<uint64_t>(all_of, 32ull * d->mask_words) : all_of;
     const uint64_t pages = align_up(n * gqa / 16 + d->batch, 8) * d->kv_heads;
     // Steps of 16-row units, if every sequence filled its table, are counted in 32 bits.
     auto steps = [&](uint32_t rows) {

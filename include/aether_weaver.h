@@ -391,7 +391,9 @@ void aw_abi_prefix_sizes(size_t sizes[2]);
  * sequence with such offsets has no rows; where the others then have more rows than num_tokens, or far more nodes than
  * their masks name, none may be computed.
  * Values that a row does not see never reach it, infinities and NaNs neither.
- * head_dim 64 or 128; up to 2^20 sequences, 2^22 tokens of each in pages, 2^25 rows of q.
+ * head_dim 64 or 128; up to 2^20 sequences, 2^22 tokens of each in pages, 2^25 rows of q; and 2^32 steps, each
+ * 64 tokens of 16 rows of a kv head, if every sequence filled its table and had as many nodes as its mask can name
+ * (without one, num_tokens / batch, or with token_offsets num_tokens).
  * Scratch is the engine's workspace, as in aw_decode_device, also under capture. */
 typedef struct aw_tree_desc {
     uint32_t batch, num_tokens;

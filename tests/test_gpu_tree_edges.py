@@ -42,3 +42,15 @@ def test_k_of_a_fused_product_as_values(ops, engine, way):
     c.out.fill_(7.0)
     ops.tree_attention(d)
     c.check("and no stride of v", v=c.k, hot_v=c.hot_k)
+
+
+def test_many_sequences_that_share_rows_equally(ops, engine):
+    """2^18 sequences of one row: each sees itself alone, its values come back as they are."""
+    import torch
+    from aether_nexus_amd import ops as O
+    n, heads, hd = 1 << 18, 8, 64
+    q, k, v = torch.randn((n, 3 * heads, hd), dtype=torch.float16, device="cuda:0").split(heads, 1)
+    out = torch.full((n, heads, hd), 7.0, dtype=torch.float16, device="cuda:0")
+    ops.tree_attention(O.make_tree_desc(batch=n, num_tokens=n, q_heads=heads, kv_heads=heads, head_dim=hd, q=q, k=k, v=v, out=out))
+    assert error_of(engine) == ""
+    assert torch.equal(out, v)

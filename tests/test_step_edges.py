@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from aether_nexus_amd import ops as O
-from aether_nexus_amd.types import AW_E_INVALID_ARG
+from aether_nexus_amd.types import AW_E_INVALID_ARG, AW_E_UNSUPPORTED
 from aether_nexus_amd.weaver import WeaverError
 from test_step import A, tree
 
@@ -162,3 +162,15 @@ def test_tree_rows_of_other_heads_are_refused(on_cpu):
         assert tree_of(**kw).q_stride == 256
     one = dict(kv_heads=1, q_heads=4)
     assert tree_of(**one, k=f16(6, 1, 64), v=f16(6, 64)).k_stride == 64
+
+
+def test_tree_plan_of_equal_parts():
+    """Rows that the sequences share equally are counted as that, not as if each had all of them."""
+    none = dict(tree_mask=0, mask_words=0, hot_count=0, refs=0, seq_held=0, hot_k=0, hot_v=0, q_heads=32, kv_heads=8)
+    p = O.tree_plan(tree(batch=1 << 18, num_tokens=1 << 18, token_offsets=0, **none))
+    assert p.work_groups
+    with pytest.raises(WeaverError) as e:  # offsets that the device alone knows
+        O.tree_plan(tree(batch=1 << 18, num_tokens=1 << 18, **none))
+    assert e.value.status == AW_E_UNSUPPORTED
+    few = dict(batch=64, num_tokens=512, tree_mask=0, mask_words=0, q_heads=8, kv_heads=2)  # 8 nodes each behind up to 48 tokens
+    assert O.tree_plan(tree(**few, token_offsets=0)).workspace_bytes == 0
