@@ -614,9 +614,9 @@ __global__ __launch_bounds__(kPrefixThreads) __attribute__((amdgpu_waves_per_eu(
 }
 
 // Small requests, in one launch: a work-group takes 16 query rows of one kv head over all
-// that they see, its waves the pages in turn.  Sequence b's work-groups begin at
-// offset_b G / 16 + b, rounded down: room for its last, partial 16 rows wherever it begins,
-// so the host need not know the lengths.  Bound: the chain offsets, lengths, refs, pages (a
+// that they see, its waves the pages in turn.  The sequences' units lie one behind another, as
+// each work-group sums up itself; the grid has one more for each sequence's last, partial 16 rows
+// than all rows fill, so the host need not know the lengths.  Bound: the chain offsets, lengths, refs, pages (a
 // round trip each), then the waves' sums: 2 sequences x 5 nodes x 14 / 2 heads x 64 behind 700
 // tokens 9.6 us, with 16 waves 3 pages of each.  As many waves as LDS holds where the work-groups
 // are no more than the CUs, else 4.
@@ -628,49 +628,56 @@ __global__ __launch_bounds__(NW * 64) void tree_pages_kernel(TreeArgs a) {
     // The heads of some rows, then the next rows, on one XCD (b % 8).
     const uint32_t j = blockIdx.x >> 3, i = uniform(j / a.kv_heads), g = j - i * a.kv_heads;
     const uint32_t unit = (blockIdx.x & 7u) * (a.work_groups / a.kv_heads >> 3) + i;
-    auto begin = [&](uint32_t b) { // of sequence b's work-groups
-        return (a.token_offsets ? min(a.token_offsets[b], a.tokens) : b * (a.tokens / a.batch)) * a.gqa / 16u + b;
-    };
-    uint32_t b = 0, n = a.batch; // the sequences that end at or before the unit are the first b .. b + n
-    while (n > 64u) {
-        const uint32_t stretch = (n + 63u) / 64u, at = (lane + 1u) * stretch - 1u;
-        const uint32_t skip = stretch * (uint32_t)__popcll(__ballot(at < n && begin(b + min(at, n - 1u) + 1u) <= unit));
-        b += skip;
-        n = n > skip ? min(n - skip, stretch) : 0u;
-    }
-    if (n) b += (uint32_t)__popcll(__ballot(lane < n && begin(b + min(lane, n - 1u) + 1u) <= unit));
-    b = uniform(b);
-    if (b < a.batch) {
-        const TreeSeq s = tree_seq(a, b, false);
-        const uint32_t first = uniform(s.first), nodes = uniform(s.nodes), held = uniform(s.held);
-        const uint32_t row0 = (unit - uniform(begin(b))) * 16u, rows = nodes * a.gqa;
-        if (row0 < rows) {
-            TreePart p{};
-            p.q = a.q + first * a.q_stride + (uint64_t)g * a.gqa * HD;
-            p.k = a.hk + (uint64_t)g * HD;
-            p.v = a.hv + (uint64_t)g * HD;
-            p.q_step = a.q_stride;
-            p.blocks = a.blocks;
-            p.rstride = a.kv_heads * (uint32_t)HD;
-            p.gqa = a.gqa;
-            p.row0 = row0;
-            p.row_end = min(row0 + 16u, rows);
-            p.q_and = a.q_and;
-            p.q_xor = a.q_xor;
-            p.scale_log2 = a.scale_log2;
-            p.out = a.out + first * a.out_stride + (uint64_t)g * a.gqa * HD;
-            p.o_step = a.out_stride;
-            p.err = a.err;
-            p.nk = a.k + first * a.k_stride + (uint64_t)g * HD;
-            p.nv = a.v + first * a.v_stride + (uint64_t)g * HD;
-            p.nk_step = a.k_stride;
-            p.nv_step = a.v_stride;
-            p.mask = a.mask ? a.mask + (uint64_t)first * a.mask_words : nullptr;
-            p.mask_words = a.mask_words;
-            const PageRun runs[2] = {{a.refs + (uint64_t)b * a.refs_stride, 0, (held + 15u) / 16u, held, held}, {nullptr, 0, (nodes + 15u) / 16u, nodes, nodes}};
-            TreePages<HD, NW, 1> pages;
-            pages.run(p, runs, prefix_lds, (int)lane, wave);
+    // The sequence that the unit is of, whose units begin behind those of the sequences before; bad offsets give none.
+    uint32_t b = a.batch, row0 = 0, first = 0, nodes = 0, held = 0;
+    for (uint32_t c0 = 0, units = 0; c0 < a.batch && b == a.batch; c0 += 256u) { // wave-uniform
+        TreeSeq s[4];
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; ++k)
+            if (c0 + 64u * k < a.batch) s[k] = tree_seq(a, min(c0 + 64u * k + lane, a.batch - 1u), false); // uniform
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; ++k) {
+            if (c0 + 64u * k >= a.batch) break; // uniform
+            const uint32_t x = c0 + 64u * k + lane < a.batch ? (s[k].nodes * a.gqa + 15u) / 16u : 0u, end = units + lanes_scan(x);
+            const uint64_t hit = __ballot(end - x <= unit && unit < end);
+            if (hit) { // one lane
+                const int l = __builtin_ctzll(hit);
+                b = c0 + 64u * k + (uint32_t)l;
+                row0 = (unit - (uint32_t)__builtin_amdgcn_readlane((int)(end - x), l)) * 16u;
+                first = (uint32_t)__builtin_amdgcn_readlane((int)s[k].first, l);
+                nodes = (uint32_t)__builtin_amdgcn_readlane((int)s[k].nodes, l);
+                held = (uint32_t)__builtin_amdgcn_readlane((int)s[k].held, l);
+            }
+            units = (uint32_t)__builtin_amdgcn_readlane((int)end, 63);
         }
+    }
+    if (b < a.batch) {
+        const uint32_t rows = nodes * a.gqa;
+        TreePart p{};
+        p.q = a.q + first * a.q_stride + (uint64_t)g * a.gqa * HD;
+        p.k = a.hk + (uint64_t)g * HD;
+        p.v = a.hv + (uint64_t)g * HD;
+        p.q_step = a.q_stride;
+        p.blocks = a.blocks;
+        p.rstride = a.kv_heads * (uint32_t)HD;
+        p.gqa = a.gqa;
+        p.row0 = row0;
+        p.row_end = min(row0 + 16u, rows);
+        p.q_and = a.q_and;
+        p.q_xor = a.q_xor;
+        p.scale_log2 = a.scale_log2;
+        p.out = a.out + first * a.out_stride + (uint64_t)g * a.gqa * HD;
+        p.o_step = a.out_stride;
+        p.err = a.err;
+        p.nk = a.k + first * a.k_stride + (uint64_t)g * HD;
+        p.nv = a.v + first * a.v_stride + (uint64_t)g * HD;
+        p.nk_step = a.k_stride;
+        p.nv_step = a.v_stride;
+        p.mask = a.mask ? a.mask + (uint64_t)first * a.mask_words : nullptr;
+        p.mask_words = a.mask_words;
+        const PageRun runs[2] = {{a.refs + (uint64_t)b * a.refs_stride, 0, (held + 15u) / 16u, held, held}, {nullptr, 0, (nodes + 15u) / 16u, nodes, nodes}};
+        TreePages<HD, NW, 1> pages;
+        pages.run(p, runs, prefix_lds, (int)lane, wave);
     }
     if (blockIdx.x == 0)
         for (uint32_t c = threadIdx.x; c < a.batch; c += NW * 64u) tree_seq(a, c, true);

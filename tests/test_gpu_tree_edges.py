@@ -5,6 +5,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
+from helpers import prefix_errors
 from test_gpu_tree import WAYS, Case, dev, error_of, host
 
 pytestmark = pytest.mark.gpu
@@ -54,3 +55,34 @@ def test_many_sequences_that_share_rows_equally(ops, engine):
     ops.tree_attention(O.make_tree_desc(batch=n, num_tokens=n, q_heads=heads, kv_heads=heads, head_dim=hd, q=q, k=k, v=v, out=out))
     assert error_of(engine) == ""
     assert torch.equal(out, v)
+
+
+# Offsets as a caller should not give them; the sequences among them that lie within the rows and ascend.
+BAD_OFFSETS = [[0, 9, 3], [0, 3, 40], [5, 2, 23], [9, 4, 7, 23], [0, 100, 7, 23], [0, 2, 1 << 31, 2, 23], [3, 3, 23, 0], [0, 0xFFFFFFFF, 0, 23, 22]]
+
+
+@pytest.mark.parametrize("spare", [0, 9000], ids=["one", "shared"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("offsets", BAD_OFFSETS, ids=lambda o: "-".join(map(str, o)))
+def test_sequences_beside_bad_offsets(ops, engine, offsets, hd, spare):
+    """Reported; each sequence whose own offsets are good is computed, and nothing is written beside those rows."""
+    import torch
+    n = len(offsets) - 1
+    good = [b for b in range(n) if offsets[b] <= offsets[b + 1] <= 23]
+    c = Case(11, 8, 2, hd, [3, 20] + [0] * (n - 2), [48, 17] + [33] * (n - 2), spare=spare)
+    around = torch.full((c.rows + 40, 8, hd), 7.0, dtype=torch.float16, device="cuda:0")
+    d = c.desc(token_offsets=dev(np.array(offsets)), out=around[20:20 + c.rows])
+    assert (plan_of(d) == 0) == (spare == 0)
+    ops.tree_attention(d)
+    assert "sequence length" in error_of(engine)
+    got = host(around).astype(np.float64)
+    left = np.ones(len(got), dtype=bool)
+    for b in good:
+        first, end = offsets[b], offsets[b + 1]
+        if first == end:
+            continue
+        left[20 + first:20 + end] = False
+        want, absolute, total = c.want(offsets=[first, end], refs=c.refs[b:b + 1], held=c.held[b:b + 1])
+        worst, _ = prefix_errors(got[20 + first:20 + end], want[first:end], absolute[first:end], total[first:end], 48 + 23, 6.0)
+        assert worst <= 1.0, (b, worst)
+    assert (got[left] == 7.0).all()
