@@ -88,14 +88,12 @@ __global__ __launch_bounds__(256) void tables_kernel(TablesArgs a) {
     uint32_t tokens = 0, pages = a.free_first ? min(a.free_first[0], 1u << 30) : 0u; // before the chunk
     bool bad_seq = false, bad_free = false;
     for (uint32_t c0 = 0; c0 < a.batch; c0 += kTablesSeqs) {
-        uint32_t held[4], had[4], n[4], need[4], got[4];
-        bool lacks[4]; // pages for the tokens that it holds
+        uint32_t held[4], had[4], n[4], need[4], lacks = 0; // bit j: pages for the tokens that it holds
         uint32_t sum = 0;
 #pragma unroll
         for (uint32_t j = 0; j < 4u; ++j) {
             const uint32_t s = c0 + 4u * tid + j;
             held[j] = had[j] = n[j] = 0;
-            lacks[j] = false;
             if (s < a.batch) {
                 held[j] = a.seq_held[s];
                 const uint32_t want = a.seq_new[s], most = held[j] < room ? room - held[j] : 0u;
@@ -104,11 +102,11 @@ __global__ __launch_bounds__(256) void tables_kernel(TablesArgs a) {
                 held[j] = min(held[j], 0xFFFFFFFFu - kPageTokens);
                 const uint32_t least = (held[j] + kPageTokens - 1u) / kPageTokens;
                 had[j] = a.seq_pages ? a.seq_pages[s] : least;
-                lacks[j] = had[j] < least;
-                bad_seq |= lacks[j];
+                lacks |= (had[j] < least ? 1u : 0u) << j;
             }
             sum = min(sum + n[j], a.tokens);
         }
+        bad_seq |= lacks != 0u;
         const uint32_t all = capped_scan(sum, a.tokens, s_wave);
         uint32_t off = min(tokens + sum, a.tokens), taken = 0;
 #pragma unroll
@@ -117,7 +115,7 @@ __global__ __launch_bounds__(256) void tables_kernel(TablesArgs a) {
             bad_seq |= end - off < n[j];
             n[j] = end - off;
             const uint32_t after = n[j] ? (held[j] + n[j] + kPageTokens - 1u) / kPageTokens : 0u;
-            need[j] = after > had[j] && !lacks[j] ? after - had[j] : 0u;
+            need[j] = after > had[j] && !(lacks >> j & 1u) ? after - had[j] : 0u;
             taken = min(taken + need[j], 1u << 30);
             s_off[4u * tid + j] = off;
             s_held[4u * tid + j] = held[j];
@@ -128,10 +126,9 @@ __global__ __launch_bounds__(256) void tables_kernel(TablesArgs a) {
         uint32_t from = min(pages + taken, 1u << 30);
 #pragma unroll
         for (uint32_t j = 0; j < 4u; ++j) {
-            s_start[4u * tid + j] = lacks[j] ? 1u << 30 : from; // past any list
-            got[j] = from < a.free_count ? min(need[j], a.free_count - from) : 0u;
+            s_start[4u * tid + j] = lacks >> j & 1u ? 1u << 30 : from; // past any list
             from = min(from + need[j], 1u << 30);
-            bad_free |= got[j] < need[j];
+            bad_free |= need[j] && from > a.free_count;
         }
         const uint32_t count = min(a.batch - c0, kTablesSeqs);
         tokens = min(tokens + all, a.tokens);
@@ -143,7 +140,7 @@ __global__ __launch_bounds__(256) void tables_kernel(TablesArgs a) {
                 const uint32_t s = c0 + 4u * tid + j;
                 if (s >= a.batch) continue;
                 a.seq_hot[s] = held[j] + n[j];
-                if (a.pages_out) a.pages_out[s] = had[j] + got[j];
+                if (a.pages_out) a.pages_out[s] = had[j] + min(need[j], a.free_count - min(s_start[4u * tid + j], a.free_count));
                 a.token_offsets[s] = s_off[4u * tid + j];
             }
         }
@@ -586,21 +583,22 @@ __global__ __launch_bounds__(256) void accept_kernel(AcceptArgs a) {
     const SeqRows rows = seq_rows(a.token_offsets, a.tokens, a.batch, b, a.err);
     const uint32_t n = min(rows.n, kMaxNodes);
     const uint32_t count = a.history && layer == 0 ? a.history_count[b] : 0u; // before a barrier: history_count_out may be it
+    const int64_t* slots = a.slots ? a.slots + rows.first : nullptr;
+    const bool none = slots && lane < n && slots[lane] == kNoSlot; // no page for the node kept lane-th
     for (uint32_t i = tid; i < n; i += 256u) {
         s_parent[i] = a.parents[rows.first + i];
         s_token[i] = a.node_tokens[rows.first + i];
         s_target[i] = a.targets[rows.first + i];
-        s_path[i] = a.slots && a.slots[rows.first + i] == kNoSlot; // until the walk: no page for the i-th kept node
     }
     __syncthreads();
     if (tid < 64u) {
         uint32_t room = n; // nodes that may be kept
-        for (uint32_t c = 0; c < n; c += 64u) {
-            const uint64_t m = __ballot(c + lane < n && s_path[min(c + lane, n - 1u)] != 0);
-            if (m) {
-                room = c + (uint32_t)__builtin_ctzll(m);
-                break;
-            }
+        uint64_t m = __ballot(none);
+        for (uint32_t c = 0;;) {
+            if (m) room = c + (uint32_t)__builtin_ctzll(m);
+            c += 64u;
+            if (m || c >= n || !slots) break;
+            m = __ballot(slots[min(c + lane, n - 1u)] == kNoSlot);
         }
         uint32_t kept = room ? 1u : 0u, cur = 0;
         if (lane == 0) s_path[0] = 0;
