@@ -428,6 +428,7 @@ struct TreeWork {
     }
     __device__ uint32_t all(uint32_t kv_heads) const { return kv_heads * tiles * steps; }
 };
+constexpr uint64_t kTreeSteps = 4294960000; // of a request: below 2^32 also when rounded up to shares of all work-groups
 
 constexpr size_t tree_lds(int HD, int NR) { return NR ? tree_pages_lds(HD, 4, NR) : prefix_lds_bytes(HD); }
 
@@ -466,30 +467,25 @@ __global__ __launch_bounds__(kPrefixThreads) __attribute__((amdgpu_waves_per_eu(
     // Work-group b runs on XCD b % 8: neighbours in the line, which read the same pages for
     // several tiles of rows, run on one XCD.
     const uint32_t w = (blockIdx.x & 7u) * (a.work_groups >> 3) + (blockIdx.x >> 3);
-    uint32_t* s_sum = (uint32_t*)prefix_lds; // [4] sums of waves, [5] the sequence found, [4] sums of waves in fp32
+    uint32_t* s_sum = (uint32_t*)prefix_lds; // [4] sums of waves, [5] the sequence found, [4] sums of waves' upper parts
     // All steps; sequence tid of each 256.
     TreeSeq s{};
-    uint32_t mine = 0;
-    // Counted in fp32 too: offsets that descend give rows to several sequences, or one has far more nodes than its
-    // mask names; steps that pass 32 bits by that (both are reported) are not taken.
-    float wide = 0.0f;
+    // Counted exactly, in two parts: offsets that descend give rows to several sequences, or one has far more nodes than its
+    // mask names; steps that pass 32 bits by that (both are reported) are not taken, and no sum below wraps.
+    uint64_t mine = 0;
     for (uint32_t b = tid; b < a.batch; b += 256u) {
         s = tree_seq(a, b, blockIdx.x == 0);
         const TreeWork<NR> work(a, s);
-        mine += work.all(a.kv_heads);
-        wide += (float)a.kv_heads * (float)work.tiles * (float)work.steps;
+        mine += min((uint64_t)a.kv_heads * work.tiles * work.steps, (uint64_t)1 << 40);
     }
-    mine = lanes_scan(mine);
-    wide = wave_sum(wide);
+    const uint32_t low = lanes_scan((uint32_t)mine & 0xFFFFu), high = lanes_scan((uint32_t)min(mine >> 16, (uint64_t)1 << 23));
     if (lane == 63u) {
-        s_sum[wave] = mine;
-        s_sum[9u + wave] = __builtin_bit_cast(uint32_t, wide);
+        s_sum[wave] = low;
+        s_sum[9u + wave] = high;
     }
     __syncthreads();
-    wide = 0.0f;
-#pragma unroll
-    for (uint32_t i = 0; i < 4u; ++i) wide += __builtin_bit_cast(float, s_sum[9u + i]);
-    const uint32_t total = uniform(wide >= 4294960000.0f ? 0u : s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]);
+    const uint64_t steps = ((uint64_t)(s_sum[9] + s_sum[10] + s_sum[11] + s_sum[12]) << 16) + s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+    const uint32_t total = uniform(steps < kTreeSteps ? (uint32_t)steps : 0u);
     const uint32_t each = uniform((total + a.work_groups - 1u) / a.work_groups);
     uint32_t pos = w * each;
     const uint32_t stop = min(pos + each, total);

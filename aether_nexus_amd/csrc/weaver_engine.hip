@@ -1272,7 +1272,7 @@ int tree_plan(const aw_tree_desc* d, uint32_t n_cu, aw::TreeArgs* out, aw_tree_p
     auto steps = [&](uint32_t rows) {
         return (double)d->kv_heads * ((double)n * gqa / rows + std::min<double>((double)n, d->batch)) * (d->hot_count / 4.0 + (double)most / 64 + 2);
     };
-    if (steps(16) >= 4294960000.0) return refuse(AW_E_UNSUPPORTED, "too many rows over too many tokens");
+    if (steps(16) >= (double)aw::kTreeSteps) return refuse(AW_E_UNSUPPORTED, "too many rows over too many tokens");
     const bool one = d->hot_count * (uint64_t)kBlock + most <= kTreeOneTokens && pages <= kTreeOneGroups * (uint64_t)n_cu;
     const uint32_t rows = one ? 16u : tree_row_tile(n * gqa / d->batch, steps(16) * 64 * d->head_dim);
     const double all = steps(rows);

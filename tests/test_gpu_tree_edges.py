@@ -86,3 +86,28 @@ def test_sequences_beside_bad_offsets(ops, engine, offsets, hd, spare):
         worst, _ = prefix_errors(got[20 + first:20 + end], want[first:end], absolute[first:end], total[first:end], 48 + 23, 6.0)
         assert worst <= 1.0, (b, worst)
     assert (got[left] == 7.0).all()
+
+
+def test_steps_just_past_32_bits_by_bad_offsets(ops, engine):
+    """Sequences of all rows each, whose steps together are a little more than 2^32: reported, and nothing is computed.  The sum
+    has to be exact: in fp32, one after another, the short sequences at its end do not count, and the rest is below 2^32."""
+    import torch
+    from aether_nexus_amd import ops as O
+    n, hd = 1 << 17, 64
+    steps = lambda nodes: -(-nodes // 16) * -(-nodes // 64)  # of a sequence without pages in units of 16 rows
+    sizes = [n] * 255
+    sizes += [max(m for m in range(n) if steps(m) + 255 * steps(n) < 4294950000)] + [320] * 600
+    total, fp32 = sum(map(steps, sizes)), np.float32(0)
+    for m in sizes:
+        fp32 += np.float32(steps(m))
+    assert 2 ** 32 < total < 2 ** 32 + 2 ** 16 and fp32 < 4294960000
+    offsets = np.zeros(256 * len(sizes) + 1, dtype=np.int64)  # every 256th sequence, which one thread counts, has rows
+    offsets[1::256] = sizes
+    q = torch.zeros((n, 1, hd), dtype=torch.float16, device="cuda:0")
+    out = torch.full_like(q, 7.0)
+    d = O.make_tree_desc(batch=len(offsets) - 1, num_tokens=n, q_heads=1, kv_heads=1, head_dim=hd, q=q, k=q, v=q, out=out,
+                         token_offsets=dev(offsets))
+    assert plan_of(d) == 16
+    ops.tree_attention(d)
+    assert "sequence length" in error_of(engine)
+    assert bool((out == 7.0).all())
