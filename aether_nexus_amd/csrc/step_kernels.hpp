@@ -355,12 +355,12 @@ __global__ __launch_bounds__(256) void logits_kernel(LogitsArgs a) {
             seq = seq_at(a.token_offsets, a.rows, a.batch, r, lane);
             seq = {(uint32_t)__builtin_amdgcn_readfirstlane((int)seq.b), (uint32_t)__builtin_amdgcn_readfirstlane((int)seq.first),
                    (uint32_t)__builtin_amdgcn_readfirstlane((int)seq.end)};
-            const bool bad = seq.b < a.batch && (seq.first > r || seq.end <= r || seq.end > a.rows); // offsets that descend, or pass the rows
+            const bool bad = seq.b < a.batch && (seq.first > r || seq.end <= r || seq.end > a.rows); // offsets that descend, pass the rows or begin behind them
             if (bad && tid == 0) flag(a.err, kErrSeq);
             if (seq.b >= a.batch || bad) { // rows of no sequence
                 for (; r < r1; ++r)
                     if (tid == 0 && a.best && a.slices > 1u) a.keys[(uint64_t)r * a.slices + slice] = kNoRow;
-                return;
+                break;
             }
             if (a.repetition) rep = a.repetition[seq.b];
             if (a.frequency) freq = a.frequency[seq.b];
@@ -534,6 +534,9 @@ __global__ __launch_bounds__(256) void logits_kernel(LogitsArgs a) {
             else a.best[r] = best_token(k);
         }
     }
+    if (blockIdx.x == 0 && a.token_offsets) // reported wherever they are, also where no row's search meets them
+        for (uint32_t b = threadIdx.x; b < a.batch; b += 256u)
+            if (a.token_offsets[b] > a.token_offsets[b + 1u] || a.token_offsets[b + 1u] > a.rows) flag(a.err, kErrSeq);
 }
 
 // The best token of a row among its slices', a wave a row.

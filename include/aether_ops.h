@@ -312,7 +312,8 @@ int aw_ops_page_tables(aw_engine* engine, const aw_tables_desc* desc, void* hip_
  * takes allowed row allowed_index[t], none where that is negative (NULL: row t); an index
  * >= allowed_rows sets "token id" and allows nothing.  History, bias and node tokens >= vocab_size
  * are passed over.  Each of the penalties, and each group of pointers, may be NULL.  Counts past their
- * stride are taken as it and set "sequence length". */
+ * stride are taken as it and set "sequence length".  So do token_offsets that do not begin at 0, descend or pass
+ * num_tokens, and rows of any sequence may then be left as they were. */
 typedef struct aw_logits_desc {
     uint32_t num_tokens, vocab_size;     /* rows <= 2^24, vocab_size <= 2^24 */
     uint32_t batch, flags;               /* batch <= 2^20; 0 or AW_LOGITS_F16 */

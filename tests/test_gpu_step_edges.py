@@ -171,3 +171,18 @@ def test_generation_over_a_list_that_ends_and_is_filled_again(ops, engine):
         rows = (run.embed[:, torch.from_numpy(history[b, :n]).cuda().long()] * run.turn[:n]).half()
         at = torch.from_numpy(refs[b, np.arange(n) // 16].astype(np.int64)).cuda(), torch.arange(n, device="cuda:0") % 16
         assert torch.equal(run.hot_k[:, at[0], at[1]], rows[:, :, HQ:HQ + HK]) and torch.equal(run.hot_v[:, at[0], at[1]], rows[:, :, HQ + HK:])
+
+
+def test_logits_report_offsets_wherever_they_descend(ops, engine):
+    """Also where no row's search meets them: here rows 2 to 9 of the second of 128 sequences."""
+    c = Logits(28, 300, [10], history=9)
+    kw = {k: np.repeat(v, 128, axis=0) for k, v in c.kw.items() if k in ("history", "history_count", "prompt_count", "repetition", "frequency", "presence")}
+    offsets = np.array([0, 0, 10] + [2] * 126)
+    c.kw.update(kw, offsets=offsets)
+    c.batch = 128
+    ops.adjust_logits(c.desc())
+    assert "sequence length" in error_of(engine)
+    offsets[3:] = 10  # all of them empty
+    ops.adjust_logits(c.desc())
+    assert error_of(engine) == ""
+    c.check()
