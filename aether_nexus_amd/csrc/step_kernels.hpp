@@ -78,7 +78,7 @@ constexpr uint32_t kTablesRows = 256, kTablesSeqs = 1024;
 
 template <bool TREE>
 __global__ __launch_bounds__(256) void tables_kernel(TablesArgs a) {
-    __shared__ uint32_t s_off[kTablesSeqs + 1], s_held[kTablesSeqs], s_pages[kTablesSeqs], s_start[kTablesSeqs], s_wave[4];
+    __shared__ uint32_t s_off[kTablesSeqs], s_held[kTablesSeqs], s_pages[kTablesSeqs], s_start[kTablesSeqs], s_wave[4];
     __shared__ int32_t s_par[TREE ? kTablesRows + kMaxNodes : 1];
     const uint32_t tid = threadIdx.x, t0 = blockIdx.x * kTablesRows, t1 = min(t0 + kTablesRows, a.tokens), t = t0 + tid;
     const uint32_t p0 = t0 > kMaxNodes ? t0 - kMaxNodes : 0u; // parents from here on are at hand
@@ -133,7 +133,6 @@ __global__ __launch_bounds__(256) void tables_kernel(TablesArgs a) {
         const uint32_t count = min(a.batch - c0, kTablesSeqs);
         tokens = min(tokens + all, a.tokens);
         pages = min(pages + all_pages, 1u << 30);
-        if (tid == 0) s_off[kTablesSeqs] = tokens; // of the last sequence's end; those past `count` are empty
         if (blockIdx.x == 0) {
 #pragma unroll
             for (uint32_t j = 0; j < 4u; ++j) {
@@ -305,8 +304,10 @@ __device__ inline SeqAt seq_at(const uint32_t* offsets, uint32_t tokens, uint32_
 // are a word a token in LDS: made once for a sequence from its history and biases (integer
 // atomics: no order shows in them), and for each row the tokens of its own nodes are added
 // and those of the row before taken off.  Logits go by in 16-byte pieces, the last of a slice
-// beginning earlier and making some values twice, from what was read before the row's first
-// write; the few tokens that have a word are taken one after another.  A row's logits, the
+// beginning earlier and making some values twice: with words from what was read before the row's
+// first write (a barrier lies between), without them perhaps from a value already written in
+// place, which the grammar alone has changed and changes no further (-inf or as it was).  The
+// few tokens that have a word are taken one after another.  A row's logits, the
 // first 2048 tokens of the history and the biases are asked for before their counts are known
 // (history_stride and bias_stride entries are there whatever the counts), so a work-group
 // waits for memory two or three times.

@@ -411,7 +411,7 @@ typedef struct aw_tree_desc {
     const uint16_t* hot_k;
     const uint16_t* hot_v;
     const uint32_t* refs;
-    const uint32_t* seq_held;            /* NULL: no tokens in pages */
+    const uint32_t* seq_held;            /* [batch]; may be NULL with hot_count 0 */
     const uint32_t* token_offsets;       /* NULL: num_tokens / batch rows each */
     const uint32_t* tree_mask;           /* [num_tokens][mask_words] */
     uint16_t*       out;

@@ -186,3 +186,14 @@ def test_logits_report_offsets_wherever_they_descend(ops, engine):
     ops.adjust_logits(c.desc())
     assert error_of(engine) == ""
     c.check()
+
+
+@pytest.mark.parametrize("vocab,half", [(257, False), (1025 + 256, False), (4096 + 769, False), (513, True), (2048 + 1537, True), (1, False), (7, True)])
+def test_masks_in_place_where_pieces_of_two_waves_overlap(ops, engine, vocab, half):
+    """Without counts a value may be made again from the output: masked twice it is what it is masked once."""
+    c = Logits(29, vocab, [40], half=half, nodes=False, allowed=0.5, extreme=True)
+    d = c.desc(token_offsets=None, batch=0)
+    d.out, d.out_stride = d.logits, d.logits_stride
+    ops.adjust_logits(d)
+    assert error_of(engine) == ""
+    c.check(out=c.src)
