@@ -14,6 +14,8 @@ namespace awo {
 constexpr uint32_t kMaxNodes = 1024u;   // of a sequence's tree
 constexpr uint32_t kErrFree = aw_engine_internal::kErrFreeBit;
 constexpr uint32_t kNoPage = kPageMask; // an entry without a page
+// A sequence's first page in the list, where it takes none: past any list.  kTooMany: of more nodes than the mask's.
+constexpr uint32_t kTakesNone = 1u << 30, kTooMany = kTakesNone + 1u;
 constexpr int64_t kNoSlot = AW_NO_SLOT;
 
 // First row and number of rows of sequence b, uniform; offsets that descend or pass the
@@ -70,7 +72,8 @@ __device__ inline uint32_t capped_scan(uint32_t& x, uint32_t cap, uint32_t* s_wa
 
 // One launch: each work-group sums the lengths of all sequences before its 256 rows
 // itself, 1024 sequences at a time (12 KB of L2 reads), and makes its rows; a page is entered
-// by the row that begins it, so nothing waits for another work-group.  The first work-group
+// by the row that begins it, so nothing waits for another work-group.  A sequence's rows are its
+// seq_new whatever its table holds, so one that is past it moves no other's.  The first work-group
 // writes what belongs to sequences.  A node's ancestors are walked in LDS.
 // Bound: a launch and the chain lengths -> sums -> search -> page -> slot: 64 sequences of
 // one new token 4.6 us, 256 trees of up to 48 nodes 6.2, 260000 rows of 509 prompts 6.8.
@@ -88,7 +91,7 @@ __global__ __launch_bounds__(256) void tables_kernel(TablesArgs a) {
     uint32_t tokens = 0, pages = a.free_first ? min(a.free_first[0], 1u << 30) : 0u; // before the chunk
     bool bad_seq = false, bad_free = false;
     for (uint32_t c0 = 0; c0 < a.batch; c0 += kTablesSeqs) {
-        uint32_t held[4], had[4], n[4], need[4], lacks = 0; // bit j: pages for the tokens that it holds
+        uint32_t held[4], had[4], n[4], need[4], lacks = 0; // bit j: pages for the tokens that it holds; bit j + 4: mask words for its nodes
         uint32_t sum = 0;
 #pragma unroll
         for (uint32_t j = 0; j < 4u; ++j) {
@@ -97,9 +100,10 @@ __global__ __launch_bounds__(256) void tables_kernel(TablesArgs a) {
             if (s < a.batch) {
                 held[j] = a.seq_held[s];
                 const uint32_t want = a.seq_new[s], most = held[j] < room ? room - held[j] : 0u;
-                n[j] = min(min(want, most), min(a.tokens, TREE ? 32u * a.mask_words : a.tokens));
-                bad_seq |= n[j] < want || held[j] > room;
-                held[j] = min(held[j], 0xFFFFFFFFu - kPageTokens);
+                n[j] = min(want, a.tokens);
+                bad_seq |= n[j] < want || want > most || held[j] > room;
+                if (TREE && want > 32u * a.mask_words) lacks |= 16u << j;
+                held[j] = min(held[j], 0xFE000000u); // no place passes 32 bits
                 const uint32_t least = (held[j] + kPageTokens - 1u) / kPageTokens;
                 had[j] = a.seq_pages ? a.seq_pages[s] : least;
                 lacks |= (had[j] < least ? 1u : 0u) << j;
@@ -114,8 +118,8 @@ __global__ __launch_bounds__(256) void tables_kernel(TablesArgs a) {
             const uint32_t end = min(off + n[j], a.tokens);
             bad_seq |= end - off < n[j];
             n[j] = end - off;
-            const uint32_t after = n[j] ? (held[j] + n[j] + kPageTokens - 1u) / kPageTokens : 0u;
-            need[j] = after > had[j] && !(lacks >> j & 1u) ? after - had[j] : 0u;
+            const uint32_t after = n[j] ? (min(held[j] + n[j], room) + kPageTokens - 1u) / kPageTokens : 0u;
+            need[j] = after > had[j] && !(lacks >> j & (TREE ? 17u : 1u)) ? after - had[j] : 0u;
             taken = min(taken + need[j], 1u << 30);
             s_off[4u * tid + j] = off;
             s_held[4u * tid + j] = held[j];
@@ -126,7 +130,7 @@ __global__ __launch_bounds__(256) void tables_kernel(TablesArgs a) {
         uint32_t from = min(pages + taken, 1u << 30);
 #pragma unroll
         for (uint32_t j = 0; j < 4u; ++j) {
-            s_start[4u * tid + j] = lacks >> j & 1u ? 1u << 30 : from; // past any list
+            s_start[4u * tid + j] = TREE && lacks >> j & 16u ? kTooMany : lacks >> j & 1u ? kTakesNone : from;
             from = min(from + need[j], 1u << 30);
             bad_free |= need[j] && from > a.free_count;
         }
@@ -150,23 +154,27 @@ __global__ __launch_bounds__(256) void tables_kernel(TablesArgs a) {
                 if (k + step < count && s_off[k + step] <= t) k += step;
             const uint32_t i = t - s_off[k], place = s_held[k] + i, page = place / kPageTokens;
             const uint64_t entry = (uint64_t)(c0 + k) * a.refs_stride + page;
-            uint32_t ref;
-            if (page >= s_pages[k]) { // a page taken here, named by the row that begins it; or there is none
-                const uint32_t f = s_start[k] + (page - s_pages[k]);
-                ref = f < a.free_count ? a.free_pages[f] & kPageMask : kNoPage;
-                if (place % kPageTokens == 0u || i == 0u) a.refs[entry] = ref;
-            } else {
-                ref = a.refs[entry] & kPageMask;
-                bad_free |= ref == kNoPage; // an entry that an earlier step found no page for
+            uint32_t ref = kNoPage;
+            if (place < room) { // else past the table
+                if (page >= s_pages[k]) { // a page taken here, named by the row that begins it; or there is none
+                    const uint32_t f = s_start[k] + (page - s_pages[k]);
+                    ref = f < a.free_count ? a.free_pages[f] & kPageMask : kNoPage;
+                    if (place % kPageTokens == 0u || i == 0u) a.refs[entry] = ref;
+                } else {
+                    ref = a.refs[entry] & kPageMask;
+                    bad_free |= ref == kNoPage; // an entry that an earlier step found no page for
+                    if (TREE && s_start[k] == kTooMany) ref = kNoPage;
+                }
             }
             if (a.slots) a.slots[t] = ref == kNoPage ? kNoSlot : (int64_t)ref * kPageTokens + place % kPageTokens;
             uint32_t position = place;
             if constexpr (TREE) {
                 uint32_t* row = a.tree_mask + (uint64_t)t * a.mask_words;
                 const uint32_t base = t - i - p0; // of the tree's parents at hand (mod 2^32: the nodes needed are)
-                uint32_t cur = i, word = i / 32u, bits = 1u << (i % 32u), depth = 0;
+                const bool inside = i < 32u * a.mask_words; // else it sees nothing, and its parents need not be at hand
+                uint32_t cur = i, word = inside ? i / 32u : 0u, bits = inside ? 1u << (i % 32u) : 0u, depth = 0;
                 for (uint32_t w = word + 1u; w < a.mask_words; ++w) row[w] = 0;
-                for (int32_t p = s_par[base + i]; p >= 0; p = s_par[base + cur]) { // nodes descend: at most i steps
+                for (int32_t p = inside ? s_par[base + i] : -1; p >= 0; p = s_par[base + cur]) { // nodes descend: at most i steps
                     if ((uint32_t)p >= cur) {
                         bad_seq = true;
                         break;

@@ -268,12 +268,14 @@ void aw_abi_ops_desc_sizes(size_t sizes[3]);
  *   tree_mask     [num_tokens][mask_words], required with parents: itself and its ancestors
  * parents [num_tokens]: node numbers within the tree, < 0 for a root; one that is not an earlier node
  * sets "sequence length" and makes a root.  Rows behind the last sequence: slot -1, position 0,
- * mask 0.  New tokens past hot_count pages, past num_tokens rows or (with parents) past 32 mask_words
- * nodes set "sequence length" and are left out.  A sequence whose seq_held needs more pages than seq_pages
- * sets "sequence length" and takes none.  New tokens without a page, there or where free_pages ends
- * ("free pages"), get AW_NO_SLOT and entries of 0x7FFFFFFF (refused by the calls that read them), which are
- * not counted in pages_out: a later step with seq_held up to 16 * pages_out takes pages for them.  One
- * of the seq_pages entries that is 0x7FFFFFFF sets "free pages" where a new token falls into it. */
+ * mask 0.  A sequence has seq_new rows whatever else is wrong with it (fewer where num_tokens end, which sets
+ * "sequence length"), so none moves the rows of those behind it.  Its new tokens past hot_count pages,
+ * all of them where seq_held needs more pages than seq_pages or (with parents) there are more than 32
+ * mask_words, set "sequence length" and take no page; those that free_pages has none for set "free pages".
+ * Each such token gets AW_NO_SLOT, and its entry, where it lies within hot_count and behind seq_pages,
+ * 0x7FFFFFFF (refused by the calls that read it), which is not counted in pages_out: a later step with
+ * seq_held up to 16 * pages_out takes a page for it.  One of the seq_pages entries that is 0x7FFFFFFF sets
+ * "free pages" where a new token falls into it.  A node past 32 mask_words sees nothing, at position held. */
 typedef struct aw_tables_desc {
     uint32_t batch, num_tokens;          /* batch <= 2^20, num_tokens <= 2^24 */
     uint32_t hot_count, refs_stride;     /* entries of a row, <= 2^26; refs_stride >= hot_count */

@@ -55,37 +55,40 @@ def page_tables(refs, held, new, pages, free, first: int, rows: int, hot_count: 
     offsets, slots, positions = [0], np.full(rows, -1, dtype=np.int64), np.zeros(rows, dtype=np.int64)
     mask = np.zeros((rows, words), dtype=np.uint32)
     for b in range(batch):
-        h, n = int(held[b]), int(new[b])
-        most = max(0, hot_count * PAGE - h)
-        n = min([n, most, rows - t] + ([32 * words] if parents is not None else []))
-        if n < int(new[b]) or h > hot_count * PAGE:
+        h, n = int(held[b]), min(int(new[b]), rows - t)
+        room = hot_count * PAGE
+        many = parents is not None and int(new[b]) > 32 * words
+        if n < int(new[b]) or int(new[b]) > max(0, room - h) or h > room or many:
             errors.add("sequence length")
         least = -(-h // PAGE)
         p = least if pages is None else int(pages[b])
         lacks = p < least
         if lacks:
             errors.add("sequence length")
-        need = max(0, -(-(h + n) // PAGE) - p) if n and not lacks else 0
+        need = max(0, -(-min(h + n, room) // PAGE) - p) if n and h < room and not lacks and not many else 0
         mine = [int(x) & REF_MASK for x in free[f:f + need]]
         if len(mine) < need:
             errors.add("free pages")
         f += need
-        tree = None if parents is None else sees_of(parents[t:t + n])
+        tree = None if parents is None else sees_of(parents[t:t + min(n, 32 * words)])
         for i in range(n):
-            at = (h + i) // PAGE
-            if at >= p:
-                ref = mine[at - p] if at - p < len(mine) else REF_MASK
-                if i == 0 or (h + i) % PAGE == 0:
-                    refs[b, at] = ref
-            else:
-                ref = int(refs[b, at]) & REF_MASK
-                if ref == REF_MASK:
-                    errors.add("free pages")
+            at, ref = (h + i) // PAGE, REF_MASK
+            if h + i < room:
+                if at >= p:
+                    ref = mine[at - p] if at - p < len(mine) else REF_MASK
+                    if i == 0 or (h + i) % PAGE == 0:
+                        refs[b, at] = ref
+                else:
+                    ref = int(refs[b, at]) & REF_MASK
+                    if ref == REF_MASK:
+                        errors.add("free pages")
+                    ref = REF_MASK if many else ref
             slots[t] = NO_SLOT if ref == REF_MASK else ref * PAGE + (h + i) % PAGE
-            positions[t] = h + (i if tree is None else tree[i][1])
+            sees, depth = (0, i) if tree is None else tree[i] if i < len(tree) else (0, 0)
+            positions[t] = h + depth
             for w in range(words):
-                mask[t, w] = tree[i][0] >> (32 * w) & 0xFFFFFFFF
-            if tree is not None and int(parents[t]) >= i:
+                mask[t, w] = sees >> (32 * w) & 0xFFFFFFFF
+            if tree is not None and i < len(tree) and int(parents[t]) >= i:
                 errors.add("sequence length")
             t += 1
         got["seq_hot"][b], got["pages_out"][b] = h + n, p + len(mine)

@@ -197,3 +197,77 @@ def test_masks_in_place_where_pieces_of_two_waves_overlap(ops, engine, vocab, ha
     ops.adjust_logits(d)
     assert error_of(engine) == ""
     c.check(out=c.src)
+
+
+@pytest.mark.parametrize("tree", ["random", "chain", None])
+@pytest.mark.parametrize("what", ["full", "past", "nodes", "many_nodes", "held", "wrap"])
+def test_tables_of_a_sequence_past_its_table_leave_the_others(ops, engine, what, tree):
+    """What is wrong with one sequence moves no row of another: their offsets, slots, positions and masks are those beside a sequence
+    that fits."""
+    held, new = [3, 20, 0, 31, 7], [14, 40, 2, 9, 30]
+    words = 2
+    if what == "nodes":
+        words = 1
+    elif what == "many_nodes":
+        new[1] = 1400
+    c = Tables(30, held, new, tree=tree, pad=3, words=words)
+    good = c.want(held=np.array(held), words=words)
+    if what == "full":
+        held[1] = 16 * c.count - 7
+    elif what == "past":
+        held[1] = 16 * c.count
+    elif what == "held":
+        held[1] = 16 * c.count + 500
+    elif what == "wrap":
+        held[1] = 0xFFFFFFFF - 20
+    c.held = np.array(held)
+    c.pages = None
+    ops.page_tables(c.desc())
+    want, text = c.want(), error_of(engine)
+    fits = tree is None and what in ("nodes", "many_nodes") and new[1] + 20 <= 16 * c.count
+    assert want["errors"] == (set() if fits else {"sequence length"})
+    assert ("sequence length" in text) == (not fits) and "free pages" not in text
+    c.check(want, skip=("seq_hot", "pages_out", "positions") if what == "wrap" else ())
+    a, e = good["token_offsets"][1:3]
+    for name in ("positions", "tree_mask"):
+        if name in c.got:
+            got = host(c.got[name]).astype(np.int64) & 0xFFFFFFFF
+            assert np.array_equal(got[:a], good[name][:a]) and np.array_equal(got[e:], good[name][e:])
+    assert np.array_equal(host(c.got["token_offsets"]), good["token_offsets"])
+
+
+def test_generation_past_the_end_of_a_table(ops, engine):
+    """A sequence whose table is full keeps what fits and then nothing; the others go on as they do beside it."""
+    import torch
+    from test_gpu_step_run import HK, HQ, PAGES, Run
+    run = Run(64)
+    run.turn = torch.cat([run.turn, torch.ones((64, 1, 1), device="cuda:0")])  # positions behind the table's end
+    run.held[0] = 16 * PAGES - 5  # of pages that hold something: the whole table is its own
+    run.pages[0] = PAGES
+    run.refs[0] = torch.arange(PAGES, device="cuda:0", dtype=torch.int32) % 3 + run.blocks
+    for p in ("hot_k", "hot_v"):
+        pool = getattr(run, p)
+        setattr(run, p, torch.cat([pool, torch.zeros((2, 3) + tuple(pool.shape[2:]), dtype=pool.dtype, device="cuda:0")], 1).contiguous())
+    from aether_nexus_amd import ops as O
+    k, v = run.rows[:, :, HQ:HQ + HK], run.rows[:, :, HQ + HK:]
+    run.d_tree = [O.make_tree_desc(batch=4, num_tokens=run.rows.shape[1], q_heads=HQ, kv_heads=HK, head_dim=64, q=run.rows[l, :, :HQ], k=k[l], v=v[l],
+                                   out=run.out[l], hot_k=run.hot_k[l], hot_v=run.hot_v[l], refs=run.refs, hot_count=PAGES, seq_held=run.held,
+                                   token_offsets=run.offsets, tree_mask=run.mask) for l in range(2)]
+    run.d_accept = O.make_accept_desc(batch=4, num_tokens=run.rows.shape[1], layers=2, kv_heads=HK, head_dim=64, parents=run.parents,
+                                      node_tokens=run.nodes, targets=run.best, token_offsets=run.offsets, seq_held=run.held, slots=run.slots, k=k, v=v,
+                                      hot_k=run.hot_k, hot_v=run.hot_v, accepted=run.accepted, next_token=run.following, seq_hot=run.after,
+                                      path=run.path, history=run.history, history_count=run.count, history_count_out=run.count)
+    before = run.held.cpu().numpy().copy()
+    starts = [len(p) for p in run.prompts]
+    for i in range(10):
+        run.step(ops)
+        assert "sequence length" in error_of(engine)
+    held = run.held.cpu().numpy()
+    assert held[0] <= 16 * PAGES and (held[1:] > before[1:]).all()
+    count, history, refs = (x.cpu().numpy() for x in (run.count, run.history, run.refs))
+    for b in range(1, 4):
+        n = int(count[b])
+        assert n == held[b] and n > starts[b]
+        rows = (run.embed[:, torch.from_numpy(history[b, :n]).cuda().long()] * run.turn[:n]).half()
+        at = torch.from_numpy(refs[b, np.arange(n) // 16].astype(np.int64)).cuda(), torch.arange(n, device="cuda:0") % 16
+        assert torch.equal(run.hot_k[:, at[0], at[1]], rows[:, :, HQ:HQ + HK])

@@ -143,3 +143,19 @@ def test_acceptance_before_a_row_without_a_slot():
     targets, offsets = [6, 7, 8, 9, 4, 2], [0, 4, 6]
     assert S.accept_tree(parents, tokens, targets, offsets, [9, -1, 2, 3, 4, 5]) == [[0, 1, 2, 3], [0, 1]]
     assert S.accept_tree(parents, tokens, targets, offsets, [9, -1, S.NO_SLOT, 3, S.NO_SLOT, 5]) == [[0, 1], []]
+
+
+def test_tables_of_a_sequence_past_its_table_leave_the_others():
+    """The second of three sequences fits, is full, or has more nodes than the mask: the rows of the third are the same."""
+    parents = [-1, 0, 1, -1, 0, 0, -1, 0, 1]
+    args = dict(pages=None, free=np.arange(5, 20), first=0, rows=9, hot_count=3, parents=parents, words=1)
+    refs = np.arange(9).reshape(3, 3)
+    good, full = S.page_tables(refs, [4, 30, 16], [3, 3, 3], **args), S.page_tables(refs, [4, 47, 16], [3, 3, 3], **args)
+    assert not good["errors"] and full["errors"] == {"sequence length"}
+    for name in ("positions", "tree_mask"):
+        assert np.array_equal(good[name][6:], full[name][6:])
+    assert full["token_offsets"].tolist() == [0, 3, 6, 9] and full["slots"][3] >= 0 and (full["slots"][4:6] == S.NO_SLOT).all()
+    assert (full["slots"][6:] % 16 == good["slots"][6:] % 16).all() and full["pages_out"].tolist() == [1, 3, 2]
+    wide = S.page_tables(refs, [4, 30, 16], [3, 40, 3], **{**args, "rows": 46, "parents": parents[:3] + [-1] * 40 + parents[6:]})
+    assert wide["errors"] == {"sequence length"} and (wide["slots"][3:43] == S.NO_SLOT).all() and not wide["tree_mask"][35:43].any()
+    assert wide["pages_out"].tolist() == [1, 2, 2] and np.array_equal(wide["tree_mask"][43:], good["tree_mask"][6:])
