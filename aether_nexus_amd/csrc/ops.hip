@@ -566,13 +566,16 @@ int accept_args(const aw_accept_desc* d, awo::AcceptArgs* a, char* msg, size_t l
         hv = {d->hot_v, pool};
     }
     const uint64_t hist = b * d->history_stride;
-    const Span out[] = {hk, hv, {d->accepted, b}, {d->next_token, b}, {d->seq_hot, b}, {d->path, 4 * t}, {d->history, hist}, {d->history_count_out, b}};
+    const Span out[] = {hk, {d->accepted, b}, {d->next_token, b}, {d->seq_hot, b}, {d->path, 4 * t}, {d->history, hist}, {d->history_count_out, b}};
+    const Span rest[] = {hv, out[1], out[2], out[3], out[4], out[5], out[6]}; // the pools' layers may lie between each other's
     const Span in[] = {k, v, {d->parents, 4 * t}, {d->node_tokens, 4 * t}, {d->targets, 4 * t}, {d->token_offsets, b + 4},
                        {d->seq_held == d->seq_hot ? nullptr : d->seq_held, b}, {d->slots, 8 * t},
                        {d->history_count == d->history_count_out ? nullptr : d->history_count, b}};
-    if (outputs_meet(out, in)) return bad("an output overlaps an input or another output");
+    const uint64_t layer = d->hot_blocks * awo::kPageTokens * row;
+    if (outputs_meet(out, in) || outputs_meet(rest, in) || (d->layers && rows_meet({d->hot_k, hl, layer, d->layers}, {d->hot_v, hl, layer, d->layers})))
+        return bad("an output overlaps an input or another output");
     // The two inputs that an output may be are nobody else's.
-    for (const Span& o : out)
+    for (const Span& o : {hk, hv, out[1], out[2], out[3], out[4], out[5], out[6]})
         if ((o.at != d->seq_hot && spans_meet(o, {d->seq_held, b})) || (o.at != d->history_count_out && spans_meet(o, {d->history_count, b})))
             return bad("an output overlaps an input or another output");
     *a = awo::AcceptArgs{};

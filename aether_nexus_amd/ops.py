@@ -470,7 +470,8 @@ def _layer_rows(t, layers: int, tokens: int, heads: int, head_dim: int, what: st
 
 def _pool(t, layers: int, heads: int, head_dim: int, blocks: Optional[int], what: str) -> tuple:
     """(blocks of a layer, elements from layer to layer) of a pool [layers][blocks][16][heads][head_dim], of at least as many
-    layers and blocks; a flat tensor or a raw pointer is taken for just that."""
+    layers and blocks, whose layers may lie apart (those of K and V in one buffer); a flat tensor or a raw pointer is taken
+    for just that."""
     page = BLOCK_SIZE * heads * head_dim
     if t is None or isinstance(t, int) or not hasattr(t, "dim") or t.dim() < 5 or layers == 0:
         if blocks is None:
@@ -483,11 +484,12 @@ def _pool(t, layers: int, heads: int, head_dim: int, blocks: Optional[int], what
         return blocks, blocks * page
     if blocks is None:
         blocks = t.shape[1]
-    if tuple(t.shape[-3:]) != (BLOCK_SIZE, heads, head_dim) or t.dim() > 5 or t.shape[0] < layers or t.shape[1] < blocks:
-        raise WeaverError(f"{what}: a pool must be [{layers}][{blocks}][{BLOCK_SIZE}][{heads}][{head_dim}], got shape {tuple(t.shape)}",
-                          AW_E_INVALID_ARG)
-    _f16(t, 0, what)
-    return blocks, t.shape[1] * page
+    if tuple(t.shape[-3:]) != (BLOCK_SIZE, heads, head_dim) or t.dim() > 5 or t.shape[0] < layers or t.shape[1] < blocks or \
+            not t[0].is_contiguous() or (layers > 1 and t.stride(0) < t.shape[1] * page):
+        raise WeaverError(f"{what}: a pool must be [{layers}][{blocks}][{BLOCK_SIZE}][{heads}][{head_dim}], its layers whole and apart, got "
+                          f"shape {tuple(t.shape)}, strides {tuple(t.stride())}", AW_E_INVALID_ARG)
+    _f16(t if t.is_contiguous() else t[:0].contiguous(), 0, what)
+    return blocks, t.stride(0) if layers > 1 else t.shape[1] * page
 
 
 def make_accept_desc(*, batch: int, num_tokens: int, parents, node_tokens, targets, seq_held, accepted, next_token, seq_hot, path,

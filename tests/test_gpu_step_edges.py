@@ -271,3 +271,14 @@ def test_generation_past_the_end_of_a_table(ops, engine):
         rows = (run.embed[:, torch.from_numpy(history[b, :n]).cuda().long()] * run.turn[:n]).half()
         at = torch.from_numpy(refs[b, np.arange(n) // 16].astype(np.int64)).cuda(), torch.arange(n, device="cuda:0") % 16
         assert torch.equal(run.hot_k[:, at[0], at[1]], rows[:, :, HQ:HQ + HK])
+
+
+def test_accept_into_pools_of_one_buffer(ops, engine):
+    """K and V pages of a layer side by side."""
+    import torch
+    c = Accept(31, [7, 12, 1], layers=3, agree=1.0)
+    both = torch.stack([dev(c.pool), dev(-c.pool)], 1).contiguous()
+    ops.accept_tree(c.desc(hot_k=both[:, 0], hot_v=both[:, 1]))
+    assert error_of(engine) == ""
+    c.hot_k, c.hot_v = both[:, 0].contiguous(), both[:, 1].contiguous()
+    c.check()

@@ -7,7 +7,7 @@ import torch
 from aether_nexus_amd import ops as O
 from aether_nexus_amd.types import AW_E_INVALID_ARG, AW_E_UNSUPPORTED
 from aether_nexus_amd.weaver import WeaverError
-from test_step import A, tree
+from test_step import A, accept, check, tree
 
 
 @pytest.mark.parametrize("kw", [dict(v_stride=257), dict(v_stride=8), dict(v_stride=1 << 40), dict(k_stride=1536, k=A["q"] + 2 * 1024, q_stride=1536)])
@@ -140,8 +140,7 @@ def test_pools_of_more_layers_or_blocks(on_cpu):
 @pytest.mark.parametrize("kw", [
     dict(hot_k=f16(2, 30, 16, 2, 64)), dict(hot_k=f16(3, 9, 16, 3, 64)), dict(hot_k=f16(3, 9, 16, 1, 128)), dict(hot_k=f16(27, 16, 4, 32)),
     dict(hot_k=f16(3, 9, 16, 2, 64), hot_blocks=10), dict(hot_k=f16(3, 9, 16, 2, 64), hot_v=f16(3, 8, 16, 2, 64)),
-    dict(hot_k=f16(3, 9, 16, 2, 64), hot_v=f16(3, 10, 16, 2, 64)), dict(hot_k=f16(3 * 9 * 16 * 128 - 1), hot_blocks=9),
-    dict(hot_k=f16(3, 12, 16, 2, 64)[:, :9])], ids=lambda d: None)
+    dict(hot_k=f16(3, 9, 16, 2, 64), hot_v=f16(3, 10, 16, 2, 64)), dict(hot_k=f16(3 * 9 * 16 * 128 - 1), hot_blocks=9)], ids=lambda d: None)
 def test_pools_of_other_pages_are_refused(on_cpu, kw):
     rows = f16(3, 6, 2, 64)
     refused(accept_of, **{**dict(k=rows, v=rows, hot_v=kw["hot_k"], hot_blocks=None), **kw})
@@ -174,3 +173,24 @@ def test_tree_plan_of_equal_parts():
     assert e.value.status == AW_E_UNSUPPORTED
     few = dict(batch=64, num_tokens=512, tree_mask=0, mask_words=0, q_heads=8, kv_heads=2)  # 8 nodes each behind up to 48 tokens
     assert O.tree_plan(tree(**few, token_offsets=0)).workspace_bytes == 0
+
+
+def test_pools_whose_layers_lie_between_each_other():
+    """K and V of a layer side by side in one buffer: no element of one is the other's."""
+    layer = 50 * 16 * 128
+    assert check(accept(hot_layer_stride=2 * layer, hot_v=A["hot_k"] + 2 * layer)) == (0, "")
+    assert check(accept(hot_layer_stride=3 * layer, hot_v=A["hot_k"] + 4 * layer)) == (0, "")
+    for kw in (dict(hot_v=A["hot_k"]), dict(hot_v=A["hot_k"] + 2 * layer - 2), dict(hot_v=A["hot_k"] + 2 * layer + 2), dict(hot_v=A["hot_k"] + 4 * layer),
+               dict(hot_v=A["hot_k"] + 2 * layer, path=A["hot_k"] + 2 * layer), dict(hot_v=A["hot_k"] + 2 * layer, k=A["hot_k"] + 6 * layer)):
+        rc, msg = check(accept(hot_layer_stride=2 * layer, **kw))
+        assert rc == AW_E_INVALID_ARG and "overlap" in msg
+
+
+def test_pools_in_one_buffer(on_cpu):
+    rows, both = f16(3, 6, 2, 64), f16(3, 2, 9, 16, 2, 64)
+    d = accept_of(k=rows, v=rows, hot_k=both[:, 0], hot_v=both[:, 1], hot_blocks=None)
+    assert (d.hot_blocks, d.hot_layer_stride) == (9, 2 * 9 * 16 * 128)
+    d = accept_of(k=rows, v=rows, hot_k=both[:, 0, :5], hot_v=both[:, 1, :5], hot_blocks=None)
+    assert (d.hot_blocks, d.hot_layer_stride) == (5, 2 * 9 * 16 * 128)
+    for pool in (both[:, 0, ::2], both[:1, 0].expand(3, 9, 16, 2, 64), f16(3, 9, 16, 2, 128)[..., ::2], f16(3, 9, 32, 2, 64)[:, :, ::2]):
+        refused(accept_of, k=rows, v=rows, hot_k=pool, hot_v=pool, hot_blocks=None)
