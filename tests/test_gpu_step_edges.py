@@ -282,3 +282,61 @@ def test_accept_into_pools_of_one_buffer(ops, engine):
     assert error_of(engine) == ""
     c.hot_k, c.hot_v = both[:, 0].contiguous(), both[:, 1].contiguous()
     c.check()
+
+
+def test_capture_refuses_workspace_growth():
+    """A captured call whose scratch does not fit yet is refused before anything is enqueued; after an eager one it is captured."""
+    import torch
+    from aether_nexus_amd.ops import OpsEngine
+    from aether_nexus_amd.types import AW_E_UNSUPPORTED
+    from aether_nexus_amd.weaver import WeaverError
+    from test_gpu_tree import Case
+    logits, tree = Logits(32, 40001, [3, 5], history=50, bias=5, allowed=0.5), Case(33, 8, 2, 64, [5, 80], [3000, 30])  # in several parts
+    for call, c, d in (("adjust_logits", logits, logits.desc()), ("tree_attention", tree, tree.desc())):
+        fresh = OpsEngine()
+        try:
+            s = torch.cuda.Stream()
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                g = torch.cuda.CUDAGraph()
+                with pytest.raises(WeaverError) as e:
+                    with torch.cuda.graph(g, stream=s):
+                        getattr(fresh, call)(d)
+                assert e.value.status == AW_E_UNSUPPORTED and "eager" in str(e.value)
+                del g
+                torch.cuda.synchronize()
+                assert bool((c.out == 7.0).all())
+                getattr(fresh, call)(d)
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g, stream=s):
+                    getattr(fresh, call)(d)
+                for _ in range(3):
+                    c.out.fill_(7.0)
+                    g.replay()
+                    s.synchronize()
+                    c.check(*(["captured"] if call == "tree_attention" else []))
+                del g
+            torch.cuda.synchronize()
+        finally:
+            fresh.close()
+
+
+def test_logits_past_32_bits(ops, engine):
+    """Rows whose elements lie past 2^32 of the tensor, in place, with masks by a row of their own and tokens of their sequences."""
+    import torch
+    from aether_nexus_amd import ops as O
+    vocab, rows = 128256, (1 << 32) // 128256 + 40
+    x = torch.zeros((rows, vocab), dtype=torch.float16, device="cuda:0")
+    c = Logits(33, vocab, [1, 8], half=True, history=40, bias=6, nodes=False)
+    c.kw["offsets"] = [0, rows - 8, rows]
+    x[-8:] = torch.from_numpy(c.x[-8:]).cuda()
+    best = empty(rows)
+    names = {"offsets": "token_offsets"}
+    d = O.make_logits_desc(num_tokens=rows, vocab_size=vocab, batch=2, logits=x, out=x, best=best,
+                           **{names.get(k, k): dev(np.asarray(v)) for k, v in c.kw.items()})
+    ops.adjust_logits(d)
+    assert error_of(engine) == ""
+    second = {k: np.asarray(v)[1:2] for k, v in c.kw.items() if k != "offsets"}
+    want, top = S.adjust_logits(c.x[-8:], offsets=[0, 8], **second)
+    assert np.array_equal(host(x[-8:]), want.astype(np.float16)) and host(best)[-8:].tolist() == top.tolist()
+    assert bool((best[:-8] == best[0]).all()) and bool((x[0] == x[rows - 9]).all())
