@@ -616,7 +616,8 @@ int launch_logits(aw_engine* e, awo::LogitsArgs& a, hipStream_t st) {
     const bool words = a.history || a.node_tokens || a.bias_ids;
     a.slices = (uint32_t)cdiv64(a.vocab, slice);
     // Rows of a work-group: a sequence's counts serve several, where that leaves 8 work-groups a
-    // CU.  544 rows x 49155 of 32 sequences, groups of 1, 2, 4, 16: 51.9, 48.3, 54.4, 86 us.
+    // CU.  526 rows x 49155 f16 of 16 sequences, groups of 1, 2, 3 (taken), 4, 16: 47.4, 44.2, 43.8, 46.8,
+    // 78.6 us; 64 rows x 128256 f32 of 64 sequences, whose rows share nothing, 1 (taken), 2, 4: 26.5, 26.8, 37.3.
     a.group = words ? (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(16, (uint64_t)a.rows * a.slices / (8ull * ei::compute_units(e)))) : 1u;
     const uint64_t grid = cdiv64(a.rows, a.group) * a.slices;
     if (grid > 0xFFFFFFull) return ei::fail(e, AW_E_UNSUPPORTED, "adjust_logits: too many rows"); // 256 threads each, below 2^32

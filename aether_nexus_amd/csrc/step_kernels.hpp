@@ -76,7 +76,7 @@ __device__ inline uint32_t capped_scan(uint32_t& x, uint32_t cap, uint32_t* s_wa
 // seq_new whatever its table holds, so one that is past it moves no other's.  The first work-group
 // writes what belongs to sequences.  A node's ancestors are walked in LDS.
 // Bound: a launch and the chain lengths -> sums -> search -> page -> slot: 64 sequences of
-// one new token 4.6 us, 256 trees of up to 48 nodes 6.2, 260000 rows of 509 prompts 6.8.
+// one new token 4.8 us, 256 trees of up to 48 nodes 6.4, 260000 rows of 509 prompts 6.9.
 constexpr uint32_t kTablesRows = 256, kTablesSeqs = 1024;
 
 template <bool TREE>
@@ -319,11 +319,11 @@ __device__ inline SeqAt seq_at(const uint32_t* offsets, uint32_t tokens, uint32_
 // first 2048 tokens of the history and the biases are asked for before their counts are known
 // (history_stride and bias_stride entries are there whatever the counts), so a work-group
 // waits for memory two or three times.
-// Bound: HBM, each logit read and written once: 544 x 49155 f16 without words 18.3 us
-// (5.8 TB/s), with the best 21.3.  With words the vector unit is busy 60 % of the time:
-// 47.3 us with histories of 2048 tokens, tree nodes, a grammar and the best (44 to 51 as
-// one of them is left out: no part alone is what it waits for); 64 x 128256 f32 with
-// histories of 4096 and 300 biases 25.8 us, 2.6 TB/s.
+// Bound: HBM, each logit read and written once: 526 x 49155 f16 that no cache holds, without
+// words, 25 us with the best (4.1 TB/s), 27 with a grammar, 31 with both.  With words the vector
+// unit is busy 60 % of the time: 47 us with histories of 2048 tokens, the nodes of 16 trees, a
+// grammar and the best (no part alone is what it waits for); 64 x 128256 f32 with histories of
+// 4096 and 300 biases 25.7 us, 2.6 TB/s.
 template <typename T, int IT, bool WORDS>
 __global__ __launch_bounds__(256) void logits_kernel(LogitsArgs a) {
     typedef typename LogitsVec<T>::type vec_t;
@@ -586,7 +586,7 @@ struct AcceptArgs {
 // those that continue the kept node with its target's token, the lowest of them) and moves
 // its layer's rows; the first layer's writes what belongs to the sequence.  VEC: rows in
 // 16-byte pieces.  Bound: the chain offsets -> nodes -> walk -> rows, 2 sequences of 24 layers
-// 4.4 us; with many layers HBM, 64 sequences of 32 layers of 8 x 128 10.5 us.
+// 4.6 us; 64 sequences of 32 layers of 8 x 128 10.6, 43 MB of rows (4 TB/s) behind the same chain.
 template <bool VEC>
 __global__ __launch_bounds__(256) void accept_kernel(AcceptArgs a) {
     __shared__ int32_t s_parent[kMaxNodes], s_path[kMaxNodes];

@@ -51,7 +51,10 @@ __device__ inline TreeSeq tree_seq(const TreeArgs& a, uint32_t b, bool report) {
 
 // ---- 16 NR query rows of a kv head: a work-group's waves take the pages (then the nodes, 16
 // at a time) in turn, each on its own until their sums meet in LDS.  Products, layouts and
-// the softmax are PrefixPages'; K and V pages are loaded one and a half to two pages ahead.
+// the softmax are PrefixPages' (weights are f16 operands of the second product, their sums
+// fp32: 2.5 to 2.8e-4 of the outputs against 64 bits, where the f16 store alone has
+// 2.1e-4; operands of more bits would double those products); K and V pages are loaded one and a
+// half to two pages ahead.
 constexpr int kTreeBufs = 5; // pages of K or of V in LDS, a wave
 constexpr size_t tree_pages_lds(int HD, int NW, int NR) {
     const size_t ring = (size_t)NW * kTreeBufs * 16 * HD * 2, sums = (size_t)NW * 16 * NR * (HD + 4) * 4 + NW * 16 * NR * 2 * 4;
@@ -455,7 +458,9 @@ __device__ inline uint32_t lanes_scan(uint32_t x) {
 // unit that begins here and is cut, 2 w for one that began before.
 // Bound: with few rows HBM (64 sequences x 8 nodes x 32 / 8 heads x 128 behind 4099 tokens, 32-row
 // units: 175 us, 4.65 TB/s, and the merge), with many a wave's chain of products, softmax, products (16 x
-// 64 nodes behind 8192, 128-row units: 127 us, 370 TFLOP/s).  Two work-groups a CU, whose
+// 64 nodes behind 8192, 128-row units: 127 us, 370 TFLOP/s, where 2104 of 3072 tile rows are
+// real, sequences of two tiles read K and V twice, 549 MB for 403, and the steps that test each
+// load, the last ones of each piece and the nodes', are 19 % of all).  Two work-groups a CU, whose
 // chains overlap: one takes 10 to 20 % longer.  Nothing may spill in the steps: a
 // reload waits for all loads in flight, those into LDS too (227 for 193 us, 173 for 142).
 template <int HD, int NR>
@@ -614,7 +619,7 @@ __global__ __launch_bounds__(kPrefixThreads) __attribute__((amdgpu_waves_per_eu(
 // each work-group sums up itself; the grid has one more for each sequence's last, partial 16 rows
 // than all rows fill, so the host need not know the lengths.  Bound: the chain offsets, lengths, refs, pages (a
 // round trip each), then the waves' sums: 2 sequences x 5 nodes x 14 / 2 heads x 64 behind 700
-// tokens 9.6 us, with 16 waves 3 pages of each.  As many waves as LDS holds where the work-groups
+// tokens 9.8 us, with 16 waves 3 pages of each.  As many waves as LDS holds where the work-groups
 // are no more than the CUs, else 4.
 template <int HD, int NW>
 __global__ __launch_bounds__(NW * 64) void tree_pages_kernel(TreeArgs a) {
