@@ -429,7 +429,8 @@ int tables_args(const aw_tables_desc* d, awo::TablesArgs* a, char* msg, size_t l
         return refuse(msg, len, AW_E_INVALID_ARG, "page_tables: refs_stride %u < hot_count %u", d->refs_stride, d->hot_count);
     if (d->free_count > 1u << 30) return refuse(msg, len, AW_E_UNSUPPORTED, "page_tables: free_count %u exceeds 2^30", d->free_count);
     if (d->mask_words > AW_MAX_NODES / 32) return refuse(msg, len, AW_E_UNSUPPORTED, "page_tables: mask_words %u exceeds 32", d->mask_words);
-    if (!d->parents != !d->mask_words || !d->parents != !d->tree_mask) return bad("parents, mask_words and tree_mask go together");
+    // Rows (and below lists) of no elements have no address.
+    if (d->num_tokens && (!d->parents != !d->mask_words || !d->parents != !d->tree_mask)) return bad("parents, mask_words and tree_mask go together");
     if (!d->token_offsets || (d->batch && (!d->seq_held || !d->seq_new || !d->seq_hot || (d->hot_count && !d->refs))) ||
         (d->free_count && !d->free_pages))
         return bad("null pointer");
@@ -475,16 +476,16 @@ int logits_args(const aw_logits_desc* d, awo::LogitsArgs* a, char* msg, size_t l
     if (d->history_stride > 1u << 20) return over("history_stride exceeds 2^20");
     if (d->bias_stride > 1023) return over("bias_stride exceeds 1023");
     if (d->mask_words > AW_MAX_NODES / 32) return over("mask_words exceeds 32");
-    if (!d->out && !d->best) return bad("neither out nor best is asked for");
+    if (!d->out && !d->best && d->num_tokens) return bad("neither out nor best is asked for");
     if (!d->logits && d->num_tokens) return bad("null pointer");
     if ((d->history || d->repetition || d->frequency || d->presence || d->bias_ids || d->node_tokens || d->token_offsets) && !d->batch &&
         d->num_tokens)
         return bad("batch is 0");
     if (d->history && !d->history_count) return bad("history needs history_count");
-    if (d->prompt_count && !d->history) return bad("prompt_count without history");
-    if (!d->node_tokens != !d->tree_mask || !d->node_tokens != !d->mask_words) return bad("node_tokens, tree_mask and mask_words go together");
-    if (!d->bias_ids != !d->bias_values || (d->bias_count && !d->bias_ids)) return bad("bias_ids and bias_values go together");
-    if (d->allowed_index && !d->allowed) return bad("allowed_index without allowed");
+    if (d->prompt_count && !d->history && d->history_stride) return bad("prompt_count without history");
+    if (d->num_tokens && (!d->node_tokens != !d->tree_mask || !d->node_tokens != !d->mask_words)) return bad("node_tokens, tree_mask and mask_words go together");
+    if (d->bias_stride && (!d->bias_ids != !d->bias_values || (d->bias_count && !d->bias_ids))) return bad("bias_ids and bias_values go together");
+    if (d->allowed_index && !d->allowed && d->allowed_rows) return bad("allowed_index without allowed");
     const uint32_t size = d->flags & AW_LOGITS_F16 ? 2u : 4u;
     const uint64_t words = cdiv64(d->vocab_size, 32);
     const uint64_t stride = d->logits_stride ? d->logits_stride : d->vocab_size, out_stride = d->out_stride ? d->out_stride : d->vocab_size;
@@ -554,7 +555,7 @@ int accept_args(const aw_accept_desc* d, awo::AcceptArgs* a, char* msg, size_t l
         if (row == 0) return bad("kv_heads or head_dim is 0");
         if (row > 1u << 20) return over("a token's row exceeds 2^20 values");
         if (t && (!d->k || !d->hot_k || !d->slots)) return bad("null pointer");
-        if (!d->v != !d->hot_v) return bad("v and hot_v go together");
+        if (t && !d->v != !d->hot_v) return bad("v and hot_v go together");
         if (d->hot_blocks == 0) return bad("hot_blocks is 0");
         if (d->hot_blocks > 1ull << 31) return bad("hot_blocks exceeds 2^31, the refs' range");
         if (ks < row || vs < row || (d->layers > 1 && hl < d->hot_blocks * awo::kPageTokens * row)) return bad("a stride is shorter than what it steps over");

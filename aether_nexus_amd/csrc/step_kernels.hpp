@@ -441,7 +441,8 @@ __global__ __launch_bounds__(256) void logits_kernel(LogitsArgs a) {
         uint32_t may[IT];
         {
             int32_t at = -1;
-            if (a.allowed) at = a.allowed_index ? a.allowed_index[r] : (int32_t)r;
+            if (a.allowed_index) at = a.allowed_index[r];
+            else if (a.allowed) at = (int32_t)r;
             const bool nothing = at >= 0 && (uint32_t)at >= a.allowed_rows;
             if (nothing && tid == 0) flag(a.err, kErrToken);
             const char* bits = (const char*)(a.allowed + (uint64_t)(uint32_t)at * a.allowed_stride + v0 / 32u);

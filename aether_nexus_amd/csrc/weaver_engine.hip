@@ -1205,7 +1205,7 @@ int tree_plan(const aw_tree_desc* d, uint32_t n_cu, aw::TreeArgs* out, aw_tree_p
     if (d->hot_count > 1u << 18) return refuse(AW_E_UNSUPPORTED, "too many tokens");
     if (d->refs_stride < d->hot_count) return refuse(AW_E_INVALID_ARG, "refs_stride is less than hot_count");
     if (d->mask_words > 32u) return refuse(AW_E_UNSUPPORTED, "mask_words exceeds 32");
-    if (!d->tree_mask != !d->mask_words) return refuse(AW_E_INVALID_ARG, "tree_mask and mask_words go together");
+    if (d->num_tokens && !d->tree_mask != !d->mask_words) return refuse(AW_E_INVALID_ARG, "tree_mask and mask_words go together");
     const uint64_t gqa = d->q_heads / d->kv_heads, n = d->num_tokens;
     if (n > 1u << 24 || gqa > 1u << 16 || n * d->q_heads > 1u << 25) return refuse(AW_E_UNSUPPORTED, "too many query rows");
     if ((uint64_t)d->kv_heads * d->head_dim > 1u << 16) return refuse(AW_E_UNSUPPORTED, "too many kv heads");

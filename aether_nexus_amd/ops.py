@@ -422,6 +422,8 @@ def make_logits_desc(*, num_tokens: int, vocab_size: int, logits, out=None, best
     states = allowed_rows if allowed_rows is not None else 0 if allowed is None else allowed.shape[0] if hasattr(allowed, "shape") else None
     if states is None:
         raise WeaverError("adjust_logits: allowed_rows is required for a raw pointer", AW_E_INVALID_ARG)
+    if allowed is not None and allowed_index is None and states < num_tokens:
+        raise WeaverError(f"adjust_logits: {states} allowed rows for {num_tokens} rows without allowed_index", AW_E_INVALID_ARG)
     _counts(num_tokens=num_tokens, vocab_size=vocab_size, batch=batch, mask_words=words, history_stride=past, bias_stride=biases,
             allowed_rows=states)
     d.num_tokens, d.vocab_size, d.batch, d.flags = num_tokens, vocab_size, batch, AW_LOGITS_F16 if half else 0
@@ -450,7 +452,7 @@ def _layer_rows(t, layers: int, tokens: int, heads: int, head_dim: int, what: st
     tensor's own, with contiguous heads, of at least as many layers and tokens.  [layers][tokens][row] and, of one layer or
     of layers one after another, [tokens][heads][head_dim] and [tokens][row] are taken too."""
     row = heads * head_dim
-    if t is None or isinstance(t, int) or not hasattr(t, "dim") or t.dim() < 2 or layers == 0:
+    if t is None or isinstance(t, int) or not hasattr(t, "dim") or t.dim() < 2 or layers == 0 or tokens == 0:
         _f16(t, layers * tokens * row, what)
         return 0, 0
     shape, strides, whole = tuple(t.shape), t.stride(), t.is_contiguous()

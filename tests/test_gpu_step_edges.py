@@ -340,3 +340,37 @@ def test_logits_past_32_bits(ops, engine):
     want, top = S.adjust_logits(c.x[-8:], offsets=[0, 8], **second)
     assert np.array_equal(host(x[-8:]), want.astype(np.float16)) and host(best)[-8:].tolist() == top.tolist()
     assert bool((best[:-8] == best[0]).all()) and bool((x[0] == x[rows - 9]).all())
+
+
+def test_a_step_of_no_rows(ops, engine):
+    """A batch without a new token: what belongs to sequences is written, nothing else is touched."""
+    import torch
+    from aether_nexus_amd import ops as O
+    c = Tables(34, [5, 16], [0, 0], tree="chain")
+    ops.page_tables(c.desc())
+    assert error_of(engine) == ""
+    c.check(c.want())
+    f16 = lambda *shape: torch.empty(shape, dtype=torch.float16, device="cuda:0")
+    offsets = dev(np.array([0, 0, 0]))
+    ops.tree_attention(O.make_tree_desc(batch=2, num_tokens=0, q_heads=4, kv_heads=2, head_dim=64, q=f16(0, 4, 64), k=f16(0, 2, 64), v=f16(0, 2, 64),
+                                        out=f16(0, 4, 64), token_offsets=offsets, tree_mask=empty(0, 2)))
+    ops.adjust_logits(O.make_logits_desc(num_tokens=0, vocab_size=50, logits=f16(0, 50), out=f16(0, 50), best=empty(0), batch=2, token_offsets=offsets,
+                                         node_tokens=empty(0), tree_mask=empty(0, 2)))
+    a = Accept(35, [0, 0])
+    ops.accept_tree(a.desc())
+    assert error_of(engine) == ""
+    a.check()
+
+
+def test_logits_of_an_empty_grammar(ops, engine):
+    """A table of no states with an index: none for -1, and a state that is not there allows nothing."""
+    import torch
+    c = Logits(36, 300, [3, 2], history=9)
+    c.kw.update(allowed=np.zeros((0, 10), dtype=np.uint32), allowed_index=np.full(5, -1))
+    ops.adjust_logits(c.desc())
+    assert error_of(engine) == ""
+    c.check()
+    c.kw["allowed_index"][2] = 0
+    ops.adjust_logits(c.desc())
+    assert "token id" in error_of(engine)
+    c.check()

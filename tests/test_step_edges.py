@@ -194,3 +194,30 @@ def test_pools_in_one_buffer(on_cpu):
     assert (d.hot_blocks, d.hot_layer_stride) == (5, 2 * 9 * 16 * 128)
     for pool in (both[:, 0, ::2], both[:1, 0].expand(3, 9, 16, 2, 64), f16(3, 9, 16, 2, 128)[..., ::2], f16(3, 9, 32, 2, 64)[:, :, ::2]):
         refused(accept_of, k=rows, v=rows, hot_k=pool, hot_v=pool, hot_blocks=None)
+
+
+def test_steps_of_no_rows_take_empty_tensors(on_cpu):
+    """A batch without a new token, whose tensors of no elements have no address."""
+    d = O.make_tables_desc(batch=2, num_tokens=0, seq_held=i32(2), seq_new=i32(2), refs=i32(2, 3), seq_hot=i32(2), token_offsets=i32(3),
+                           parents=i32(0), tree_mask=i32(0, 2), slots=torch.zeros(0, dtype=torch.int64), positions=i32(0))
+    assert check(d) == (0, "")
+    d = O.make_tree_desc(batch=2, num_tokens=0, q_heads=4, kv_heads=2, head_dim=64, q=f16(0, 4, 64), k=f16(0, 2, 64), v=f16(0, 2, 64),
+                         out=f16(0, 4, 64), token_offsets=i32(3), tree_mask=i32(0, 2))
+    O.tree_plan(d)
+    none = dict(rows=0, logits=torch.zeros(0, 1000), best=i32(0), out=torch.zeros(0, 1000), batch=2, token_offsets=i32(3))
+    assert check(logits_of(**none)) == (0, "")
+    assert check(logits_of(**none, node_tokens=i32(0), tree_mask=i32(0, 2), allowed=i32(3, 32), allowed_index=i32(0))) == (0, "")
+    own = {n: i32(2) for n in ("seq_held", "accepted", "next_token", "seq_hot")}
+    d = O.make_accept_desc(batch=2, num_tokens=0, layers=3, kv_heads=2, head_dim=64, parents=i32(0), node_tokens=i32(0), targets=i32(0), path=i32(0),
+                           token_offsets=i32(3), slots=torch.zeros(0, dtype=torch.int64), k=torch.empty_strided((3, 0, 2, 64), (0, 0, 0, 0), dtype=torch.float16), v=f16(3, 0, 2, 64),
+                           hot_k=f16(3, 9, 16, 2, 64), hot_v=f16(3, 9, 16, 2, 64), **own)
+    assert check(d) == (0, "")
+
+
+def test_lists_of_no_entries_take_empty_tensors(on_cpu):
+    """No history, biases or grammar states yet: the counts beside them and an index of -1 stay."""
+    own = dict(batch=2, token_offsets=i32(3))
+    assert check(logits_of(**own, history=i32(2, 0), history_count=i32(2), prompt_count=i32(2))) == (0, "")
+    assert check(logits_of(**own, bias_ids=i32(2, 0), bias_values=torch.zeros(2, 0), bias_count=i32(2))) == (0, "")
+    assert check(logits_of(**own, allowed=i32(0, 32), allowed_index=i32(3))) == (0, "")
+    assert "allowed" in refused(logits_of, **own, allowed=i32(0, 32))
