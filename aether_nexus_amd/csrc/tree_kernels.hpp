@@ -458,8 +458,8 @@ __device__ inline uint32_t lanes_scan(uint32_t x) {
 // unit that begins here and is cut, 2 w for one that began before.
 // Bound: with few rows HBM (64 sequences x 8 nodes x 32 / 8 heads x 128 behind 4099 tokens, 32-row
 // units: 175 us, 4.65 TB/s, and the merge), with many a wave's chain of products, softmax, products (16 x
-// 64 nodes behind 8192, 128-row units: 127 us, 370 TFLOP/s, where 2104 of 3072 tile rows are
-// real, sequences of two tiles read K and V twice, 549 MB for 403, and the steps that test each
+// 64 nodes behind 8192, 128-row units: 127 us, 370 TFLOP/s, where 24 tiles a kv head hold
+// 2104 rows, sequences of two tiles read K and V twice, 549 MB for 403, and the steps that test each
 // load, the last ones of each piece and the nodes', are 19 % of all).  Two work-groups a CU, whose
 // chains overlap: one takes 10 to 20 % longer.  Nothing may spill in the steps: a
 // reload waits for all loads in flight, those into LDS too (227 for 193 us, 173 for 142).

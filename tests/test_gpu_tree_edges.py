@@ -111,3 +111,43 @@ def test_steps_just_past_32_bits_by_bad_offsets(ops, engine):
     ops.tree_attention(d)
     assert "sequence length" in error_of(engine)
     assert bool((out == 7.0).all())
+
+
+@pytest.mark.parametrize("way", SPLITS, ids=IDS)
+def test_bad_refs_and_unseen_infinities_in_each_split(ops, engine, way):
+    """Bad refs hide their pages, whatever lies in the page that is read in their place; NaN and infinities of nodes reach the rows that
+    see them alone."""
+    hq, hk, hd, nodes, held, spare, tile = way
+    c = Case(42, hq, hk, hd, nodes, held, pad=1, spare=spare, qscale=1.0)
+    # Page 0, which is read for a bad ref, holds no token and NaN and inf alone.
+    free = [p for p in range(c.blocks) if p not in set((c.refs & 0x7FFFFFFF).ravel().tolist())][0]
+    moved = (c.refs & 0x7FFFFFFF) == 0
+    c.refs[moved] = c.refs[moved] & (1 << 31) | free
+    for p in (c.hot_k, c.hot_v):
+        p[free] = p[0]
+        p[0] = np.inf
+        p[0, ::2] = np.nan
+    longest = int(np.argmax(held))
+    pages = -(-held[longest] // 16)
+    c.refs[longest, [0, pages // 2, pages - 1]] = c.blocks, 0x7FFFFFFF, c.blocks + 7
+    # A node of the widest tree that only the last row sees, and one that none sees.
+    wide = int(np.argmax(nodes))
+    first, last = c.offsets[wide], c.offsets[wide + 1] - 1
+    c.mask[first:last, 0] &= ~np.uint32(1 << 1)
+    c.mask[last, 0] |= 1 << 1
+    c.v[first + 1, 0, 5] = np.inf
+    d = c.desc()
+    assert plan_of(d) == tile
+    ops.tree_attention(d)
+    assert "hot block ref" in error_of(engine)
+    got = host(c.out)[:c.offsets[-1]].astype(np.float64)
+    heads = range(hq // hk)
+    bad = sorted(map(tuple, np.argwhere(~np.isfinite(got))))
+    assert bad == [(last, h, 5) for h in heads] and all(got[i] == np.inf for i in bad)
+    c.v[first + 1, 0, 5] = 0.0  # its weight counts in every dim; with 0 in this one the oracle is finite
+    want, absolute, total = c.want()
+    n = int(c.offsets[-1])
+    for i in bad:
+        got[i] = want[i]
+    worst, _ = prefix_errors(got, want[:n], absolute[:n], total[:n], max(held) + max(nodes), 6.0)
+    assert worst <= 1.0
